@@ -217,9 +217,10 @@ def _plain_reserve(lens, add, table, free, num_free, page, tokens):
     n = num_free.long()[0]
     cum_need, cum_back = need.cumsum(0), back.cumsum(0)
     top = n + cum_back[-1]
-    granted = (ad <= 0) | (fits & ((need == 0) | (cum_need <= top)))
+    granted = (ad > 0) & fits & ((need == 0) | (cum_need <= top))
+    kept = (ad > 0) & ~granted
     take = torch.where(granted, need, 0).cumsum(0)
-    out_len = torch.where(granted, want, ln)
+    out_len = torch.where(kept, ln, want)
     # the stack with the pages given back, read from the top: entry x below the top
     P = free.numel()
     x = torch.arange(P + 1, device=dev)
@@ -228,7 +229,7 @@ def _plain_reserve(lens, add, table, free, num_free, page, tokens):
     from_top = torch.where(x < cum_back[-1], given, free.long()[(top - 1 - x).clamp(0, P - 1)])
     # table entries of the pages taken
     col = torch.arange(width, device=dev)[None, :]
-    fresh = (col >= old_p[:, None]) & (col < new_p[:, None]) & (granted & (ad > 0))[:, None]
+    fresh = (col >= old_p[:, None]) & (col < new_p[:, None]) & granted[:, None]
     which = (take - torch.where(granted, need, 0))[:, None] + col - old_p[:, None]
     tab = torch.where(fresh, from_top[which.clamp(0, P)], tab)
     # the stack afterwards: pages given back and not taken again
@@ -335,7 +336,7 @@ def exact(case, seed):
         stack += back[::-1]
         new, slots, positions, granted, asked, room = [], [], [], [], 0, len(stack)
         for b, (ln, ad) in enumerate(zip(lens, add)):
-            ok = True
+            ok = ad > 0
             if ad > 0:
                 need = _pages(ln + ad, page) - _pages(ln, page)
                 ok = _pages(ln + ad, page) <= table.shape[1]
@@ -348,7 +349,7 @@ def exact(case, seed):
                 for p in range(ln, ln + ad):
                     slots.append(int(table[b, p // page]) * page + p % page if ok else -1)
                     positions.append(p if ok else -1)
-            new.append(max(0, ln + ad) if ok else ln)
+            new.append(ln if ad > 0 and not ok else max(0, ln + ad))
             granted.append(ok)
         disk[n:len(stack)] = stack[n:]
         return {"lens": np.array(new), "num_free": np.array([len(stack)]), "slots": np.array(slots), "positions": np.array(positions),
