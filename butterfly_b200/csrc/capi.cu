@@ -38,6 +38,12 @@ int launch_selection_dump(const bna_route*, int, int32_t*, int32_t*, cudaStream_
 int take_device_error(int, int32_t*);
 int launch_probe(int, cudaStream_t);
 void set_prefill_trace(uint64_t*);
+int launch_reserve(const int32_t*, const int32_t*, int, int32_t*, int64_t, int, int32_t*, int, const int32_t*, int,
+                   int32_t*, int32_t*, uint8_t*, int64_t*, int32_t*, int64_t, cudaStream_t);
+int launch_paged_append(const bna_tensor4*, const bna_tensor4*, bna_tensor4*, bna_tensor4*, const int64_t*, cudaStream_t);
+int launch_paged_decode(const bna_tensor4*, bna_tensor4*, bna_tensor4*, const bna_tensor4*, const bna_tensor4*,
+                        const uint8_t*, bna_tensor4*, float*, int64_t, int64_t, int, const int32_t*, int64_t, int, const int32_t*, int,
+                        float, cudaStream_t);
 
 // ---------------------------------------------------------------- validation helpers
 static bool null4(const bna_tensor4* t) { return t == nullptr || t->data == nullptr; }
@@ -408,6 +414,102 @@ int bna_decode_step_qk(const bna_tensor4* q_raw, const bna_tensor4* k_raw, const
   return decode_step_impl(q_raw, k_raw, v_new, ring_k, ring_v, sum_k, sum_v, out, lse, lse_stride_b, lse_stride_h,
                           dtype, route, window, pos, ring, close_block, close_slot, num_summary_limit, scale, stream,
                           &prep);
+}
+
+// ---------------------------------------------------------------- paged key/value cache
+// A pool [pages, Hkv, page_size, dh] that the kernels write through (no two rows may share memory).
+static int check_pools(const bna_tensor4* kp, const bna_tensor4* vp, int64_t dh) {
+  if (dh != 64 && dh != 128 && dh != 256) return fail(BNA_UNSUPPORTED, "paged cache: head_dim must be 64, 128 or 256");
+  const char* names[2] = {"k_pages", "v_pages"};
+  const bna_tensor4* ts[2] = {kp, vp};
+  for (int i = 0; i < 2; ++i) {
+    if (int rc = check_rows(ts[i], names[i], dh)) return rc;
+    for (int d = 0; d < 3; ++d) {
+      if (ts[i]->size[d] <= 0 || ts[i]->size[d] > INT32_MAX) return fail(BNA_BAD_SHAPE, std::string(names[i]) + " is empty or too large");
+      if (ts[i]->size[d] > 1 && ts[i]->stride[d] < dh)
+        return fail(BNA_BAD_STRIDE, std::string(names[i]) + ": rows must not overlap (strides of at least head_dim)");
+    }
+  }
+  for (int d = 0; d < 3; ++d)
+    if (kp->size[d] != vp->size[d]) return fail(BNA_BAD_SHAPE, "k_pages and v_pages shapes differ");
+  if (kp->size[2] % 16) return fail(BNA_UNSUPPORTED, "paged cache: page_size must be a multiple of 16");
+  return BNA_OK;
+}
+
+int bna_paged_reserve(const int32_t* lens, const int32_t* add, int32_t requests, int32_t* block_table,
+                      int64_t table_stride, int32_t table_width, int32_t* free_pages, int32_t num_pages,
+                      const int32_t* num_free, int32_t page_size, int32_t* lens_out, int32_t* num_free_out,
+                      uint8_t* granted, int64_t* slot_map, int32_t* positions, int64_t num_tokens, void* stream) {
+  if (requests < 0 || num_tokens < 0 || num_tokens > INT32_MAX) return fail(BNA_BAD_SHAPE, "paged_reserve: bad request or token count");
+  if (requests == 0) return num_tokens ? fail(BNA_BAD_SHAPE, "paged_reserve: tokens without requests") : BNA_OK;
+  if (table_width <= 0 || num_pages <= 0 || page_size <= 0 || table_stride < table_width)
+    return fail(BNA_BAD_SHAPE, "paged_reserve: table width, pages and page_size must be positive, rows must not overlap");
+  if (!lens || !add || !block_table || !free_pages || !num_free || !lens_out || !num_free_out || !granted ||
+      (num_tokens && (!slot_map || !positions)))
+    return fail(BNA_BAD_SHAPE, "paged_reserve: null pointer");
+  if (lens_out == lens || num_free_out == num_free)
+    return fail(BNA_BAD_SHAPE, "paged_reserve: lens_out / num_free_out must not be the inputs");
+  for (const void* p : {(const void*)lens, (const void*)add, (const void*)block_table, (const void*)free_pages, (const void*)num_free,
+                        (const void*)lens_out, (const void*)num_free_out, (const void*)positions})
+    if (reinterpret_cast<uintptr_t>(p) & 3) return fail(BNA_BAD_STRIDE, "paged_reserve: pointers must be 4-byte aligned");
+  if (reinterpret_cast<uintptr_t>(slot_map) & 7) return fail(BNA_BAD_STRIDE, "paged_reserve: slot_map must be 8-byte aligned");
+  return launch_reserve(lens, add, requests, block_table, table_stride, table_width, free_pages, num_pages, num_free,
+                        page_size, lens_out, num_free_out, granted, slot_map, positions, num_tokens, (cudaStream_t)stream);
+}
+
+int bna_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* k_pages, bna_tensor4* v_pages,
+                     const int64_t* slot_map, int32_t dtype, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (!k || !v || !k_pages || !v_pages) return fail(BNA_BAD_SHAPE, "paged_append: null tensor");
+  if (k->size[0] != 1 || v->size[0] != 1 || k->size[1] != v->size[1] || k->size[2] != v->size[2])
+    return fail(BNA_BAD_SHAPE, "paged_append: k and v must be [1, Hkv, tokens, dh] of one shape");
+  if (int rc = check_pools(k_pages, v_pages, k->size[3])) return rc;
+  if (k->size[1] != k_pages->size[1]) return fail(BNA_BAD_SHAPE, "paged_append: head counts of the rows and the pool differ");
+  if (k->size[2] == 0) return BNA_OK;
+  if (int rc = check_rows(k, "k", k_pages->size[3])) return rc;
+  if (int rc = check_rows(v, "v", k_pages->size[3])) return rc;
+  if (!slot_map) return fail(BNA_BAD_SHAPE, "paged_append: null slot_map");
+  if (reinterpret_cast<uintptr_t>(slot_map) & 7) return fail(BNA_BAD_STRIDE, "paged_append: slot_map must be 8-byte aligned");
+  return launch_paged_append(k, v, k_pages, v_pages, slot_map, (cudaStream_t)stream);
+}
+
+int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_tensor4* v_pages, const bna_tensor4* k_new,
+                     const bna_tensor4* v_new, const uint8_t* active, bna_tensor4* out, float* lse,
+                     int64_t lse_stride_b, int64_t lse_stride_h, int32_t dtype, const int32_t* block_table, int64_t table_stride, int32_t table_width,
+                     const int32_t* lens, int32_t window, float scale, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (!q || !k_pages || !v_pages || !out) return fail(BNA_BAD_SHAPE, "paged_decode: null tensor");
+  const int64_t dh = q->size[3], B = q->size[0], Hq = q->size[1], Hkv = k_pages->size[1];
+  if (int rc = check_pools(k_pages, v_pages, dh)) return rc;
+  if (Hq <= 0 || Hq % Hkv) return fail(BNA_BAD_SHAPE, "num query heads must be a multiple of num kv heads");
+  if (Hq > 65535 || Hkv > 65535) return fail(BNA_UNSUPPORTED, "paged_decode: too many heads");
+  if (q->size[2] != 1) return fail(BNA_BAD_SHAPE, "paged_decode: q must be [B, Hq, 1, dh], one new token per request");
+  if (B == 0) return BNA_OK;
+  if (B < 0 || B > INT32_MAX) return fail(BNA_BAD_SHAPE, "paged_decode: bad batch size");
+  if (int rc = check_rows(q, "q", dh)) return rc;
+  if (int rc = check_rows(out, "out", dh)) return rc;
+  for (int i = 0; i < 3; ++i)
+    if (out->size[i] != q->size[i]) return fail(BNA_BAD_SHAPE, "out shape mismatch");
+  if ((k_new == nullptr) != (v_new == nullptr)) return fail(BNA_BAD_SHAPE, "paged_decode: k_new and v_new go together");
+  if (active && !k_new) return fail(BNA_BAD_SHAPE, "paged_decode: active says which requests have a k_new / v_new row");
+  if (k_new) {
+    const char* names[2] = {"k_new", "v_new"};
+    const bna_tensor4* ts[2] = {k_new, v_new};
+    for (int i = 0; i < 2; ++i) {
+      if (int rc = check_rows(ts[i], names[i], dh)) return rc;
+      if (ts[i]->size[0] != B || ts[i]->size[1] != Hkv || ts[i]->size[2] != 1)
+        return fail(BNA_BAD_SHAPE, std::string(names[i]) + " must be [B, Hkv, 1, dh]");
+    }
+  }
+  if (!block_table || !lens) return fail(BNA_BAD_SHAPE, "paged_decode: null block_table or lens");
+  if ((reinterpret_cast<uintptr_t>(block_table) & 3) || (reinterpret_cast<uintptr_t>(lens) & 3))
+    return fail(BNA_BAD_STRIDE, "paged_decode: block_table and lens must be 4-byte aligned");
+  if (table_width <= 0 || (B > 1 && table_stride < 0)) return fail(BNA_BAD_SHAPE, "paged_decode: bad block_table shape");
+  if ((int64_t)table_width * k_pages->size[2] > INT32_MAX) return fail(BNA_UNSUPPORTED, "paged_decode: a table row covers 2^31 tokens or more");
+  if (window < 0) return fail(BNA_BAD_SHAPE, "window must be >= 0 (0: every key)");
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(BNA_BAD_SHAPE, "scale must be positive");
+  return launch_paged_decode(q, k_pages, v_pages, k_new, v_new, active, out, lse, lse_stride_b, lse_stride_h, dtype, block_table,
+                             table_stride, table_width, lens, window, scale, (cudaStream_t)stream);
 }
 
 }  // extern "C"

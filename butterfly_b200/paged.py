@@ -1,0 +1,211 @@
+"""Paged key/value cache: requests of different lengths, and decode over their whole context.
+
+``CompressedKVCache`` keeps one offset for a whole batch and a bounded window per sequence.  The
+layers that keep ordinary (dense) attention, served to requests that come and go, need the
+other kind: keys and values in pages of ``page_size`` tokens from one pool, a block table per
+request, and attention that reads through the table.
+
+  paged_reserve            pages, slots and positions for a step's tokens, from the requests'
+                           lengths (block tables and the free-page stack stay on the GPU)
+  paged_append             the tokens' key / value rows into their slots
+  paged_decode_attention   one new token per request over its pages, optionally writing that
+                           token's rows in the same launch
+  PagedKVCache             the three of them over per-layer pools
+
+Pools are ``[pages, Hkv, page_size, dh]`` views (``page_size`` a multiple of 16, ``dh`` 64, 128
+or 256; rows of ``dh`` contiguous), so token-major pages are a transposed view.  Everything is
+enqueued on the current stream and nothing waits for the host.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from . import _lib
+
+RELEASE = -2 ** 31  # an ``add`` entry that gives all of a request's pages back
+
+
+class PagedReservation(NamedTuple):
+    """What ``paged_reserve`` returns, all on the device."""
+    lens: torch.Tensor        # [B] int32 lengths after the call
+    num_free: torch.Tensor    # [1] int32 pages left on the stack
+    slot_map: torch.Tensor    # [num_tokens] int64, -1 for refused and unused entries
+    positions: torch.Tensor   # [num_tokens] int32, -1 likewise
+    granted: torch.Tensor     # [B] bool: this request's added tokens have slots
+
+
+def _ints(name: str, x: torch.Tensor, dim: int) -> None:
+    if x.dtype != torch.int32 or x.dim() != dim or x.stride(-1) != 1 and x.shape[-1] > 1:
+        raise ValueError(f"{name} must be a {dim}-D int32 tensor with a contiguous last dim")
+
+
+def paged_reserve(lens: torch.Tensor, add: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                  num_free: torch.Tensor, *, page_size: int, num_tokens: int) -> PagedReservation:
+    """Room for ``add[b]`` more tokens of every request (``lens``, ``add`` [B] int32).
+
+    ``add > 0`` takes the pages the request's ``block_table`` row [B, width] lacks from the top
+    of the stack ``free_pages[:num_free]``; ``add < 0`` takes tokens back (a rollback; ``RELEASE``
+    for a request that is done) and returns pages emptied by it.  Requests are served in order
+    while pages last; one that is refused (``add > 0`` and not ``granted``) keeps its length.  The added
+    tokens of request 0, then 1, ... are entries 0, 1, ... of ``slot_map`` and ``positions``
+    (``num_tokens`` of them: at least the sum of the positive ``add``).  ``block_table`` and
+    ``free_pages`` are updated in place, the lengths and the stack height are returned."""
+    _lib.require_cuda(lens, add, block_table, free_pages, num_free)
+    for name, x, d in (("lens", lens, 1), ("add", add, 1), ("block_table", block_table, 2),
+                       ("free_pages", free_pages, 1), ("num_free", num_free, 1)):
+        _ints(name, x, d)
+    B, width = block_table.shape
+    if lens.shape[0] != B or add.shape[0] != B or num_free.shape[0] != 1:
+        raise ValueError(f"lens and add must be [{B}] as block_table's rows, num_free [1]")
+    dev, n = lens.device, int(num_tokens)
+    out = torch.empty(B, dtype=torch.int32, device=dev)
+    left = torch.empty(1, dtype=torch.int32, device=dev)
+    granted = torch.empty(B, dtype=torch.bool, device=dev)
+    slots = torch.empty(n, dtype=torch.int64, device=dev)
+    positions = torch.empty(n, dtype=torch.int32, device=dev)
+    _lib.check(_lib.lib().bna_paged_reserve(
+        lens.data_ptr(), add.data_ptr(), B, block_table.data_ptr(), block_table.stride(0) if B > 1 else width, width,
+        free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), int(page_size), out.data_ptr(), left.data_ptr(),
+        granted.data_ptr(), slots.data_ptr(), positions.data_ptr(), n, _lib.stream_ptr(dev)))
+    return PagedReservation(out, left, slots, positions, granted)
+
+
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype) -> None:
+    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise ValueError("the pools must have the dtype of the rows")
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 slot_map: torch.Tensor) -> None:
+    """Write token t's rows ``k[t]`` / ``v[t]`` ([tokens, Hkv, dh], any token and head strides)
+    into slot ``slot_map[t]`` (int64) of the pools; negative slots are skipped."""
+    _lib.require_cuda(k, v, k_pages, v_pages, slot_map)
+    if k.dim() != 3 or v.dim() != 3:
+        raise ValueError("k and v must be [tokens, Hkv, dh]")
+    if v.dtype != k.dtype:
+        raise ValueError("k and v dtype mismatch")
+    _pools(k_pages, v_pages, k.dtype)
+    if slot_map.dtype != torch.int64 or slot_map.dim() != 1 or slot_map.shape[0] != k.shape[0] \
+            or slot_map.stride(0) != 1 and k.shape[0] > 1:
+        raise ValueError(f"slot_map must be a contiguous [{k.shape[0]}] int64 tensor")
+    tk, tv = _lib.t4(k.transpose(0, 1).unsqueeze(0)), _lib.t4(v.transpose(0, 1).unsqueeze(0))
+    tkp, tvp = _lib.t4(k_pages), _lib.t4(v_pages)
+    _lib.check(_lib.lib().bna_paged_append(ctypes.byref(tk), ctypes.byref(tv), ctypes.byref(tkp), ctypes.byref(tvp),
+                                           slot_map.data_ptr(), _lib.dtype_code(k.dtype), _lib.stream_ptr(k.device)))
+
+
+def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                           lens: torch.Tensor, *, k_new: Optional[torch.Tensor] = None,
+                           v_new: Optional[torch.Tensor] = None, active: Optional[torch.Tensor] = None,
+                           window: int = 0, scale: Optional[float] = None, return_lse: bool = False):
+    """Attention of one new token per request: q [B,Hq,1,dh] over the first ``lens[b]`` tokens of
+    request b (the last ``window`` of them where ``window`` > 0).  ``lens`` counts the new token.
+
+    With ``k_new`` / ``v_new`` [B,Hkv,1,dh] the new token's rows are read from there and written
+    into their slot by the same launch (in place of ``paged_append``) for the requests that
+    ``active`` [B] bool names (default: all; pass ``PagedReservation.granted`` where some
+    requests got no room, or rest).  Returns [B,Hq,1,dh]
+    (storage [B,1,Hq,dh]) in q's dtype; with ``return_lse`` also the fp32 natural-log sums
+    [B,Hq,1].  A request of length 0 gives zeros and -inf."""
+    _lib.require_cuda(q, k_pages, v_pages, block_table, lens)
+    if q.dim() != 4:
+        raise ValueError("q must be [B, Hq, 1, dh]")
+    B, Hq, Tq, dh = q.shape
+    _pools(k_pages, v_pages, q.dtype)
+    _ints("block_table", block_table, 2)
+    _ints("lens", lens, 1)
+    if block_table.shape[0] != B or lens.shape[0] != B:
+        raise ValueError(f"block_table and lens must have {B} rows")
+    nk = nv = act = None
+    if k_new is not None or v_new is not None:
+        if k_new is None or v_new is None:
+            raise ValueError("k_new and v_new go together")
+        _lib.require_cuda(q, k_new, v_new)
+        if k_new.dtype != q.dtype or v_new.dtype != q.dtype:
+            raise ValueError("q, k_new, v_new dtype mismatch")
+        nk, nv = ctypes.byref(_lib.t4(k_new)), ctypes.byref(_lib.t4(v_new))
+    if active is not None:
+        _lib.require_cuda(q, active)
+        if active.dtype != torch.bool or active.shape != (B,) or not active.is_contiguous():
+            raise ValueError(f"active must be a contiguous [{B}] bool tensor")
+        act = active.data_ptr()
+    out = torch.empty((B, Tq, Hq, dh), device=q.device, dtype=q.dtype).transpose(1, 2)
+    lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if return_lse else None
+    tq, tkp, tvp, to = (_lib.t4(x) for x in (q, k_pages, v_pages, out))
+    _lib.check(_lib.lib().bna_paged_decode(
+        ctypes.byref(tq), ctypes.byref(tkp), ctypes.byref(tvp), nk, nv, act, ctypes.byref(to),
+        lse.data_ptr() if return_lse else None, Hq, 1, _lib.dtype_code(q.dtype), block_table.data_ptr(),
+        block_table.stride(0), block_table.shape[1], lens.data_ptr(), int(window),
+        float(scale) if scale is not None else 1.0 / math.sqrt(dh), _lib.stream_ptr(q.device)))
+    return (out, lse) if return_lse else out
+
+
+class PagedKVCache:
+    """Pools of ``num_layers`` layers under one set of block tables, lengths and free pages.
+
+    The requests are the ``max_requests`` rows of the tables; a row of length 0 is vacant."""
+
+    def __init__(self, *, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+                 max_requests: int, max_tokens_per_request: int, dtype: torch.dtype = torch.bfloat16,
+                 device: torch.device | str = "cuda") -> None:
+        self.page_size = int(page_size)
+        shape = (int(num_pages), int(num_kv_heads), self.page_size, int(head_dim))
+        # every read goes through a row written before, so the pools need no clearing
+        self.k_pages = [torch.empty(shape, dtype=dtype, device=device) for _ in range(int(num_layers))]
+        self.v_pages = [torch.empty(shape, dtype=dtype, device=device) for _ in range(int(num_layers))]
+        width = -(-int(max_tokens_per_request) // self.page_size)
+        self.block_table = torch.full((int(max_requests), width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(int(max_requests), dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(int(num_pages) - 1, -1, -1, dtype=torch.int32, device=device)
+        self.num_free = torch.full((1,), int(num_pages), dtype=torch.int32, device=device)
+
+    @property
+    def max_requests(self) -> int:
+        return int(self.lens.shape[0])
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes of all pools (what the cache holds on the device, used or not)."""
+        return sum(x.numel() * x.element_size() for x in self.k_pages + self.v_pages)
+
+    def reserve(self, add: torch.Tensor | Sequence[int], num_tokens: Optional[int] = None) -> PagedReservation:
+        """Advance every request by ``add`` tokens (see ``paged_reserve``); done once per step, for
+        all layers.  ``num_tokens`` may be left out when ``add`` is a host sequence."""
+        if not isinstance(add, torch.Tensor):
+            add = [int(x) for x in add]
+            if num_tokens is None:
+                num_tokens = sum(max(x, 0) for x in add)
+            add = torch.tensor(add, dtype=torch.int32).to(self.lens.device, non_blocking=True)
+        if num_tokens is None:
+            raise ValueError("num_tokens is needed when add is a device tensor")
+        r = paged_reserve(self.lens, add, self.block_table, self.free_pages, self.num_free, page_size=self.page_size,
+                          num_tokens=num_tokens)
+        self.lens, self.num_free = r.lens, r.num_free
+        return r
+
+    def release(self, rows: Sequence[int]) -> None:
+        """Give back all pages of the requests in ``rows``."""
+        add = [0] * self.max_requests
+        for b in rows:
+            add[int(b)] = RELEASE
+        self.reserve(add)
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
+        """The reserved tokens' rows [tokens, Hkv, dh] of one layer into their slots."""
+        paged_append(k, v, self.k_pages[layer], self.v_pages[layer], slot_map)
+
+    def attend(self, layer: int, q: torch.Tensor, *, k_new: Optional[torch.Tensor] = None,
+               v_new: Optional[torch.Tensor] = None, active: Optional[torch.Tensor] = None, window: int = 0,
+               scale: Optional[float] = None, return_lse: bool = False):
+        """One new token per request, q [max_requests,Hq,1,dh], over its cached context (see
+        ``paged_decode_attention``)."""
+        return paged_decode_attention(q, self.k_pages[layer], self.v_pages[layer], self.block_table, self.lens,
+                                      k_new=k_new, v_new=v_new, active=active, window=window, scale=scale,
+                                      return_lse=return_lse)
+
+
+__all__ = ["PagedKVCache", "PagedReservation", "RELEASE", "paged_append", "paged_decode_attention", "paged_reserve"]

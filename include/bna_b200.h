@@ -353,6 +353,51 @@ BNA_API int bna_prefill_attention_static_scratch(const bna_tensor4* q, const bna
                                                  const bna_route* route, int32_t window, float scale,
                                                  void* stream);
 
+/* ---- Paged key/value cache: requests of different lengths, full-context decode --------------
+ * No counterpart in the reference (its caches hold one offset for the whole batch).  A pool is
+ * [pages, Hkv, page_size, dh] (any strides with rows of dh contiguous and 16-byte aligned, so
+ * token-major pages are a transposed view), page_size a multiple of 16, dh 64, 128 or 256.
+ * Row b of the int32 block table names the pages of request b in order; its token p lies in
+ * page block_table[b][p / page_size] at offset p % page_size: slot = page * page_size + offset. */
+
+/* Pages and slots for the tokens that `add` gives each request (device arrays throughout).
+ * Request b goes from lens[b] to max(0, lens[b] + add[b]) tokens: add > 0 takes the pages its
+ * table row lacks from the top of the stack free_pages[0 .. num_free[0]), add < 0 (a rollback;
+ * INT32_MIN for a request that is done) puts its last pages back on the stack.  Pages given
+ * back can be taken in the same call; a call followed by its opposite restores the stack.
+ * Requests are served in order while the pages last: granted[b] = 1 where add[b] > 0 tokens got
+ * their slots.  A request whose pages ran out, or whose length would pass table_width *
+ * page_size, keeps its length, its tokens get slot and position -1, and later requests that
+ * need pages are refused too once the pages asked for so far exceed the stack.  slot_map / positions [num_tokens] hold the added tokens
+ * of request 0, then 1, ... (-1 past the last).  lens and num_free are read only; lens_out
+ * [requests] and num_free_out [1] are written (not in place).  block_table and free_pages are
+ * updated in place; entries past a request's pages keep their old values.  requests <= 4096. */
+BNA_API int bna_paged_reserve(const int32_t* lens, const int32_t* add, int32_t requests, int32_t* block_table,
+                              int64_t table_stride, int32_t table_width, int32_t* free_pages, int32_t num_pages,
+                              const int32_t* num_free, int32_t page_size, int32_t* lens_out, int32_t* num_free_out,
+                              uint8_t* granted, int64_t* slot_map, int32_t* positions, int64_t num_tokens,
+                              void* stream);
+
+/* Rows t of k / v [1, Hkv, tokens, dh] into slot slot_map[t] of every head's pages; a slot outside
+ * the pool (-1) is skipped.  Two tokens with one slot: either may be kept. */
+BNA_API int bna_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* k_pages, bna_tensor4* v_pages,
+                             const int64_t* slot_map, int32_t dtype, void* stream);
+
+/* Attention of one new token per request: q / out [B, Hq, 1, dh] over keys
+ * [max(0, lens[b] - window), lens[b]) of request b (window 0: all of them), Hq a multiple of Hkv;
+ * lse (optional, fp32, natural log, element strides) of the softmax.  lens[b] counts the new
+ * token.  A request of length 0 gets out = 0, lse = -inf, and so does a row whose scores are
+ * all -inf; what pages hold beyond the keys attended to (NaN included) does not matter.  With
+ * k_new / v_new [B, Hkv, 1, dh] the row at position lens[b] - 1 is taken from them and written
+ * into its page, for the requests with active[b] != 0 (null: all; the others attend to what
+ * their pages hold).  A length is cut to table_width * page_size; a page number outside the pool reads
+ * as zeros. */
+BNA_API int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_tensor4* v_pages,
+                             const bna_tensor4* k_new, const bna_tensor4* v_new, const uint8_t* active,
+                             bna_tensor4* out, float* lse, int64_t lse_stride_b, int64_t lse_stride_h, int32_t dtype,
+                             const int32_t* block_table, int64_t table_stride, int32_t table_width,
+                             const int32_t* lens, int32_t window, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
