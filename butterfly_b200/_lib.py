@@ -25,7 +25,7 @@ EXPORTED = (
     "bna_rmsnorm", "bna_qk_norm_rope", "bna_gate_sigmoid_mul", "bna_swiglu", "bna_gemv_rmsnorm", "bna_gemv_gated",
     "bna_gemv", "bna_launch_probe", "bna_decode_step_qk", "bna_prefill_attention_gated",
     "bna_gemm_swiglu", "bna_gemm_qkv_norm_rope", "bna_gemm_residual", "bna_row_sumsq",
-    "bna_paged_reserve", "bna_paged_append", "bna_paged_decode",
+    "bna_paged_reserve", "bna_paged_append", "bna_paged_decode", "bna_paged_decode_workspace_bytes",
 )
 
 
@@ -95,7 +95,8 @@ def lib() -> ctypes.CDLL:
             "bna_gemv": (i32, [vp, i64, vp, i64, i64, vp, i64, vp, i64, i32, i32, vp]),
             "bna_paged_reserve": (i32, [vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, i64, vp]),
             "bna_paged_append": (i32, [T4, T4, T4, T4, vp, i32, vp]),
-            "bna_paged_decode": (i32, [T4, T4, T4, T4, T4, vp, T4, vp, i64, i64, i32, vp, i64, i32, vp, i32, f32, vp]),
+            "bna_paged_decode": (i32, [T4, T4, T4, T4, T4, vp, T4, vp, i64, i64, i32, vp, i64, i32, vp, i32, f32, vp, i64, vp]),
+            "bna_paged_decode_workspace_bytes": (i64, []),
             "bna_decode_step": (i32, [T4, T4, T4, T4, T4, T4, T4, T4, vp, i64, i64, i32, R, i32, i64, i64, i64, i64, i32, f32, vp]),
         }
         for name, (res, args) in sig.items():

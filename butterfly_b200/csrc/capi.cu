@@ -43,7 +43,8 @@ int launch_reserve(const int32_t*, const int32_t*, int, int32_t*, int64_t, int, 
 int launch_paged_append(const bna_tensor4*, const bna_tensor4*, bna_tensor4*, bna_tensor4*, const int64_t*, cudaStream_t);
 int launch_paged_decode(const bna_tensor4*, bna_tensor4*, bna_tensor4*, const bna_tensor4*, const bna_tensor4*,
                         const uint8_t*, bna_tensor4*, float*, int64_t, int64_t, int, const int32_t*, int64_t, int, const int32_t*, int,
-                        float, cudaStream_t);
+                        float, void*, cudaStream_t);
+int64_t paged_decode_workspace_bytes();
 
 // ---------------------------------------------------------------- validation helpers
 static bool null4(const bna_tensor4* t) { return t == nullptr || t->data == nullptr; }
@@ -473,10 +474,13 @@ int bna_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* k_
   return launch_paged_append(k, v, k_pages, v_pages, slot_map, (cudaStream_t)stream);
 }
 
+int64_t bna_paged_decode_workspace_bytes(void) { return paged_decode_workspace_bytes(); }
+
 int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_tensor4* v_pages, const bna_tensor4* k_new,
                      const bna_tensor4* v_new, const uint8_t* active, bna_tensor4* out, float* lse,
                      int64_t lse_stride_b, int64_t lse_stride_h, int32_t dtype, const int32_t* block_table, int64_t table_stride, int32_t table_width,
-                     const int32_t* lens, int32_t window, float scale, void* stream) {
+                     const int32_t* lens, int32_t window, float scale, void* workspace, int64_t workspace_bytes,
+                     void* stream) {
   if (int rc = check_dtype(dtype)) return rc;
   if (!q || !k_pages || !v_pages || !out) return fail(BNA_BAD_SHAPE, "paged_decode: null tensor");
   const int64_t dh = q->size[3], B = q->size[0], Hq = q->size[1], Hkv = k_pages->size[1];
@@ -508,8 +512,11 @@ int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_tensor4* v_
   if ((int64_t)table_width * k_pages->size[2] > INT32_MAX) return fail(BNA_UNSUPPORTED, "paged_decode: a table row covers 2^31 tokens or more");
   if (window < 0) return fail(BNA_BAD_SHAPE, "window must be >= 0 (0: every key)");
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(BNA_BAD_SHAPE, "scale must be positive");
+  if (!workspace || workspace_bytes < paged_decode_workspace_bytes())
+    return fail(BNA_CAPACITY, "paged_decode: workspace smaller than bna_paged_decode_workspace_bytes()");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BNA_BAD_STRIDE, "paged_decode: workspace must be 16-byte aligned");
   return launch_paged_decode(q, k_pages, v_pages, k_new, v_new, active, out, lse, lse_stride_b, lse_stride_h, dtype, block_table,
-                             table_stride, table_width, lens, window, scale, (cudaStream_t)stream);
+                             table_stride, table_width, lens, window, scale, workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

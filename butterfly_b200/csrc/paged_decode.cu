@@ -1,20 +1,50 @@
 // paged_decode.cu — attention of one new token per request over a paged key/value cache.
 //   s_j = scale * q . k_j   for keys j in [max(0, len - window), len)
 //   out = sum_j softmax(s)_j v_j,   lse = log sum_j exp(s_j);  no key: out = 0, lse = -inf
+// One pass over the keys with a running maximum m, sum l and output o; a set of keys cut into
+// parts is joined by  M = max m_i,  L = sum l_i 2^(m_i - M),  out = sum o_i 2^(m_i - M) / L
+// (m in the exp2 domain).
+//
+// Each key and value is read once and serves the G = Hq / Hkv query heads of its KV head:
+// 2 G FLOP per byte, far below the tensor cores' balance, so the kernel is bound by HBM and is
+// built to keep its reads in flight:
+//   * Work is cut evenly by bytes, not by request: the granules (16 keys of one KV head) of all
+//     requests form one line, and each of the persistent CTAs (one per SM) takes an equal
+//     stretch of it.  One long request spreads over all SMs, many short ones share an SM.
+//   * A producer warp walks the CTA's stretch, looks the pages up and issues one TMA tile copy
+//     for a granule's keys and one for its values into a ring of granule slots (192 KB a CTA); it runs ahead across the ends of requests.
+//   * Eight consumer warps (four at head_dim 256) take the granules in turn, each with its own m, l and o in
+//     registers: no barrier between warps until a request's stretch ends.
+//   * A (request, KV head) that lies in one CTA is finished there.  Of one cut by CTA
+//     boundaries each CTA leaves a part in the workspace, and the CTA that arrives last joins
+//     the parts in their order on the line, so the result does not depend on the arrival order.
+#include <cuda.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
+#include <algorithm>
+#include <climits>
 #include <cmath>
+#include <map>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
 #include "common.cuh"
+#include "mma.cuh"
+#include "sm100.cuh"
 
 namespace bna {
-namespace {
+int* device_error_word();
 
-constexpr int kWarps = 8;
-// Query heads of one KV head served by a CTA (the partial outputs fit 32 KB of shared memory).
-__host__ __device__ constexpr int rows_of(int dh) { return dh > 128 ? 4 : 8; }
+namespace {
+using namespace sm100;
+
+constexpr int kGran = 16;       // keys of a granule
+constexpr int kMaxCtas = 160;   // workspace parts are sized for this many CTAs
+constexpr int kRows = 16;       // query heads of one KV head served together
+constexpr int kMinPart = 16;    // granules a CTA gets at least (fewer CTAs otherwise)
+constexpr int kErrSite = 0x40;  // device error sites of this file
 
 struct PagedArgs {
   const uint8_t* q;
@@ -32,105 +62,665 @@ struct PagedArgs {
   int64_t table_stride;
   const int32_t* lens;
   int B, Hkv, G, width, num_pages, page_size, window;
+  int chunks, chunk_rows;  // the G heads in `chunks` groups of chunk_rows <= kRows
   float scale_log2;
+  uint8_t* ws;
+  int* err;
 };
 
-// One CTA per (request, KV head, group of up to 8 of its query heads); each warp walks every
-// 8th key with an online softmax (a lane holds head_dim / 32 dims), and the warps' partial
-// (max, sum, output) are joined through shared memory.
-template <typename T, int DH>
-__global__ void __launch_bounds__(kWarps * 32) paged_decode_kernel(const PagedArgs a) {
-  constexpr int E = DH / 32, kRows = rows_of(DH);
-  __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows], sm_o[kWarps][kRows][DH];
+// Workspace: arrival counters (zero between calls), (m, l) of every part, then the outputs.
+constexpr int64_t kWsMl = 4096;
+constexpr int64_t kWsO = kWsMl + (int64_t)2 * kMaxCtas * kRows * 8;
+constexpr int64_t kWsBytes = kWsO + (int64_t)2 * kMaxCtas * kRows * 256 * 4;
+
+// One stretch of a (request, KV head, head group) inside a CTA.
+struct Seg {
+  int b, h, r0, rows;  // request, KV head, first query head of the group (within G) and their count
+  int g0, n;           // granules (16-key blocks of the request) [g0, g0 + n); n < 0: no more
+  int lo, hi;          // keys attended to
+  int first_cta, parts, slot;  // parts of a cut pair, the CTA of the first one, this part's slot (-1: uncut)
+};
+
+template <int DH>
+struct Layout {
+  // Consumer warps.  head_dim 256: four, as the output and score registers of eight would not
+  // fit beside each other.
+  static constexpr int kCons = DH == 256 ? 4 : 8;
+  static constexpr int kThreads = 32 * (kCons + 1);  // and the producer
+  static constexpr int kSlotBytes = 2 * kGran * DH * 2;      // keys, then values
+  static constexpr int kSlots = 192 * 1024 / kSlotBytes;
+  // Granule i goes to warp i % kCons and slot i % kSlots: a slot has to stay with one warp,
+  // because a barrier's parity tells a wait that is one use ahead nothing about the use before.
+  static_assert(kSlots % kCons == 0, "a slot belongs to one warp");
+  static constexpr int kQPitch = 2 * DH + 16;                         // spreads the rows over the banks
+  static constexpr int kQBytes = kRows * kQPitch;
+  static constexpr int kQ = kSlots * kSlotBytes;
+  static constexpr int kBuf = kQ + 2 * kQBytes;
+  // merge of the warps: 16 rows x 32 columns, 8 x 64 or 4 x 128 (rows padded by 8 floats), or
+  // the weights and partial sums of a join
+  static constexpr int kMergeFloats = kCons * kRows * (32 + 8), kJoinFloats = kMaxCtas * kRows + 4 * 32 * kCons;
+  static constexpr int kBufBytes = 4 * (kMergeFloats > kJoinFloats ? kMergeFloats : kJoinFloats);
+  static constexpr int kMl = kBuf + kBufBytes;
+  static constexpr int kBars = kMl + 2 * kCons * kRows * 8;
+  static constexpr int kNumBars = 2 * kSlots + 5;
+  static constexpr int kSeg = kBars + kNumBars * 8;
+  static constexpr int kFlags = kSeg + 2 * (int)sizeof(Seg);
+  static constexpr int kBytes = (kFlags + 16 + 15) / 16 * 16;
+  static constexpr int kAlloc = kBytes + 1024;  // the base is aligned to 1024 (swizzle atom)
+  static_assert(kAlloc <= 232448, "shared memory of a CTA");
+};
+
+__device__ __forceinline__ int clamp_len(const PagedArgs& a, int len) {
+  return (int)min((int64_t)max(len, 0), (int64_t)a.width * a.page_size);
+}
+__device__ __forceinline__ int first_key(const PagedArgs& a, int len) {
+  return a.window > 0 ? max(0, len - a.window) : 0;
+}
+__device__ __forceinline__ int granules_of(const PagedArgs& a, int len) {
+  return len == 0 ? 0 : (len + kGran - 1) / kGran - first_key(a, len) / kGran;
+}
+
+// Offset of 16-byte chunk c of row r in a granule tile: 64-column boxes of 16 rows x 128 bytes,
+// 128-byte swizzle.
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+  return (uint32_t)((c >> 3) * (kGran * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(uint8_t* p, const float4& v, float f) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(ElemTraits<T>::pack2(v.x * f, v.y * f), ElemTraits<T>::pack2(v.z * f, v.w * f));
+}
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// WIDE: 9 to 16 query heads, the rows of the 16-row MMA.  Otherwise the heads are rows 0-7, and rows
+// 8-15 of the P V product carry the low part of the probabilities.  A probability is held
+// as hi + lo in the 16-bit type (relative error u^2 instead of u: rounding it once would add
+// as much error to the output as its final rounding does); with at most 8 heads lo rides in rows
+// that the MMA computes anyway, with more it costs a second MMA, which the memory hides.
+template <typename T, int DH, bool WIDE>
+__global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
+    paged_decode_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const PagedArgs a) {
+  using Lay = Layout<DH>;
+  constexpr int kCons = Lay::kCons;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + Lay::kBars);
+  uint64_t* empty = full + Lay::kSlots;
+  uint64_t* seg_full = empty + Lay::kSlots;
+  uint64_t* seg_empty = seg_full + 2;
+  uint64_t* cons_bar = seg_empty + 2;
+  Seg* segs = reinterpret_cast<Seg*>(sm + Lay::kSeg);
+  volatile int* abort_flag = reinterpret_cast<int*>(sm + Lay::kFlags);
+  volatile int* last_flag = abort_flag + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.x, h = blockIdx.y, r0 = blockIdx.z * kRows;
-  const int rows = min(kRows, a.G - r0);
-  int64_t len = max(a.lens[b], 0);
-  len = min(len, (int64_t)a.width * a.page_size);
-  const int64_t lo = a.window > 0 ? max((int64_t)0, len - a.window) : 0;
-  float q[kRows][E], o[kRows][E], m[kRows], l[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      o[r][e] = 0.f;
-      const T* row = reinterpret_cast<const T*>(a.q) + b * a.q_b + (h * a.G + r0 + min(r, rows - 1)) * a.q_h;
-      q[r][e] = (float)row[lane * E + e];
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Lay::kSlots; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(seg_full + i, 1);
+      mbar_init(seg_empty + i, kCons);
+    }
+    mbar_init(cons_bar, kCons);
+    fence_mbar_init();
+    *abort_flag = 0;
+    prefetch_tmap(&mk);
+    prefetch_tmap(&mv);
   }
-  for (int64_t j = lo + warp; j < len; j += kWarps) {
-    const int page = a.table[b * a.table_stride + j / a.page_size];
-    const int64_t off = j % a.page_size;
-    const bool inside = page >= 0 && page < a.num_pages;  // a page outside the pool reads as zeros
-    const bool fresh = a.kn && j == len - 1 && (!a.active || a.active[b]);
-    T* kr = reinterpret_cast<T*>(a.kp) + page * a.kp_p + h * a.kp_h + off * a.kp_t + lane * E;
-    T* vr = reinterpret_cast<T*>(a.vp) + page * a.vp_p + h * a.vp_h + off * a.vp_t + lane * E;
-    float kf[E], vf[E];
+  __syncthreads();
+  // every input may come from the previous kernel of the stream; the next one may be set up
+  // once that kernel is done
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, kErrSite + site, a.err));
+  };
+
+  if (warp == kCons) {
+    // ------------------------------------------------------------------ producer
+    const int per_b = a.Hkv * a.chunks;
+    int64_t total = 0;
+    for (int i = lane; i < a.B; i += 32) total += granules_of(a, clamp_len(a, a.lens[i]));
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (fresh) {
-        const T kx = reinterpret_cast<const T*>(a.kn)[b * a.kn_b + h * a.kn_h + lane * E + e];
-        const T vx = reinterpret_cast<const T*>(a.vn)[b * a.vn_b + h * a.vn_h + lane * E + e];
-        kf[e] = (float)kx;
-        vf[e] = (float)vx;
-        if (inside && blockIdx.z == 0) {
-          kr[e] = kx;
-          vr[e] = vx;
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int64_t U = total * per_b;
+    const int64_t C = max((int64_t)1, min((int64_t)gridDim.x, (U + kMinPart - 1) / kMinPart));
+    int64_t cur = blockIdx.x < C ? U * blockIdx.x / C : U;
+    const int64_t end = blockIdx.x < C ? U * (blockIdx.x + 1) / C : U;
+    int cnt = 0;      // granules issued
+    int nseg = 0;
+    bool ok = true;
+    if (cur < end) {
+      // the request holding granule `cur`, and the granules before it
+      int wb = 0, b = 0;
+      int64_t before = 0;
+      int len_w = 0;  // lane i: length of request wb + i
+      for (;; wb += 32) {
+        len_w = wb + lane < a.B ? clamp_len(a, a.lens[wb + lane]) : 0;
+        const int64_t mine = (int64_t)granules_of(a, len_w) * per_b;
+        int64_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += x;
         }
+        const unsigned past = __ballot_sync(0xffffffffu, before + incl > cur);
+        if (past) {
+          const int f = __ffs(past) - 1;
+          b = wb + f;
+          before += __shfl_sync(0xffffffffu, incl - mine, f);
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      int slot = 0;
+      uint32_t phase = 1;  // parity of the empty barriers' first use
+      int len = __shfl_sync(0xffffffffu, len_w, b - wb), nt = granules_of(a, len);
+      int pair = (int)((cur - before) / nt), t0 = (int)((cur - before) - (int64_t)pair * nt);
+      while (ok && cur < end) {
+        const int n = (int)min((int64_t)(nt - t0), end - cur);
+        const int si = nseg & 1;
+        if (!(ok = wait(seg_empty + si, (uint32_t)(((nseg >> 1) & 1) ^ 1), 0))) break;
+        Seg s;
+        s.b = b;
+        s.h = pair / a.chunks;
+        s.r0 = (pair - s.h * a.chunks) * a.chunk_rows;
+        s.rows = min(a.chunk_rows, a.G - s.r0);
+        s.lo = first_key(a, len);
+        s.hi = len;
+        s.g0 = s.lo / kGran + t0;
+        s.n = n;
+        s.slot = -1;
+        s.parts = 1;
+        s.first_cta = 0;
+        if (n < nt) {
+          const int64_t p0 = cur - t0;
+          s.first_cta = (int)(((p0 + 1) * C - 1) / U);
+          s.parts = (int)(((p0 + nt) * C - 1) / U) - s.first_cta + 1;
+          s.slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+        }
+        uint8_t* qdst = sm + Lay::kQ + si * Lay::kQBytes;
+        if (lane == 0) {
+          segs[si] = s;
+          mbar_arrive_expect_tx(seg_full + si, (uint32_t)(s.rows * 2 * DH));
+        }
+        __syncwarp();
+        if (lane < s.rows)
+          bulk_copy_g2s(qdst + lane * Lay::kQPitch, a.q + 2 * (b * a.q_b + (int64_t)(s.h * a.G + s.r0 + lane) * a.q_h), 2 * DH,
+                        seg_full + si);
+        const int32_t* trow = a.table + b * a.table_stride;
+        for (int i0 = 0; i0 < n && ok; i0 += 32) {
+          int page = -1, row = 0;
+          if (i0 + lane < n) {
+            const int pos = (s.g0 + i0 + lane) * kGran, pi = pos / a.page_size;
+            row = pos - pi * a.page_size;
+            page = trow[pi];
+          }
+          const int m = min(32, n - i0);
+          for (int j = 0; j < m; ++j) {
+            const int pg = __shfl_sync(0xffffffffu, page, j), rw = __shfl_sync(0xffffffffu, row, j);
+            if (!(ok = wait(empty + slot, phase, 1))) break;
+            if (lane == 0) {
+              // a page number outside the pool fills the tile with zeros
+              uint8_t* dst = sm + slot * Lay::kSlotBytes;
+              mbar_arrive_expect_tx(full + slot, Lay::kSlotBytes);
+              tma_load_5d(dst, &mk, full + slot, 0, rw, 0, s.h, pg);
+              tma_load_5d(dst + Lay::kSlotBytes / 2, &mv, full + slot, 0, rw, 0, s.h, pg);
+            }
+            ++cnt;
+            if (++slot == Lay::kSlots) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
+        }
+        ++nseg;
+        cur += n;
+        t0 = 0;
+        if (++pair == per_b) {
+          pair = 0;
+          do {  // the next request that has keys (there is one while cur < end)
+            if (++b >= wb + 32) {
+              wb = b;
+              len_w = wb + lane < a.B ? clamp_len(a, a.lens[wb + lane]) : 0;
+            }
+            len = __shfl_sync(0xffffffffu, len_w, b - wb);
+          } while (len == 0 && b + 1 < a.B);
+          nt = granules_of(a, len);
+        }
+      }
+    }
+    if (ok) {
+      const int si = nseg & 1;
+      if ((ok = wait(seg_empty + si, (uint32_t)(((nseg >> 1) & 1) ^ 1), 2)) && lane == 0) {
+        segs[si].n = -1;
+        mbar_arrive(seg_full + si);
+      }
+    }
+    // requests without keys
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      if (clamp_len(a, a.lens[b]) != 0) continue;
+      const int hq = a.Hkv * a.G;
+      for (int i = lane; i < hq * (DH / 8); i += 32)
+        st_128(a.out + 2 * (b * a.o_b + (int64_t)(i / (DH / 8)) * a.o_h) + 16 * (i % (DH / 8)), make_uint4(0, 0, 0, 0));
+      if (a.lse)
+        for (int i = lane; i < hq; i += 32) a.lse[b * a.ls_b + i * a.ls_h] = -INFINITY;
+    }
+    // no copy of this CTA is in flight when it ends, whatever the consumers did
+    for (int i = max(0, cnt - Lay::kSlots); i < cnt; ++i)
+      for (int tries = 0; tries < 1000; ++tries)
+        if (mbar_try_wait_suspend(full + i % Lay::kSlots, (i / Lay::kSlots) & 1, 20000u)) break;
+    return;
+  }
+
+  // -------------------------------------------------------------------- consumers
+  constexpr int NT = DH / 8;   // 8-column output tiles
+  constexpr int KS = DH / 16;  // 16-dim steps of the scores
+  constexpr bool kKeepQ = DH <= 128;
+  constexpr int kRowSets = WIDE ? 2 : 1;
+  float* buf = reinterpret_cast<float*>(sm + Lay::kBuf);
+  const uint32_t sm32 = smem_u32(sm);
+  const int gid = lane >> 2, tig = lane & 3;
+  const int tid = threadIdx.x;
+  uint32_t cons_phase = 0;
+  auto cons_sync = [&]() -> bool {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(cons_bar);
+    const bool ok = wait(cons_bar, cons_phase, 3);
+    cons_phase ^= 1;
+    return ok;
+  };
+  // ldmatrix lane offsets: keys as B operand (plain), values as B operand (transposed)
+  const int k_row = ((lane >> 4) << 3) + (lane & 7), k_chunk = (lane >> 3) & 1;
+  const int v_row = (((lane >> 3) & 1) << 3) + (lane & 7), v_chunk = lane >> 4;
+
+  int gbase = 0;  // granules of the CTA before this segment
+  for (int nseg = 0;; ++nseg) {
+    const int si = nseg & 1;
+    if (!wait(seg_full + si, (uint32_t)((nseg >> 1) & 1), 4)) return;
+    const Seg s = segs[si];
+    if (s.n < 0) break;
+    const uint32_t q32 = sm32 + Lay::kQ + si * Lay::kQBytes;
+    uint32_t qf[kKeepQ ? KS : 1][4];
+    // Q fragment of step ks: rows 0-7 in registers 0 and 2, rows 8-15 in 1 and 3 (zero if !WIDE)
+    auto load_q = [&](int ks, uint32_t (&f)[4]) {
+      if (WIDE) {
+        ldsm_x4(q32 + ((((lane >> 3) & 1) << 3) + (lane & 7)) * Lay::kQPitch + ks * 32 + (lane >> 4) * 16, f);
       } else {
-        kf[e] = inside ? (float)kr[e] : 0.f;
-        vf[e] = inside ? (float)vr[e] : 0.f;
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
+                     : "=r"(f[0]), "=r"(f[2])
+                     : "r"(q32 + (lane & 7) * Lay::kQPitch + ks * 32 + ((lane >> 3) & 1) * 16)
+                     : "memory");
+        f[1] = f[3] = 0;
+      }
+    };
+    if (kKeepQ) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) load_q(ks, qf[ks]);
+    }
+    float o[NT][4], m[kRowSets], l[kRowSets];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kRowSets; ++x) {
+      m[x] = -INFINITY;
+      l[x] = 0.f;
+    }
+    const bool fresh = a.kn && (!a.active || a.active[s.b]);
+
+    for (int i = (warp - gbase) & (kCons - 1); i < s.n; i += kCons) {
+      const int slot = (gbase + i) % Lay::kSlots;
+      const uint32_t par = (uint32_t)(((gbase + i) / Lay::kSlots) & 1);
+      const int pos = (s.g0 + i) * kGran;
+      const bool edge = pos < s.lo || pos + kGran > s.hi;
+      const bool owns_new = fresh && pos + kGran >= s.hi;  // the granule of key hi - 1
+      if (!wait(full + slot, par, 5)) return;
+      uint8_t* kt = sm + slot * Lay::kSlotBytes;
+      const uint32_t k32 = sm32 + slot * Lay::kSlotBytes, v32 = k32 + Lay::kSlotBytes / 2;
+      if (edge || owns_new) {
+        // values of masked keys count as zero (0 times what the page holds could be NaN)
+        if (edge)
+          for (int x = lane; x < kGran * (DH / 8); x += 32) {
+            const int r = x / (DH / 8), c = x % (DH / 8);
+            if (pos + r < s.lo || pos + r >= s.hi)
+              *reinterpret_cast<uint4*>(kt + Lay::kSlotBytes / 2 + tile_off(r, c)) = make_uint4(0, 0, 0, 0);
+          }
+        if (owns_new) {  // the new token's rows: into the tile, and into the page
+          const int r = s.hi - 1 - pos, last = s.hi - 1;
+          const int64_t page = a.table[s.b * a.table_stride + last / a.page_size];
+          const int off = last % a.page_size;
+          for (int x = lane; x < 2 * (DH / 8); x += 32) {
+            const bool isv = x >= DH / 8;
+            const int c = isv ? x - DH / 8 : x;
+            const uint4 u = isv ? ld_128(a.vn + 2 * (s.b * a.vn_b + s.h * a.vn_h) + 16 * c)
+                                : ld_128(a.kn + 2 * (s.b * a.kn_b + s.h * a.kn_h) + 16 * c);
+            *reinterpret_cast<uint4*>(kt + (isv ? Lay::kSlotBytes / 2 : 0) + tile_off(r, c)) = u;
+            if (s.r0 == 0 && page >= 0 && page < a.num_pages)
+              st_128((isv ? a.vp + 2 * (page * a.vp_p + s.h * a.vp_h + off * a.vp_t)
+                          : a.kp + 2 * (page * a.kp_p + s.h * a.kp_h + off * a.kp_t)) + 16 * c, u);
+          }
+        }
+        fence_proxy_async_smem();  // the slot's next copy comes through the async proxy
+        __syncwarp();
+      }
+
+      // scores of the 16 keys: two 8-key column tiles, even and odd steps in separate chains
+      float sc[2][2][4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[x][y][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t kf[4];
+        ldsm_x4(k32 + tile_off(k_row, 2 * ks + k_chunk), kf);
+        if (!kKeepQ) load_q(ks, qf[0]);
+        const uint32_t(&qq)[4] = qf[kKeepQ ? ks : 0];
+        mma_16816<T>(sc[ks & 1][0], qq, kf[0], kf[1]);
+        mma_16816<T>(sc[ks & 1][1], qq, kf[2], kf[3]);
+      }
+      // online softmax of rows gid (and gid + 8): this lane's keys are pos + 8 y + 2 tig + {0, 1}
+      uint32_t ph[4] = {0, 0, 0, 0}, pl[4] = {0, 0, 0, 0};  // P as A operand: high and low parts
+      float al[kRowSets];
+      bool moved = false;
+#pragma unroll
+      for (int x = 0; x < kRowSets; ++x) {
+        float v[4];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float t = (sc[0][y][2 * x + e] + sc[1][y][2 * x + e]) * a.scale_log2;
+            const int key = pos + 8 * y + 2 * tig + e;
+            if (edge && (key < s.lo || key >= s.hi)) t = -INFINITY;
+            v[2 * y + e] = t;
+          }
+        float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[x], mx), base = mn == -INFINITY ? 0.f : mn;
+        al[x] = ex2_approx(m[x] - base);
+        moved |= mn != m[x];
+        m[x] = mn;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ex2_approx(v[e] - base);
+        l[x] = l[x] * al[x] + ((v[0] + v[1]) + (v[2] + v[3]));
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t hi = ElemTraits<T>::pack2(v[2 * y], v[2 * y + 1]);
+          const float2 f = ElemTraits<T>::unpack2(hi);
+          const uint32_t lo = ElemTraits<T>::pack2(v[2 * y] - f.x, v[2 * y + 1] - f.y);
+          if (WIDE) {
+            ph[2 * y + x] = hi;
+            pl[2 * y + x] = lo;
+          } else {
+            ph[2 * y] = hi;
+            ph[2 * y + 1] = lo;
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          o[j][0] *= al[0];
+          o[j][1] *= al[0];
+          o[j][2] *= al[kRowSets - 1];
+          o[j][3] *= al[kRowSets - 1];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NT; j += 2) {
+        uint32_t vf[4];
+        ldsm_x4_trans(v32 + tile_off(v_row, j + v_chunk), vf);
+        mma_16816<T>(o[j], ph, vf[0], vf[1]);
+        mma_16816<T>(o[j + 1], ph, vf[2], vf[3]);
+        if (WIDE) {
+          mma_16816<T>(o[j], pl, vf[0], vf[1]);
+          mma_16816<T>(o[j + 1], pl, vf[2], vf[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + slot);
+    }
+    gbase += s.n;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(seg_empty + si);  // the descriptor and Q have been read
+
+    // join the warps: maxima and sums first, then the outputs rescaled to the common maximum
+    float2* ml = reinterpret_cast<float2*>(sm + Lay::kMl) + (nseg & 1) * kCons * kRows;
+#pragma unroll
+    for (int x = 0; x < kRowSets; ++x) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+      if (tig == 0) ml[warp * kRows + gid + 8 * x] = make_float2(m[x], l[x]);
+    }
+    if (!cons_sync()) return;
+    auto joined = [&](int r) {  // (max, sum) of row r over the warps
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kCons; ++w) M = fmaxf(M, ml[w * kRows + r].x);
+      const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int w = 0; w < kCons; ++w) L += ml[w * kRows + r].y * ex2_approx(ml[w * kRows + r].x - base);
+      return make_float2(M, L);
+    };
+    if (!WIDE) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {  // high and low parts
+        o[j][0] += o[j][2];
+        o[j][1] += o[j][3];
       }
     }
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      float s = 0.f;
+    for (int x = 0; x < kRowSets; ++x) {
+      const int r = gid + 8 * x;
+      if (r < s.rows) {
+        const float M = joined(r).x;
+        const float f = ex2_approx(m[x] - (M == -INFINITY ? 0.f : M));
 #pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf(q[r][e], kf[e], s);
-      s = warp_sum(s) * a.scale_log2;
-      const float mn = fmaxf(m[r], s), base = mn == -INFINITY ? 0.f : mn;
-      const float alpha = ex2_approx(m[r] - base), p = ex2_approx(s - base);
-      m[r] = mn;
-      l[r] = l[r] * alpha + p;
+        for (int j = 0; j < NT; ++j) {
+          o[j][2 * x] *= f;
+          o[j][2 * x + 1] *= f;
+        }
+      }
+    }
+    // columns joined at a time: what the buffer holds of s.rows rows (rows padded by 8 floats
+    // to spread the stores over the banks)
+    const int cw = s.rows <= 4 ? (DH < 128 ? DH : 128) : s.rows <= 8 ? 64 : 32;
+    const int pitch = cw + 8;
+    float* part_o = reinterpret_cast<float*>(a.ws + kWsO) + (int64_t)s.slot * kRows * DH;
+    for (int c0 = 0; c0 < DH; c0 += cw) {
+      if (c0 > 0 && !cons_sync()) return;  // the buffer has been read
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[r][e] = fmaf(o[r][e], alpha, p * vf[e]);
+      for (int x = 0; x < kRowSets; ++x)
+        if (gid + 8 * x < s.rows) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const int c = 8 * j + 2 * tig - c0;
+            if (c >= 0 && c < cw)
+              *reinterpret_cast<float2*>(buf + (warp * s.rows + gid + 8 * x) * pitch + c) = make_float2(o[j][2 * x], o[j][2 * x + 1]);
+          }
+        }
+      if (!cons_sync()) return;
+      const int quads = cw / 4;
+      for (int it = tid; it < s.rows * quads; it += 32 * kCons) {
+        const int r = it / quads, c = (it - r * quads) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kCons; ++w) {
+          const float4 u = *reinterpret_cast<const float4*>(buf + (w * s.rows + r) * pitch + c);
+          v.x += u.x;
+          v.y += u.y;
+          v.z += u.z;
+          v.w += u.w;
+        }
+        const float2 t = joined(r);
+        if (s.slot < 0) {
+          const int hq = s.h * a.G + s.r0 + r;
+          store4<T>(a.out + 2 * (s.b * a.o_b + hq * a.o_h + c0 + c), v, t.y == 0.f ? 0.f : 1.f / t.y);
+          if (a.lse && c0 + c == 0) a.lse[s.b * a.ls_b + hq * a.ls_h] = lse_of(t.x, t.y);
+        } else {
+          *reinterpret_cast<float4*>(part_o + r * DH + c0 + c) = v;
+          if (c0 + c == 0) reinterpret_cast<float2*>(a.ws + kWsMl)[s.slot * kRows + r] = t;
+        }
+      }
+    }
+    if (s.slot < 0) continue;
+
+    // a cut pair: the CTA whose part arrives last joins the parts
+    __threadfence();
+    if (!cons_sync()) return;
+    if (tid == 0) {
+      int* counter = reinterpret_cast<int*>(a.ws) + s.first_cta;
+      const int arrived = atomicAdd(counter, 1) + 1;
+      if (arrived == s.parts) *counter = 0;  // as the next call finds it
+      *last_flag = arrived == s.parts;
+    }
+    if (!cons_sync()) return;
+    if (!*last_flag) continue;
+    __threadfence();
+    auto slot_of = [&](int p) { return 2 * (s.first_cta + p) + (p == 0 ? 1 : 0); };
+    float* wt = buf;                               // [parts][rows] weights
+    float* red = buf + kMaxCtas * kRows;           // [groups][items] partial sums
+    const float2* gml = reinterpret_cast<const float2*>(a.ws + kWsMl);
+    const float* go = reinterpret_cast<const float*>(a.ws + kWsO);
+    for (int r = warp; r < s.rows; r += kCons) {
+      float M = -INFINITY, L = 0.f;
+      for (int p = lane; p < s.parts; p += 32) M = fmaxf(M, __ldcg(gml + slot_of(p) * kRows + r).x);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+      const float base = M == -INFINITY ? 0.f : M;
+      for (int p = lane; p < s.parts; p += 32) {
+        const float2 t = __ldcg(gml + slot_of(p) * kRows + r);
+        const float f = ex2_approx(t.x - base);
+        wt[p * s.rows + r] = f;
+        L += t.y * f;
+      }
+      L = warp_sum(L);
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      __syncwarp();
+      for (int p = lane; p < s.parts; p += 32) wt[p * s.rows + r] *= inv;
+      if (lane == 0 && a.lse) a.lse[s.b * a.ls_b + (int64_t)(s.h * a.G + s.r0 + r) * a.ls_h] = lse_of(M, L);
+    }
+    if (!cons_sync()) return;
+    const int items = s.rows * (DH / 4);
+    const int groups = items >= 32 * kCons ? 1 : 32 * kCons / items;  // threads that share an item's parts
+    for (int base = 0; base < items; base += 32 * kCons) {
+      const int grp = groups == 1 ? 0 : tid / items, it = groups == 1 ? base + tid : tid % items;
+      const int r = it / (DH / 4), c = (it % (DH / 4)) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (it < items && grp < groups) {
+#pragma unroll 8
+        for (int p = grp; p < s.parts; p += groups) {
+          const float4 u = __ldcg(reinterpret_cast<const float4*>(go + ((int64_t)slot_of(p) * kRows + r) * DH + c));
+          const float f = wt[p * s.rows + r];
+          v.x = fmaf(u.x, f, v.x);
+          v.y = fmaf(u.y, f, v.y);
+          v.z = fmaf(u.z, f, v.z);
+          v.w = fmaf(u.w, f, v.w);
+        }
+        if (groups > 1) *reinterpret_cast<float4*>(red + (grp * items + it) * 4) = v;
+      }
+      if (groups > 1) {
+        if (!cons_sync()) return;
+        if (grp == 0)
+          for (int g = 1; g < groups; ++g) {
+            const float4 u = *reinterpret_cast<const float4*>(red + (g * items + it) * 4);
+            v.x += u.x;
+            v.y += u.y;
+            v.z += u.z;
+            v.w += u.w;
+          }
+      }
+      if (it < items && grp == 0)
+        store4<T>(a.out + 2 * (s.b * a.o_b + (int64_t)(s.h * a.G + s.r0 + r) * a.o_h + c), v, 1.f);
     }
   }
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    if (lane == 0) {
-      sm_m[warp][r] = m[r];
-      sm_l[warp][r] = l[r];
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) sm_o[warp][r][lane * E + e] = o[r][e];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * DH; i += blockDim.x) {
-    const int r = i / DH, d = i - r * DH;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][r]);
-    const float base = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2_approx(sm_m[w][r] - base);
-      L += sm_l[w][r] * f;
-      O += sm_o[w][r][d] * f;
-    }
-    const int hq = h * a.G + r0 + r;
-    const uint32_t u = ElemTraits<T>::pack2(L == 0.f ? 0.f : O / L, 0.f);
-    *reinterpret_cast<uint16_t*>(a.out + 2 * (b * a.o_b + hq * a.o_h + d)) = (uint16_t)u;
-    if (a.lse && d == 0) a.lse[b * a.ls_b + hq * a.ls_h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-  }
+}
+
+using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    cudaDriverEntryPointQueryResult qr;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) != cudaSuccess ||
+        qr != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// A pool [pages, Hkv, page_size, dh] as (64 columns, token, 64-column box, head, page), so that one
+// copy brings 16 tokens of one head and page, all columns, in boxes of 16 rows x 128 bytes.
+int encode_pool(CUtensorMap* m, const bna_tensor4* t, int dtype, const char* name) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return fail(BNA_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t boxes = (cuuint64_t)t->size[3] / 64;
+  const cuuint64_t dims[5] = {64, (cuuint64_t)t->size[2], boxes, (cuuint64_t)t->size[1], (cuuint64_t)t->size[0]};
+  // a dim of size 1 is never stepped over: any valid stride will do
+  auto st = [&](int d) { return t->size[d] > 1 ? (cuuint64_t)t->stride[d] * 2 : (cuuint64_t)t->size[3] * 2; };
+  const cuuint64_t strides[4] = {st(2), 128, st(1), st(0)};
+  const cuuint32_t box[5] = {64, kGran, (cuuint32_t)boxes, 1, 1};
+  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(m, dtype == BNA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, t->data,
+                         dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(BNA_BAD_STRIDE, std::string(name) + ": cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return BNA_OK;
+}
+
+int sm_count() {
+  static std::mutex mu;
+  static std::map<int, int> cache;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> g(mu);
+  auto it = cache.find(dev);
+  if (it != cache.end()) return it->second;
+  int n = 0;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return cache[dev] = n;
+}
+
+template <typename T, int DH, bool WIDE>
+int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, unsigned grid, cudaStream_t s) {
+  auto kern = paged_decode_kernel<T, DH, WIDE>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DH>::kAlloc);
+  if (e != cudaSuccess) return check_cuda(e, "paged_decode attributes");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(Layout<DH>::kThreads);
+  cfg.dynamicSmemBytes = Layout<DH>::kAlloc;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, mk, mv, a), "paged_decode launch");
 }
 
 }  // namespace
 
+int64_t paged_decode_workspace_bytes() { return kWsBytes; }
+
 int launch_paged_decode(const bna_tensor4* q, bna_tensor4* kp, bna_tensor4* vp, const bna_tensor4* kn,
-                        const bna_tensor4* vn, const uint8_t* active, bna_tensor4* out, float* lse, int64_t ls_b, int64_t ls_h, int dtype,
-                        const int32_t* table, int64_t table_stride, int width, const int32_t* lens, int window,
-                        float scale, cudaStream_t s) {
+                        const bna_tensor4* vn, const uint8_t* active, bna_tensor4* out, float* lse, int64_t ls_b,
+                        int64_t ls_h, int dtype, const int32_t* table, int64_t table_stride, int width,
+                        const int32_t* lens, int window, float scale, void* ws, cudaStream_t s) {
+  CUtensorMap mk, mv;
+  if (int rc = encode_pool(&mk, kp, dtype, "k_pages")) return rc;
+  if (int rc = encode_pool(&mv, vp, dtype, "v_pages")) return rc;
   PagedArgs a{};
   a.q = static_cast<const uint8_t*>(q->data);
   a.q_b = q->stride[0], a.q_h = q->stride[1];
@@ -148,18 +738,31 @@ int launch_paged_decode(const bna_tensor4* q, bna_tensor4* kp, bna_tensor4* vp, 
   a.table = table, a.table_stride = table_stride, a.lens = lens;
   a.B = (int)q->size[0], a.Hkv = (int)kp->size[1], a.G = (int)(q->size[1] / kp->size[1]);
   a.width = width, a.num_pages = (int)kp->size[0], a.page_size = (int)kp->size[2], a.window = window;
+  a.chunks = (a.G + kRows - 1) / kRows;
+  a.chunk_rows = (a.G + a.chunks - 1) / a.chunks;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const int kRows = rows_of((int)q->size[3]);
-  const dim3 grid((unsigned)a.B, (unsigned)a.Hkv, (unsigned)((a.G + kRows - 1) / kRows));
-  auto launch = [&](auto kern) { kern<<<grid, kWarps * 32, 0, s>>>(a); };
-  const bool bf = dtype == BNA_BF16;
+  a.ws = static_cast<uint8_t*>(ws);
+  a.err = device_error_word();
+  // no more CTAs than the longest possible requests could occupy
+  const int64_t keys = window > 0 ? std::min((int64_t)width * a.page_size, (int64_t)window + 2 * kGran) : (int64_t)width * a.page_size;
+  const double most = (double)a.B * a.Hkv * a.chunks * (double)((keys + kGran - 1) / kGran);
+  const unsigned grid = (unsigned)std::max(1.0, std::min((double)std::min(sm_count(), kMaxCtas), std::ceil(most / kMinPart)));
+  const bool bf = dtype == BNA_BF16, wide = a.chunk_rows > 8;
+#define BNA_PAGED(T_, DH_) \
+  return wide ? launch_decode<T_, DH_, true>(mk, mv, a, grid, s) : launch_decode<T_, DH_, false>(mk, mv, a, grid, s)
   switch (q->size[3]) {
-    case 64: bf ? launch(paged_decode_kernel<__nv_bfloat16, 64>) : launch(paged_decode_kernel<__half, 64>); break;
-    case 128: bf ? launch(paged_decode_kernel<__nv_bfloat16, 128>) : launch(paged_decode_kernel<__half, 128>); break;
-    case 256: bf ? launch(paged_decode_kernel<__nv_bfloat16, 256>) : launch(paged_decode_kernel<__half, 256>); break;
+    case 64:
+      if (bf) BNA_PAGED(__nv_bfloat16, 64);
+      BNA_PAGED(__half, 64);
+    case 128:
+      if (bf) BNA_PAGED(__nv_bfloat16, 128);
+      BNA_PAGED(__half, 128);
+    case 256:
+      if (bf) BNA_PAGED(__nv_bfloat16, 256);
+      BNA_PAGED(__half, 256);
     default: return fail(BNA_UNSUPPORTED, "paged_decode_attention: head_dim must be 64, 128 or 256");
   }
-  return check_cuda(cudaGetLastError(), "paged_decode launch");
+#undef BNA_PAGED
 }
 
 }  // namespace bna

@@ -98,10 +98,32 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                                            slot_map.data_ptr(), _lib.dtype_code(k.dtype), _lib.stream_ptr(k.device)))
 
 
+_workspaces: dict = {}
+
+
+def decode_workspace(device: torch.device | str = "cuda") -> torch.Tensor:
+    """A workspace for ``paged_decode_attention`` calls that follow one another on a stream."""
+    ws = torch.empty(_lib.lib().bna_paged_decode_workspace_bytes(), dtype=torch.uint8, device=device)
+    ws[:4096].zero_()  # the arrival counters; every call leaves them zero
+    return ws
+
+
+def _workspace_for(device: torch.device, stream: int) -> torch.Tensor:
+    """The workspace kept for a stream.  A capture gets its own (zeroed inside the graph): its
+    replays may run beside later calls on the stream."""
+    if torch.cuda.is_current_stream_capturing():
+        return decode_workspace(device)
+    ws = _workspaces.get((device.index, stream))
+    if ws is None:
+        ws = _workspaces[(device.index, stream)] = decode_workspace(device)
+    return ws
+
+
 def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                            lens: torch.Tensor, *, k_new: Optional[torch.Tensor] = None,
                            v_new: Optional[torch.Tensor] = None, active: Optional[torch.Tensor] = None,
-                           window: int = 0, scale: Optional[float] = None, return_lse: bool = False):
+                           window: int = 0, scale: Optional[float] = None, return_lse: bool = False,
+                           workspace: Optional[torch.Tensor] = None):
     """Attention of one new token per request: q [B,Hq,1,dh] over the first ``lens[b]`` tokens of
     request b (the last ``window`` of them where ``window`` > 0).  ``lens`` counts the new token.
 
@@ -110,7 +132,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     ``active`` [B] bool names (default: all; pass ``PagedReservation.granted`` where some
     requests got no room, or rest).  Returns [B,Hq,1,dh]
     (storage [B,1,Hq,dh]) in q's dtype; with ``return_lse`` also the fp32 natural-log sums
-    [B,Hq,1].  A request of length 0 gives zeros and -inf."""
+    [B,Hq,1].  A request of length 0 gives zeros and -inf.  ``workspace`` (``decode_workspace``)
+    defaults to one kept per stream; calls that may overlap need one each."""
     _lib.require_cuda(q, k_pages, v_pages, block_table, lens)
     if q.dim() != 4:
         raise ValueError("q must be [B, Hq, 1, dh]")
@@ -136,11 +159,15 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     out = torch.empty((B, Tq, Hq, dh), device=q.device, dtype=q.dtype).transpose(1, 2)
     lse = torch.empty((B, Hq, Tq), device=q.device, dtype=torch.float32) if return_lse else None
     tq, tkp, tvp, to = (_lib.t4(x) for x in (q, k_pages, v_pages, out))
+    stream = _lib.stream_ptr(q.device)
+    ws = workspace if workspace is not None else _workspace_for(q.device, stream)
+    if ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.device != q.device:
+        raise ValueError("workspace must be a contiguous uint8 tensor on q's device (decode_workspace)")
     _lib.check(_lib.lib().bna_paged_decode(
         ctypes.byref(tq), ctypes.byref(tkp), ctypes.byref(tvp), nk, nv, act, ctypes.byref(to),
         lse.data_ptr() if return_lse else None, Hq, 1, _lib.dtype_code(q.dtype), block_table.data_ptr(),
         block_table.stride(0), block_table.shape[1], lens.data_ptr(), int(window),
-        float(scale) if scale is not None else 1.0 / math.sqrt(dh), _lib.stream_ptr(q.device)))
+        float(scale) if scale is not None else 1.0 / math.sqrt(dh), ws.data_ptr(), ws.numel(), stream))
     return (out, lse) if return_lse else out
 
 
@@ -208,4 +235,4 @@ class PagedKVCache:
                                       return_lse=return_lse)
 
 
-__all__ = ["PagedKVCache", "PagedReservation", "RELEASE", "paged_append", "paged_decode_attention", "paged_reserve"]
+__all__ = ["PagedKVCache", "PagedReservation", "RELEASE", "decode_workspace", "paged_append", "paged_decode_attention", "paged_reserve"]

@@ -391,12 +391,17 @@ BNA_API int bna_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_ten
  * k_new / v_new [B, Hkv, 1, dh] the row at position lens[b] - 1 is taken from them and written
  * into its page, for the requests with active[b] != 0 (null: all; the others attend to what
  * their pages hold).  A length is cut to table_width * page_size; a page number outside the pool reads
- * as zeros. */
+ * as zeros.
+ * workspace: bna_paged_decode_workspace_bytes() of device memory, 16-byte aligned, whose first
+ * 4096 bytes were zeroed once; every call leaves them zero again (after BNA_DEVICE_TIMEOUT zero
+ * them anew).  Calls that may overlap on the GPU need a workspace each. */
+BNA_API int64_t bna_paged_decode_workspace_bytes(void);
 BNA_API int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_tensor4* v_pages,
                              const bna_tensor4* k_new, const bna_tensor4* v_new, const uint8_t* active,
                              bna_tensor4* out, float* lse, int64_t lse_stride_b, int64_t lse_stride_h, int32_t dtype,
                              const int32_t* block_table, int64_t table_stride, int32_t table_width,
-                             const int32_t* lens, int32_t window, float scale, void* stream);
+                             const int32_t* lens, int32_t window, float scale, void* workspace,
+                             int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

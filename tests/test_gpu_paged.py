@@ -144,6 +144,16 @@ def test_long_requests_are_split_and_joined():
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("Hq,Hkv,dh,page,step", [(4, 4, 256, 16, True), (8, 2, 128, 16, False), (12, 6, 64, 48, True)])
+def test_many_requests_cut_between_ctas(Hq, Hkv, dh, page, step):
+    # adjacent requests that each cross a boundary between CTAs, in different orders
+    for seed in range(4):
+        lens = np.random.default_rng(seed).permutation(np.geomspace(301, 8191, 24).astype(int)).tolist()
+        c = Case(lens, Hq, Hkv, dh, page, seed=seed, step=step)
+        for _ in range(2):
+            c.check(*c.run())
+
+
 def test_many_short_requests():
     rng = np.random.default_rng(5)
     lens = rng.integers(0, 90, 1500).tolist()

@@ -73,12 +73,12 @@ def test_append_refusals():
 
 
 def _decode(q=(3, 8, 1, 128), kp=(9, 2, 16, 128), vp=None, kn=None, vn=None, active=None, out=None, dt=BF, table=P, ts=6,
-            width=6, lens=P, window=0, scale=0.1, qd=P):
+            width=6, lens=P, window=0, scale=0.1, qd=P, ws=P, wsb=1 << 40):
     t = [_t(q, data=qd), _t(kp), _t(vp or kp)]
     new = [ctypes.byref(_t(x)) if x else None for x in (kn, vn)]
     o = _t(out or q)
     return _lib.lib().bna_paged_decode(*(ctypes.byref(x) for x in t), *new, active, ctypes.byref(o), None, 0, 0, dt, table, ts,
-                                       width, lens, window, scale, None)
+                                       width, lens, window, scale, ws, wsb, None)
 
 
 def test_decode_refusals():
@@ -100,6 +100,7 @@ def test_decode_refusals():
     assert _decode(width=0) == BAD_SHAPE
     assert _decode(width=1 << 28) == UNSUPPORTED
     assert _decode(window=-1) == BAD_SHAPE
+    assert _decode(ws=None) == _lib.CAPACITY and _decode(wsb=4096) == _lib.CAPACITY and _decode(ws=P + 8) == BAD_STRIDE
     assert _decode(scale=0.0) == BAD_SHAPE and _decode(scale=float("nan")) == BAD_SHAPE
 
 
@@ -135,7 +136,7 @@ def test_wrappers_check_types_and_shapes():
     kn = torch.zeros(2, 2, 1, 128, dtype=torch.bfloat16, device=dev)
     for bad in (dict(q=q.half()), dict(q=q[0]), dict(lens=i[:1]), dict(block_table=table.long()), dict(k_new=kn),
                 dict(k_new=kn.half(), v_new=kn.half()), dict(k_new=kn, v_new=kn, active=i), dict(window=-2), dict(scale=-1.0),
-                dict(active=torch.ones(2, dtype=torch.bool, device=dev))):
+                dict(active=torch.ones(2, dtype=torch.bool, device=dev)), dict(workspace=torch.zeros(8, device=dev))):
         a = dict(q=q, k_pages=pool, v_pages=pool.clone(), block_table=table, lens=i)
         a.update(bad)
         with pytest.raises(ValueError):
