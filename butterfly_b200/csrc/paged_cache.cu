@@ -4,6 +4,7 @@
 // its block-table row names, page_size to a page; slot = page * page_size + offset.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <string>
 
@@ -14,6 +15,7 @@ namespace {
 
 constexpr int kMaxRequests = 4096;  // three prefix sums and the lengths of a call: 64 KB of shared memory
 constexpr int kReserveThreads = 256;
+constexpr int kReserveCtas = 148;
 
 struct ReserveArgs {
   const int32_t* lens;
@@ -42,106 +44,140 @@ __device__ __forceinline__ int upper_bound(const int32_t* c, int n, int64_t x) {
   return lo;
 }
 
-__device__ __forceinline__ int pages_of(int64_t tokens, int page_size) {
-  return (int)((tokens + page_size - 1) / page_size);
+__device__ __forceinline__ int pages_of(unsigned tokens, unsigned page_size) {
+  return (int)((tokens + page_size - 1) / page_size);  // tokens <= INT_MAX, page_size <= INT_MAX
 }
 
 // What a request asks for: its length after the call, and pages taken (need) or given back.
 struct Ask {
-  int len, add, old_pages, new_pages, need, back;
-  int64_t want;
+  int want, old_pages, new_pages, need, back;
   bool fits;
 };
-__device__ __forceinline__ Ask ask_of(const ReserveArgs& a, int b) {
+__device__ __forceinline__ Ask ask_of(int len, int add, int capacity, int page_size) {
   Ask r;
-  // a length outside the table is cut to it, so that no later index leaves the row
-  r.len = min(max(a.lens[b], 0), (int)min((int64_t)a.width * a.page_size, (int64_t)INT_MAX));
-  r.add = a.add[b];
-  r.want = max((int64_t)0, (int64_t)r.len + r.add);
-  r.old_pages = pages_of(r.len, a.page_size);
-  r.fits = r.want <= (int64_t)a.width * a.page_size && r.want <= INT_MAX;
-  r.new_pages = r.fits ? pages_of(r.want, a.page_size) : r.old_pages;
-  r.need = r.add > 0 && r.fits ? r.new_pages - r.old_pages : 0;
-  r.back = r.add < 0 ? r.old_pages - r.new_pages : 0;
+  const int64_t want = (int64_t)len + add;
+  r.fits = want <= capacity;
+  r.want = (int)min(max(want, (int64_t)0), (int64_t)capacity);
+  r.old_pages = pages_of(len, page_size);
+  r.new_pages = r.fits ? pages_of(r.want, page_size) : r.old_pages;
+  r.need = add > 0 ? r.new_pages - r.old_pages : 0;
+  r.back = add < 0 ? r.old_pages - r.new_pages : 0;
   return r;
 }
 
-// One CTA.  Prefix sums over the requests of the tokens added, the pages needed and the pages
-// given back (shared memory), from which every table entry, slot and stack entry follows by a
-// binary search; the j-th page given back lies j below the new top of the free stack and the
-// i-th page taken comes from i below it, so a call followed by its opposite restores the stack.
+// Every CTA computes the prefix sums over the requests of the tokens added, the pages needed
+// and the pages given back (shared memory; at most 4096 requests, read through L2), from which any
+// table entry, slot and stack entry follows by a binary search, and the grid shares these
+// out: no CTA waits for another.  Nothing that is read is written in the call: lengths and stack
+// height go to other places, table entries written lie past those read, and stack entries
+// are written only where pages stay given back (then none is taken from below them).
+// The j-th page given back lies j below the new top of the stack and the i-th page taken
+// comes from i below it, so a call followed by its opposite restores the stack.
+// Bound by launch and dependent-read latency: the largest calls move about 1 MB.
 __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveArgs a) {
   extern __shared__ int32_t sm[];
-  int32_t* cum_add = sm;                 // inclusive prefix sums
+  int32_t* cum_add = sm;            // inclusive prefix sums (capped at INT_MAX)
   int32_t* cum_need = sm + a.B;
   int32_t* cum_back = sm + 2 * a.B;
-  if (threadIdx.x == 0) {
-    int64_t ca = 0, cn = 0, cb = 0;
-    for (int b = 0; b < a.B; ++b) {
-      const Ask r = ask_of(a, b);
-      ca += max(r.add, 0);
-      cn += r.need;
-      cb += r.back;
-      cum_add[b] = (int32_t)min(ca, (int64_t)INT_MAX);
-      cum_need[b] = (int32_t)min(cn, (int64_t)INT_MAX);
-      cum_back[b] = (int32_t)min(cb, (int64_t)INT_MAX);
+  int32_t* lens = sm + 3 * a.B;     // cut to the table, so that no later index leaves a row
+  __shared__ int64_t warp_sums[3][kReserveThreads / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int capacity = (int)min((int64_t)a.width * a.page_size, (int64_t)INT_MAX);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = min(max(a.num_free[0], 0), a.num_pages);
+
+  // each thread sums a run of requests, then the runs are scanned
+  const int per = (a.B + kReserveThreads - 1) / kReserveThreads;
+  const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
+  int64_t sum[3] = {0, 0, 0};
+  for (int b = b0; b < b1; ++b) {
+    const int len = min(max(a.lens[b], 0), capacity), add = a.add[b];
+    const Ask r = ask_of(len, add, capacity, a.page_size);
+    lens[b] = len;
+    sum[0] += max(add, 0);
+    sum[1] += r.need;
+    sum[2] += r.back;
+  }
+  int64_t at[3];
+#pragma unroll
+  for (int x = 0; x < 3; ++x) {
+    int64_t v = sum[x];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
     }
+    if (lane == 31) warp_sums[x][warp] = v;
+    at[x] = v - sum[x];
   }
   __syncthreads();
-  const int n = min(max(a.num_free[0], 0), a.num_pages);
+#pragma unroll
+  for (int x = 0; x < 3; ++x)
+    for (int w = 0; w < warp; ++w) at[x] += warp_sums[x][w];
+  for (int b = b0; b < b1; ++b) {
+    const int add = a.add[b];
+    const Ask r = ask_of(lens[b], add, capacity, a.page_size);
+    at[0] += max(add, 0);
+    at[1] += r.need;
+    at[2] += r.back;
+    cum_add[b] = (int32_t)min(at[0], (int64_t)INT_MAX);
+    cum_need[b] = (int32_t)min(at[1], (int64_t)INT_MAX);
+    cum_back[b] = (int32_t)min(at[2], (int64_t)INT_MAX);
+  }
+  __syncthreads();
+
   const int R = cum_back[a.B - 1];
   const int64_t top = (int64_t)n + R;
   // requests are served in order while their pages last: pages taken = the largest prefix <= top
-  const int served = upper_bound(cum_need, a.B, top);
+  const int served = cum_need[a.B - 1] <= top ? a.B : upper_bound(cum_need, a.B, top);
   const int A = served > 0 ? cum_need[served - 1] : 0;
-
+  auto before = [](const int32_t* c, int b) { return b > 0 ? c[b - 1] : 0; };
   // Page x below the top of the stack with the pages given back on it.
   auto from_top = [&](int64_t x) -> int {
     if (x < R) {
       const int b = upper_bound(cum_back, a.B, x);
-      const Ask r = ask_of(a, b);
-      return a.table[b * a.table_stride + r.new_pages + (x - (cum_back[b] - r.back))];
+      const int first = pages_of(lens[b], a.page_size) - (cum_back[b] - before(cum_back, b));
+      return a.table[b * a.table_stride + first + (x - before(cum_back, b))];
     }
     const int64_t i = top - 1 - x;
     return i >= 0 && i < n ? a.free_pages[i] : -1;
   };
-  auto granted = [&](const Ask& r, int b) { return r.add > 0 && r.fits && (r.need == 0 || cum_need[b] <= top); };
+  // Tokens were added to b and have slots: it fits, and needs no page or was served.
+  auto granted = [&](int b) {
+    const int tokens = cum_add[b] - before(cum_add, b);
+    return tokens > 0 && (int64_t)lens[b] + tokens <= capacity && (b < served || cum_need[b] == before(cum_need, b));
+  };
+  const int64_t stride = (int64_t)gridDim.x * kReserveThreads, tid = (int64_t)blockIdx.x * kReserveThreads + threadIdx.x;
 
-  for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
-    const Ask r = ask_of(a, b);
-    const bool ok = granted(r, b);
-    a.lens_out[b] = ok || r.add <= 0 ? (int)r.want : r.len;
-    a.granted[b] = ok;
-  }
-  if (threadIdx.x == 0) a.num_free_out[0] = (int)min(top - A, (int64_t)a.num_pages);
-  // table entries of the pages taken
-  for (int i = threadIdx.x; i < A; i += blockDim.x) {
-    const int b = upper_bound(cum_need, a.B, i);
-    const Ask r = ask_of(a, b);
-    a.table[b * a.table_stride + r.old_pages + (i - (cum_need[b] - r.need))] = from_top(i);
-  }
-  // stack entries of the pages given back and not taken again (from index n up; a page taken
-  // comes from below n only when every page given back was taken, so no entry is read here
-  // that is written here)
-  for (int64_t i = n + threadIdx.x; i < top - A && i < a.num_pages; i += blockDim.x) a.free_pages[i] = from_top(top - 1 - i);
   // slots and positions of the added tokens, packed request by request
-  for (int64_t t = threadIdx.x; t < a.num_tokens; t += blockDim.x) {
+  for (int64_t t = tid; t < a.num_tokens; t += stride) {
     int64_t slot = -1;
     int pos = -1;
     const int b = upper_bound(cum_add, a.B, t);
-    if (b < a.B) {
-      const Ask r = ask_of(a, b);
-      if (granted(r, b)) {
-        pos = (int)(r.len + (t - (cum_add[b] - r.add)));
-        const int pi = pos / a.page_size;
-        const int page = pi < r.old_pages ? a.table[b * a.table_stride + pi]
-                                          : from_top(cum_need[b] - r.need + pi - r.old_pages);
-        slot = page < 0 ? -1 : (int64_t)page * a.page_size + pos % a.page_size;
-      }
+    if (b < a.B && granted(b)) {
+      pos = lens[b] + (int)(t - before(cum_add, b));
+      const int pi = (unsigned)pos / (unsigned)a.page_size, have = pages_of(lens[b], a.page_size);
+      const int page = pi < have ? a.table[b * a.table_stride + pi] : from_top((int64_t)before(cum_need, b) + pi - have);
+      slot = page < 0 ? -1 : (int64_t)page * a.page_size + (pos - pi * a.page_size);
     }
     a.slots[t] = slot;
     a.positions[t] = pos;
   }
+  for (int64_t b = tid; b < a.B; b += stride) {
+    const bool ok = granted((int)b);
+    const int add = a.add[b];
+    a.lens_out[b] = add > 0 && !ok ? lens[b] : max(0, (int)((int64_t)lens[b] + add));
+    a.granted[b] = ok;
+  }
+  if (tid == 0) a.num_free_out[0] = (int)min(top - A, (int64_t)a.num_pages);
+  // table entries of the pages taken
+  for (int64_t i = tid; i < A; i += stride) {
+    const int b = upper_bound(cum_need, a.B, i);
+    a.table[b * a.table_stride + pages_of(lens[b], a.page_size) + (i - before(cum_need, b))] = from_top(i);
+  }
+  // stack entries of the pages given back and not taken again, from index n up
+  for (int64_t i = n + tid; i < top - A && i < a.num_pages; i += stride) a.free_pages[i] = from_top(top - 1 - i);
 }
 
 // ------------------------------------------------------------------------------ append
@@ -153,22 +189,59 @@ struct PagedAppendArgs {
   const int64_t* slots;
   int64_t rows;  // tokens * heads
   int64_t num_slots;
-  int heads, page_size, vecs;  // 16-byte vectors per row
+  int heads, page_size, vec_shift;  // 2^vec_shift 16-byte vectors per row
 };
 
-// One thread per 16-byte vector of a (token, head) row, of the keys and of the values.
+// A thread moves one 16-byte vector of the keys and of the values of N (token, head) rows that lie a
+// block apart, with all 2 N loads in flight before the first store (they do not wait for the
+// slots).  Bound by HBM: each row is read and written once.
+template <int N>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppendArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t row = i / a.vecs;
-  const int c = (int)(i - row * a.vecs);
-  if (row >= a.rows) return;
-  const int64_t t = row / a.heads;
-  const int h = (int)(row - t * a.heads);
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >= a.num_slots) return;
-  const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
-  st_128(a.kp + 2 * (page * a.kp_p + h * a.kp_h + off * a.kp_t) + 16 * c, ld_128(a.k + 2 * (t * a.k_t + h * a.k_h) + 16 * c));
-  st_128(a.vp + 2 * (page * a.vp_p + h * a.vp_h + off * a.vp_t) + 16 * c, ld_128(a.v + 2 * (t * a.v_t + h * a.v_h) + 16 * c));
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int c = threadIdx.x & ((1 << a.vec_shift) - 1);
+  const int step = 256 >> a.vec_shift;  // rows of a block side by side
+  const int64_t row0 = (int64_t)blockIdx.x * (N * step) + (threadIdx.x >> a.vec_shift);
+  uint4 k[N], v[N];
+  int64_t slot[N];
+  int head[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t row = row0 + i * step;
+    slot[i] = -1;
+    if (row < a.rows) {
+      const int64_t t = a.rows <= UINT_MAX ? (int64_t)((unsigned)row / (unsigned)a.heads) : row / a.heads;
+      head[i] = (int)(row - t * a.heads);
+      slot[i] = a.slots[t];
+      k[i] = ld_nc_128(a.k + 2 * (t * a.k_t + head[i] * a.k_h) + 16 * c);
+      v[i] = ld_nc_128(a.v + 2 * (t * a.v_t + head[i] * a.v_h) + 16 * c);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (slot[i] < 0 || slot[i] >= a.num_slots) continue;
+    const int64_t page = a.num_slots <= UINT_MAX ? (int64_t)((unsigned)slot[i] / (unsigned)a.page_size) : slot[i] / a.page_size;
+    const int64_t off = slot[i] - page * a.page_size;
+    st_128(a.kp + 2 * (page * a.kp_p + head[i] * a.kp_h + off * a.kp_t) + 16 * c, k[i]);
+    st_128(a.vp + 2 * (page * a.vp_p + head[i] * a.vp_h + off * a.vp_t) + 16 * c, v[i]);
+  }
+}
+
+// Launch that may be set up while the stream's previous kernel runs (the kernel waits for it).
+template <typename Args>
+int launch_dependent(void (*kern)(Args), const std::remove_const_t<Args>& a, unsigned grid, unsigned block, int smem, cudaStream_t s,
+                     const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a), what);
 }
 
 }  // namespace
@@ -180,25 +253,32 @@ int launch_reserve(const int32_t* lens, const int32_t* add, int B, int32_t* tabl
   if (B > kMaxRequests) return fail(BNA_UNSUPPORTED, "paged_reserve: at most 4096 requests per call");
   ReserveArgs a{lens, add, table, table_stride, free_pages, num_free, lens_out, num_free_out, granted, slots, positions,
                 num_tokens, B, width, num_pages, page_size};
-  const int smem = 3 * B * 4;
-  cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * kMaxRequests * 4);
-  reserve_kernel<<<1, kReserveThreads, smem, s>>>(a);
-  return check_cuda(cudaGetLastError(), "paged_reserve launch");
+  const int smem = 4 * B * 4;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMaxRequests * 4);
+    if (e != cudaSuccess) return check_cuda(e, "paged_reserve attributes");
+  }
+  // enough CTAs for the tokens and for every page the requests could give back
+  const int64_t items = num_tokens + std::min((int64_t)num_pages, (int64_t)B * width);
+  const unsigned grid = (unsigned)std::min<int64_t>(kReserveCtas, (items + 2 * kReserveThreads - 1) / (2 * kReserveThreads));
+  return launch_dependent(reserve_kernel, a, grid, kReserveThreads, smem, s, "paged_reserve launch");
 }
 
 int launch_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* kp, bna_tensor4* vp,
                         const int64_t* slots, cudaStream_t s) {
   const int heads = (int)k->size[1];
   const int64_t rows = k->size[2] * heads;
-  const int vecs = (int)(k->size[3] / 8);
+  const int vecs = (int)(k->size[3] / 8), vec_shift = vecs == 8 ? 3 : vecs == 16 ? 4 : 5;
   PagedAppendArgs a{static_cast<const uint8_t*>(k->data), static_cast<const uint8_t*>(v->data),
                     static_cast<uint8_t*>(kp->data), static_cast<uint8_t*>(vp->data), k->stride[1], k->stride[2],
                     v->stride[1], v->stride[2], kp->stride[0], kp->stride[1], kp->stride[2], vp->stride[0],
-                    vp->stride[1], vp->stride[2], slots, rows, kp->size[0] * kp->size[2], heads, (int)kp->size[2], vecs};
-  const int64_t blocks = (rows * vecs + 255) / 256;
+                    vp->stride[1], vp->stride[2], slots, rows, kp->size[0] * kp->size[2], heads, (int)kp->size[2], vec_shift};
+  // four rows a thread once that still fills the GPU; one row a thread has the shorter latency
+  const int n = rows * vecs >= (int64_t)4 * 256 * 148 * 4 ? 4 : 1;
+  const int64_t per = (int64_t)n * (256 >> vec_shift), blocks = (rows + per - 1) / per;
   if (blocks > INT_MAX) return fail(BNA_UNSUPPORTED, "paged_append: too many elements");
-  paged_append_kernel<<<(unsigned)blocks, 256, 0, s>>>(a);
-  return check_cuda(cudaGetLastError(), "paged_append launch");
+  return launch_dependent(n == 4 ? paged_append_kernel<4> : paged_append_kernel<1>, a, (unsigned)blocks, 256, 0, s,
+                          "paged_append launch");
 }
 
 }  // namespace bna

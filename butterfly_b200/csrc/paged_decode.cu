@@ -23,6 +23,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <map>
@@ -695,8 +696,14 @@ int sm_count() {
 template <typename T, int DH, bool WIDE>
 int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, unsigned grid, cudaStream_t s) {
   auto kern = paged_decode_kernel<T, DH, WIDE>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DH>::kAlloc);
-  if (e != cudaSuccess) return check_cuda(e, "paged_decode attributes");
+  static std::atomic<uint64_t> ready{0};  // devices (bits) whose kernel has its shared memory allowed
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DH>::kAlloc);
+    if (e != cudaSuccess) return check_cuda(e, "paged_decode attributes");
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(Layout<DH>::kThreads);
