@@ -11,8 +11,9 @@
 //   * Work is cut evenly by bytes, not by request: the granules (16 keys of one KV head) of all
 //     requests form one line, and each of the persistent CTAs (one per SM) takes an equal
 //     stretch of it.  One long request spreads over all SMs, many short ones share an SM.
-//   * A producer warp walks the CTA's stretch, looks the pages up and issues one TMA tile copy
-//     for a granule's keys and one for its values into a ring of granule slots (192 KB a CTA); it runs ahead across the ends of requests.
+//   * Producer warps walk the CTA's stretch, look the pages up and issue one TMA tile copy for a
+//     granule's keys and one for its values into a ring of granule slots (192 KB a CTA); they
+//     run ahead across the ends of requests.
 //   * Eight consumer warps (four at head_dim 256) take the granules in turn, each with its own m, l and o in
 //     registers: no barrier between warps until a request's stretch ends.
 //   * A (request, KV head) that lies in one CTA is finished there.  Of one cut by CTA
@@ -87,12 +88,13 @@ struct Layout {
   // Consumer warps.  head_dim 256: four, as the output and score registers of eight would not
   // fit beside each other.
   static constexpr int kCons = DH == 256 ? 4 : 8;
-  static constexpr int kThreads = 32 * (kCons + 1);  // and the producer
+  static constexpr int kProd = 4;                        // producer warps
+  static constexpr int kThreads = 32 * (kCons + kProd);
   static constexpr int kSlotBytes = 2 * kGran * DH * 2;      // keys, then values
   static constexpr int kSlots = 192 * 1024 / kSlotBytes;
   // Granule i goes to warp i % kCons and slot i % kSlots: a slot has to stay with one warp,
   // because a barrier's parity tells a wait that is one use ahead nothing about the use before.
-  static_assert(kSlots % kCons == 0, "a slot belongs to one warp");
+  static_assert(kSlots % kCons == 0 && kSlots % kProd == 0, "a slot belongs to one consumer and one producer warp");
   static constexpr int kQPitch = 2 * DH + 16;                         // spreads the rows over the banks
   static constexpr int kQBytes = kRows * kQPitch;
   static constexpr int kQ = kSlots * kSlotBytes;
@@ -144,7 +146,7 @@ template <typename T, int DH, bool WIDE>
 __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const PagedArgs a) {
   using Lay = Layout<DH>;
-  constexpr int kCons = Lay::kCons;
+  constexpr int kCons = Lay::kCons, kProd = Lay::kProd;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + Lay::kBars);
@@ -181,8 +183,12 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, kErrSite + site, a.err));
   };
 
-  if (warp == kCons) {
-    // ------------------------------------------------------------------ producer
+  if (warp >= kCons) {
+    // ------------------------------------------------------------------ producers
+    // All walk the CTA's stretch; warp `pw` issues the copies of every kProd-th granule (one warp
+    // takes about 400 cycles a granule, and the memory delivers one in 350), and the first
+    // one publishes the segments and their queries.
+    const int pw = warp - kCons;
     const int per_b = a.Hkv * a.chunks;
     int64_t total = 0;
     for (int i = lane; i < a.B; i += 32) total += granules_of(a, clamp_len(a, a.lens[i]));
@@ -192,7 +198,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
     const int64_t C = max((int64_t)1, min((int64_t)gridDim.x, (U + kMinPart - 1) / kMinPart));
     int64_t cur = blockIdx.x < C ? U * blockIdx.x / C : U;
     const int64_t end = blockIdx.x < C ? U * (blockIdx.x + 1) / C : U;
-    int cnt = 0;      // granules issued
+    int cnt = 0;      // granules so far
     int nseg = 0;
     bool ok = true;
     if (cur < end) {
@@ -218,14 +224,14 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
         }
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
-      int slot = 0;
+      int slot = pw;
       uint32_t phase = 1;  // parity of the empty barriers' first use
       int len = __shfl_sync(0xffffffffu, len_w, b - wb), nt = granules_of(a, len);
       int pair = (int)((cur - before) / nt), t0 = (int)((cur - before) - (int64_t)pair * nt);
       while (ok && cur < end) {
         const int n = (int)min((int64_t)(nt - t0), end - cur);
         const int si = nseg & 1;
-        if (!(ok = wait(seg_empty + si, (uint32_t)(((nseg >> 1) & 1) ^ 1), 0))) break;
+        if (pw == 0 && !(ok = wait(seg_empty + si, (uint32_t)(((nseg >> 1) & 1) ^ 1), 0))) break;
         Seg s;
         s.b = b;
         s.h = pair / a.chunks;
@@ -245,12 +251,12 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
           s.slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
         }
         uint8_t* qdst = sm + Lay::kQ + si * Lay::kQBytes;
-        if (lane == 0) {
+        if (pw == 0 && lane == 0) {
           segs[si] = s;
           mbar_arrive_expect_tx(seg_full + si, (uint32_t)(s.rows * 2 * DH));
         }
         __syncwarp();
-        if (lane < s.rows)
+        if (pw == 0 && lane < s.rows)
           bulk_copy_g2s(qdst + lane * Lay::kQPitch, a.q + 2 * (b * a.q_b + (int64_t)(s.h * a.G + s.r0 + lane) * a.q_h), 2 * DH,
                         seg_full + si);
         const int32_t* trow = a.table + b * a.table_stride;
@@ -262,7 +268,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
             page = trow[pi];
           }
           const int m = min(32, n - i0);
-          for (int j = 0; j < m; ++j) {
+          for (int j = (pw - cnt) & (kProd - 1); j < m; j += kProd) {
             const int pg = __shfl_sync(0xffffffffu, page, j), rw = __shfl_sync(0xffffffffu, row, j);
             if (!(ok = wait(empty + slot, phase, 1))) break;
             if (lane == 0) {
@@ -272,12 +278,12 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
               tma_load_5d(dst, &mk, full + slot, 0, rw, 0, s.h, pg);
               tma_load_5d(dst + Lay::kSlotBytes / 2, &mv, full + slot, 0, rw, 0, s.h, pg);
             }
-            ++cnt;
-            if (++slot == Lay::kSlots) {
-              slot = 0;
+            if ((slot += kProd) >= Lay::kSlots) {
+              slot = pw;
               phase ^= 1;
             }
           }
+          cnt += m;
         }
         ++nseg;
         cur += n;
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
         }
       }
     }
-    if (ok) {
+    if (ok && pw == 0) {
       const int si = nseg & 1;
       if ((ok = wait(seg_empty + si, (uint32_t)(((nseg >> 1) & 1) ^ 1), 2)) && lane == 0) {
         segs[si].n = -1;
@@ -303,7 +309,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
       }
     }
     // requests without keys
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    for (int b = blockIdx.x * kProd + pw; b < a.B; b += gridDim.x * kProd) {
       if (clamp_len(a, a.lens[b]) != 0) continue;
       const int hq = a.Hkv * a.G;
       for (int i = lane; i < hq * (DH / 8); i += 32)
@@ -311,9 +317,9 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
       if (a.lse)
         for (int i = lane; i < hq; i += 32) a.lse[b * a.ls_b + i * a.ls_h] = -INFINITY;
     }
-    // no copy of this CTA is in flight when it ends, whatever the consumers did
+    // none of this warp's copies is in flight when the CTA ends, whatever the consumers did
     for (int i = max(0, cnt - Lay::kSlots); i < cnt; ++i)
-      for (int tries = 0; tries < 1000; ++tries)
+      for (int tries = 0; i % kProd == pw && tries < 1000; ++tries)
         if (mbar_try_wait_suspend(full + i % Lay::kSlots, (i / Lay::kSlots) & 1, 20000u)) break;
     return;
   }
