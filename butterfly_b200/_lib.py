@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 
 import torch
 
@@ -95,9 +94,8 @@ def lib() -> ctypes.CDLL:
                                          f32, vp, vp, vp, vp, i64, i32, f32, vp]),
             "bna_gemv": (i32, [vp, i64, vp, i64, i64, vp, i64, vp, i64, i32, i32, vp]),
             "bna_paged_reserve": (i32, [vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, i64, vp]),
-            # (their tensors are passed as packed bytes, see pack4)
-            "bna_paged_append": (i32, [vp, vp, vp, vp, vp, i32, vp]),
-            "bna_paged_decode": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i32, vp, i64, i32, vp, i32, f32, vp, i64, vp]),
+            "bna_paged_append": (i32, [T4, T4, T4, T4, vp, i32, vp]),
+            "bna_paged_decode": (i32, [T4, T4, T4, T4, T4, vp, T4, vp, i64, i64, i32, vp, i64, i32, vp, i32, f32, vp, i64, vp]),
             "bna_paged_decode_workspace_bytes": (i64, []),
             "bna_decode_step": (i32, [T4, T4, T4, T4, T4, T4, T4, T4, vp, i64, i64, i32, R, i32, i64, i64, i64, i64, i32, f32, vp]),
         }
@@ -134,11 +132,6 @@ def t4(x: torch.Tensor) -> Tensor4:
     if x.dim() != 4:
         raise ValueError(f"expected a 4-D tensor, got shape {tuple(x.shape)}")
     return Tensor4(x.data_ptr(), _I64x4(*x.shape), _I64x4(*x.stride()))
-
-
-# The nine int64 of a Tensor4 as bytes, which ctypes passes by address: a third of the time of
-# building the structure, in calls whose kernel takes a few microseconds.
-pack4 = struct.Struct("9q").pack
 
 
 def stream_ptr(device: torch.device) -> int:

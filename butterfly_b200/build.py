@@ -1,9 +1,10 @@
-"""Build libbna_b200.so (sm_100a) in-tree with nvcc.
+"""Build libbna_b200.so (sm_100a) in-tree with nvcc, and the CPython binding of the paged cache.
 
     python -m butterfly_b200.build          # or __graft_entry__.build()
 
 Each .cu under csrc/ is compiled to an object in csrc/_build/ (rebuilt when it or a
-header is newer), then linked into butterfly_b200/libbna_b200.so.
+header is newer), then linked into butterfly_b200/libbna_b200.so.  csrc/binding.cpp becomes
+butterfly_b200/_native.so (g++, against the installed torch's headers and libraries).
 """
 from __future__ import annotations
 
@@ -12,11 +13,14 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libbna_b200.so")
 BUILD = os.path.join(CSRC, "_build")
+BINDING = os.path.join(CSRC, "binding.cpp")
+NATIVE = os.path.join(HERE, "_native.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",
@@ -43,11 +47,29 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_binding() -> str:
+    if os.path.exists(NATIVE) and os.path.getmtime(NATIVE) >= max(os.path.getmtime(BINDING), _headers()):
+        return NATIVE
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc, libs = os.path.join(root, "include"), os.path.join(root, "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", BINDING, "-o", NATIVE,
+           f"-I{inc}", f"-I{inc}/torch/csrc/api/include", f"-I{sysconfig.get_path('include')}", f"-L{libs}",
+           f"-Wl,-rpath,{libs}", "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING}:\n{r.stdout}\n{r.stderr}")
+    return NATIVE
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        native = ex.submit(_build_binding)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+        native.result()
     if not os.path.exists(OUT) or os.path.getmtime(OUT) < max(os.path.getmtime(o) for o in objs):
         cmd = [NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", OUT, *objs,
                "-lcudart"]

@@ -18,6 +18,7 @@ enqueued on the current stream and nothing waits for the host.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import NamedTuple, Optional, Sequence
 
@@ -38,20 +39,27 @@ class PagedReservation(NamedTuple):
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object
+_native = None
 
 
-def _device(*xs: torch.Tensor) -> int:
-    """The index of the CUDA device that all of ``xs`` are on."""
-    d = xs[0].get_device()
-    for x in xs:
-        if x.get_device() != d or not x.is_cuda:
-            _lib.require_cuda(*xs)
-    return d
+def _binding():
+    """The compiled binding (csrc/binding.cpp), given the C entry points of the loaded library."""
+    global _native
+    if _native is None:
+        try:
+            from . import _native as mod
+        except ImportError as e:
+            raise ImportError(f"butterfly_b200/_native.so is missing or stale: build it with "
+                              f"`python -m butterfly_b200.build` ({e})") from e
+        L = _lib.lib()
+        mod.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in (L.bna_paged_reserve, L.bna_paged_append,
+                                                                  L.bna_paged_decode)))
+        _native = mod
+    return _native
 
 
-def _ints(name: str, x: torch.Tensor, dim: int) -> None:
-    if x.dtype != torch.int32 or x.dim() != dim or x.stride(-1) != 1 and x.shape[-1] > 1:
-        raise ValueError(f"{name} must be a {dim}-D int32 tensor with a contiguous last dim")
+def _stream(x: torch.Tensor) -> int:
+    return _raw_stream(x.get_device()) if x.is_cuda else 0  # (a CPU tensor is refused further on)
 
 
 def paged_reserve(lens: torch.Tensor, add: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -65,54 +73,17 @@ def paged_reserve(lens: torch.Tensor, add: torch.Tensor, block_table: torch.Tens
     tokens of request 0, then 1, ... are entries 0, 1, ... of ``slot_map`` and ``positions``
     (``num_tokens`` of them: at least the sum of the positive ``add``).  ``block_table`` and
     ``free_pages`` are updated in place, the lengths and the stack height are returned."""
-    dev = _device(lens, add, block_table, free_pages, num_free)
-    i32 = torch.int32
-    if not (lens.dtype is i32 and add.dtype is i32 and block_table.dtype is i32 and free_pages.dtype is i32
-            and num_free.dtype is i32 and block_table.dim() == 2 and block_table.is_contiguous() and lens.dim() == 1
-            and add.dim() == 1 and free_pages.dim() == 1 and lens.is_contiguous() and add.is_contiguous()
-            and free_pages.is_contiguous()):  # the usual case in one expression, else name what is wrong
-        for name, x, d in (("lens", lens, 1), ("add", add, 1), ("block_table", block_table, 2),
-                           ("free_pages", free_pages, 1), ("num_free", num_free, 1)):
-            _ints(name, x, d)
-    B, width = block_table.shape
-    n = int(num_tokens)
-    if lens.shape[0] != B or add.shape[0] != B or num_free.shape != (1,) or n < 0:
-        raise ValueError(f"lens and add must be [{B}] as block_table's rows, num_free [1], num_tokens >= 0")
-    # one allocation for the int32 results
-    out, left, positions = lens.new_empty(B + 1 + n).split_with_sizes((B, 1, n))
-    slots = lens.new_empty(n, dtype=torch.int64)
-    granted = lens.new_empty(B, dtype=torch.bool)
-    _lib.check(_lib.lib().bna_paged_reserve(
-        lens.data_ptr(), add.data_ptr(), B, block_table.data_ptr(), block_table.stride(0) if B > 1 else width, width,
-        free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), int(page_size), out.data_ptr(), left.data_ptr(),
-        granted.data_ptr(), slots.data_ptr(), positions.data_ptr(), n, _raw_stream(dev)))
-    return PagedReservation(out, left, slots, positions, granted)
-
-
-def _t4(name: str, x: torch.Tensor) -> bytes:
-    if x.dim() != 4:
-        raise ValueError(f"{name} must be a 4-D tensor, got shape {tuple(x.shape)}")
-    return _lib.pack4(x.data_ptr(), *x.shape, *x.stride())
+    r = (_native or _binding()).reserve(lens, add, block_table, free_pages, num_free, page_size, num_tokens, _stream(lens))
+    if r.__class__ is int:
+        _lib.check(r)
+    return PagedReservation(*r)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  slot_map: torch.Tensor) -> None:
     """Write token t's rows ``k[t]`` / ``v[t]`` ([tokens, Hkv, dh], any token and head strides)
     into slot ``slot_map[t]`` (int64) of the pools; negative slots are skipped."""
-    dev = _device(k, v, k_pages, v_pages, slot_map)
-    if k.dim() != 3 or v.dim() != 3:
-        raise ValueError("k and v must be [tokens, Hkv, dh]")
-    dt = k.dtype
-    if v.dtype != dt or k_pages.dtype != dt or v_pages.dtype != dt:
-        raise ValueError("k, v and the pools must have one dtype")
-    n, heads, dh = k.shape
-    if slot_map.dtype != torch.int64 or slot_map.shape != (n,) or n > 1 and slot_map.stride(0) != 1:
-        raise ValueError(f"slot_map must be a contiguous [{n}] int64 tensor")
-    ks, vs, (nv, hv, dv) = k.stride(), v.stride(), v.shape
-    _lib.check(_lib.lib().bna_paged_append(
-        _lib.pack4(k.data_ptr(), 1, heads, n, dh, 0, ks[1], ks[0], ks[2]),
-        _lib.pack4(v.data_ptr(), 1, hv, nv, dv, 0, vs[1], vs[0], vs[2]),
-        _t4("k_pages", k_pages), _t4("v_pages", v_pages), slot_map.data_ptr(), _lib.dtype_code(dt), _raw_stream(dev)))
+    _lib.check((_native or _binding()).append(k, v, k_pages, v_pages, slot_map, _stream(k)))
 
 
 _workspaces: dict = {}
@@ -125,14 +96,16 @@ def decode_workspace(device: torch.device | str | int = "cuda") -> torch.Tensor:
     return ws
 
 
-def _workspace_for(device: int, stream: int) -> torch.Tensor:
+def _workspace_for(x: torch.Tensor, stream: int) -> torch.Tensor:
     """The workspace kept for a stream.  A capture gets its own (zeroed inside the graph): its
     replays may run beside later calls on the stream."""
+    if not x.is_cuda:
+        raise ValueError("butterfly_b200 kernels run on CUDA tensors only (no CPU path)")
     if torch.cuda.is_current_stream_capturing():
-        return decode_workspace(device)
-    ws = _workspaces.get((device, stream))
+        return decode_workspace(x.device)
+    ws = _workspaces.get((x.get_device(), stream))
     if ws is None:
-        ws = _workspaces[(device, stream)] = decode_workspace(device)
+        ws = _workspaces[(x.get_device(), stream)] = decode_workspace(x.device)
     return ws
 
 
@@ -151,43 +124,14 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     ``transpose(1, 2)`` is [B,1,Hq,dh] storage); with ``return_lse`` also the fp32 natural-log sums
     [B,Hq,1].  A request of length 0 gives zeros and -inf.  ``workspace`` (``decode_workspace``)
     defaults to one kept per stream; calls that may overlap need one each."""
-    dev = _device(q, k_pages, v_pages, block_table, lens)
-    tq = _t4("q", q)
-    B, Hq, Tq, dh = q.shape
-    dt = q.dtype
-    if k_pages.dtype != dt or v_pages.dtype != dt:
-        raise ValueError("the pools must have q's dtype")
-    _ints("block_table", block_table, 2)
-    _ints("lens", lens, 1)
-    if block_table.shape[0] != B or lens.shape[0] != B:
-        raise ValueError(f"block_table and lens must have {B} rows")
-    nk = nv = act = None
-    if k_new is not None or v_new is not None:
-        if k_new is None or v_new is None:
-            raise ValueError("k_new and v_new go together")
-        _device(q, k_new, v_new)
-        if k_new.dtype != dt or v_new.dtype != dt:
-            raise ValueError("q, k_new, v_new dtype mismatch")
-        nk, nv = _t4("k_new", k_new), _t4("v_new", v_new)
-    if active is not None:
-        _device(q, active)
-        if active.dtype != torch.bool or active.shape != (B,) or not active.is_contiguous():
-            raise ValueError(f"active must be a contiguous [{B}] bool tensor")
-        act = active.data_ptr()
-    stream = _raw_stream(dev)
-    if workspace is None:
-        workspace = _workspace_for(dev, stream)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.get_device() != dev:
-        raise ValueError("workspace must be a contiguous uint8 tensor on q's device (decode_workspace)")
-    out = q.new_empty((B, Hq, Tq, dh))
-    lse = q.new_empty((B, Hq, Tq), dtype=torch.float32) if return_lse else None
-    _lib.check(_lib.lib().bna_paged_decode(
-        tq, _t4("k_pages", k_pages), _t4("v_pages", v_pages), nk, nv, act,
-        _lib.pack4(out.data_ptr(), B, Hq, Tq, dh, Hq * Tq * dh, Tq * dh, dh, 1), lse.data_ptr() if return_lse else None, Hq, 1,
-        _lib.dtype_code(dt), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], lens.data_ptr(),
-        int(window), float(scale) if scale is not None else 1.0 / math.sqrt(dh), workspace.data_ptr(), workspace.numel(),
-        stream))
-    return (out, lse) if return_lse else out
+    stream = _stream(q)
+    r = (_native or _binding()).decode(
+        q, k_pages, v_pages, block_table, lens, k_new, v_new, active, window,
+        1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else scale, return_lse,
+        _workspace_for(q, stream) if workspace is None else workspace, stream)
+    if r.__class__ is int:
+        _lib.check(r)
+    return r
 
 
 class PagedKVCache:
