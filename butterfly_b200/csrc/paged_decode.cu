@@ -47,6 +47,7 @@ constexpr int kGran = 16;       // keys of a granule
 constexpr int kMaxCtas = 160;   // workspace parts are sized for this many CTAs
 constexpr int kRows = 16;       // query heads of one KV head served together
 constexpr int kMinPart = 16;    // granules a CTA gets at least of an even cut (fewer CTAs otherwise)
+constexpr int kFan = 16;        // parts of a pair joined at a time; up to kFan + 4 where that is all
 constexpr int kLanes = 8;       // producer lanes that issue copies side by side
 constexpr int kErrSite = 0x40;  // device error sites of this file
 
@@ -72,12 +73,13 @@ struct PagedArgs {
   int* err;
 };
 
-// Workspace: counters (zero between calls: arrivals at each CTA's last part, then pairs claimed),
+// Workspace: counters (zero between calls: pairs claimed, arrivals at a pair by its first CTA, at a
+// group of its parts by the first one's slot),
 // (m, l) of every part, then the outputs.
 constexpr int64_t kWsMl = 4096;
 constexpr int64_t kWsO = kWsMl + (int64_t)2 * kMaxCtas * kRows * 8;
 constexpr int64_t kWsBytes = kWsO + (int64_t)2 * kMaxCtas * kRows * 256 * 4;
-static_assert(4 * (kMaxCtas + 1) <= kWsMl, "counters");
+static_assert(4 * (3 * kMaxCtas + 1) <= kWsMl && kMaxCtas <= kFan * (kFan + 4), "counters, rounds");
 
 // One stretch of a (request, KV head, head group) inside a CTA.
 struct Seg {
@@ -109,7 +111,7 @@ struct Layout {
   static constexpr int kBuf = kQ + 2 * kQBytes;
   // merge of the warps: 16 rows x 32 columns, 8 x 64 or 4 x 128 (rows padded by 8 floats), or
   // the weights and partial sums of a join
-  static constexpr int kMergeFloats = kCons * kRows * (32 + 8), kJoinFloats = kMaxCtas * kRows + 4 * 32 * kCons;
+  static constexpr int kMergeFloats = kCons * kRows * (32 + 8), kJoinFloats = 32 * kRows + 4 * 32 * kCons;
   static constexpr int kBufBytes = 4 * (kMergeFloats > kJoinFloats ? kMergeFloats : kJoinFloats);
   static constexpr int kStage = kBuf + 2 * kBufBytes;  // (segments alternate between two buffers)
   static constexpr int kHalf = 20 * 1024;  // parts of a join arrive in two halves of this size
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
     // items: the pairs, or the stretches of C CTAs
     const int64_t C = whole ? N : max((int64_t)1, min(grid, quot(U + kMinPart - 1, kMinPart)));
     const Cut cut(U, max((int64_t)1, C));
-    int* claims = reinterpret_cast<int*>(a.ws) + kMaxCtas;
+    int* claims = reinterpret_cast<int*>(a.ws);
 
     // The line that items are cut from: granules, or whole pairs.  Window of 32 requests (lane i:
     // request wb + i): length, its stretch of the line, and the line up to that stretch's end.
@@ -666,120 +668,126 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
     }
     if (s.slot < 0) continue;
 
-    // a cut pair: the CTA whose part arrives last joins the parts
-    cons_sync<kNT>();
-    if (tid == 0) {
-      // release: the CTA's part (ordered before this by the barrier) before the count
-      int arrived, *counter = reinterpret_cast<int*>(a.ws) + s.first_cta;
-      asm volatile("atom.add.release.gpu.global.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(counter) : "memory");
-      const bool last = arrived + 1 == s.parts;
-      if (last) {
-        *counter = 0;  // as the next call finds it
-        asm volatile("fence.acq_rel.gpu;" ::: "memory");
-      }
-      *last_flag = last;
-    }
-    cons_sync<kNT>();
-    if (!*last_flag) continue;
-    // The parts come to shared memory by bulk copies, in batches, two in flight (plain loads bring
-    // one SM about 34 GB/s here: 5 us for 74 parts of 4 heads); a thread sums 4 columns of a
-    // row, and where the rows are few, groups of threads share the parts.
-    auto slot_of = [&](int p) { return (int64_t)(2 * (s.first_cta + p) + (p == 0 ? 1 : 0)); };
+    // A cut pair: the CTA whose part arrives last joins the parts.  Of many parts, groups of kFan
+    // first: most groups are complete before the last CTA arrives, and a CTA reads only some
+    // 30 GB/s here (74 parts of 4 heads at once took 8 us after the last arrival).
     const float2* gml = reinterpret_cast<const float2*>(a.ws + kWsMl);
     const float* go = reinterpret_cast<const float*>(a.ws + kWsO);
-    constexpr int kItems = (kRows * DH / 4 + kNT - 1) / kNT;
-    const int items = s.rows * (DH / 4);
-    const int batch = Lay::kHalf / 16 / items, batches = (s.parts + batch - 1) / batch;
-    auto fetch = [&](int k) {  // by warp 0
-      if (k >= batches) return;
-      const int half = (fetched + k) & 1, n = min(batch, s.parts - k * batch);
-      if (lane == 0) mbar_arrive_expect_tx(stage_full + half, (uint32_t)(n * items * 16));
-      __syncwarp();
-      for (int p = lane; p < n; p += 32)
-        bulk_copy_g2s(sm + Lay::kStage + half * Lay::kHalf + p * items * 16, go + slot_of(k * batch + p) * kRows * DH, items * 16,
-                      stage_full + half);
-    };
-    if (warp == 0) {
-      asm volatile("fence.proxy.async;" ::: "memory");  // the parts were written by plain stores
-      fetch(0);
-      fetch(1);
-    }
-    float* wt = buf;  // [parts][rows] weights
-    for (int r = warp; r < s.rows; r += kCons) {
-      constexpr int kPer = kMaxCtas / 32;
-      float2 t[kPer];
-#pragma unroll
-      for (int x = 0; x < kPer; ++x) {
-        const int p = x * 32 + lane;
-        t[x] = p < s.parts ? __ldcg(gml + slot_of(p) * kRows + r) : make_float2(-INFINITY, 0.f);
+    bool final = s.parts <= kFan + 4;
+    int base = final ? 0 : (int)(blockIdx.x - s.first_cta) / kFan * kFan;  // first part of the round's group,
+    int members = final ? s.parts : min(kFan, s.parts - base), step = 1;   // their number, and their distance
+    for (;;) {
+      auto slot_of = [&](int p) {
+        const int part = base + p * step;
+        return (int64_t)(2 * (s.first_cta + part) + (part == 0 ? 1 : 0));
+      };
+      cons_sync<kNT>();
+      if (tid == 0) {
+        // release: the CTA's part (ordered before this by the barrier) before the count
+        int arrived, *counter = reinterpret_cast<int*>(a.ws) + 1 + (final ? s.first_cta : kMaxCtas + (int)slot_of(0));
+        asm volatile("atom.add.release.gpu.global.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(counter) : "memory");
+        const bool last = arrived + 1 == members;
+        if (last) {
+          *counter = 0;  // as the next call finds it
+          asm volatile("fence.acq_rel.gpu;" ::: "memory");
+        }
+        *last_flag = last;
       }
-      float M = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int x = 0; x < kPer; ++x) M = fmaxf(M, t[x].x);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-      const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll
-      for (int x = 0; x < kPer; ++x) {
-        t[x].x = ex2_approx(t[x].x - base);
-        L += t[x].y * t[x].x;
+      cons_sync<kNT>();
+      if (!*last_flag) break;
+      // The parts come to shared memory by bulk copies, in batches, two in flight; a thread sums
+      // 4 columns of a row, and where the rows are few, groups of threads share the parts.
+      constexpr int kItems = (kRows * DH / 4 + kNT - 1) / kNT;
+      const int items = s.rows * (DH / 4);
+      const int batch = Lay::kHalf / 16 / items, batches = (members + batch - 1) / batch;
+      auto fetch = [&](int k) {  // by warp 0
+        if (k >= batches) return;
+        const int half = (fetched + k) & 1, n = min(batch, members - k * batch);
+        if (lane == 0) mbar_arrive_expect_tx(stage_full + half, (uint32_t)(n * items * 16));
+        __syncwarp();
+        if (lane < n)
+          bulk_copy_g2s(sm + Lay::kStage + half * Lay::kHalf + lane * items * 16, go + slot_of(k * batch + lane) * kRows * DH,
+                        items * 16, stage_full + half);
+      };
+      if (warp == 0) {
+        asm volatile("fence.proxy.async;" ::: "memory");  // the parts were written by plain stores
+        fetch(0);
+        fetch(1);
       }
-      L = warp_sum(L);
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+      float* wt = buf;  // [members][rows] weights
+      for (int r = warp; r < s.rows; r += kCons) {
+        const float2 t = lane < members ? __ldcg(gml + slot_of(lane) * kRows + r) : make_float2(-INFINITY, 0.f);
+        float M = t.x;
 #pragma unroll
-      for (int x = 0; x < kPer; ++x)
-        if (x * 32 + lane < s.parts) wt[(x * 32 + lane) * s.rows + r] = t[x].x * inv;
-      if (lane == 0 && a.lse) a.lse[s.b * a.ls_b + (int64_t)(s.h * a.G + s.r0 + r) * a.ls_h] = lse_of(M, L);
-    }
-    cons_sync<kNT>();
-    const int groups = items >= kNT ? 1 : kNT / items, grp = groups == 1 ? 0 : tid / items;
-    const int it0 = groups == 1 ? tid : tid % items;
-    float4 v[kItems];
+        for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+        const float f = ex2_approx(t.x - (M == -INFINITY ? 0.f : M));
+        const float L = warp_sum(t.y * f);
+        if (lane < members) wt[lane * s.rows + r] = f * (!final ? 1.f : L == 0.f ? 0.f : 1.f / L);
+        if (lane == 0) {
+          if (!final) const_cast<float2*>(gml)[slot_of(0) * kRows + r] = make_float2(M, L);
+          else if (a.lse) a.lse[s.b * a.ls_b + (int64_t)(s.h * a.G + s.r0 + r) * a.ls_h] = lse_of(M, L);
+        }
+      }
+      cons_sync<kNT>();
+      const int groups = items >= kNT ? 1 : kNT / items, grp = groups == 1 ? 0 : tid / items;
+      const int it0 = groups == 1 ? tid : tid % items;
+      float4 v[kItems];
 #pragma unroll
-    for (int x = 0; x < kItems; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < batches; ++k) {
-      const int half = (fetched + k) & 1;
-      wait(stage_full + half, (uint32_t)(((fetched + k) >> 1) & 1), 6);  // (the next segment's wait sees a failure)
-      const float4* src = reinterpret_cast<const float4*>(sm + Lay::kStage + half * Lay::kHalf);
-      const int n = min(batch, s.parts - k * batch);
-      if (grp < groups)
+      for (int x = 0; x < kItems; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < batches; ++k) {
+        const int half = (fetched + k) & 1;
+        wait(stage_full + half, (uint32_t)(((fetched + k) >> 1) & 1), 6);  // (the next segment's wait sees a failure)
+        const float4* src = reinterpret_cast<const float4*>(sm + Lay::kStage + half * Lay::kHalf);
+        const int n = min(batch, members - k * batch);
+        if (grp < groups)
+#pragma unroll
+          for (int x = 0; x < kItems; ++x) {
+            const int it = it0 + x * kNT;
+            if (it < items)
+              for (int p = grp; p < n; p += groups) {
+                const float4 u = src[p * items + it];
+                const float f = wt[(k * batch + p) * s.rows + it / (DH / 4)];
+                v[x].x = fmaf(u.x, f, v[x].x);
+                v[x].y = fmaf(u.y, f, v[x].y);
+                v[x].z = fmaf(u.z, f, v[x].z);
+                v[x].w = fmaf(u.w, f, v[x].w);
+              }
+          }
+        if (k + 2 < batches) {
+          cons_sync<kNT>();  // the half has been read
+          if (warp == 0) fetch(k + 2);
+        }
+      }
+      fetched += batches;
+      if (groups > 1) {
+        float4* red = reinterpret_cast<float4*>(wt + 32 * kRows);  // [group][item]
+        if (grp < groups) red[grp * items + it0] = v[0];
+        cons_sync<kNT>();
+        if (grp == 0)
+          for (int g = 1; g < groups; ++g) {
+            const float4 w = red[g * items + it0];
+            v[0].x += w.x;
+            v[0].y += w.y;
+            v[0].z += w.z;
+            v[0].w += w.w;
+          }
+      }
+      if (grp == 0)
 #pragma unroll
         for (int x = 0; x < kItems; ++x) {
           const int it = it0 + x * kNT;
-          if (it < items)
-            for (int p = grp; p < n; p += groups) {
-              const float4 u = src[p * items + it];
-              const float f = wt[(k * batch + p) * s.rows + it / (DH / 4)];
-              v[x].x = fmaf(u.x, f, v[x].x);
-              v[x].y = fmaf(u.y, f, v[x].y);
-              v[x].z = fmaf(u.z, f, v[x].z);
-              v[x].w = fmaf(u.w, f, v[x].w);
-            }
+          if (it >= items) break;
+          if (final)
+            store4<T>(a.out + 2 * (s.b * a.o_b + (int64_t)(s.h * a.G + s.r0 + it / (DH / 4)) * a.o_h + (it % (DH / 4)) * 4), v[x], 1.f);
+          else
+            reinterpret_cast<float4*>(const_cast<float*>(go) + slot_of(0) * kRows * DH)[it] = v[x];
         }
-      cons_sync<kNT>();  // the half has been read
-      if (warp == 0) fetch(k + 2);
+      if (final) break;
+      members = (s.parts + kFan - 1) / kFan;
+      base = 0;
+      step = kFan;
+      final = true;
     }
-    fetched += batches;
-    if (groups > 1) {
-      float4* red = reinterpret_cast<float4*>(wt + kMaxCtas * kRows);  // [group][item]
-      if (grp < groups) red[grp * items + it0] = v[0];
-      cons_sync<kNT>();
-      if (grp == 0)
-        for (int g = 1; g < groups; ++g) {
-          const float4 w = red[g * items + it0];
-          v[0].x += w.x;
-          v[0].y += w.y;
-          v[0].z += w.z;
-          v[0].w += w.w;
-        }
-    }
-    if (grp == 0)
-#pragma unroll
-      for (int x = 0; x < kItems; ++x) {
-        const int it = it0 + x * kNT;
-        if (it < items)
-          store4<T>(a.out + 2 * (s.b * a.o_b + (int64_t)(s.h * a.G + s.r0 + it / (DH / 4)) * a.o_h + (it % (DH / 4)) * 4), v[x], 1.f);
-      }
   }
 }
 
