@@ -48,6 +48,7 @@ constexpr int kMaxCtas = 160;   // workspace parts are sized for this many CTAs
 constexpr int kRows = 16;       // query heads of one KV head served together
 constexpr int kMinPart = 16;    // granules a CTA gets at least of an even cut (fewer CTAs otherwise)
 constexpr int kFan = 16;        // parts of a pair joined at a time; up to kFan + 4 where that is all
+constexpr int kKeepLens = 1024;  // lengths kept in shared memory, once read
 constexpr int kLanes = 8;       // producer lanes that issue copies side by side
 constexpr int kErrSite = 0x40;  // device error sites of this file
 
@@ -67,6 +68,7 @@ struct PagedArgs {
   int64_t table_stride;
   const int32_t* lens;
   int B, Hkv, G, width, num_pages, page_size, window;
+  int page_shift;          // log2(page_size), or -1
   int chunks, chunk_rows;  // the G heads in `chunks` groups of chunk_rows <= kRows
   float scale_log2;
   uint8_t* ws;
@@ -120,7 +122,8 @@ struct Layout {
   static constexpr int kNumBars = 2 * kSlots + 6;
   static constexpr int kSeg = kBars + kNumBars * 8;
   static constexpr int kFlags = kSeg + 2 * (int)sizeof(Seg);
-  static constexpr int kBytes = (kFlags + 16 + 15) / 16 * 16;
+  static constexpr int kLens = (kFlags + 16 + 15) / 16 * 16;  // the first kKeepLens requests' lengths
+  static constexpr int kBytes = kLens + 4 * kKeepLens;
   static constexpr int kAlloc = kBytes + 1024;  // the base is aligned to 1024 (swizzle atom)
   static_assert(kAlloc <= 232448, "shared memory of a CTA");
 };
@@ -142,8 +145,11 @@ __device__ __forceinline__ int64_t quot(int64_t x, int64_t y) {
 
 // U granules over C CTAs: the first U % C take one more.
 struct Cut {
-  int64_t q, r;
-  __device__ Cut(int64_t U, int64_t C) : q(quot(U, C)), r(U - q * C) {}
+  int64_t q = 1, r = 0;
+  __device__ void set(int64_t U, int64_t C) {
+    q = quot(U, C);
+    r = U - q * C;
+  }
   __device__ int64_t start(int64_t c) const { return c * q + min(c, r); }
   __device__ int cta_of(int64_t x) const {  // the CTA that holds granule x
     const int64_t wide = r * (q + 1);
@@ -234,16 +240,31 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
     // ------------------------------------------------------------------ producer
     const int per_b = a.Hkv * a.chunks;
     const int64_t grid = gridDim.x;
-    const int len0 = lane < a.B ? clamp_len(a, a.lens[lane]) : 0;  // the first 32 requests stay in registers
-    auto len_at = [&](int i) { return i < 32 ? len0 : i < a.B ? clamp_len(a, a.lens[i]) : 0; };  // i = lane + 32 k
+    int* lens = reinterpret_cast<int*>(sm + Lay::kLens);
+    // The first claim of a pair goes out before it is known whether there is one to take: with
+    // all CTAs claiming at once the answer takes 3 us.
+    int* claims = reinterpret_cast<int*>(a.ws);
+    int claim = lane == 0 ? atomicAdd(claims, 1) : 0;
     int64_t U = 0, N = 0;  // granules, and pairs that have any
     int longest = 0;
-    for (int i = lane; i < a.B; i += 32) {
-      const int nt = granules_of(a, len_at(i));
+    auto count = [&](int len) {
+      const int nt = granules_of(a, len);
       U += nt;
       N += nt > 0;
       longest = max(longest, nt);
+    };
+    for (int i0 = lane; i0 < a.B; i0 += 256) {  // eight loads in flight
+      int len[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) len[x] = i0 + 32 * x < a.B ? a.lens[i0 + 32 * x] : 0;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        len[x] = clamp_len(a, len[x]);
+        if (i0 + 32 * x < kKeepLens) lens[i0 + 32 * x] = len[x];
+        count(len[x]);
+      }
     }
+    __syncwarp();
     if (__all_sync(0xffffffffu, U < 1 << 26)) {
       U = __reduce_add_sync(0xffffffffu, (unsigned)U);
     } else {
@@ -264,15 +285,16 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
     const bool whole = (N <= grid ? longest : share + longest / 2) <= even;
     // items: the pairs, or the stretches of C CTAs
     const int64_t C = whole ? N : max((int64_t)1, min(grid, quot(U + kMinPart - 1, kMinPart)));
-    const Cut cut(U, max((int64_t)1, C));
-    int* claims = reinterpret_cast<int*>(a.ws);
+    Cut cut;
+    if (!whole) cut.set(U, C);
 
     // The line that items are cut from: granules, or whole pairs.  Window of 32 requests (lane i:
     // request wb + i): length, its stretch of the line, and the line up to that stretch's end.
     int wb = 0, len_w = 0;
     int64_t mine_w = 0, incl_w = 0, before = 0;
     auto load_window = [&]() {
-      len_w = len_at(wb + lane);
+      const int i = wb + lane;
+      len_w = i >= a.B ? 0 : i < kKeepLens ? lens[i] : clamp_len(a, a.lens[i]);
       const int nt = granules_of(a, len_w);
       mine_w = incl_w = (int64_t)(whole ? (nt > 0) : nt) * per_b;
       if (__all_sync(0xffffffffu, mine_w < 1 << 26)) {
@@ -302,91 +324,115 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
       }
       return __ffs(past) - 1;
     };
+    // Segments (a pair, or the CTA's part of one) in their order, each with the pages of its first
+    // 32 granules asked for.  Taking one starts the claim of the pair after it.
+    struct Next {
+      Seg s;
+      int page, row;
+    };
+    auto look_up = [&](Next& x, int i) {
+      if (i < x.s.n) {
+        const int pos = (x.s.g0 + i) * kGran, pi = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.page_size;
+        x.row = pos - pi * a.page_size;
+        x.page = a.table[x.s.b * a.table_stride + pi];
+      }
+    };
+    int64_t item = blockIdx.x, cur = 0, end = 0;  // the next item, and what is left of the last one taken
+    bool first = true, pending = true;
+    // A claim comes with every CTA and with every pair claimed: the last of all finds nothing and
+    // leaves the count as the next call needs it.
+    const int64_t last_claim = (whole && C > grid ? C : grid) - 1;
+    auto answer = [&]() -> int64_t {
+      const int c = __shfl_sync(0xffffffffu, claim, 0);
+      if (c == last_claim && lane == 0) *claims = 0;
+      pending = false;
+      return grid + c;
+    };
+    auto take = [&](Next& x) -> bool {
+      if (cur >= end) {
+        if (!first) {
+          item = pending ? answer() : C;
+          if (!whole) item = C;
+          if (item < C) {
+            if (lane == 0) claim = atomicAdd(claims, 1);
+            pending = true;
+          }
+        }
+        first = false;
+        if (item >= C) return false;
+        cur = whole ? item : cut.start(item);
+        end = whole ? item + 1 : cut.start(item + 1);
+      }
+      const int f = find(cur), len = __shfl_sync(0xffffffffu, len_w, f), nt = granules_of(a, len);
+      const int64_t local = cur - before - __shfl_sync(0xffffffffu, incl_w - mine_w, f);
+      const int pair = whole ? (int)local : (int)quot(local, nt), t0 = whole ? 0 : (int)(local - (int64_t)pair * nt);
+      Seg& s = x.s;
+      s.b = wb + f;
+      s.lo = first_key(a, len);
+      s.hi = len;
+      s.g0 = s.lo / kGran + t0;
+      s.n = whole ? nt : (int)min((int64_t)(nt - t0), end - cur);
+      x.page = -1;
+      x.row = 0;
+      look_up(x, lane);
+      s.h = a.chunks == 1 ? pair : pair / a.chunks;
+      s.r0 = (pair - s.h * a.chunks) * a.chunk_rows;
+      s.rows = min(a.chunk_rows, a.G - s.r0);
+      s.slot = -1;
+      s.parts = 1;
+      s.first_cta = 0;
+      if (s.n < nt) {
+        const int64_t p0 = cur - t0;
+        s.first_cta = cut.cta_of(p0);
+        s.parts = cut.cta_of(p0 + nt - 1) - s.first_cta + 1;
+        s.slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+      }
+      cur += whole ? 1 : s.n;
+      return true;
+    };
     int used = 0, nseg = 0;  // granules given to warp lane % kCons, and segments, so far
     bool ok = true;
-    int64_t item = blockIdx.x;
-    while (ok && item < C) {
-      int claim = 0;  // of the pair after this one; the answer is needed when this one has been issued
-      if (whole && C > grid && lane == 0) claim = atomicAdd(claims, 1);
-      int64_t cur = whole ? item : cut.start(item);
-      const int64_t end = whole ? item + 1 : cut.start(item + 1);
-      while (ok && cur < end) {  // segments: a pair, or the CTA's part of one
-        const int f = find(cur);
-        const int len = __shfl_sync(0xffffffffu, len_w, f), nt = granules_of(a, len);
-        const int64_t local = cur - before - __shfl_sync(0xffffffffu, incl_w - mine_w, f);
-        const int pair = whole ? (int)local : (int)quot(local, nt), t0 = whole ? 0 : (int)(local - (int64_t)pair * nt);
-        Seg s;
-        s.b = wb + f;
-        s.h = pair / a.chunks;
-        s.r0 = (pair - s.h * a.chunks) * a.chunk_rows;
-        s.rows = min(a.chunk_rows, a.G - s.r0);
-        s.lo = first_key(a, len);
-        s.hi = len;
-        s.g0 = s.lo / kGran + t0;
-        s.n = whole ? nt : (int)min((int64_t)(nt - t0), end - cur);
-        s.slot = -1;
-        s.parts = 1;
-        s.first_cta = 0;
-        if (s.n < nt) {
-          const int64_t p0 = cur - t0;
-          s.first_cta = cut.cta_of(p0);
-          s.parts = cut.cta_of(p0 + nt - 1) - s.first_cta + 1;
-          s.slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
-        }
-        // the first pages, asked for before the wait for a place to put the segment
-        const int32_t* trow = a.table + s.b * a.table_stride;
-        int page = -1, row = 0;
-        auto look_up = [&](int i) {
-          if (i < s.n) {
-            const int pos = (s.g0 + i) * kGran, pi = pos / a.page_size;
-            row = pos - pi * a.page_size;
-            page = trow[pi];
-          }
-        };
-        look_up(lane);
-        const int si = nseg & 1;
-        if (!(ok = wait(seg_empty + si, (uint32_t)(((nseg >> 1) & 1) ^ 1), 0))) break;
-        if (lane == 0) {
-          segs[si] = s;
-          mbar_arrive_expect_tx(seg_full + si, (uint32_t)(s.rows * 2 * DH));
-        }
-        __syncwarp();
-        if (lane < s.rows)
-          bulk_copy_g2s(sm + Lay::kQ + si * Lay::kQBytes + lane * Lay::kQPitch,
-                        a.q + 2 * (s.b * a.q_b + (int64_t)(s.h * a.G + s.r0 + lane) * a.q_h), 2 * DH, seg_full + si);
-        for (int i0 = 0; i0 < s.n && ok; i0 += 32) {
-          const int m = min(32, s.n - i0), page_i = page, row_i = row;
-          look_up(i0 + 32 + lane);
-          // lane i issues granule i0 + i; several lanes at once, as one takes about 400 cycles a
-          // granule and the memory delivers one in 350 (one lane: 758, eight: 615 us at 64 x 65,536)
-          for (int w = 0; w < m && ok; w += kLanes) {
-            bool mine = true;
-            if (lane >= w && lane < w + kLanes && lane < m) {
-              const int use = used + (i0 + lane) / kCons, slot = use % Lay::kRing * kCons + lane % kCons;
-              mine = mbar_wait(empty + slot, (uint32_t)((use / Lay::kRing) & 1) ^ 1, abort_flag, kErrSite + 1, a.err);
-              if (mine) {  // (a page number outside the pool fills the tile with zeros)
-                uint8_t* dst = sm + slot * Lay::kSlotBytes;
-                mbar_arrive_expect_tx(full + slot, Lay::kSlotBytes);
-                tma_load_5d(dst, &mk, full + slot, 0, row_i, 0, s.h, page_i);
-                tma_load_5d(dst + Lay::kSlotBytes / 2, &mv, full + slot, 0, row_i, 0, s.h, page_i);
-              }
+    Next next;
+    bool more = take(next);
+    while (ok && more) {
+      Next now = next;
+      // the next one's page numbers arrive while this one's granules are issued (the first one's
+      // copies go out at once)
+      if (nseg > 0) more = take(next);
+      const Seg& s = now.s;
+      const int si = nseg & 1;
+      if (!(ok = wait(seg_empty + si, (uint32_t)(((nseg >> 1) & 1) ^ 1), 0))) break;
+      if (lane == 0) {
+        segs[si] = s;
+        mbar_arrive_expect_tx(seg_full + si, (uint32_t)(s.rows * 2 * DH));
+      }
+      __syncwarp();
+      if (lane < s.rows)
+        bulk_copy_g2s(sm + Lay::kQ + si * Lay::kQBytes + lane * Lay::kQPitch,
+                      a.q + 2 * (s.b * a.q_b + (int64_t)(s.h * a.G + s.r0 + lane) * a.q_h), 2 * DH, seg_full + si);
+      for (int i0 = 0; i0 < s.n && ok; i0 += 32) {
+        const int m = min(32, s.n - i0), page = now.page, row = now.row;
+        look_up(now, i0 + 32 + lane);
+        // lane i issues granule i0 + i; several lanes at once, as one takes about 400 cycles a
+        // granule and the memory delivers one in 350 (one lane: 758, eight: 615 us at 64 x 65,536)
+        for (int w = 0; w < m && ok; w += kLanes) {
+          bool mine = true;
+          if (lane >= w && lane < w + kLanes && lane < m) {
+            const int use = used + (i0 + lane) / kCons, slot = use % Lay::kRing * kCons + lane % kCons;
+            mine = mbar_wait(empty + slot, (uint32_t)((use / Lay::kRing) & 1) ^ 1, abort_flag, kErrSite + 1, a.err);
+            if (mine) {  // (a page number outside the pool fills the tile with zeros)
+              uint8_t* dst = sm + slot * Lay::kSlotBytes;
+              mbar_arrive_expect_tx(full + slot, Lay::kSlotBytes);
+              tma_load_5d(dst, &mk, full + slot, 0, row, 0, s.h, page);
+              tma_load_5d(dst + Lay::kSlotBytes / 2, &mv, full + slot, 0, row, 0, s.h, page);
             }
-            ok = __all_sync(0xffffffffu, mine);
           }
+          ok = __all_sync(0xffffffffu, mine);
         }
-        used += (s.n - lane % kCons + kCons - 1) / kCons;
-        ++nseg;
-        cur += whole ? 1 : s.n;
       }
-      if (whole && C > grid) {
-        // One claim a pair: the last of them finds nothing and leaves the count as the next call
-        // needs it.
-        claim = __shfl_sync(0xffffffffu, claim, 0);
-        item = grid + claim;
-        if (claim == C - 1 && lane == 0) *claims = 0;
-      } else {
-        item = C;
-      }
+      used += (s.n - lane % kCons + kCons - 1) / kCons;
+      if (nseg == 0) more = take(next);
+      ++nseg;
     }
     if (ok) {
       const int si = nseg & 1;
@@ -395,6 +441,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
         mbar_arrive(seg_full + si);
       }
     }
+    if (pending) answer();
     // requests without keys
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
       if (clamp_len(a, a.lens[b]) != 0) continue;
@@ -889,6 +936,7 @@ int launch_paged_decode(const bna_tensor4* q, bna_tensor4* kp, bna_tensor4* vp, 
   a.table = table, a.table_stride = table_stride, a.lens = lens;
   a.B = (int)q->size[0], a.Hkv = (int)kp->size[1], a.G = (int)(q->size[1] / kp->size[1]);
   a.width = width, a.num_pages = (int)kp->size[0], a.page_size = (int)kp->size[2], a.window = window;
+  a.page_shift = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.page_size) : -1;
   a.chunks = (a.G + kRows - 1) / kRows;
   a.chunk_rows = (a.G + a.chunks - 1) / a.chunks;
   a.scale_log2 = scale * 1.4426950408889634f;
