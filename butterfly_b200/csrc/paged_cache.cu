@@ -14,7 +14,6 @@ namespace bna {
 namespace {
 
 constexpr int kMaxRequests = 4096;  // three prefix sums and the lengths of a call: 64 KB of shared memory
-constexpr int kReserveThreads = 256;
 constexpr int kReserveCtas = 148;
 
 struct ReserveArgs {
@@ -31,6 +30,7 @@ struct ReserveArgs {
   int32_t* positions;
   int64_t num_tokens;
   int B, width, num_pages, page_size;
+  int vector_out;  // slots and positions are 16-byte aligned
 };
 
 // First index b in [0, n) with c[b] > x (c non-decreasing), n if there is none.
@@ -73,14 +73,18 @@ __device__ __forceinline__ Ask ask_of(int len, int add, int capacity, int page_s
 // are written only where pages stay given back (then none is taken from below them).
 // The j-th page given back lies j below the new top of the stack and the i-th page taken
 // comes from i below it, so a call followed by its opposite restores the stack.
-// Bound by launch and dependent-read latency: the largest calls move about 1 MB.
-__global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveArgs a) {
+// Bound by launch and dependent-read latency: the largest calls move about 1 MB.  A thread takes K
+// tokens in a row: one where the tokens are few, four (one search and one page for most of
+// them) where there are many.
+template <int K>
+__global__ void __launch_bounds__(1024) reserve_kernel(const ReserveArgs a) {
   extern __shared__ int32_t sm[];
   int32_t* cum_add = sm;            // inclusive prefix sums (capped at INT_MAX)
   int32_t* cum_need = sm + a.B;
   int32_t* cum_back = sm + 2 * a.B;
   int32_t* lens = sm + 3 * a.B;     // cut to the table, so that no later index leaves a row
-  __shared__ int64_t warp_sums[3][kReserveThreads / 32];
+  __shared__ int64_t warp_sums[3][32];
+  const int threads = blockDim.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int capacity = (int)min((int64_t)a.width * a.page_size, (int64_t)INT_MAX);
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveA
   const int n = min(max(a.num_free[0], 0), a.num_pages);
 
   // each thread sums a run of requests, then the runs are scanned
-  const int per = (a.B + kReserveThreads - 1) / kReserveThreads;
+  const int per = (a.B + threads - 1) / threads;
   const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
   int64_t sum[3] = {0, 0, 0};
   for (int b = b0; b < b1; ++b) {
@@ -148,21 +152,54 @@ __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveA
     const int tokens = cum_add[b] - before(cum_add, b);
     return tokens > 0 && (int64_t)lens[b] + tokens <= capacity && (b < served || cum_need[b] == before(cum_need, b));
   };
-  const int64_t stride = (int64_t)gridDim.x * kReserveThreads, tid = (int64_t)blockIdx.x * kReserveThreads + threadIdx.x;
+  const int64_t stride = (int64_t)gridDim.x * threads, tid = (int64_t)blockIdx.x * threads + threadIdx.x;
 
-  // slots and positions of the added tokens, packed request by request
-  for (int64_t t = tid; t < a.num_tokens; t += stride) {
-    int64_t slot = -1;
-    int pos = -1;
-    const int b = upper_bound(cum_add, a.B, t);
-    if (b < a.B && granted(b)) {
-      pos = lens[b] + (int)(t - before(cum_add, b));
-      const int pi = (unsigned)pos / (unsigned)a.page_size, have = pages_of(lens[b], a.page_size);
-      const int page = pi < have ? a.table[b * a.table_stride + pi] : from_top((int64_t)before(cum_need, b) + pi - have);
-      slot = page < 0 ? -1 : (int64_t)page * a.page_size + (pos - pi * a.page_size);
+  // slots and positions of the added tokens, packed request by request, and the table entries
+  // of the pages taken, each written with the page's first token
+  const int64_t limit = max(a.num_tokens, (int64_t)cum_add[a.B - 1]);
+  for (int64_t t0 = tid * K; t0 < limit; t0 += stride * K) {
+    int b = upper_bound(cum_add, a.B, t0);
+    int64_t slot[K];
+    int pos[K], at_b = -1, at_page = -1, page = -1, have = 0, first = 0;
+    bool ok = false;
+#pragma unroll
+    for (int x = 0; x < K; ++x) {
+      const int64_t t = t0 + x;
+      slot[x] = -1;
+      pos[x] = -1;
+      while (b < a.B && cum_add[b] <= t) ++b;
+      if (b >= a.B) continue;
+      if (b != at_b) {
+        at_b = b;
+        at_page = -1;
+        ok = granted(b);
+        have = pages_of(lens[b], a.page_size);
+        first = before(cum_need, b);
+      }
+      if (!ok) continue;
+      pos[x] = lens[b] + (int)(t - before(cum_add, b));
+      const int pi = (unsigned)pos[x] / (unsigned)a.page_size, off = pos[x] - pi * a.page_size;
+      if (pi != at_page) {
+        at_page = pi;
+        page = pi < have ? a.table[b * a.table_stride + pi] : from_top((int64_t)first + pi - have);
+        if (pi >= have && off == 0) a.table[b * a.table_stride + pi] = page;
+      }
+      slot[x] = page < 0 ? -1 : (int64_t)page * a.page_size + off;
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
+    if (K == 4 && a.vector_out && t0 + K <= a.num_tokens) {
+      st_128(a.slots + t0, make_uint4((uint32_t)slot[0], (uint32_t)(slot[0] >> 32), (uint32_t)slot[1 % K],
+                                      (uint32_t)(slot[1 % K] >> 32)));
+      st_128(a.slots + t0 + 2, make_uint4((uint32_t)slot[2 % K], (uint32_t)(slot[2 % K] >> 32), (uint32_t)slot[3 % K],
+                                          (uint32_t)(slot[3 % K] >> 32)));
+      st_128(a.positions + t0, make_uint4(pos[0], pos[1 % K], pos[2 % K], pos[3 % K]));
+    } else {
+#pragma unroll
+      for (int x = 0; x < K; ++x)
+        if (t0 + x < a.num_tokens) {
+          a.slots[t0 + x] = slot[x];
+          a.positions[t0 + x] = pos[x];
+        }
+    }
   }
   for (int64_t b = tid; b < a.B; b += stride) {
     const bool ok = granted((int)b);
@@ -171,11 +208,6 @@ __global__ void __launch_bounds__(kReserveThreads) reserve_kernel(const ReserveA
     a.granted[b] = ok;
   }
   if (tid == 0) a.num_free_out[0] = (int)min(top - A, (int64_t)a.num_pages);
-  // table entries of the pages taken
-  for (int64_t i = tid; i < A; i += stride) {
-    const int b = upper_bound(cum_need, a.B, i);
-    a.table[b * a.table_stride + pages_of(lens[b], a.page_size) + (i - before(cum_need, b))] = from_top(i);
-  }
   // stack entries of the pages given back and not taken again, from index n up
   for (int64_t i = n + tid; i < top - A && i < a.num_pages; i += stride) a.free_pages[i] = from_top(top - 1 - i);
 }
@@ -251,17 +283,26 @@ int launch_reserve(const int32_t* lens, const int32_t* add, int B, int32_t* tabl
                    int32_t* num_free_out, uint8_t* granted, int64_t* slots, int32_t* positions, int64_t num_tokens,
                    cudaStream_t s) {
   if (B > kMaxRequests) return fail(BNA_UNSUPPORTED, "paged_reserve: at most 4096 requests per call");
+  const bool aligned = ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions)) & 15) == 0;
   ReserveArgs a{lens, add, table, table_stride, free_pages, num_free, lens_out, num_free_out, granted, slots, positions,
-                num_tokens, B, width, num_pages, page_size};
+                num_tokens, B, width, num_pages, page_size, aligned};
+  // Four tokens a thread once one would need more than a CTA of 256 on every SM.  Small CTAs on many
+  // SMs, as a token's searches keep the issue slots busy (33 CTAs of 1,024 threads took 6 us
+  // over 131,072 tokens), unless the scan over the requests is the longer part.
+  const int k = num_tokens > 256 * kReserveCtas ? 4 : 1;
+  auto kern = k == 4 ? reserve_kernel<4> : reserve_kernel<1>;
+  const unsigned threads = B > 1024 ? 1024 : 256;
   const int smem = 4 * B * 4;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMaxRequests * 4);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMaxRequests * 4);
     if (e != cudaSuccess) return check_cuda(e, "paged_reserve attributes");
   }
-  // enough CTAs for the tokens and for every page the requests could give back
-  const int64_t items = num_tokens + std::min((int64_t)num_pages, (int64_t)B * width);
-  const unsigned grid = (unsigned)std::min<int64_t>(kReserveCtas, (items + 2 * kReserveThreads - 1) / (2 * kReserveThreads));
-  return launch_dependent(reserve_kernel, a, grid, kReserveThreads, smem, s, "paged_reserve launch");
+  // enough CTAs for the tokens and for every page the requests could give back (these in several
+  // rounds: they are rarely many)
+  const int64_t given = std::min((int64_t)num_pages, (int64_t)B * width) / 2;
+  const int64_t items = std::max((num_tokens + k - 1) / k, std::max(given, (int64_t)B));
+  const unsigned grid = (unsigned)std::min<int64_t>(kReserveCtas, (items + threads - 1) / threads);
+  return launch_dependent(kern, a, grid, threads, smem, s, "paged_reserve launch");
 }
 
 int launch_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* kp, bna_tensor4* vp,

@@ -407,6 +407,24 @@ def test_reserve_follows_the_model(B, pages, page, width):
     assert sorted(owned) == list(range(pages))  # no page lost, none owned twice
 
 
+def test_reserve_many_tokens():
+    # prompts of all lengths, some ending inside a page, and more tokens than entries of one CTA
+    rng = np.random.default_rng(3)
+    for B, extra, start in ((70, 0, 0), (3, 5, 37), (2000, 3, 1)):
+        add = rng.integers(0, 160000 // B, B).tolist()
+        add[1] = 0
+        pages = sum(_pages(a + start, 16) for a in add) - 2
+        cache = bb.PagedKVCache(num_layers=1, num_pages=pages + B, page_size=16, num_kv_heads=1, head_dim=64, max_requests=B,
+                                max_tokens_per_request=max(add) + 64)
+        model = Model(B, pages + B, -(-(max(add) + 64) // 16), 16)
+        if start:
+            first = [start] * B
+            _same(cache, model, cache.reserve(first), model.reserve(first), 0)
+        want = model.reserve(add)
+        r = cache.reserve(torch.tensor(add, dtype=torch.int32, device=DEV), sum(add) + extra)
+        _same(cache, model, r, want, extra)
+
+
 def test_reserve_then_rollback_is_the_identity():
     cache = bb.PagedKVCache(num_layers=1, num_pages=64, page_size=16, num_kv_heads=1, head_dim=64, max_requests=4,
                             max_tokens_per_request=512)
