@@ -74,6 +74,16 @@ at::Tensor empty(const at::Tensor& like, at::IntArrayRef size, at::ScalarType ty
   return at::empty(size, like.options().dtype(type));
 }
 
+// n elements of `type` at byte `offset` of a byte buffer, sharing its storage (a fraction of the
+// time of an allocation).
+at::Tensor part(const at::Tensor& bytes, int64_t offset, int64_t n, at::ScalarType type) {
+  auto impl = c10::make_intrusive<at::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(),
+                                                  caffe2::TypeMeta::fromScalarType(type));
+  impl->set_sizes_contiguous({n});
+  impl->set_storage_offset(bytes.storage_offset() + offset / (int64_t)c10::elementSize(type));
+  return at::Tensor(std::move(impl));
+}
+
 PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
   PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
   if (!r) throw python_error();
@@ -112,8 +122,11 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
        "lens and add must have block_table's rows, num_free one entry, num_tokens must be >= 0");
   need(B <= INT32_MAX && width <= INT32_MAX && free_pages.size(0) <= INT32_MAX && page_size >= 0 && page_size <= INT32_MAX,
        "paged_reserve: sizes beyond 32 bits");
-  at::Tensor out = empty(lens, {B}, at::kInt), left = empty(lens, {1}, at::kInt), slots = empty(lens, {tokens}, at::kLong),
-             positions = empty(lens, {tokens}, at::kInt), granted = empty(lens, {B}, at::kBool);
+  // one allocation for what lives on as the cache's state, one for the step's tokens
+  const int64_t round = (tokens + 1) / 2 * 16;  // slots, to a multiple of 16 bytes
+  const at::Tensor state = empty(lens, {4 * B + 4 + B}, at::kByte), step = empty(lens, {round + 4 * tokens}, at::kByte);
+  at::Tensor out = part(state, 0, B, at::kInt), left = part(state, 4 * B, 1, at::kInt), granted = part(state, 4 * B + 4, B, at::kBool),
+             slots = part(step, 0, tokens, at::kLong), positions = part(step, round, tokens, at::kInt);
   const int st = g_reserve(static_cast<const int32_t*>(lens.data_ptr()), static_cast<const int32_t*>(add.data_ptr()), (int32_t)B,
                            static_cast<int32_t*>(table.data_ptr()), B > 1 ? table.stride(0) : width, (int32_t)width,
                            static_cast<int32_t*>(free_pages.data_ptr()), (int32_t)free_pages.size(0),
