@@ -44,7 +44,8 @@ namespace {
 using namespace sm100;
 
 constexpr int kGran = 16;       // keys of a granule
-constexpr int kMaxCtas = 160;   // workspace parts are sized for this many CTAs
+constexpr int kMaxSms = 160;    // the workspace is sized for this many, with two CTAs each
+constexpr int kMaxCtas = 2 * kMaxSms;
 constexpr int kRows = 16;       // query heads of one KV head served together
 constexpr int kMinPart = 16;    // granules a CTA gets at least of an even cut (fewer CTAs otherwise)
 constexpr int kFan = 16;        // parts of a pair joined at a time; up to kFan + 4 where that is all
@@ -93,14 +94,17 @@ struct Seg {
 
 template <int DH>
 struct Layout {
-  // Consumer warps.  head_dim 256: four, as the output and score registers of eight would not
-  // fit beside each other.
-  static constexpr int kCons = DH == 256 ? 4 : 8;
+  // CTAs of an SM, and consumer warps of a CTA.  head_dim 64: two CTAs of four warps, so that the end
+  // of one's pair overlaps the other's reads (96 x 3 pairs of up to 1,000 keys: 22 us with
+  // one of eight).  head_dim 256: four warps, as the output and score registers of eight
+  // would not fit beside each other.
+  static constexpr int kCtas = DH == 64 ? 2 : 1;
+  static constexpr int kCons = DH == 128 ? 8 : 4;
   static constexpr int kThreads = 32 * (kCons + 1);      // and the producer
   static constexpr int kSlotBytes = 2 * kGran * DH * 2;  // keys, then values
-  // 128 KB of ring keeps the memory busy; with 192 KB requests queue and the SMs that a loaded
+  // 128 KB of ring an SM keeps the memory busy; with 192 KB requests queue and the SMs that a loaded
   // GPU serves last fall further behind (640 against 615 us at 64 x 65,536 tokens).
-  static constexpr int kSlots = 128 * 1024 / kSlotBytes;
+  static constexpr int kSlots = 128 * 1024 / kCtas / kSlotBytes;
   // Every consumer warp has a ring of its own (slot = use % kRing * kCons + warp): a barrier's parity
   // tells a wait that is one use ahead nothing about the use before, so a slot has to stay
   // with one warp.  Granule i of a segment goes to warp i % kCons, whatever came before it,
@@ -116,7 +120,7 @@ struct Layout {
   static constexpr int kMergeFloats = kCons * kRows * (32 + 8), kJoinFloats = 32 * kRows + 4 * 32 * kCons;
   static constexpr int kBufBytes = 4 * (kMergeFloats > kJoinFloats ? kMergeFloats : kJoinFloats);
   static constexpr int kStage = kBuf + 2 * kBufBytes;  // (segments alternate between two buffers)
-  static constexpr int kHalf = 20 * 1024;  // parts of a join arrive in two halves of this size
+  static constexpr int kHalf = (kCtas == 2 ? 8 : 20) * 1024;  // parts of a join arrive in two halves of this size
   static constexpr int kMl = kStage + 2 * kHalf;
   static constexpr int kBars = kMl + 2 * kCons * kRows * 8;
   static constexpr int kNumBars = 2 * kSlots + 6;
@@ -125,7 +129,7 @@ struct Layout {
   static constexpr int kLens = (kFlags + 16 + 15) / 16 * 16;  // the first kKeepLens requests' lengths
   static constexpr int kBytes = kLens + 4 * kKeepLens;
   static constexpr int kAlloc = kBytes + 1024;  // the base is aligned to 1024 (swizzle atom)
-  static_assert(kAlloc <= 232448, "shared memory of a CTA");
+  static_assert(kCtas * (kAlloc + 1024) <= 233472, "shared memory of an SM");
 };
 
 __device__ __forceinline__ int clamp_len(const PagedArgs& a, int len) {
@@ -196,7 +200,7 @@ __device__ __forceinline__ bool cons_any(bool bad) {
 // as much error to the output as its final rounding does); with at most 8 heads lo rides in rows
 // that the MMA computes anyway, with more it costs a second MMA, which the memory hides.
 template <typename T, int DH, bool WIDE>
-__global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
+__global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     paged_decode_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const PagedArgs a) {
   using Lay = Layout<DH>;
   constexpr int kCons = Lay::kCons;
@@ -280,7 +284,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, 1)
     // and their join, about 10 us, in which the SM could have read kCut granules.  Measured
     // whole / cut: 96 x 3 pairs of up to 1,000 keys (head_dim 64) 17 / 29 us; 256 pairs of 2,048
     // keys (head_dim 128) 56 / 50 us.
-    constexpr int kCut = 8192 / DH;
+    constexpr int kCut = 8192 / DH / Lay::kCtas;
     const int64_t share = quot(U, grid), even = max(share, (int64_t)kMinPart) + kCut;
     const bool whole = (N <= grid ? longest : share + longest / 2) <= even;
     // items: the pairs, or the stretches of C CTAs
@@ -885,7 +889,7 @@ int sm_count() {
 }
 
 template <typename T, int DH, bool WIDE>
-int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, unsigned grid, cudaStream_t s) {
+int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, double most, cudaStream_t s) {
   auto kern = paged_decode_kernel<T, DH, WIDE>;
   static std::atomic<uint64_t> ready{0};  // devices (bits) whose kernel has its shared memory allowed
   int dev = 0;
@@ -896,7 +900,7 @@ int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs&
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3((unsigned)std::min((double)std::min(sm_count(), kMaxSms) * Layout<DH>::kCtas, most));
   cfg.blockDim = dim3(Layout<DH>::kThreads);
   cfg.dynamicSmemBytes = Layout<DH>::kAlloc;
   cfg.stream = s;
@@ -945,10 +949,10 @@ int launch_paged_decode(const bna_tensor4* q, bna_tensor4* kp, bna_tensor4* vp, 
   // no more CTAs than there could be pairs, or stretches of an even cut
   const int64_t keys = window > 0 ? std::min((int64_t)width * a.page_size, (int64_t)window + 2 * kGran) : (int64_t)width * a.page_size;
   const double pairs = (double)a.B * a.Hkv * a.chunks, stretches = std::ceil(pairs * (double)((keys + kGran - 1) / kGran) / kMinPart);
-  const unsigned grid = (unsigned)std::min((double)std::min(sm_count(), kMaxCtas), std::max(pairs, stretches));
+  const double most = std::max(pairs, stretches);
   const bool bf = dtype == BNA_BF16, wide = a.chunk_rows > 8;
 #define BNA_PAGED(T_, DH_) \
-  return wide ? launch_decode<T_, DH_, true>(mk, mv, a, grid, s) : launch_decode<T_, DH_, false>(mk, mv, a, grid, s)
+  return wide ? launch_decode<T_, DH_, true>(mk, mv, a, most, s) : launch_decode<T_, DH_, false>(mk, mv, a, most, s)
   switch (q->size[3]) {
     case 64:
       if (bf) BNA_PAGED(__nv_bfloat16, 64);
