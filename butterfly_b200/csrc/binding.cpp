@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -112,6 +113,7 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor &lens = tensor(a[0], "lens"), &add = tensor(a[1], "add"), &table = tensor(a[2], "block_table"),
                    &free_pages = tensor(a[3], "free_pages"), &num_free = tensor(a[4], "num_free");
   need_cuda({&lens, &add, &table, &free_pages, &num_free});
+  const c10::DeviceGuard guard(lens.device());
   need_ints(lens, 1, "lens");
   need_ints(add, 1, "add");
   need_ints(table, 2, "block_table");
@@ -146,6 +148,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &kp = tensor(a[2], "k_pages"), &vp = tensor(a[3], "v_pages"),
                    &slots = tensor(a[4], "slot_map");
   need_cuda({&k, &v, &kp, &vp, &slots});
+  const c10::DeviceGuard guard(k.device());
   need(k.dim() == 3 && v.dim() == 3, "k and v must be [tokens, Hkv, dh]");
   const auto dt = k.scalar_type();
   need(v.scalar_type() == dt && kp.scalar_type() == dt && vp.scalar_type() == dt, "k, v and the pools must have one dtype");
@@ -171,6 +174,7 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor &q = tensor(a[0], "q"), &kp = tensor(a[1], "k_pages"), &vp = tensor(a[2], "v_pages"),
                    &table = tensor(a[3], "block_table"), &lens = tensor(a[4], "lens"), &ws = tensor(a[11], "workspace");
   need_cuda({&q, &kp, &vp, &table, &lens, &ws});
+  const c10::DeviceGuard guard(q.device());
   const bna_tensor4 tq = view4(q, "q");
   bna_tensor4 tkp = view4(kp, "k_pages"), tvp = view4(vp, "v_pages");
   const int64_t B = q.size(0), Hq = q.size(1), Tq = q.size(2), dh = q.size(3);

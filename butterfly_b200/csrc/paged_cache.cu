@@ -73,7 +73,8 @@ __device__ __forceinline__ Ask ask_of(int len, int add, int capacity, int page_s
 // are written only where pages stay given back (then none is taken from below them).
 // The j-th page given back lies j below the new top of the stack and the i-th page taken
 // comes from i below it, so a call followed by its opposite restores the stack.
-// Bound by launch and dependent-read latency: the largest calls move about 1 MB.  A thread takes K
+// Bound by launch and dependent-read latency: the largest calls move about 1.6 MB (1,000 requests
+// with 131,072 prompt tokens 9.0 us, one request 3.0 us on the GPU).  A thread takes K
 // tokens in a row: one where the tokens are few, four (one search and one page for most of
 // them) where there are many.
 template <int K>
@@ -226,7 +227,8 @@ struct PagedAppendArgs {
 
 // A thread moves one 16-byte vector of the keys and of the values of N (token, head) rows that lie a
 // block apart, with all 2 N loads in flight before the first store (they do not wait for the
-// slots).  Bound by HBM: each row is read and written once.
+// slots).  Bound by HBM: each row is read and written once (131,072 tokens x 2 heads of 128:
+// 42.0 us = 6.4 TB/s, the rate of a plain copy; one row a thread 53 us).
 template <int N>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppendArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
