@@ -9,7 +9,7 @@
 // 2 G FLOP per byte, far below the tensor cores' balance, so the kernel is bound by HBM and is
 // built to keep its reads in flight:
 //   * The keys of a pair (request, KV head) come in granules of 16.  One persistent CTA per SM
-//     takes either whole pairs, one after the other as they are claimed, or, where single pairs
+//     takes either whole pairs, as they are claimed (in turn, if all are short), or, where single pairs
 //     are long beside an even share, an equal stretch of the line of all granules: one long
 //     request spreads over all SMs, and only its parts have to be joined.
 //   * The producer warp looks the pages up and issues one TMA tile copy for a granule's keys and
@@ -350,7 +350,8 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     bool first = true, pending = true;
     // A claim comes with every CTA and with every pair claimed: the last of all finds nothing and
     // leaves the count as the next call needs it.
-    const int64_t last_claim = (whole && C > grid ? C : grid) - 1;
+    const bool claiming = whole && C > grid && longest > kCons;
+    const int64_t last_claim = (claiming ? C : grid) - 1;
     auto answer = [&]() -> int64_t {
       const int c = __shfl_sync(0xffffffffu, claim, 0);
       if (c == last_claim && lane == 0) *claims = 0;
@@ -360,11 +361,14 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     auto take = [&](Next& x) -> bool {
       if (cur >= end) {
         if (!first) {
-          item = pending ? answer() : C;
-          if (!whole) item = C;
-          if (item < C) {
-            if (lane == 0) claim = atomicAdd(claims, 1);
-            pending = true;
+          if (!claiming) {
+            item = whole ? item + grid : C;
+          } else {
+            item = answer();
+            if (item < C) {
+              if (lane == 0) claim = atomicAdd(claims, 1);
+              pending = true;
+            }
           }
         }
         first = false;
@@ -658,14 +662,10 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     __syncwarp();
     if (lane == 0) mbar_arrive(seg_empty + si);  // the descriptor and Q have been read
 
-    // Join the warps: each leaves (m, l) and its outputs, which are scaled to the common maximum as
-    // they are summed.  Two buffers: a warp may start on the next segment before all are done.
-    float2* ml = reinterpret_cast<float2*>(sm + Lay::kMl) + si * kCons * kRows;
 #pragma unroll
     for (int x = 0; x < kRowSets; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      if (tig == 0) ml[warp * kRows + gid + 8 * x] = make_float2(m[x], l[x]);
     }
     if (!WIDE) {
 #pragma unroll
@@ -674,6 +674,30 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
         o[j][1] += o[j][3];
       }
     }
+    if (s.n == 1 && s.slot < 0) {  // a pair of one granule: the first warp has all of it
+      if (cons_any<kNT>(bad)) return;
+#pragma unroll
+      for (int x = 0; x < kRowSets; ++x) {
+        const int r = gid + 8 * x;
+        if (warp == 0 && r < s.rows) {
+          const int64_t hq = s.h * a.G + s.r0 + r;
+          uint8_t* dst = a.out + 2 * (s.b * a.o_b + hq * a.o_h + 2 * tig);
+          const float f = l[x] == 0.f ? 0.f : 1.f / l[x];
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            *reinterpret_cast<uint32_t*>(dst + 16 * j) = ElemTraits<T>::pack2(o[j][2 * x] * f, o[j][2 * x + 1] * f);
+          if (a.lse && tig == 0) a.lse[s.b * a.ls_b + hq * a.ls_h] = lse_of(m[x], l[x]);
+        }
+      }
+      continue;
+    }
+
+    // Join the warps: each leaves (m, l) and its outputs, which are scaled to the common maximum as
+    // they are summed.  Two buffers: a warp may start on the next segment before all are done.
+    float2* ml = reinterpret_cast<float2*>(sm + Lay::kMl) + si * kCons * kRows;
+#pragma unroll
+    for (int x = 0; x < kRowSets; ++x)
+      if (tig == 0) ml[warp * kRows + gid + 8 * x] = make_float2(m[x], l[x]);
     // columns joined at a time: what the buffer holds of s.rows rows (rows padded by 8 floats
     // to spread the stores over the banks)
     const int shift = s.rows <= 4 ? (DH < 128 ? 6 : 7) : s.rows <= 8 ? 6 : 5, cw = 1 << shift;
