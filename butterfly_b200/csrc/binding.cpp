@@ -129,6 +129,7 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor state = empty(lens, {4 * B + 4 + B}, at::kByte), step = empty(lens, {round + 4 * tokens}, at::kByte);
   at::Tensor out = part(state, 0, B, at::kInt), left = part(state, 4 * B, 1, at::kInt), granted = part(state, 4 * B + 4, B, at::kBool),
              slots = part(step, 0, tokens, at::kLong), positions = part(step, round, tokens, at::kInt);
+  if (B == 0) left.copy_(num_free);  // (no request: the call writes nothing)
   const int st = g_reserve(static_cast<const int32_t*>(lens.data_ptr()), static_cast<const int32_t*>(add.data_ptr()), (int32_t)B,
                            static_cast<int32_t*>(table.data_ptr()), B > 1 ? table.stride(0) : width, (int32_t)width,
                            static_cast<int32_t*>(free_pages.data_ptr()), (int32_t)free_pages.size(0),

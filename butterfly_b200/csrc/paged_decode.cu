@@ -221,17 +221,13 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
   volatile int* last_flag = abort_flag + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < Lay::kSlots; ++i) {
-      mbar_init(full + i, 1);
-      mbar_init(empty + i, 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(seg_full + i, 1);
-      mbar_init(seg_empty + i, kCons);
-      mbar_init(stage_full + i, 1);
-    }
+  // full and empty (one arrival), seg_full (one), seg_empty (each consumer warp), stage_full (one)
+  for (int i = threadIdx.x; i < Lay::kNumBars; i += Lay::kThreads) {
+    const int k = i - 2 * Lay::kSlots;
+    mbar_init(full + i, k == 2 || k == 3 ? kCons : 1);
     fence_mbar_init();
+  }
+  if (threadIdx.x == 0) {
     *abort_flag = 0;
     prefetch_tmap(&mk);
     prefetch_tmap(&mv);
@@ -290,8 +286,8 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     // whole / cut: 96 x 3 pairs of up to 1,000 keys (head_dim 64) 15 / 24 us; at head_dim 128, 256
     // pairs of 2,048 keys 47 / 50 us and 16 pairs of 2,048 keys 18 / 11 us.
     constexpr int kCut = 8192 / DH / Lay::kCtas;
-    const int64_t share = quot(U, grid), even = max(share, (int64_t)kMinPart) + kCut;
-    const bool whole = (N <= grid ? longest : share + longest / 2) <= even;
+    const float share = (float)U * __frcp_rn((float)grid), even = fmaxf(share, (float)kMinPart) + (float)kCut;
+    const bool whole = (N <= grid ? (float)longest : share + 0.5f * (float)longest) <= even;
     // items: the pairs, or the stretches of C CTAs
     const int64_t C = whole ? N : max((int64_t)1, min(grid, quot(U + kMinPart - 1, kMinPart)));
     Cut cut;

@@ -371,7 +371,8 @@ BNA_API int bna_prefill_attention_static_scratch(const bna_tensor4* q, const bna
  * need pages are refused too once the pages asked for so far exceed the stack.  slot_map / positions [num_tokens] hold the added tokens
  * of request 0, then 1, ... (-1 past the last).  lens and num_free are read only; lens_out
  * [requests] and num_free_out [1] are written (not in place).  block_table and free_pages are
- * updated in place; entries past a request's pages keep their old values.  requests <= 4096. */
+ * updated in place; entries past a request's pages keep their old values.  requests <= 4096;
+ * with none nothing is written. */
 BNA_API int bna_paged_reserve(const int32_t* lens, const int32_t* add, int32_t requests, int32_t* block_table,
                               int64_t table_stride, int32_t table_width, int32_t* free_pages, int32_t num_pages,
                               const int32_t* num_free, int32_t page_size, int32_t* lens_out, int32_t* num_free_out,

@@ -435,6 +435,13 @@ def test_reserve_then_rollback_is_the_identity():
     assert all(torch.equal(a, b) for a, b in zip(before, (cache.lens, cache.num_free, cache.free_pages)))
 
 
+def test_reserve_without_requests():
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    free = torch.arange(5, dtype=torch.int32, device=DEV)
+    r = bb.paged_reserve(none, none, torch.empty(0, 3, dtype=torch.int32, device=DEV), free, free[4:], page_size=16, num_tokens=0)
+    assert r.num_free.tolist() == [4] and all(x.numel() == 0 for x in (r.lens, r.slot_map, r.positions, r.granted))
+
+
 def test_reserve_does_not_change_its_inputs_and_repeats():
     lens = torch.tensor([5, 20], dtype=torch.int32, device=DEV)
     add = torch.tensor([40, -20], dtype=torch.int32, device=DEV)
