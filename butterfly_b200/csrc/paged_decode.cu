@@ -20,7 +20,7 @@
 //   * Of a pair cut by CTA boundaries each CTA leaves a part in the workspace, and the CTA that
 //     arrives last joins the parts in their order on the line.  Every sum has its order fixed by
 //     the lengths and the grid, whichever CTA runs when: equal calls give equal bits.
-// Measured (GPU time, bf16, 8 / 2 heads of 128): 64 x 65,536 tokens 615 us = 7.0 TB/s (a copy reaches
+// Measured (GPU time, bf16, 8 / 2 heads of 128): 64 x 65,536 tokens 610 us = 7.0 TB/s (a copy reaches
 // 6.45 TB/s here), DRAM reads equal to the keys and values, tensor pipe 17% busy; one request of
 // 131,072 tokens 34.5 us = 3.9 TB/s: 4 us until the first granule, 19 to 22 us of reads, 7 us from
 // the last CTA's arrival through two rounds of joins; four requests of 37 to 513 tokens 9.0 us,
