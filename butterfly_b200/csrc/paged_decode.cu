@@ -8,17 +8,17 @@
 // Each key and value is read once and serves the G = Hq / Hkv query heads of its KV head:
 // 2 G FLOP per byte, far below the tensor cores' balance, so the kernel is bound by HBM and is
 // built to keep its reads in flight:
-//   * The keys of a pair (request, KV head) come in granules of 16.  One persistent CTA per SM
-//     takes either whole pairs, as they are claimed (in turn, if all are short), or, where single pairs
+//   * The keys of a pair (request, KV head) come in granules of 16.  One persistent CTA per SM (two
+//     at head_dim 64) takes either whole pairs, as they are claimed (in turn, if all are short), or, where single pairs
 //     are long beside an even share, an equal stretch of the line of all granules: one long
 //     request spreads over all SMs, and only its parts have to be joined.
 //   * The producer warp looks the pages up and issues one TMA tile copy for a granule's keys and
-//     one for its values into a ring of granule slots (128 KB); it runs ahead into the next
-//     pairs.
-//   * Eight consumer warps (four at head_dim 256) take the granules in turn, each with its own m,
+//     one for its values into a ring of granule slots (128 KB an SM); it runs ahead into the
+//     next pairs.
+//   * Eight consumer warps (four at head_dim 64 and 256) take the granules in turn, each with its own m,
 //     l and o in registers: no barrier between warps until a pair, or a CTA's part of it, ends.
 //   * Of a pair cut by CTA boundaries each CTA leaves a part in the workspace, and the CTA that
-//     arrives last joins the parts in their order on the line.  Every sum has its order fixed by
+//     arrives last joins the parts in their order on the line (of many, groups first).  Every sum has its order fixed by
 //     the lengths and the grid, whichever CTA runs when: equal calls give equal bits.
 // Measured (GPU time, bf16, 8 / 2 heads of 128): 64 x 65,536 tokens 610 us = 7.0 TB/s (a copy reaches
 // 6.45 TB/s here), DRAM reads equal to the keys and values, tensor pipe 17% busy; one request of
@@ -319,12 +319,14 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
       }
     };
     if (blockIdx.x < C) load_window();
-    // lane of the request, in the window moved to it, that holds place `at` of the line
+    // lane of the request, in the window moved to it, that holds place `at` of the line (-1: none,
+    // if lengths changed under the call)
     auto find = [&](int64_t at) -> int {
       unsigned past;
       while (!(past = __ballot_sync(0xffffffffu, before + incl_w > at))) {
         before += __shfl_sync(0xffffffffu, incl_w, 31);
         wb += 32;
+        if (wb >= a.B) return -1;
         load_window();
       }
       return __ffs(past) - 1;
@@ -372,7 +374,9 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
         cur = whole ? item : cut.start(item);
         end = whole ? item + 1 : cut.start(item + 1);
       }
-      const int f = find(cur), len = __shfl_sync(0xffffffffu, len_w, f), nt = granules_of(a, len);
+      const int f = find(cur);
+      if (f < 0) return false;
+      const int len = __shfl_sync(0xffffffffu, len_w, f), nt = granules_of(a, len);
       const int64_t local = cur - before - __shfl_sync(0xffffffffu, incl_w - mine_w, f);
       const int pair = whole ? (int)local : (int)quot(local, nt), t0 = whole ? 0 : (int)(local - (int64_t)pair * nt);
       Seg& s = x.s;
