@@ -97,8 +97,8 @@ def decode_workspace(device: torch.device | str | int = "cuda") -> torch.Tensor:
 
 
 def _workspace_for(x: torch.Tensor, stream: int) -> torch.Tensor:
-    """The workspace kept for a stream.  A capture gets its own (zeroed inside the graph): its
-    replays may run beside later calls on the stream."""
+    """The workspace kept for a stream.  A call under capture gets its own (zeroed inside the graph;
+    pass one to share it): its replays may run beside later calls on the stream."""
     if not x.is_cuda:
         raise ValueError("butterfly_b200 kernels run on CUDA tensors only (no CPU path)")
     if torch.cuda.is_current_stream_capturing():
@@ -137,7 +137,9 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 class PagedKVCache:
     """Pools of ``num_layers`` layers under one set of block tables, lengths and free pages.
 
-    The requests are the ``max_requests`` rows of the tables; a row of length 0 is vacant."""
+    The requests are the ``max_requests`` rows of the tables; a row of length 0 is vacant.  The
+    attention's workspace is the cache's own, in graph captures too: calls on one cache (and
+    replays of graphs that hold them) follow one another."""
 
     def __init__(self, *, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  max_requests: int, max_tokens_per_request: int, dtype: torch.dtype = torch.bfloat16,
@@ -152,6 +154,7 @@ class PagedKVCache:
         self.lens = torch.zeros(int(max_requests), dtype=torch.int32, device=device)
         self.free_pages = torch.arange(int(num_pages) - 1, -1, -1, dtype=torch.int32, device=device)
         self.num_free = torch.full((1,), int(num_pages), dtype=torch.int32, device=device)
+        self.workspace = decode_workspace(device)
 
     @property
     def max_requests(self) -> int:
@@ -195,7 +198,7 @@ class PagedKVCache:
         ``paged_decode_attention``)."""
         return paged_decode_attention(q, self.k_pages[layer], self.v_pages[layer], self.block_table, self.lens,
                                       k_new=k_new, v_new=v_new, active=active, window=window, scale=scale,
-                                      return_lse=return_lse)
+                                      return_lse=return_lse, workspace=self.workspace)
 
 
 __all__ = ["PagedKVCache", "PagedReservation", "RELEASE", "decode_workspace", "paged_append", "paged_decode_attention", "paged_reserve"]

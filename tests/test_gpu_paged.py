@@ -283,6 +283,34 @@ def test_graph_capture_replays():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_cache_step_in_a_graph():
+    # reservation and both layers' attention captured; each replay starts from the captured lengths
+    cache = bb.PagedKVCache(num_layers=2, num_pages=40, page_size=16, num_kv_heads=2, head_dim=128, max_requests=3,
+                            max_tokens_per_request=256)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    r = cache.reserve([30, 200, 16])
+    for layer in range(2):
+        cache.append(layer, rnd(246, 2, 128), rnd(246, 2, 128), r.slot_map)
+    q, kn, vn, add = rnd(3, 8, 1, 128), rnd(3, 2, 1, 128), rnd(3, 2, 1, 128), torch.ones(3, dtype=torch.int32, device=DEV)
+    lens, num_free = cache.lens, cache.num_free
+
+    def step():
+        cache.lens, cache.num_free = lens, num_free
+        r = cache.reserve(add, 3)
+        return [cache.attend(layer, q, k_new=kn, v_new=vn, active=r.granted) for layer in range(2)] + [r.lens, r.slot_map]
+
+    want = [x.clone() for x in step()]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[2].tolist() == [31, 201, 17]
+
+
 def test_empty_batch():
     c = Case([5], 8, 2, seed=1)
     out, lse = bb.paged_decode_attention(c.q[:0], c.kp, c.vp, c.table[:0], c.lens[:0], return_lse=True)
