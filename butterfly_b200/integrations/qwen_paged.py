@@ -105,16 +105,18 @@ class PagedQwenDecoder:
     @torch.no_grad()
     def step(self, tokens: torch.Tensor):
         """One token for every live request: ``tokens`` [max_requests] (entries of other rows do not
-        matter).  Returns the next-token logits [max_requests, vocab] and ``granted`` [max_requests]
+        matter, whatever they hold).  Returns the next-token logits [max_requests, vocab] and ``granted`` [max_requests]
         bool on the device: False for rows that are not live, or whose page could not be had
         (such a request stays as it was: finish others and step again)."""
         R = self.cache.max_requests
         if self._live_add is None:
             self._live_add = torch.tensor([int(x) for x in self.live], dtype=torch.int32, device=self.cache.lens.device)
+        # rows that are not live embed token 0: their ids may be padding that no table holds
+        ids = tokens.reshape(R, 1) * self._live_add[:, None]
         r = self.cache.reserve(self._live_add, sum(self.live))
         few = R <= 8  # rows the weight-streaming GEMVs take
         pos = (r.lens - 1).clamp(min=0).long()[:, None]
-        x = self.decoder.embed_tokens(tokens.reshape(R, 1))
+        x = self.decoder.embed_tokens(ids)
         cos, sin = self.decoder.rotary_emb(x, pos)
         x = x.view(R, -1)
         for i, st in enumerate(self.layers):

@@ -1,0 +1,82 @@
+"""Host logic of PagedQwenDecoder on the CPU: a stand-in cache keeps the lengths and free pages, the
+kernels are replaced by plain functions, so that ids, failures and refusals can be followed
+without a GPU."""
+import pytest
+import torch
+
+pytest.importorskip("transformers")
+from transformers import Qwen3_5TextConfig  # noqa: E402
+from transformers.models.qwen3_5.modeling_qwen3_5 import Qwen3_5ForCausalLM  # noqa: E402
+
+from butterfly_b200 import glue  # noqa: E402
+from butterfly_b200.integrations import qwen_torch as qt  # noqa: E402
+from butterfly_b200.integrations.qwen_paged import PagedQwenDecoder  # noqa: E402
+from butterfly_b200.paged import RELEASE, PagedReservation  # noqa: E402
+
+PAGE, ROWS, VOCAB = 16, 4, 500
+
+
+def _model(layers=2):
+    qt.patch_qwen35_full_attention_decode()
+    cfg = Qwen3_5TextConfig(hidden_size=256, num_attention_heads=4, num_key_value_heads=1, head_dim=128,
+                            num_hidden_layers=layers, layer_types=["full_attention"] * layers,
+                            intermediate_size=256, vocab_size=VOCAB, partial_rotary_factor=0.25)
+    torch.manual_seed(0)
+    return Qwen3_5ForCausalLM(cfg).eval()
+
+
+class _Cache:
+    """Lengths, free pages and the appended slots of a PagedKVCache, on the host."""
+
+    def __init__(self, pages=12):
+        self.max_requests, self.lens, self.free = ROWS, torch.zeros(ROWS, dtype=torch.int32), pages
+        self.written = 0
+
+    def reserve(self, add, num_tokens=None):
+        add = [int(x) for x in add]
+        assert num_tokens is None or num_tokens >= sum(max(x, 0) for x in add)
+        granted, lens = [], self.lens.tolist()
+        for b, a in enumerate(add):
+            want = max(0, lens[b] + a)
+            need = -(-want // PAGE) + (-lens[b] // PAGE)
+            ok = need <= self.free
+            granted.append(ok and a > 0)
+            if ok:
+                lens[b], self.free = want, self.free - need
+        self.lens = torch.tensor(lens, dtype=torch.int32)
+        total = sum(max(x, 0) for x in add)
+        return PagedReservation(self.lens, torch.tensor([self.free]), torch.arange(total), torch.arange(total, dtype=torch.int32),
+                                torch.tensor(granted))
+
+    def release(self, rows):
+        self.reserve([RELEASE if b in set(rows) else 0 for b in range(ROWS)])
+
+    def append(self, layer, k, v, slots):
+        assert k.shape[0] == v.shape[0] == slots.shape[0]
+        self.written += 1
+
+    def attend(self, layer, q, **kw):
+        return torch.zeros(ROWS, q.shape[1], 1, 128, dtype=q.dtype)
+
+
+@pytest.fixture
+def dec(monkeypatch):
+    """A decoder of no layers (what surrounds them is left) whose norm and head run on the CPU."""
+    d = PagedQwenDecoder(_model(), max_requests=ROWS, num_pages=12, page_size=PAGE, max_tokens_per_request=64)
+    d.cache, d.layers = _Cache(), []
+    monkeypatch.setattr(glue, "rmsnorm", lambda x, w, eps, **kw: x)
+    monkeypatch.setattr(glue, "gemv", lambda x, w, **kw: x @ w.t())
+    return d
+
+
+def _ids(n, seed=0):
+    return torch.randint(0, VOCAB, (n,), generator=torch.Generator().manual_seed(seed))
+
+
+def test_ids_of_rows_that_are_not_live_do_not_matter(dec):
+    dec.add({1: _ids(5)})
+    tokens = torch.tensor([-1, 7, VOCAB, 2 ** 40])  # padding ids that no embedding table holds
+    logits, granted = dec.step(tokens)
+    assert granted.tolist() == [False, True, False, False]
+    want = dec.model.lm_head(dec.decoder.embed_tokens(torch.tensor(7)))
+    torch.testing.assert_close(logits[1], want)
