@@ -40,6 +40,7 @@
 
 #include "common.cuh"
 #include "mma.cuh"
+#include "ring.cuh"
 #include "sm100.cuh"
 
 namespace bna {
@@ -110,12 +111,9 @@ struct Layout {
   // 128 KB of ring an SM keeps the memory busy; with 192 KB requests queue and the SMs that a loaded
   // GPU serves last fall further behind (640 against 615 us at 64 x 65,536 tokens).
   static constexpr int kSlots = 128 * 1024 / kCtas / kSlotBytes;
-  // Every consumer warp has a ring of its own (slot = use % kRing * kCons + warp): a barrier's parity
-  // tells a wait that is one use ahead nothing about the use before, so a slot has to stay
-  // with one warp.  Granule i of a segment goes to warp i % kCons, whatever came before it,
-  // so that the segment's sums do not depend on that.
-  static_assert(kSlots % kCons == 0, "a slot belongs to one warp");
-  static constexpr int kRing = kSlots / kCons;
+  // Every consumer warp has slots of its own (ring.cuh).  Granule i of a segment goes to warp
+  // i % kCons, whatever came before it, so that the segment's sums do not depend on that.
+  using Uses = Ring<kCons, kSlots>;
   static constexpr int kQPitch = 2 * DH + 16;                         // spreads the rows over the banks
   static constexpr int kQBytes = kRows * kQPitch;
   static constexpr int kQ = kSlots * kSlotBytes;
@@ -131,7 +129,8 @@ struct Layout {
   static constexpr int kNumBars = 2 * kSlots + 6;
   static constexpr int kSeg = kBars + kNumBars * 8;
   static constexpr int kFlags = kSeg + 2 * (int)sizeof(Seg);
-  static constexpr int kLens = (kFlags + 16 + 15) / 16 * 16;  // the first kKeepLens requests' lengths
+  static constexpr int kIssued = kFlags + 16;  // the log of tile copies
+  static constexpr int kLens = (kIssued + 4 * kSlots + 15) / 16 * 16;  // the first kKeepLens requests' lengths
   static constexpr int kBytes = kLens + 4 * kKeepLens;
   static constexpr int kAlloc = kBytes + 1024;  // the base is aligned to 1024 (swizzle atom)
   static_assert(kCtas * (kAlloc + 1024) <= 233472, "shared memory of an SM");
@@ -208,6 +207,7 @@ template <typename T, int DH, bool WIDE>
 __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     paged_decode_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const PagedArgs a) {
   using Lay = Layout<DH>;
+  using Uses = typename Lay::Uses;
   constexpr int kCons = Lay::kCons;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
   Seg* segs = reinterpret_cast<Seg*>(sm + Lay::kSeg);
   volatile int* abort_flag = reinterpret_cast<int*>(sm + Lay::kFlags);
   volatile int* last_flag = abort_flag + 1;
+  int* issued = reinterpret_cast<int*>(sm + Lay::kIssued);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // full and empty (one arrival), seg_full (one), seg_empty (each consumer warp), stage_full (one)
@@ -226,6 +227,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     const int k = i - 2 * Lay::kSlots;
     mbar_init(full + i, k == 2 || k == 3 ? kCons : 1);
     fence_mbar_init();
+    if (i < Lay::kSlots) issued[i] = 0;
   }
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -239,6 +241,12 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, kErrSite + site, a.err));
+  };
+  // Wait for a copy that is in flight, whatever went wrong elsewhere (20 ms at most): none may land in
+  // the shared memory of a CTA that has ended.
+  auto settle = [&](uint64_t* bar, uint32_t parity) {
+    for (int tries = 0; tries < 1000; ++tries)
+      if (mbar_try_wait_suspend(bar, parity, 20000u)) break;
   };
 
   if (warp == kCons) {
@@ -404,6 +412,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
       return true;
     };
     int used = 0, nseg = 0;  // granules given to warp lane % kCons, and segments, so far
+    int queries = 0;         // segments whose Q copies were issued
     bool ok = true;
     Next next;
     bool more = take(next);
@@ -420,6 +429,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
         mbar_arrive_expect_tx(seg_full + si, (uint32_t)(s.rows * 2 * DH));
       }
       __syncwarp();
+      queries = nseg + 1;
       if (lane < s.rows)
         bulk_copy_g2s(sm + Lay::kQ + si * Lay::kQBytes + lane * Lay::kQPitch,
                       a.q + 2 * (s.b * a.q_b + (int64_t)(s.h * a.G + s.r0 + lane) * a.q_h), 2 * DH, seg_full + si);
@@ -431,9 +441,10 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
         for (int w = 0; w < m && ok; w += kLanes) {
           bool mine = true;
           if (lane >= w && lane < w + kLanes && lane < m) {
-            const int use = used + (i0 + lane) / kCons, slot = use % Lay::kRing * kCons + lane % kCons;
-            mine = mbar_wait(empty + slot, (uint32_t)((use / Lay::kRing) & 1) ^ 1, abort_flag, kErrSite + 1, a.err);
+            const int use = used + (i0 + lane) / kCons, slot = Uses::slot(use, lane % kCons);
+            mine = mbar_wait(empty + slot, Uses::parity(use) ^ 1, abort_flag, kErrSite + 1, a.err);
             if (mine) {  // (a page number outside the pool fills the tile with zeros)
+              Uses::log(issued, use, lane % kCons);
               uint8_t* dst = sm + slot * Lay::kSlotBytes;
               mbar_arrive_expect_tx(full + slot, Lay::kSlotBytes);
               tma_load_5d(dst, &mk, full + slot, 0, row, 0, s.h, page);
@@ -447,6 +458,9 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
       if (nseg == 0) more = take(next);
       ++nseg;
     }
+    // the Q copies, while their barriers still stand at them (the end's mark comes next)
+    if (lane < 2 && lane < queries) settle(seg_full + ((queries - 1 - lane) & 1), (uint32_t)((queries - 1 - lane) >> 1) & 1);
+    __syncwarp();
     if (ok) {
       const int si = nseg & 1;
       if (wait(seg_empty + si, (uint32_t)(((nseg >> 1) & 1) ^ 1), 2) && lane == 0) {
@@ -464,11 +478,9 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
       if (a.lse)
         for (int i = lane; i < hq; i += 32) a.lse[b * a.ls_b + i * a.ls_h] = -INFINITY;
     }
-    // no copy is in flight when the CTA ends, whatever the consumers did
-    if (lane < kCons)
-      for (int use = max(0, used - Lay::kRing); use < used; ++use)
-        for (int tries = 0; tries < 1000; ++tries)
-          if (mbar_try_wait_suspend(full + use % Lay::kRing * kCons + lane, (use / Lay::kRing) & 1, 20000u)) break;
+    // no tile copy is in flight when the CTA ends, wherever this warp or the consumers gave up
+    __syncwarp();
+    Uses::settle(issued, lane, 32, [&](int slot, uint32_t parity) { settle(full + slot, parity); });
     return;
   }
 
@@ -529,8 +541,8 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     const bool fresh = a.kn && (!a.active || a.active[s.b]);
 
     for (int i = warp; i < s.n; i += kCons, ++use) {
-      const int slot = use % Lay::kRing * kCons + warp;
-      const uint32_t par = (uint32_t)((use / Lay::kRing) & 1);
+      const int slot = Uses::slot(use, warp);
+      const uint32_t par = Uses::parity(use);
       const int pos = (s.g0 + i) * kGran;
       const bool edge = pos < s.lo || pos + kGran > s.hi;
       const bool owns_new = fresh && pos + kGran >= s.hi;  // the granule of key hi - 1
@@ -816,7 +828,8 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
       for (int x = 0; x < kItems; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = 0; k < batches; ++k) {
         const int half = (fetched + k) & 1;
-        wait(stage_full + half, (uint32_t)(((fetched + k) >> 1) & 1), 6);  // (the next segment's wait sees a failure)
+        const uint32_t par = (uint32_t)(((fetched + k) >> 1) & 1);
+        if (!wait(stage_full + half, par, 6)) settle(stage_full + half, par);  // (the next segment's wait sees a failure)
         const float4* src = reinterpret_cast<const float4*>(sm + Lay::kStage + half * Lay::kHalf);
         const int n = min(batch, members - k * batch);
         if (grp < groups)
