@@ -175,8 +175,15 @@ template <typename T>
 __device__ __forceinline__ void store4(uint8_t* p, const float4& v, float f) {
   *reinterpret_cast<uint2*>(p) = make_uint2(ElemTraits<T>::pack2(v.x * f, v.y * f), ElemTraits<T>::pack2(v.z * f, v.w * f));
 }
+// Probabilities are held times 2^kShift, and so are the sums l and outputs o, which the final division
+// undoes.  fp16 has steps of 2^-24 below 2^-14: unscaled, with the row's largest at 1, what lies 17
+// nats below it would vanish from the output (but not from l).  At 2^15 (the largest still fits, the
+// sums are fp32) the steps are 2^-39 of it.
+template <typename T>
+constexpr float kShift = std::is_same<T, __half>::value ? 15.f : 0.f;
+template <typename T>
 __device__ __forceinline__ float lse_of(float m, float l) {
-  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  return l == 0.f ? -INFINITY : (m + log2f(l * (std::is_same<T, __half>::value ? 0x1p-15f : 1.f))) * 0.6931471805599453f;
 }
 
 // Barrier of the consumer warps.  Every path of every warp between two of them ends by itself
@@ -200,7 +207,7 @@ __device__ __forceinline__ bool cons_any(bool bad) {
 
 // WIDE: 9 to 16 query heads, the rows of the 16-row MMA.  Otherwise the heads are rows 0-7, and rows
 // 8-15 of the P V product carry the low part of the probabilities.  A probability is held
-// as hi + lo in the 16-bit type (relative error u^2 instead of u: rounding it once would add
+// as hi + lo in the 16-bit type, scaled (kShift; relative error u^2 instead of u: rounding it once would add
 // as much error to the output as its final rounding does); with at most 8 heads lo rides in rows
 // that the MMA computes anyway, with more it costs a second MMA, which the memory hides.
 template <typename T, int DH, bool WIDE>
@@ -626,8 +633,8 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
         float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[x], mx), base = mn == -INFINITY ? 0.f : mn;
-        al[x] = ex2_approx(m[x] - base);
+        const float mn = fmaxf(m[x], mx), top = mn == -INFINITY ? 0.f : mn, base = top - kShift<T>;
+        al[x] = ex2_approx(m[x] - top);
         moved |= mn != m[x];
         m[x] = mn;
 #pragma unroll
@@ -698,7 +705,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
 #pragma unroll
           for (int j = 0; j < NT; ++j)
             *reinterpret_cast<uint32_t*>(dst + 16 * j) = ElemTraits<T>::pack2(o[j][2 * x] * f, o[j][2 * x + 1] * f);
-          if (a.lse && tig == 0) a.lse[s.b * a.ls_b + hq * a.ls_h] = lse_of(m[x], l[x]);
+          if (a.lse && tig == 0) a.lse[s.b * a.ls_b + hq * a.ls_h] = lse_of<T>(m[x], l[x]);
         }
       }
       continue;
@@ -751,7 +758,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
         if (s.slot < 0) {
           const int hq = s.h * a.G + s.r0 + r;
           store4<T>(a.out + 2 * (s.b * a.o_b + hq * a.o_h + c0 + c), v, L == 0.f ? 0.f : 1.f / L);
-          if (a.lse && c0 + c == 0) a.lse[s.b * a.ls_b + hq * a.ls_h] = lse_of(M, L);
+          if (a.lse && c0 + c == 0) a.lse[s.b * a.ls_b + hq * a.ls_h] = lse_of<T>(M, L);
         } else {
           *reinterpret_cast<float4*>(part_o + r * DH + c0 + c) = v;
           if (c0 + c == 0) reinterpret_cast<float2*>(a.ws + kWsMl)[s.slot * kRows + r] = make_float2(M, L);
@@ -817,7 +824,7 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
         if (lane < members) wt[lane * s.rows + r] = f * (!final ? 1.f : L == 0.f ? 0.f : 1.f / L);
         if (lane == 0) {
           if (!final) const_cast<float2*>(gml)[slot_of(0) * kRows + r] = make_float2(M, L);
-          else if (a.lse) a.lse[s.b * a.ls_b + (int64_t)(s.h * a.G + s.r0 + r) * a.ls_h] = lse_of(M, L);
+          else if (a.lse) a.lse[s.b * a.ls_b + (int64_t)(s.h * a.G + s.r0 + r) * a.ls_h] = lse_of<T>(M, L);
         }
       }
       cons_sync<kNT>();
