@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kMaxRequests = 4096;  // three prefix sums and the lengths of a call: 64 KB of shared memory
 constexpr int kReserveCtas = 148;
+constexpr int kScanBytes = 3 * 32 * 8;  // static shared memory: a warp's part of each sum
 
 struct ReserveArgs {
   const int32_t* lens;
@@ -85,6 +86,7 @@ __global__ void __launch_bounds__(1024) reserve_kernel(const ReserveArgs a) {
   int32_t* cum_back = sm + 2 * a.B;
   int32_t* lens = sm + 3 * a.B;     // cut to the table, so that no later index leaves a row
   __shared__ int64_t warp_sums[3][32];
+  static_assert(sizeof(warp_sums) == kScanBytes, "static shared memory");
   const int threads = blockDim.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -294,8 +296,9 @@ int launch_reserve(const int32_t* lens, const int32_t* add, int B, int32_t* tabl
   const int k = num_tokens > 256 * kReserveCtas ? 4 : 1;
   auto kern = k == 4 ? reserve_kernel<4> : reserve_kernel<1>;
   const unsigned threads = B > 1024 ? 1024 : 256;
+  // What a launch may use unasked, 48 KB, covers the static warp sums too.
   const int smem = 4 * B * 4;
-  if (smem > 48 * 1024) {
+  if (smem + kScanBytes > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMaxRequests * 4);
     if (e != cudaSuccess) return check_cuda(e, "paged_reserve attributes");
   }

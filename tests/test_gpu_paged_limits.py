@@ -1,9 +1,12 @@
-"""The paged cache at its limits: probabilities far below their row's maximum.
+"""The paged cache at its limits: request counts around the shared-memory bounds, probabilities far below their row's maximum.
 
 Bars as in tests/test_gpu_paged.py, where the second part of an fp16 probability that is subnormal
 counts in steps of 2^-39 of the row's largest (rounding: 2^-40), probabilities being held times 2^15;
 an fp16 result that is subnormal is off by 2^-25."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -12,6 +15,7 @@ import butterfly_b200 as bb
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 # ------------------------------------------------------------------------------ attention
@@ -55,3 +59,28 @@ def test_tail_below_a_dominant_key(dtype, Hq, Hkv, dh, lens, gap):
         assert bool((err <= bar).all()), (b, float((err / bar).max()), float((err / ref.abs()).max()))
         lbar = ds[:, 0] + 2.0 ** -20 + ln * 2.0 ** -23 + 2.0 ** -21 * rl.abs()
         assert bool(((lse[b, :, 0].double() - rl).abs() <= lbar).all())
+
+
+# ------------------------------------------------------------------------------ reserve
+_ONE_CALL = """
+import sys
+import torch
+import butterfly_b200 as bb
+B, tokens = int(sys.argv[1]), int(sys.argv[2])
+z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+free = torch.arange(B, dtype=torch.int32, device="cuda")
+table = torch.full((B, 1), -1, dtype=torch.int32, device="cuda")
+r = bb.paged_reserve(z(B), z(B) + 1, table, free, z(1) + B, page_size=16, num_tokens=tokens)
+want = (B - 1 - torch.arange(B, device="cuda"))
+assert bool((table[:, 0] == want).all()) and bool(r.granted.all()) and int(r.num_free) == 0
+assert bool((r.slot_map[:B] == want * 16).all()) and bool((r.slot_map[B:] == -1).all())
+"""
+
+
+@pytest.mark.parametrize("B", [2048, 2560, 2816, 3024, 3025, 3048, 3072, 3073, 4096])
+@pytest.mark.parametrize("tokens", [0, 50000])  # (one token a thread, or four)
+def test_reserve_first_call_at_every_request_count(B, tokens):
+    # in a process of its own: an earlier, larger call would have raised the shared-memory limit
+    r = subprocess.run([sys.executable, "-c", _ONE_CALL, str(B), str(max(tokens, B))], cwd=ROOT, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
