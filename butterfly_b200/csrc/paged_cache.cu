@@ -13,8 +13,9 @@
 namespace bna {
 namespace {
 
-constexpr int kMaxRequests = 4096;  // three prefix sums and the lengths of a call: 64 KB of shared memory
+constexpr int kMaxRequests = 4096;  // three prefix sums, the lengths and flags of a call: 68 KB of shared memory
 constexpr int kReserveCtas = 148;
+constexpr int kRequestBytes = 4 * 4 + 1;  // dynamic shared memory of a request
 constexpr int kScanBytes = 3 * 32 * 8;  // static shared memory: a warp's part of each sum
 
 struct ReserveArgs {
@@ -50,6 +51,7 @@ __device__ __forceinline__ int pages_of(unsigned tokens, unsigned page_size) {
 }
 
 // What a request asks for: its length after the call, and pages taken (need) or given back.
+enum : uint8_t { kGrows = 1, kNeeds = 2 };  // tokens are added and fit the table; they need pages
 struct Ask {
   int want, old_pages, new_pages, need, back;
   bool fits;
@@ -81,10 +83,13 @@ __device__ __forceinline__ Ask ask_of(int len, int add, int capacity, int page_s
 template <int K>
 __global__ void __launch_bounds__(1024) reserve_kernel(const ReserveArgs a) {
   extern __shared__ int32_t sm[];
-  int32_t* cum_add = sm;            // inclusive prefix sums (capped at INT_MAX)
+  // Inclusive prefix sums, capped at INT_MAX: exact for every token below num_tokens and every page
+  // there is.  What a request asks for is not read off their differences, which the cap falsifies.
+  int32_t* cum_add = sm;
   int32_t* cum_need = sm + a.B;
   int32_t* cum_back = sm + 2 * a.B;
   int32_t* lens = sm + 3 * a.B;     // cut to the table, so that no later index leaves a row
+  uint8_t* asks = reinterpret_cast<uint8_t*>(sm + 4 * a.B);  // kGrows, kNeeds
   __shared__ int64_t warp_sums[3][32];
   static_assert(sizeof(warp_sums) == kScanBytes, "static shared memory");
   const int threads = blockDim.x;
@@ -128,6 +133,7 @@ __global__ void __launch_bounds__(1024) reserve_kernel(const ReserveArgs a) {
     at[0] += max(add, 0);
     at[1] += r.need;
     at[2] += r.back;
+    asks[b] = (add > 0 && r.fits ? kGrows : 0) | (r.need > 0 ? kNeeds : 0);
     cum_add[b] = (int32_t)min(at[0], (int64_t)INT_MAX);
     cum_need[b] = (int32_t)min(at[1], (int64_t)INT_MAX);
     cum_back[b] = (int32_t)min(at[2], (int64_t)INT_MAX);
@@ -150,17 +156,13 @@ __global__ void __launch_bounds__(1024) reserve_kernel(const ReserveArgs a) {
     const int64_t i = top - 1 - x;
     return i >= 0 && i < n ? a.free_pages[i] : -1;
   };
-  // Tokens were added to b and have slots: it fits, and needs no page or was served.
-  auto granted = [&](int b) {
-    const int tokens = cum_add[b] - before(cum_add, b);
-    return tokens > 0 && (int64_t)lens[b] + tokens <= capacity && (b < served || cum_need[b] == before(cum_need, b));
-  };
+  // Tokens were added to b and have slots: they fit, and need no page or were served.
+  auto granted = [&](int b) { return (asks[b] & kGrows) && (b < served || !(asks[b] & kNeeds)); };
   const int64_t stride = (int64_t)gridDim.x * threads, tid = (int64_t)blockIdx.x * threads + threadIdx.x;
 
   // slots and positions of the added tokens, packed request by request, and the table entries
   // of the pages taken, each written with the page's first token
-  const int64_t limit = max(a.num_tokens, (int64_t)cum_add[a.B - 1]);
-  for (int64_t t0 = tid * K; t0 < limit; t0 += stride * K) {
+  for (int64_t t0 = tid * K; t0 < a.num_tokens; t0 += stride * K) {
     int b = upper_bound(cum_add, a.B, t0);
     int64_t slot[K];
     int pos[K], at_b = -1, at_page = -1, page = -1, have = 0, first = 0;
@@ -204,6 +206,13 @@ __global__ void __launch_bounds__(1024) reserve_kernel(const ReserveArgs a) {
         }
     }
   }
+  // more tokens than slot_map holds: the entries of the pages past it, page by page
+  if (cum_add[a.B - 1] > a.num_tokens)
+    for (int64_t i = tid; i < A; i += stride) {
+      const int b = upper_bound(cum_need, a.B, i);
+      const int64_t pi = pages_of(lens[b], a.page_size) + i - before(cum_need, b);
+      if (before(cum_add, b) + pi * a.page_size - lens[b] >= a.num_tokens) a.table[b * a.table_stride + pi] = from_top(i);
+    }
   for (int64_t b = tid; b < a.B; b += stride) {
     const bool ok = granted((int)b);
     const int add = a.add[b];
@@ -297,9 +306,9 @@ int launch_reserve(const int32_t* lens, const int32_t* add, int B, int32_t* tabl
   auto kern = k == 4 ? reserve_kernel<4> : reserve_kernel<1>;
   const unsigned threads = B > 1024 ? 1024 : 256;
   // What a launch may use unasked, 48 KB, covers the static warp sums too.
-  const int smem = 4 * B * 4;
+  const int smem = kRequestBytes * B;
   if (smem + kScanBytes > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMaxRequests * 4);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRequestBytes * kMaxRequests);
     if (e != cudaSuccess) return check_cuda(e, "paged_reserve attributes");
   }
   // enough CTAs for the tokens and for every page the requests could give back (these in several

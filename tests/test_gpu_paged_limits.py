@@ -1,4 +1,5 @@
-"""The paged cache at its limits: request counts around the shared-memory bounds, probabilities far below their row's maximum.
+"""The paged cache at its limits: request counts around the shared-memory bounds, additions that no
+request can hold, probabilities far below their row's maximum.
 
 Bars as in tests/test_gpu_paged.py, where the second part of an fp16 probability that is subnormal
 counts in steps of 2^-39 of the row's largest (rounding: 2^-40), probabilities being held times 2^15;
@@ -84,3 +85,49 @@ def test_reserve_first_call_at_every_request_count(B, tokens):
     r = subprocess.run([sys.executable, "-c", _ONE_CALL, str(B), str(max(tokens, B))], cwd=ROOT, capture_output=True, text=True,
                        timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def _i(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("add", [(2 ** 31 - 1, 5), (2 ** 31 - 3, 5), (2 ** 30, 2 ** 30, 2 ** 30, 5), (2 ** 31 - 1,) * 40 + (5,),
+                                 (7, 2 ** 31 - 1, 5, 2 ** 31 - 1, 70, 20)])
+def test_oversized_additions_are_refused_and_take_nothing(add):
+    # the sum of the additions passes 32 bits; those that fit are served all the same
+    B, page, width, pages, tokens = len(add), 16, 4, 9, 10
+    table, free = torch.full((B, width), -1, dtype=torch.int32, device=DEV), _i(*range(pages))
+    r = bb.paged_reserve(_i(*[0] * B), _i(*add), table, free, _i(pages), page_size=page, num_tokens=tokens)
+    stack, slots, positions = list(range(pages)), [], []
+    for b, n in enumerate(add):
+        ok = n <= width * page
+        rows = [stack.pop() for _ in range(-(-n // page))] if ok else []
+        assert table[b].tolist() == rows + [-1] * (width - len(rows)), b
+        assert r.granted[b].item() == ok and r.lens[b].item() == (n if ok else 0), b
+        for p in range(min(n, tokens - len(slots))):
+            slots.append(rows[p // page] * page + p % page if ok else -1)
+            positions.append(p if ok else -1)
+    assert int(r.num_free) == len(stack)
+    assert r.slot_map.tolist() == slots and r.positions.tolist() == positions
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 30, 47, 48, 49, 119, 120, 500])
+def test_table_entries_past_the_slot_map(tokens):
+    # the pages of granted tokens that slot_map has no entry for are in the table all the same
+    lens, add, page = [5, 16, 0, 31], [40, 0, 70, 10], 16
+    table = torch.full((4, 6), -1, dtype=torch.int32, device=DEV)
+    table[0, 0], table[1, 0], table[3, :2] = 20, 21, _i(22, 23)
+    r = bb.paged_reserve(_i(*lens), _i(*add), table, _i(*range(20)), _i(20), page_size=page, num_tokens=tokens)
+    assert table.tolist() == [[20, 19, 18, -1, -1, -1], [21, -1, -1, -1, -1, -1], [17, 16, 15, 14, 13, -1], [22, 23, 12, -1, -1, -1]]
+    assert int(r.num_free) == 12 and r.lens.tolist() == [45, 16, 70, 41]
+    want = [int(table[b, p // page]) * page + p % page for b in range(4) for p in range(lens[b], lens[b] + add[b])]
+    assert r.slot_map.tolist() == (want + [-1] * tokens)[:tokens]
+
+
+def test_pages_asked_for_past_32_bits():
+    # four requests of 2^30 pages each over a stack of ten: all are refused, and a later one too
+    table = torch.empty(5, 2 ** 30, dtype=torch.int32, device=DEV)
+    table[:, :3] = -1
+    r = bb.paged_reserve(_i(0, 0, 0, 0, 0), _i(*[2 ** 30] * 4, 3), table, _i(*range(10)), _i(10), page_size=1, num_tokens=7)
+    assert r.granted.tolist() == [False] * 5 and r.lens.tolist() == [0] * 5 and int(r.num_free) == 10
+    assert r.slot_map.tolist() == [-1] * 7 and bool((table[:, :3] == -1).all())
