@@ -68,7 +68,8 @@ class PagedQwenDecoder:
     @torch.no_grad()
     def add(self, prompts: Mapping[int, torch.Tensor]) -> dict[int, torch.Tensor]:
         """Admit prompts (1-D token ids) into vacant rows; returns their next-token logits.  Raises
-        RuntimeError, with nothing admitted, if the pages do not suffice for all of them."""
+        RuntimeError if the pages do not suffice for all of them; nothing is admitted then, nor
+        when the model's forward raises."""
         from transformers import DynamicCache
         rows = sorted(prompts)
         for b in rows:
@@ -78,19 +79,23 @@ class PagedQwenDecoder:
                 raise ValueError("a prompt needs at least one token")
         add = [int(prompts[b].numel()) if b in prompts else 0 for b in range(self.cache.max_requests)]
         r = self.cache.reserve(add)
-        granted = r.granted.tolist()
-        if not all(granted[b] for b in rows):
-            self.cache.release(rows)
-            raise RuntimeError("not enough free pages for the prompts")
         logits, at = {}, 0
+        try:
+            granted = r.granted.tolist()
+            if not all(granted[b] for b in rows):
+                raise RuntimeError("not enough free pages for the prompts")
+            for b in rows:
+                n = add[b]
+                kv = DynamicCache(config=self.model.config)
+                out = self.model(input_ids=prompts[b].reshape(1, n), past_key_values=kv, use_cache=True, logits_to_keep=1)
+                for i, layer in enumerate(kv.layers):
+                    self.cache.append(i, layer.keys[0].transpose(0, 1), layer.values[0].transpose(0, 1), r.slot_map[at:at + n])
+                logits[b] = out.logits[0, -1]
+                at += n
+        except BaseException:  # the rows were vacant: nothing of them is kept
+            self.cache.release(rows)
+            raise
         for b in rows:
-            n = add[b]
-            kv = DynamicCache(config=self.model.config)
-            out = self.model(input_ids=prompts[b].reshape(1, n), past_key_values=kv, use_cache=True, logits_to_keep=1)
-            for i, layer in enumerate(kv.layers):
-                self.cache.append(i, layer.keys[0].transpose(0, 1), layer.values[0].transpose(0, 1), r.slot_map[at:at + n])
-            logits[b] = out.logits[0, -1]
-            at += n
             self.live[b] = True
         self._live_add = None
         return logits

@@ -80,3 +80,37 @@ def test_ids_of_rows_that_are_not_live_do_not_matter(dec):
     assert granted.tolist() == [False, True, False, False]
     want = dec.model.lm_head(dec.decoder.embed_tokens(torch.tensor(7)))
     torch.testing.assert_close(logits[1], want)
+
+
+def _state(d):
+    return d.cache.lens.tolist(), d.cache.free, list(d.live)
+
+
+@pytest.mark.parametrize("calls", [0, 1, 2])
+def test_prompts_are_given_back_when_the_model_raises(dec, calls):
+    dec.add({2: _ids(20)})
+    before, forward, made = _state(dec), dec.model.forward, []
+
+    def failing(*a, **kw):
+        if len(made) == calls:
+            raise MemoryError("out of memory")
+        made.append(1)
+        return forward(*a, **kw)
+
+    dec.model.forward = failing
+    prompts = {0: _ids(40, 1), 1: _ids(3, 2), 3: _ids(17, 3)}
+    with pytest.raises(MemoryError):
+        dec.add(prompts)
+    assert _state(dec) == before
+    assert dec.step(torch.zeros(ROWS, dtype=torch.long))[1].tolist() == [False, False, True, False]
+    dec.model.forward = forward
+    logits = dec.add(prompts)
+    assert sorted(logits) == [0, 1, 3] and dec.live == [True] * 4 and dec.cache.lens.tolist() == [40, 3, 21, 17]
+
+
+def test_prompts_are_given_back_when_an_append_raises(dec):
+    before = _state(dec)
+    dec.cache.append = lambda *a: (_ for _ in ()).throw(RuntimeError("append"))
+    with pytest.raises(RuntimeError, match="append"):
+        dec.add({0: _ids(40, 1), 1: _ids(3, 2)})
+    assert _state(dec) == before
