@@ -29,7 +29,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import glue
-from ..paged import PagedKVCache
+from ..paged import PagedKVCache, PagedReservation
 from .qwen_fused import _is_qwen35_norm, _merge_weights
 from .qwen_torch import _get_decoder_with_layers, _has_required_qwen_attention_attrs, patch_qwen35_full_attention_decode
 
@@ -112,13 +112,22 @@ class PagedQwenDecoder:
         """One token for every live request: ``tokens`` [max_requests] (entries of other rows do not
         matter, whatever they hold).  Returns the next-token logits [max_requests, vocab] and ``granted`` [max_requests]
         bool on the device: False for rows that are not live, or whose page could not be had
-        (such a request stays as it was: finish others and step again)."""
+        (such a request stays as it was: finish others and step again).  If the step raises, all
+        requests stay as they were."""
         R = self.cache.max_requests
         if self._live_add is None:
             self._live_add = torch.tensor([int(x) for x in self.live], dtype=torch.int32, device=self.cache.lens.device)
         # rows that are not live embed token 0: their ids may be padding that no table holds
         ids = tokens.reshape(R, 1) * self._live_add[:, None]
         r = self.cache.reserve(self._live_add, sum(self.live))
+        try:
+            return self._forward(ids, r), r.granted
+        except BaseException:  # a token without rows in every layer must not count
+            self.cache.reserve(-(self._live_add * r.granted), 0)
+            raise
+
+    def _forward(self, ids: torch.Tensor, r: PagedReservation) -> torch.Tensor:
+        R = self.cache.max_requests
         few = R <= 8  # rows the weight-streaming GEMVs take
         pos = (r.lens - 1).clamp(min=0).long()[:, None]
         x = self.decoder.embed_tokens(ids)
@@ -145,7 +154,7 @@ class PagedQwenDecoder:
                 x = x2 + F.linear(glue.swiglu(F.linear(h, st.w_gu), st.inter), st.mlp.down_proj.weight)
         x = glue.rmsnorm(x, self.decoder.norm.weight, self.decoder.norm.eps)
         w = self.model.lm_head.weight
-        return (glue.gemv(x, w) if few else F.linear(x, w)), r.granted
+        return glue.gemv(x, w) if few else F.linear(x, w)
 
 
 def main() -> None:

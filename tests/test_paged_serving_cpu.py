@@ -114,3 +114,18 @@ def test_prompts_are_given_back_when_an_append_raises(dec):
     with pytest.raises(RuntimeError, match="append"):
         dec.add({0: _ids(40, 1), 1: _ids(3, 2)})
     assert _state(dec) == before
+
+
+def test_a_step_that_raises_advances_no_request(dec, monkeypatch):
+    dec.add({0: _ids(16, 1), 2: _ids(20, 2), 3: _ids(64, 3)})  # row 0 needs a page for its next token
+    dec.cache.free = 1
+    before = _state(dec)
+    tokens = torch.zeros(ROWS, dtype=torch.long)
+    with monkeypatch.context() as m:
+        m.setattr(glue, "gemv", lambda *a, **kw: (_ for _ in ()).throw(RuntimeError("head")))
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="head"):
+                dec.step(tokens)
+            assert _state(dec) == before
+    granted = dec.step(tokens)[1].tolist()
+    assert granted == [True, False, True, False] and dec.cache.lens.tolist() == [17, 0, 21, 64]
