@@ -341,7 +341,10 @@ __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
       while (!(past = __ballot_sync(0xffffffffu, before + incl_w > at))) {
         before += __shfl_sync(0xffffffffu, incl_w, 31);
         wb += 32;
-        if (wb >= a.B) return -1;
+        if (wb >= a.B) {
+          if (lane == 0 && a.err) atomicCAS(a.err, 0, 0x1000 | (kErrSite + 7));
+          return -1;
+        }
         load_window();
       }
       return __ffs(past) - 1;

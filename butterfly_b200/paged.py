@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import weakref
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -86,14 +87,49 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     _lib.check((_native or _binding()).append(k, v, k_pages, v_pages, slot_map, _stream(k)))
 
 
-_workspaces: dict = {}
+_workspaces: dict = {}  # (device, stream) -> the workspace kept for it
+_made: dict = {}  # id -> weak reference to every workspace there is, for reset_workspaces
 
 
 def decode_workspace(device: torch.device | str | int = "cuda") -> torch.Tensor:
     """A workspace for ``paged_decode_attention`` calls that follow one another on a stream."""
     ws = torch.empty(_lib.lib().bna_paged_decode_workspace_bytes(), dtype=torch.uint8, device=device)
     ws[:4096].zero_()  # the arrival counters; every call leaves them zero
+    key = id(ws)
+    _made[key] = weakref.ref(ws, lambda _: _made.pop(key, None))
     return ws
+
+
+def reset_workspaces(device: torch.device | str | int = "cuda") -> None:
+    """Zero the counters of every ``decode_workspace`` of a device (those kept per stream and the caches'
+    own among them), after its kernels have ended.  Needed where a call did not run to its end (see
+    ``take_device_error``) or its lengths were changed while it ran: counts left by such a call
+    would make later ones leave out work."""
+    device = torch.empty(0, device=device).device
+    torch.cuda.synchronize(device)
+    for ref in list(_made.values()):
+        ws = ref()
+        if ws is not None and ws.device == device:
+            ws[:4096].zero_()
+    torch.cuda.synchronize(device)
+
+
+def _read_device_error(device: int) -> int:
+    code = ctypes.c_int32()
+    _lib.check(_lib.lib().bna_take_device_error(device, ctypes.byref(code)))
+    return code.value
+
+
+def take_device_error(device: torch.device | str | int = "cuda") -> int:
+    """Read and clear a device's error word, once its kernels have ended: 0, or the site of the first wait
+    that a kernel gave up since the last call.  What kernels wrote since then is not to be used;
+    the workspaces are made usable again (``reset_workspaces``)."""
+    device = torch.empty(0, device=device).device
+    torch.cuda.synchronize(device)
+    code = _read_device_error(device.index)
+    if code:
+        reset_workspaces(device)
+    return code
 
 
 def _workspace_for(x: torch.Tensor, stream: int) -> torch.Tensor:
@@ -123,7 +159,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     requests got no room, or rest).  Returns [B,Hq,1,dh] in q's dtype, contiguous (so that
     ``transpose(1, 2)`` is [B,1,Hq,dh] storage); with ``return_lse`` also the fp32 natural-log sums
     [B,Hq,1].  A request of length 0 gives zeros and -inf.  ``workspace`` (``decode_workspace``)
-    defaults to one kept per stream; calls that may overlap need one each."""
+    defaults to one kept per stream; calls that may overlap need one each.  Lengths and tables
+    must not change while the call runs; ``take_device_error`` tells whether a kernel gave up."""
     stream = _stream(q)
     r = (_native or _binding()).decode(
         q, k_pages, v_pages, block_table, lens, k_new, v_new, active, window,
@@ -201,4 +238,5 @@ class PagedKVCache:
                                       return_lse=return_lse, workspace=self.workspace)
 
 
-__all__ = ["PagedKVCache", "PagedReservation", "RELEASE", "decode_workspace", "paged_append", "paged_decode_attention", "paged_reserve"]
+__all__ = ["PagedKVCache", "PagedReservation", "RELEASE", "decode_workspace", "paged_append", "paged_decode_attention", "paged_reserve",
+           "reset_workspaces", "take_device_error"]

@@ -394,8 +394,9 @@ BNA_API int bna_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_ten
  * their pages hold).  A length is cut to table_width * page_size; a page number outside the pool reads
  * as zeros.
  * workspace: bna_paged_decode_workspace_bytes() of device memory, 16-byte aligned, whose first
- * 4096 bytes were zeroed once; every call leaves them zero again (after BNA_DEVICE_TIMEOUT zero
- * them anew).  Calls that may overlap on the GPU need a workspace each. */
+ * 4096 bytes were zeroed once; every call leaves them zero again.  After a call that did not run to
+ * its end (bna_take_device_error gives a code), or whose lens changed while it ran, zero them anew.
+ * Calls that may overlap on the GPU need a workspace each. */
 BNA_API int64_t bna_paged_decode_workspace_bytes(void);
 BNA_API int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_tensor4* v_pages,
                              const bna_tensor4* k_new, const bna_tensor4* v_new, const uint8_t* active,
