@@ -106,10 +106,12 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // The functions below return their tensors, or the status of a refused call as an int.
 
-// reserve(lens, add, block_table, free_pages, num_free, page_size, num_tokens, stream)
+// reserve(lens, add, block_table, free_pages, num_free, page_size, num_tokens, stream, keep): `keep`
+// [B + 1] int32 (or None) gets the new lengths and stack height after the kernel, which may have
+// read the old ones from there (its CTAs read them at different times, so it cannot write there).
 PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arity(n, 8);
+  arity(n, 9);
   const at::Tensor &lens = tensor(a[0], "lens"), &add = tensor(a[1], "add"), &table = tensor(a[2], "block_table"),
                    &free_pages = tensor(a[3], "free_pages"), &num_free = tensor(a[4], "num_free");
   need_cuda({&lens, &add, &table, &free_pages, &num_free});
@@ -122,6 +124,12 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t B = table.size(0), width = table.size(1), page_size = integer(a[5]), tokens = integer(a[6]);
   need(lens.size(0) == B && add.size(0) == B && num_free.size(0) == 1 && tokens >= 0,
        "lens and add must have block_table's rows, num_free one entry, num_tokens must be >= 0");
+  const at::Tensor* keep = a[8] == Py_None ? nullptr : &tensor(a[8], "keep");
+  if (keep) {
+    need_cuda({&lens, keep});
+    need_ints(*keep, 1, "keep");
+    need(keep->size(0) == B + 1, "keep must have one entry more than block_table has rows");
+  }
   need(B <= INT32_MAX && width <= INT32_MAX && free_pages.size(0) <= INT32_MAX && page_size >= 0 && page_size <= INT32_MAX,
        "paged_reserve: sizes beyond 32 bits");
   // one allocation for what lives on as the cache's state, one for the step's tokens
@@ -138,6 +146,7 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
                            static_cast<uint8_t*>(granted.data_ptr()), static_cast<int64_t*>(slots.data_ptr()),
                            static_cast<int32_t*>(positions.data_ptr()), tokens, address(a[7]));
   if (st != BNA_OK) return PyLong_FromLong(st);
+  if (keep) keep->copy_(part(state, 0, B + 1, at::kInt));
   return tuple_of({out, left, slots, positions, granted});
   END_HANDLE_TH_ERRORS
 }

@@ -116,7 +116,7 @@ class PagedQwenDecoder:
         requests stay as they were."""
         R = self.cache.max_requests
         if self._live_add is None:
-            self._live_add = torch.tensor([int(x) for x in self.live], dtype=torch.int32, device=self.cache.lens.device)
+            self._live_add = torch.tensor([int(x) for x in self.live], dtype=torch.int32, device=self.cache.block_table.device)
         # rows that are not live embed token 0: their ids may be padding that no table holds
         ids = tokens.reshape(R, 1) * self._live_add[:, None]
         r = self.cache.reserve(self._live_add, sum(self.live))

@@ -74,7 +74,8 @@ def paged_reserve(lens: torch.Tensor, add: torch.Tensor, block_table: torch.Tens
     tokens of request 0, then 1, ... are entries 0, 1, ... of ``slot_map`` and ``positions``
     (``num_tokens`` of them: at least the sum of the positive ``add``).  ``block_table`` and
     ``free_pages`` are updated in place, the lengths and the stack height are returned."""
-    r = (_native or _binding()).reserve(lens, add, block_table, free_pages, num_free, page_size, num_tokens, _stream(lens))
+    r = (_native or _binding()).reserve(lens, add, block_table, free_pages, num_free, page_size, num_tokens, _stream(lens),
+                                        None)
     if r.__class__ is int:
         _lib.check(r)
     return PagedReservation(*r)
@@ -175,8 +176,10 @@ class PagedKVCache:
     """Pools of ``num_layers`` layers under one set of block tables, lengths and free pages.
 
     The requests are the ``max_requests`` rows of the tables; a row of length 0 is vacant.  The
-    attention's workspace is the cache's own, in graph captures too: calls on one cache (and
-    replays of graphs that hold them) follow one another."""
+    cache's state (lengths, stack height, tables, the attention's workspace) stays at one address
+    and moves on in stream order, so calls may be captured: a replayed ``reserve`` (with a device
+    tensor) advances the requests from wherever they are then, a replayed ``attend`` reads their
+    lengths of then.  Calls on one cache, and replays of graphs that hold them, follow one another."""
 
     def __init__(self, *, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  max_requests: int, max_tokens_per_request: int, dtype: torch.dtype = torch.bfloat16,
@@ -188,14 +191,33 @@ class PagedKVCache:
         self.v_pages = [torch.empty(shape, dtype=dtype, device=device) for _ in range(int(num_layers))]
         width = -(-int(max_tokens_per_request) // self.page_size)
         self.block_table = torch.full((int(max_requests), width), -1, dtype=torch.int32, device=device)
-        self.lens = torch.zeros(int(max_requests), dtype=torch.int32, device=device)
+        self._state = torch.zeros(int(max_requests) + 1, dtype=torch.int32, device=device)
+        self._lens, self._num_free = self._state[:-1], self._state[-1:]
+        self._num_free.fill_(int(num_pages))
         self.free_pages = torch.arange(int(num_pages) - 1, -1, -1, dtype=torch.int32, device=device)
-        self.num_free = torch.full((1,), int(num_pages), dtype=torch.int32, device=device)
         self.workspace = decode_workspace(device)
 
     @property
     def max_requests(self) -> int:
-        return int(self.lens.shape[0])
+        return int(self._lens.shape[0])
+
+    @property
+    def lens(self) -> torch.Tensor:
+        """The requests' lengths [max_requests] int32, as of now (a copy; assign to set them)."""
+        return self._lens.clone()
+
+    @lens.setter
+    def lens(self, value: torch.Tensor) -> None:
+        self._lens.copy_(value)
+
+    @property
+    def num_free(self) -> torch.Tensor:
+        """The free pages' number [1] int32, as of now (a copy; assign to set it)."""
+        return self._num_free.clone()
+
+    @num_free.setter
+    def num_free(self, value: torch.Tensor) -> None:
+        self._num_free.copy_(value)
 
     @property
     def nbytes(self) -> int:
@@ -209,13 +231,14 @@ class PagedKVCache:
             add = [int(x) for x in add]
             if num_tokens is None:
                 num_tokens = sum(max(x, 0) for x in add)
-            add = torch.tensor(add, dtype=torch.int32).to(self.lens.device, non_blocking=True)
+            add = torch.tensor(add, dtype=torch.int32).to(self._state.device, non_blocking=True)
         if num_tokens is None:
             raise ValueError("num_tokens is needed when add is a device tensor")
-        r = paged_reserve(self.lens, add, self.block_table, self.free_pages, self.num_free, page_size=self.page_size,
-                          num_tokens=num_tokens)
-        self.lens, self.num_free = r.lens, r.num_free
-        return r
+        r = (_native or _binding()).reserve(self._lens, add, self.block_table, self.free_pages, self._num_free, self.page_size,
+                                            num_tokens, _stream(self._state), self._state)
+        if r.__class__ is int:
+            _lib.check(r)
+        return PagedReservation(*r)
 
     def release(self, rows: Sequence[int]) -> None:
         """Give back all pages of the requests in ``rows``."""
@@ -233,7 +256,7 @@ class PagedKVCache:
                scale: Optional[float] = None, return_lse: bool = False):
         """One new token per request, q [max_requests,Hq,1,dh], over its cached context (see
         ``paged_decode_attention``)."""
-        return paged_decode_attention(q, self.k_pages[layer], self.v_pages[layer], self.block_table, self.lens,
+        return paged_decode_attention(q, self.k_pages[layer], self.v_pages[layer], self.block_table, self._lens,
                                       k_new=k_new, v_new=v_new, active=active, window=window, scale=scale,
                                       return_lse=return_lse, workspace=self.workspace)
 

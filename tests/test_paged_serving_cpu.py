@@ -30,6 +30,7 @@ class _Cache:
 
     def __init__(self, pages=12):
         self.max_requests, self.lens, self.free = ROWS, torch.zeros(ROWS, dtype=torch.int32), pages
+        self.block_table = torch.zeros(ROWS, 4, dtype=torch.int32)
         self.written = 0
 
     def reserve(self, add, num_tokens=None):
