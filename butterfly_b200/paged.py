@@ -27,6 +27,7 @@ import torch
 
 from . import _lib
 
+MAX_REQUESTS = 4096  # requests of one reservation call
 RELEASE = -2 ** 31  # an ``add`` entry that gives all of a request's pages back
 
 
@@ -184,6 +185,8 @@ class PagedKVCache:
     def __init__(self, *, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  max_requests: int, max_tokens_per_request: int, dtype: torch.dtype = torch.bfloat16,
                  device: torch.device | str = "cuda") -> None:
+        if not 0 < int(max_requests) <= MAX_REQUESTS:
+            raise ValueError(f"max_requests must be in [1, {MAX_REQUESTS}], what one reservation serves")
         self.page_size = int(page_size)
         shape = (int(num_pages), int(num_kv_heads), self.page_size, int(head_dim))
         # every read goes through a row written before, so the pools need no clearing

@@ -1,0 +1,21 @@
+"""Refusals of PagedKVCache that need no device."""
+import pytest
+
+import butterfly_b200 as bb
+
+
+def _cache(**kw):
+    a = dict(num_layers=1, num_pages=4, page_size=16, num_kv_heads=1, head_dim=64, max_requests=3, max_tokens_per_request=64,
+             device="cpu")
+    a.update(kw)
+    return bb.PagedKVCache(**a)
+
+
+@pytest.mark.parametrize("requests", [0, -1, 4097, 10000])
+def test_request_counts_that_no_reservation_takes(requests):
+    with pytest.raises(ValueError, match="max_requests"):
+        _cache(max_requests=requests)
+
+
+def test_the_most_requests():
+    assert _cache(max_requests=4096).max_requests == 4096
