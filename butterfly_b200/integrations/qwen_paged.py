@@ -65,6 +65,11 @@ class PagedQwenDecoder:
         self.live = [False] * max_requests
         self._live_add = None  # device tensor of one token per live request, renewed when they change
 
+    def _check_rows(self, rows: Sequence[int]) -> None:
+        for b in rows:
+            if not 0 <= b < self.cache.max_requests:
+                raise ValueError(f"there is no row {b}: the cache has {self.cache.max_requests}")
+
     @torch.no_grad()
     def add(self, prompts: Mapping[int, torch.Tensor]) -> dict[int, torch.Tensor]:
         """Admit prompts (1-D token ids) into vacant rows; returns their next-token logits.  Raises
@@ -72,6 +77,7 @@ class PagedQwenDecoder:
         when the model's forward raises."""
         from transformers import DynamicCache
         rows = sorted(prompts)
+        self._check_rows(rows)
         for b in rows:
             if self.live[b]:
                 raise ValueError(f"row {b} is in use")
@@ -102,6 +108,7 @@ class PagedQwenDecoder:
 
     def finish(self, rows: Sequence[int]) -> None:
         """Give the rows' pages back."""
+        self._check_rows(rows)
         self.cache.release(rows)
         for b in rows:
             self.live[b] = False

@@ -247,6 +247,8 @@ class PagedKVCache:
         """Give back all pages of the requests in ``rows``."""
         add = [0] * self.max_requests
         for b in rows:
+            if not 0 <= int(b) < self.max_requests:
+                raise ValueError(f"there is no row {int(b)}: the cache has {self.max_requests}")
             add[int(b)] = RELEASE
         self.reserve(add)
 

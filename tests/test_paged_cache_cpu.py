@@ -19,3 +19,9 @@ def test_request_counts_that_no_reservation_takes(requests):
 
 def test_the_most_requests():
     assert _cache(max_requests=4096).max_requests == 4096
+
+
+@pytest.mark.parametrize("rows", [[-1], [3], [0, 7]])
+def test_release_of_rows_that_are_not_there(rows):
+    with pytest.raises(ValueError, match="row"):
+        _cache().release(rows)

@@ -130,3 +130,14 @@ def test_a_step_that_raises_advances_no_request(dec, monkeypatch):
             assert _state(dec) == before
     granted = dec.step(tokens)[1].tolist()
     assert granted == [True, False, True, False] and dec.cache.lens.tolist() == [17, 0, 21, 64]
+
+
+@pytest.mark.parametrize("row", [-1, ROWS, ROWS + 3])
+def test_rows_that_are_not_there(dec, row):
+    dec.add({0: _ids(5), ROWS - 1: _ids(20)})
+    before = _state(dec)
+    with pytest.raises(ValueError, match="row"):
+        dec.add({row: _ids(4), 1: _ids(3)})
+    with pytest.raises(ValueError, match="row"):
+        dec.finish([0, row])
+    assert _state(dec) == before
