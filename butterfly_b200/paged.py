@@ -232,8 +232,13 @@ class PagedKVCache:
         all layers.  ``num_tokens`` may be left out when ``add`` is a host sequence."""
         if not isinstance(add, torch.Tensor):
             add = [int(x) for x in add]
+            if len(add) != self.max_requests:
+                raise ValueError("add must have one entry per row")
+            added = sum(max(x, 0) for x in add)
             if num_tokens is None:
-                num_tokens = sum(max(x, 0) for x in add)
+                num_tokens = added
+            elif num_tokens < added:
+                raise ValueError(f"num_tokens is {num_tokens}, but add has {added} tokens to give slots to")
             add = torch.tensor(add, dtype=torch.int32).to(self._state.device, non_blocking=True)
         if num_tokens is None:
             raise ValueError("num_tokens is needed when add is a device tensor")

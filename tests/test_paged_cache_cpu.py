@@ -25,3 +25,14 @@ def test_the_most_requests():
 def test_release_of_rows_that_are_not_there(rows):
     with pytest.raises(ValueError, match="row"):
         _cache().release(rows)
+
+
+@pytest.mark.parametrize("add,tokens", [([3, 0, 2], 4), ([1, 1, 1], 0), ([-5, 40, 0], 39)])
+def test_slot_maps_shorter_than_the_tokens_of_a_host_list(add, tokens):
+    with pytest.raises(ValueError, match="num_tokens"):
+        _cache().reserve(add, tokens)
+
+
+def test_host_lists_of_another_length():
+    with pytest.raises(ValueError, match="one entry per row"):
+        _cache().reserve([1, 1])
