@@ -37,9 +37,16 @@ from .qwen_torch import _get_decoder_with_layers, _has_required_qwen_attention_a
 class _Layer:
     def __init__(self, layer: nn.Module):
         attn, mlp = getattr(layer, "self_attn", None), getattr(layer, "mlp", None)
-        if (attn is None or not _has_required_qwen_attention_attrs(attn) or int(attn.head_dim) != 128
-                or not _is_qwen35_norm(getattr(attn, "q_norm", None)) or not _is_qwen35_norm(layer.input_layernorm)):
+        if attn is None or mlp is None or not _has_required_qwen_attention_attrs(attn) or int(attn.head_dim) != 128:
             raise ValueError("PagedQwenDecoder needs dense Qwen3.5 full-attention layers with head_dim 128")
+        norms = [getattr(attn, "q_norm", None), getattr(attn, "k_norm", None), layer.input_layernorm, layer.post_attention_layernorm]
+        # (one launch normalises q and k, with one eps)
+        if not all(_is_qwen35_norm(x) for x in norms) or norms[0].eps != norms[1].eps:
+            raise ValueError("PagedQwenDecoder needs Qwen3.5 RMSNorms, q_norm and k_norm with one eps")
+        if type(getattr(mlp, "act_fn", None)).__name__ not in ("SiLU", "SiLUActivation"):
+            raise ValueError("PagedQwenDecoder needs the SiLU activation")
+        if abs(float(getattr(attn, "scaling", 128 ** -0.5)) - 128 ** -0.5) > 1e-6:
+            raise ValueError("PagedQwenDecoder needs attention scaled by head_dim ** -0.5")
         for lin in (attn.q_proj, attn.k_proj, attn.v_proj, attn.o_proj, mlp.gate_proj, mlp.up_proj, mlp.down_proj):
             if getattr(lin, "bias", None) is not None:
                 raise ValueError("PagedQwenDecoder needs bias-free projections")
@@ -57,6 +64,9 @@ class PagedQwenDecoder:
                  page_size: int = 64):
         patch_qwen35_full_attention_decode()
         self.model, self.decoder = model, _get_decoder_with_layers(model)
+        head = getattr(model, "lm_head", None)
+        if not _is_qwen35_norm(getattr(self.decoder, "norm", None)) or not isinstance(head, nn.Linear) or head.bias is not None:
+            raise ValueError("PagedQwenDecoder needs a Qwen3.5 final norm and a bias-free lm_head")
         self.layers = [_Layer(layer) for layer in self.decoder.layers]
         w = self.layers[0].w_qkv
         self.cache = PagedKVCache(num_layers=len(self.layers), num_pages=num_pages, page_size=page_size,

@@ -141,3 +141,26 @@ def test_rows_that_are_not_there(dec, row):
     with pytest.raises(ValueError, match="row"):
         dec.finish([0, row])
     assert _state(dec) == before
+
+
+def _plain_norm(n):
+    return torch.nn.RMSNorm(n)
+
+
+@pytest.mark.parametrize("change", [
+    lambda m: setattr(m.model.layers[1].self_attn, "q_norm", _plain_norm(128)),
+    lambda m: setattr(m.model.layers[1].self_attn, "k_norm", _plain_norm(128)),
+    lambda m: setattr(m.model.layers[0], "input_layernorm", _plain_norm(256)),
+    lambda m: setattr(m.model.layers[0], "post_attention_layernorm", _plain_norm(256)),
+    lambda m: setattr(m.model.layers[0].self_attn.k_norm, "eps", 1e-3),
+    lambda m: setattr(m.model.layers[0].self_attn, "scaling", 0.5),
+    lambda m: setattr(m.model.layers[1].mlp, "act_fn", torch.nn.GELU()),
+    lambda m: setattr(m.model, "norm", _plain_norm(256)),
+    lambda m: setattr(m, "lm_head", torch.nn.Linear(256, VOCAB, bias=True)),
+    lambda m: setattr(m.model.layers[1].mlp, "down_proj", torch.nn.Linear(256, 256, bias=True)),
+])
+def test_models_that_the_step_would_not_follow_are_refused(change):
+    m = _model()
+    change(m)
+    with pytest.raises(ValueError, match="PagedQwenDecoder needs"):
+        PagedQwenDecoder(m, max_requests=ROWS, num_pages=12, page_size=PAGE, max_tokens_per_request=64)
