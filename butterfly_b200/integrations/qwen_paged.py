@@ -11,7 +11,8 @@ into pages (``paged_append``); a decode step advances all requests by one token:
                 paged_decode_attention (writes the token's rows, attends), gate + o_proj +
                 residual, rmsnorm + SwiGLU, down_proj + residual
 
-with the fused glue of ``butterfly_b200.glue`` (weight-streaming GEMVs for up to 8 rows).
+with the fused glue of ``butterfly_b200.glue`` (weight-streaming GEMVs for up to 8 rows and input
+sizes that are multiples of 256 up to 8,192).
 
     dec = PagedQwenDecoder(model, max_requests=8, num_pages=4096, max_tokens_per_request=32768)
     logits = dec.add({0: ids0, 3: ids3})                # {row: next-token logits}
@@ -72,6 +73,9 @@ class PagedQwenDecoder:
         self.cache = PagedKVCache(num_layers=len(self.layers), num_pages=num_pages, page_size=page_size,
                                   num_kv_heads=self.layers[0].hkv, head_dim=128, max_requests=max_requests,
                                   max_tokens_per_request=max_tokens_per_request, dtype=w.dtype, device=w.device)
+        # the weight-streaming GEMVs take up to 8 rows, and inputs of these sizes; else library products
+        sizes = [n for st in self.layers for n in (st.w_qkv.shape[1], 128 * st.hq, st.inter)]
+        self._few = max_requests <= 8 and all(n % 256 == 0 and n <= 8192 for n in sizes)
         self.live = [False] * max_requests
         self._live_add = None  # device tensor of one token per live request, renewed when they change
 
@@ -145,7 +149,7 @@ class PagedQwenDecoder:
 
     def _forward(self, ids: torch.Tensor, r: PagedReservation) -> torch.Tensor:
         R = self.cache.max_requests
-        few = R <= 8  # rows the weight-streaming GEMVs take
+        few = self._few
         pos = (r.lens - 1).clamp(min=0).long()[:, None]
         x = self.decoder.embed_tokens(ids)
         cos, sin = self.decoder.rotary_emb(x, pos)
