@@ -191,6 +191,9 @@ def main() -> None:
     ap.add_argument("--prompt", type=int, default=4096, help="longest prompt; request i has a 1 / (i + 1) of it")
     ap.add_argument("--steps", type=int, default=64)
     args = ap.parse_args()
+    if args.steps < 1:
+        ap.error("--steps must be at least 1")
+    untimed = min(3, args.steps - 1)
     cfg = Qwen3_5TextConfig(hidden_size=1024, num_attention_heads=8, num_key_value_heads=2, head_dim=128,
                             num_hidden_layers=args.layers, layer_types=["full_attention"] * args.layers,
                             intermediate_size=3584, vocab_size=32000, partial_rotary_factor=0.25)
@@ -204,13 +207,13 @@ def main() -> None:
     logits = dec.add({i: torch.randint(0, 32000, (n,), device="cuda") for i, n in enumerate(lens)})
     tokens = torch.stack([logits[i].argmax() for i in range(args.requests)])
     for s in range(args.steps):
-        if s == 3:
+        if s == untimed:
             torch.cuda.synchronize()
             t0 = time.perf_counter()
         logits, _ = dec.step(tokens)
         tokens = logits.argmax(-1)
     torch.cuda.synchronize()
-    ms = (time.perf_counter() - t0) / max(1, args.steps - 3) * 1e3
+    ms = (time.perf_counter() - t0) / (args.steps - untimed) * 1e3
     print(f"{args.requests} requests of {min(lens)} to {max(lens)} prompt tokens: {ms:.3f} ms a step, "
           f"{args.requests / ms * 1e3:.0f} tokens/s; lengths now {dec.cache.lens.tolist()}, "
           f"{int(dec.cache.num_free)} of {int(dec.cache.free_pages.numel())} pages free")

@@ -44,3 +44,11 @@ def test_intermediate_sizes(inter, heads, rows):
         for b, ids in prompts.items():
             ref = model(input_ids=ids[None]).logits[0, -1].float()
             assert float((logits[b].float() - ref).abs().max()) <= 3e-2 * float(ref.abs().max())
+
+
+@pytest.mark.parametrize("steps", [1, 3, 5])
+def test_example_of_a_few_steps(steps, monkeypatch, capsys):
+    from butterfly_b200.integrations import qwen_paged
+    monkeypatch.setattr("sys.argv", ["qwen_paged", "--layers", "1", "--requests", "2", "--prompt", "40", "--steps", str(steps)])
+    qwen_paged.main()
+    assert f"lengths now [{40 + steps}, {20 + steps}]" in capsys.readouterr().out
