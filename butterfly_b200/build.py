@@ -14,6 +14,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from importlib import metadata
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -48,8 +49,12 @@ def _compile(src: str, verbose: bool) -> str:
 
 
 def _build_binding() -> str:
-    if os.path.exists(NATIVE) and os.path.getmtime(NATIVE) >= max(os.path.getmtime(BINDING), _headers()):
-        return NATIVE
+    # what it was built against, beside the objects: another torch or Python may lay its types out anew
+    stamp, built_for = os.path.join(BUILD, "_native.for"), f"torch {metadata.version('torch')}, python {sys.version}"
+    if os.path.exists(NATIVE) and os.path.getmtime(NATIVE) >= max(os.path.getmtime(BINDING), _headers()) and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == built_for:
+                return NATIVE
     import torch
     root = os.path.dirname(torch.__file__)
     inc, libs = os.path.join(root, "include"), os.path.join(root, "lib")
@@ -60,6 +65,8 @@ def _build_binding() -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {BINDING}:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(built_for)
     return NATIVE
 
 
