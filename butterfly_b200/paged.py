@@ -139,7 +139,12 @@ def _workspace_for(x: torch.Tensor, stream: int) -> torch.Tensor:
     pass one to share it): its replays may run beside later calls on the stream."""
     if not x.is_cuda:
         raise ValueError("butterfly_b200 kernels run on CUDA tensors only (no CPU path)")
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_getDevice() == x.get_device():
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(x.device):  # (the question is about the current device's stream)
+            capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
         return decode_workspace(x.device)
     ws = _workspaces.get((x.get_device(), stream))
     if ws is None:

@@ -36,3 +36,33 @@ def test_slot_maps_shorter_than_the_tokens_of_a_host_list(add, tokens):
 def test_host_lists_of_another_length():
     with pytest.raises(ValueError, match="one entry per row"):
         _cache().reserve([1, 1])
+
+
+def test_capture_is_looked_up_on_the_tensors_device(monkeypatch):
+    # a call on device 1, whose stream captures, while device 0 is current (the devices are stand-ins)
+    from types import SimpleNamespace
+
+    import torch
+
+    from butterfly_b200 import paged
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *a):
+            current[0] = self.before
+
+    x = SimpleNamespace(is_cuda=True, get_device=lambda: 1, device=1)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == 1)
+    monkeypatch.setattr(paged, "decode_workspace", lambda device: object())
+    monkeypatch.setattr(paged, "_workspaces", {})
+    assert paged._workspace_for(x, 7) is not paged._workspace_for(x, 7) and not paged._workspaces
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert paged._workspace_for(x, 7) is paged._workspace_for(x, 7) and current == [0]
