@@ -95,8 +95,9 @@ _made: dict = {}  # id -> weak reference to every workspace there is, for reset_
 
 def decode_workspace(device: torch.device | str | int = "cuda") -> torch.Tensor:
     """A workspace for ``paged_decode_attention`` calls that follow one another on a stream."""
-    ws = torch.empty(_lib.lib().bna_paged_decode_workspace_bytes(), dtype=torch.uint8, device=device)
-    ws[:4096].zero_()  # the arrival counters; every call leaves them zero
+    with torch.inference_mode(False):  # (an inference tensor could not be zeroed again outside that mode)
+        ws = torch.empty(_lib.lib().bna_paged_decode_workspace_bytes(), dtype=torch.uint8, device=device)
+        ws[:4096].zero_()  # the arrival counters; every call leaves them zero
     key = id(ws)
     _made[key] = weakref.ref(ws, lambda _: _made.pop(key, None))
     return ws
@@ -199,9 +200,10 @@ class PagedKVCache:
         self.v_pages = [torch.empty(shape, dtype=dtype, device=device) for _ in range(int(num_layers))]
         width = -(-int(max_tokens_per_request) // self.page_size)
         self.block_table = torch.full((int(max_requests), width), -1, dtype=torch.int32, device=device)
-        self._state = torch.zeros(int(max_requests) + 1, dtype=torch.int32, device=device)
-        self._lens, self._num_free = self._state[:-1], self._state[-1:]
-        self._num_free.fill_(int(num_pages))
+        with torch.inference_mode(False):  # (updated in place, in whichever mode the caller is then)
+            self._state = torch.zeros(int(max_requests) + 1, dtype=torch.int32, device=device)
+            self._lens, self._num_free = self._state[:-1], self._state[-1:]
+            self._num_free.fill_(int(num_pages))
         self.free_pages = torch.arange(int(num_pages) - 1, -1, -1, dtype=torch.int32, device=device)
         self.workspace = decode_workspace(device)
 

@@ -131,3 +131,18 @@ def test_lengths_handed_out_are_of_their_time():
     assert r.lens.tolist() == [4, 50, 0] and cache.lens.tolist() == [5, 51, 1]
     cache.lens, cache.num_free = before, free
     assert cache.lens.tolist() == [3, 0, 40] and torch.equal(cache.num_free, free)
+
+
+@pytest.mark.parametrize("inside", ["make", "use", "both"])
+def test_inference_mode(inside):
+    with torch.inference_mode(inside != "use"):
+        rnd, cache = _filled(6, [30, 0, 5])
+    with torch.inference_mode(inside != "make"):
+        q, kn, vn = rnd(3, 8, 1, 128), rnd(3, 2, 1, 128), rnd(3, 2, 1, 128)
+        add = torch.tensor([1, 0, 1], dtype=torch.int32, device=DEV)
+        for i in range(2):
+            out = _step(cache, add, q, kn, vn)
+            assert cache.lens.tolist() == [31 + i, 0, 6 + i] == out[2].tolist()
+        cache.lens = cache.lens - 1
+        assert cache.lens.tolist() == [31, -1, 6]
+        paged.reset_workspaces()
