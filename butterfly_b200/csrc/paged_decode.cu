@@ -5,9 +5,11 @@
 // parts is joined by  M = max m_i,  L = sum l_i 2^(m_i - M),  out = sum o_i 2^(m_i - M) / L
 // (m in the exp2 domain).
 //
-// Each key and value is read once and serves the G = Hq / Hkv query heads of its KV head:
-// 2 G FLOP per byte, far below the tensor cores' balance, so the kernel is bound by HBM and is
-// built to keep its reads in flight:
+// Each key and value is read once and serves the G = Hq / Hkv query heads of its KV head (more than 16
+// in chunks of equal size, each of which reads them: 16 requests of 16,384 tokens, 2 KV heads of
+// 128, take 56.5 us with 16 query heads per KV head and 93.3 us with 32): 2 G FLOP per byte,
+// far below the tensor cores' balance, so the kernel is bound by HBM and is built to keep its
+// reads in flight:
 //   * The keys of a pair (request, KV head) come in granules of 16.  One persistent CTA per SM (two
 //     at head_dim 64) takes either whole pairs, as they are claimed (in turn, if all are short), or, where single pairs
 //     are long beside an even share, an equal stretch of the line of all granules: one long
@@ -22,8 +24,8 @@
 //     the lengths and the grid, whichever CTA runs when: equal calls give equal bits.
 // Measured (GPU time, bf16, 8 / 2 heads of 128): 64 x 65,536 tokens 610 us = 7.0 TB/s (a copy reaches
 // 6.45 TB/s here), DRAM reads equal to the keys and values, tensor pipe 17% busy; one request of
-// 131,072 tokens 34.5 us = 3.9 TB/s: 4 us until the first granule, 19 to 22 us of reads, 7 us from
-// the last CTA's arrival through two rounds of joins; four requests of 37 to 513 tokens 9.0 us,
+// 131,072 tokens 34.4 us = 3.9 TB/s: 4 us until the first granule, 19 to 22 us of reads, 7 us from
+// the last CTA's arrival through two rounds of joins; four requests of 37 to 513 tokens 9.1 us,
 // a chain of dependent reads (lengths, pages, keys) and one pass of the code.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -209,7 +211,10 @@ __device__ __forceinline__ bool cons_any(bool bad) {
 // 8-15 of the P V product carry the low part of the probabilities.  A probability is held
 // as hi + lo in the 16-bit type, scaled (kShift; relative error u^2 instead of u: rounding it once would add
 // as much error to the output as its final rounding does); with at most 8 heads lo rides in rows
-// that the MMA computes anyway, with more it costs a second MMA, which the memory hides.
+// that the MMA computes anyway, with more it costs a second MMA, which the memory hides.  The MMA
+// cuts its fp32 sums off instead of rounding them, some hundreds of steps a warp and part: of 64
+// requests with 65,536 tokens 0.37% of the bf16 results (2.1% in fp16) are the neighbours of the
+// correctly rounded ones, of 400 tokens 0.12% (0.19%); fp32 arithmetic gives 0.06% (0.48%).
 template <typename T, int DH, bool WIDE>
 __global__ void __launch_bounds__(Layout<DH>::kThreads, Layout<DH>::kCtas)
     paged_decode_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const PagedArgs a) {

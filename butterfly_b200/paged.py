@@ -74,7 +74,8 @@ def paged_reserve(lens: torch.Tensor, add: torch.Tensor, block_table: torch.Tens
     while pages last; one that is refused (``add > 0`` and not ``granted``) keeps its length.  The added
     tokens of request 0, then 1, ... are entries 0, 1, ... of ``slot_map`` and ``positions``
     (``num_tokens`` of them: at least the sum of the positive ``add``).  ``block_table`` and
-    ``free_pages`` are updated in place, the lengths and the stack height are returned."""
+    ``free_pages`` are updated in place, the lengths and the stack height are returned.  A page
+    belongs to one row: one that two rows name would come back on the stack twice."""
     r = (_native or _binding()).reserve(lens, add, block_table, free_pages, num_free, page_size, num_tokens, _stream(lens),
                                         None)
     if r.__class__ is int:
@@ -166,7 +167,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     ``active`` [B] bool names (default: all; pass ``PagedReservation.granted`` where some
     requests got no room, or rest).  Returns [B,Hq,1,dh] in q's dtype, contiguous (so that
     ``transpose(1, 2)`` is [B,1,Hq,dh] storage); with ``return_lse`` also the fp32 natural-log sums
-    [B,Hq,1].  A request of length 0 gives zeros and -inf.  ``workspace`` (``decode_workspace``)
+    [B,Hq,1].  A request of length 0 gives zeros and -inf; an infinite value attended to gives an
+    infinity or NaN in its column.  ``workspace`` (``decode_workspace``)
     defaults to one kept per stream; calls that may overlap need one each.  Lengths and tables
     must not change while the call runs; ``take_device_error`` tells whether a kernel gave up."""
     stream = _stream(q)

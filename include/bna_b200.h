@@ -371,8 +371,10 @@ BNA_API int bna_prefill_attention_static_scratch(const bna_tensor4* q, const bna
  * need pages are refused too once the pages asked for so far exceed the stack.  slot_map / positions [num_tokens] hold the added tokens
  * of request 0, then 1, ... (-1 past the last).  lens and num_free are read only; lens_out
  * [requests] and num_free_out [1] are written (not in place).  block_table and free_pages are
- * updated in place; entries past a request's pages keep their old values.  requests <= 4096;
- * with none nothing is written. */
+ * updated in place; entries past a request's pages keep their old values.  A page belongs to one row:
+ * one that two rows name would come back on the stack twice.  Where slot_map is shorter than the
+ * added tokens, the tables and lengths still cover all of them.  requests <= 4096; with none
+ * nothing is written. */
 BNA_API int bna_paged_reserve(const int32_t* lens, const int32_t* add, int32_t requests, int32_t* block_table,
                               int64_t table_stride, int32_t table_width, int32_t* free_pages, int32_t num_pages,
                               const int32_t* num_free, int32_t page_size, int32_t* lens_out, int32_t* num_free_out,
@@ -388,7 +390,8 @@ BNA_API int bna_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_ten
  * [max(0, lens[b] - window), lens[b]) of request b (window 0: all of them), Hq a multiple of Hkv;
  * lse (optional, fp32, natural log, element strides) of the softmax.  lens[b] counts the new
  * token.  A request of length 0 gets out = 0, lse = -inf, and so does a row whose scores are
- * all -inf; what pages hold beyond the keys attended to (NaN included) does not matter.  With
+ * all -inf; what pages hold beyond the keys attended to (NaN included) does not matter.  An infinite
+ * value among those attended to gives an infinity or NaN in its column.  With
  * k_new / v_new [B, Hkv, 1, dh] the row at position lens[b] - 1 is taken from them and written
  * into its page, for the requests with active[b] != 0 (null: all; the others attend to what
  * their pages hold).  A length is cut to table_width * page_size; a page number outside the pool reads
