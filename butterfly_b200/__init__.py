@@ -9,6 +9,7 @@ from .topology import (BlockHamiltonianLayout, build_block_butterfly_layout, bui
                        butterfly_stage_meta, butterfly_width, num_blocks_for_seq_len)
 from .attention import (block_mean_summaries, butterfly_compressed_attention,
                         butterfly_compressed_attention_active)
+from .logits import TokenLogprobs, token_logprobs
 from .paged import PagedKVCache, paged_append, paged_decode_attention, paged_reserve
 
 __all__ = [
@@ -16,4 +17,5 @@ __all__ = [
     "butterfly_stage_meta", "butterfly_width", "num_blocks_for_seq_len", "block_mean_summaries",
     "butterfly_compressed_attention", "butterfly_compressed_attention_active",
     "PagedKVCache", "paged_append", "paged_decode_attention", "paged_reserve",
+    "TokenLogprobs", "token_logprobs",
 ]

@@ -26,6 +26,7 @@ EXPORTED = (
     "bna_gemv", "bna_launch_probe", "bna_decode_step_qk", "bna_prefill_attention_gated",
     "bna_gemm_swiglu", "bna_gemm_qkv_norm_rope", "bna_gemm_residual", "bna_row_sumsq",
     "bna_paged_reserve", "bna_paged_append", "bna_paged_decode", "bna_paged_decode_workspace_bytes",
+    "bna_token_logprobs",
 )
 
 
@@ -97,6 +98,7 @@ def lib() -> ctypes.CDLL:
             "bna_paged_append": (i32, [T4, T4, T4, T4, vp, i32, vp]),
             "bna_paged_decode": (i32, [T4, T4, T4, T4, T4, vp, T4, vp, i64, i64, i32, vp, i64, i32, vp, i32, f32, vp, i64, vp]),
             "bna_paged_decode_workspace_bytes": (i64, []),
+            "bna_token_logprobs": (i32, [vp, i64, i64, i64, i64, i64, i32, vp, i32, vp, vp, vp, vp, i32, vp]),
             "bna_decode_step": (i32, [T4, T4, T4, T4, T4, T4, T4, T4, vp, i64, i64, i32, R, i32, i64, i64, i64, i64, i32, f32, vp]),
         }
         for name, (res, args) in sig.items():
@@ -105,6 +107,34 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+# The compiled binding's calls (csrc/binding.cpp), in the order of their addresses in its init.
+_BOUND = ("bna_paged_reserve", "bna_paged_append", "bna_paged_decode", "bna_token_logprobs")
+_native = None
+
+
+def native():
+    """The compiled binding, given the C entry points of the loaded library."""
+    global _native
+    if _native is None:
+        try:
+            from . import _native as mod
+        except ImportError as e:
+            raise ImportError(f"butterfly_b200/_native.so is missing or stale: build it with "
+                              f"`python -m butterfly_b200.build` ({e})") from e
+        L = lib()
+        mod.init(*(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BOUND))
+        _native = mod
+    return _native
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object
+
+
+def raw_stream(x: torch.Tensor) -> int:
+    """The handle of the current stream of x's device."""
+    return _raw_stream(x.get_device()) if getattr(x, "is_cuda", False) else 0  # (other things are refused further on)
 
 
 def check(status: int) -> None:

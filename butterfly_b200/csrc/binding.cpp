@@ -1,5 +1,5 @@
-// binding.cpp — CPython functions behind butterfly_b200.paged: argument checks, output tensors and
-// the C call in one step.  The kernels of a serving step take 2 to 10 us, and the same work in
+// binding.cpp — CPython functions behind butterfly_b200.paged and butterfly_b200.logits: argument checks, output
+// tensors and the C call in one step.  The kernels of a serving step take 2 to 10 us, and the same work in
 // Python (a ctypes call, packed descriptors, torch.empty) took 7 to 19 us a call.
 // The C entry points come in as addresses (init), from the library that ctypes has loaded.
 #define PY_SSIZE_T_CLEAN
@@ -19,6 +19,7 @@ namespace {
 decltype(&bna_paged_reserve) g_reserve = nullptr;
 decltype(&bna_paged_append) g_append = nullptr;
 decltype(&bna_paged_decode) g_decode = nullptr;
+decltype(&bna_token_logprobs) g_logprobs = nullptr;
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) throw torch::TypeError(std::string(name) + " must be a torch.Tensor");
@@ -93,13 +94,14 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
   return r;
 }
 
-// init(reserve, append, decode): addresses of the C entry points.
+// init(reserve, append, decode, logprobs): addresses of the C entry points.
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arity(n, 3);
+  arity(n, 4);
   g_reserve = reinterpret_cast<decltype(g_reserve)>(address(a[0]));
   g_append = reinterpret_cast<decltype(g_append)>(address(a[1]));
   g_decode = reinterpret_cast<decltype(g_decode)>(address(a[2]));
+  g_logprobs = reinterpret_cast<decltype(g_logprobs)>(address(a[3]));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -235,6 +237,74 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// logprobs(logits, tokens, k, stream) -> logprobs (or None), entropy, top_ids, top_logprobs
+PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 4);
+  const at::Tensor& x = tensor(a[0], "logits");
+  need_cuda({&x});
+  const c10::DeviceGuard guard(x.device());
+  const int64_t dims = x.dim();
+  need(dims >= 1 && (x.size(-1) <= 1 || x.stride(-1) == 1), "logits must have a contiguous last dim");
+  const auto type = x.scalar_type();
+  need(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "logits must be bfloat16, float16 or float32");
+  const int64_t V = x.size(-1), rows = V ? x.numel() / V : 0, k = integer(a[2]);
+  need(V > 0, "logits must have at least one entry a row");
+  need(k >= 0 && k <= 64 && k <= V, "top_k must be in [0, min(64, the vocabulary)]");
+  // the leading dims as runs of `inner` evenly spaced rows, evenly spaced themselves
+  int64_t inner = 1, stride = 0, outer = 1, outer_stride = 0;
+  bool runs = false;
+  for (int64_t d = dims - 2; d >= 0; --d) {
+    const int64_t size = x.size(d), st = x.stride(d);
+    if (size <= 1) continue;
+    if (!runs && inner == 1) {
+      inner = size;
+      stride = st;
+    } else if (!runs && st == stride * inner) {
+      inner *= size;
+    } else if (!runs) {
+      runs = true;
+      outer = size;
+      outer_stride = st;
+    } else {
+      need(st == outer_stride * outer, "the leading dims of logits must be two evenly strided ones at most");
+      outer *= size;
+    }
+  }
+  const auto lead = x.sizes().slice(0, dims - 1);
+  at::Tensor tokens;
+  if (a[1] != Py_None) {
+    const at::Tensor& t = tensor(a[1], "tokens");
+    need_cuda({&x, &t});
+    need(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, "tokens must be int64 or int32");
+    need(t.sizes() == lead, "tokens must have logits' leading shape");
+    tokens = t.contiguous();
+  }
+  // one allocation: ids, then log probabilities of the top, entropies, log probabilities of the tokens
+  const int64_t top = rows * k;
+  const at::Tensor all = empty(x, {12 * top + 8 * rows}, at::kByte);
+  at::Tensor ids = part(all, 0, top, at::kLong), top_lp = part(all, 8 * top, top, at::kFloat),
+             entropy = part(all, 12 * top, rows, at::kFloat), lp;
+  if (tokens.defined()) lp = part(all, 12 * top + 4 * rows, rows, at::kFloat);
+  const int st = g_logprobs(x.data_ptr(), stride, outer_stride, rows, inner, V,
+                            type == at::kFloat ? BNA_F32 : type == at::kHalf ? BNA_F16 : BNA_BF16,
+                            tokens.defined() && rows ? tokens.data_ptr() : nullptr, tokens.defined() && tokens.scalar_type() == at::kLong,
+                            tokens.defined() && rows ? static_cast<float*>(lp.data_ptr()) : nullptr,
+                            static_cast<float*>(entropy.data_ptr()), static_cast<int64_t*>(ids.data_ptr()),
+                            static_cast<float*>(top_lp.data_ptr()), (int32_t)k, address(a[3]));
+  if (st != BNA_OK) return PyLong_FromLong(st);
+  c10::SmallVector<int64_t, 6> shape(lead.begin(), lead.end());
+  if (dims != 2) {
+    entropy.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    if (lp.defined()) lp.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+  }
+  shape.push_back(k);
+  ids.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+  top_lp.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+  return tuple_of({lp, entropy, ids, top_lp});
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyCFunction fast() {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F));
@@ -244,6 +314,7 @@ PyMethodDef methods[] = {{"init", fast<init>(), METH_FASTCALL, nullptr},
                          {"reserve", fast<reserve>(), METH_FASTCALL, nullptr},
                          {"append", fast<append>(), METH_FASTCALL, nullptr},
                          {"decode", fast<decode>(), METH_FASTCALL, nullptr},
+                         {"logprobs", fast<logprobs>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

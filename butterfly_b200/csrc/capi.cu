@@ -45,6 +45,8 @@ int launch_paged_decode(const bna_tensor4*, bna_tensor4*, bna_tensor4*, const bn
                         const uint8_t*, bna_tensor4*, float*, int64_t, int64_t, int, const int32_t*, int64_t, int, const int32_t*, int,
                         float, void*, cudaStream_t);
 int64_t paged_decode_workspace_bytes();
+int launch_token_logprobs(const void*, int64_t, int64_t, int64_t, int64_t, int, int, const void*, int, float*, float*, int64_t*, float*, int,
+                          cudaStream_t);
 
 // ---------------------------------------------------------------- validation helpers
 static bool null4(const bna_tensor4* t) { return t == nullptr || t->data == nullptr; }
@@ -517,6 +519,27 @@ int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_tensor4* v_
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BNA_BAD_STRIDE, "paged_decode: workspace must be 16-byte aligned");
   return launch_paged_decode(q, k_pages, v_pages, k_new, v_new, active, out, lse, lse_stride_b, lse_stride_h, dtype, block_table,
                              table_stride, table_width, lens, window, scale, workspace, (cudaStream_t)stream);
+}
+
+// ---------------------------------------------------------------- token log probabilities
+int bna_token_logprobs(const void* logits, int64_t stride, int64_t stride_outer, int64_t rows, int64_t inner, int64_t vocab, int32_t dtype,
+                       const void* tokens, int32_t tokens64, float* logprob, float* entropy, int64_t* top_ids, float* top_logprob,
+                       int32_t k, void* stream) {
+  if (dtype != BNA_BF16 && dtype != BNA_F16 && dtype != BNA_F32)
+    return fail(BNA_BAD_DTYPE, "token_logprobs: logits must be bfloat16, float16 or float32");
+  if (rows < 0 || vocab < 1 || vocab > INT32_MAX - 16) return fail(BNA_BAD_SHAPE, "token_logprobs: bad row count or vocabulary");
+  if (k < 0 || k > 64 || k > vocab) return fail(BNA_BAD_SHAPE, "token_logprobs: top_k must be in [0, min(64, vocabulary)]");
+  if (rows == 0) return BNA_OK;
+  if (inner < 1) return fail(BNA_BAD_SHAPE, "token_logprobs: inner must be positive");
+  if (!logits || !entropy || (tokens == nullptr) != (logprob == nullptr) || (k && (!top_ids || !top_logprob)))
+    return fail(BNA_BAD_SHAPE, "token_logprobs: null pointer");
+  const uintptr_t size = dtype == BNA_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % size || reinterpret_cast<uintptr_t>(tokens) % (tokens64 ? 8 : 4) ||
+      ((reinterpret_cast<uintptr_t>(logprob) | reinterpret_cast<uintptr_t>(entropy) | reinterpret_cast<uintptr_t>(top_logprob)) & 3) ||
+      (reinterpret_cast<uintptr_t>(top_ids) & 7))
+    return fail(BNA_BAD_STRIDE, "token_logprobs: pointers must be aligned to their elements");
+  return launch_token_logprobs(logits, stride, stride_outer, rows, inner, (int)vocab, dtype, tokens, tokens64 != 0, logprob, entropy, top_ids,
+                               top_logprob, k, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -40,28 +40,14 @@ class PagedReservation(NamedTuple):
     granted: torch.Tensor     # [B] bool: this request's added tokens have slots
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object
 _native = None
+_stream = _lib.raw_stream
 
 
 def _binding():
-    """The compiled binding (csrc/binding.cpp), given the C entry points of the loaded library."""
     global _native
-    if _native is None:
-        try:
-            from . import _native as mod
-        except ImportError as e:
-            raise ImportError(f"butterfly_b200/_native.so is missing or stale: build it with "
-                              f"`python -m butterfly_b200.build` ({e})") from e
-        L = _lib.lib()
-        mod.init(*(ctypes.cast(f, ctypes.c_void_p).value for f in (L.bna_paged_reserve, L.bna_paged_append,
-                                                                  L.bna_paged_decode)))
-        _native = mod
+    _native = _lib.native()
     return _native
-
-
-def _stream(x: torch.Tensor) -> int:
-    return _raw_stream(x.get_device()) if x.is_cuda else 0  # (a CPU tensor is refused further on)
 
 
 def paged_reserve(lens: torch.Tensor, add: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,

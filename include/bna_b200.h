@@ -44,7 +44,7 @@ typedef enum {
   BNA_DEVICE_TIMEOUT = 7  /* a kernel gave up a bounded wait and returned early               */
 } bna_status;
 
-typedef enum { BNA_BF16 = 0, BNA_F16 = 1 } bna_dtype;
+typedef enum { BNA_BF16 = 0, BNA_F16 = 1, BNA_F32 = 2 /* logits only */ } bna_dtype;
 
 /* Partner rules of bna/topology/butterfly.py:108-141 used by the block-sparse layout. */
 typedef enum {
@@ -407,6 +407,19 @@ BNA_API int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_ten
                              const int32_t* block_table, int64_t table_stride, int32_t table_width,
                              const int32_t* lens, int32_t window, float scale, void* workspace,
                              int64_t workspace_bytes, void* stream);
+
+/* ---- Token log probabilities -----------------------------------------------------------------
+ * No counterpart in the reference.  Row r of the logits (bf16, fp16 or fp32, `vocab` contiguous entries) starts at element
+ * (r / inner) * stride_outer + (r % inner) * stride.  Per row, in fp32 and natural logarithms, with p = softmax(row):
+ *   logprob[r] = log p[tokens[r]]: 0 for a negative token (padding), -inf for one that is not below vocab
+ *   entropy[r] = -sum p log p
+ *   top_ids / top_logprob [rows, k]: the k <= 64 likeliest entries, of equal ones the lowest index first
+ * A row whose entries are all -inf has log probabilities -inf and entropy 0.  A row with a NaN or +inf has NaN for
+ * both; its ids are in range, with NaN ordered as -inf.  tokens (int64, or int32 where tokens64 is 0) and
+ * logprob may both be null, and top_ids and top_logprob where k is 0.  Equal calls give equal bits. */
+BNA_API int bna_token_logprobs(const void* logits, int64_t stride, int64_t stride_outer, int64_t rows, int64_t inner, int64_t vocab,
+                               int32_t dtype, const void* tokens, int32_t tokens64, float* logprob, float* entropy,
+                               int64_t* top_ids, float* top_logprob, int32_t k, void* stream);
 
 #ifdef __cplusplus
 }
