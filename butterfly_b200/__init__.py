@@ -10,12 +10,14 @@ from .topology import (BlockHamiltonianLayout, build_block_butterfly_layout, bui
 from .attention import (block_mean_summaries, butterfly_compressed_attention,
                         butterfly_compressed_attention_active)
 from .logits import TokenLogprobs, token_logprobs
-from .paged import PagedKVCache, paged_append, paged_decode_attention, paged_reserve
+from .paged import (PagedKVCache, paged_append, paged_append_int4, paged_decode_attention,
+                    paged_decode_attention_int4, paged_read_int4, paged_reserve)
 
 __all__ = [
     "BlockHamiltonianLayout", "build_block_butterfly_layout", "build_block_wayfinder_layout",
     "butterfly_stage_meta", "butterfly_width", "num_blocks_for_seq_len", "block_mean_summaries",
     "butterfly_compressed_attention", "butterfly_compressed_attention_active",
     "PagedKVCache", "paged_append", "paged_decode_attention", "paged_reserve",
+    "paged_append_int4", "paged_read_int4", "paged_decode_attention_int4",
     "TokenLogprobs", "token_logprobs",
 ]

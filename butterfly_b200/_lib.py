@@ -26,7 +26,7 @@ EXPORTED = (
     "bna_gemv", "bna_launch_probe", "bna_decode_step_qk", "bna_prefill_attention_gated",
     "bna_gemm_swiglu", "bna_gemm_qkv_norm_rope", "bna_gemm_residual", "bna_row_sumsq",
     "bna_paged_reserve", "bna_paged_append", "bna_paged_decode", "bna_paged_decode_workspace_bytes",
-    "bna_token_logprobs",
+    "bna_paged_append_int4", "bna_paged_read_int4", "bna_paged_decode_int4", "bna_paged_decode_int4_workspace_bytes", "bna_token_logprobs",
 )
 
 
@@ -98,6 +98,10 @@ def lib() -> ctypes.CDLL:
             "bna_paged_append": (i32, [T4, T4, T4, T4, vp, i32, vp]),
             "bna_paged_decode": (i32, [T4, T4, T4, T4, T4, vp, T4, vp, i64, i64, i32, vp, i64, i32, vp, i32, f32, vp, i64, vp]),
             "bna_paged_decode_workspace_bytes": (i64, []),
+            "bna_paged_append_int4": (i32, [T4, T4, T4, vp, i32, vp]),
+            "bna_paged_read_int4": (i32, [T4, vp, T4, T4, i32, vp]),
+            "bna_paged_decode_int4": (i32, [T4, T4, T4, T4, vp, T4, vp, i64, i64, i32, vp, i64, i32, vp, i32, f32, vp, i64, vp]),
+            "bna_paged_decode_int4_workspace_bytes": (i64, []),
             "bna_token_logprobs": (i32, [vp, i64, i64, i64, i64, i64, i32, vp, i32, vp, vp, vp, vp, i32, vp]),
             "bna_decode_step": (i32, [T4, T4, T4, T4, T4, T4, T4, T4, vp, i64, i64, i32, R, i32, i64, i64, i64, i64, i32, f32, vp]),
         }
@@ -110,7 +114,8 @@ def lib() -> ctypes.CDLL:
 
 
 # The compiled binding's calls (csrc/binding.cpp), in the order of their addresses in its init.
-_BOUND = ("bna_paged_reserve", "bna_paged_append", "bna_paged_decode", "bna_token_logprobs")
+_BOUND = ("bna_paged_reserve", "bna_paged_append", "bna_paged_decode", "bna_token_logprobs", "bna_paged_append_int4",
+          "bna_paged_read_int4", "bna_paged_decode_int4")
 _native = None
 
 

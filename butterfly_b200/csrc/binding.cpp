@@ -20,6 +20,9 @@ decltype(&bna_paged_reserve) g_reserve = nullptr;
 decltype(&bna_paged_append) g_append = nullptr;
 decltype(&bna_paged_decode) g_decode = nullptr;
 decltype(&bna_token_logprobs) g_logprobs = nullptr;
+decltype(&bna_paged_append_int4) g_append_int4 = nullptr;
+decltype(&bna_paged_read_int4) g_read_int4 = nullptr;
+decltype(&bna_paged_decode_int4) g_decode_int4 = nullptr;
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) throw torch::TypeError(std::string(name) + " must be a torch.Tensor");
@@ -94,14 +97,17 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
   return r;
 }
 
-// init(reserve, append, decode, logprobs): addresses of the C entry points.
+// init(reserve, append, decode, logprobs, append_int4, read_int4, decode_int4): addresses of the C entry points.
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arity(n, 4);
+  arity(n, 7);
   g_reserve = reinterpret_cast<decltype(g_reserve)>(address(a[0]));
   g_append = reinterpret_cast<decltype(g_append)>(address(a[1]));
   g_decode = reinterpret_cast<decltype(g_decode)>(address(a[2]));
   g_logprobs = reinterpret_cast<decltype(g_logprobs)>(address(a[3]));
+  g_append_int4 = reinterpret_cast<decltype(g_append_int4)>(address(a[4]));
+  g_read_int4 = reinterpret_cast<decltype(g_read_int4)>(address(a[5]));
+  g_decode_int4 = reinterpret_cast<decltype(g_decode_int4)>(address(a[6]));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -153,6 +159,16 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// [tokens, heads, dh] as [1, heads, tokens, dh]
+bna_tensor4 rows4(const at::Tensor& x) {
+  return bna_tensor4{x.data_ptr(), {1, x.size(1), x.size(0), x.size(2)}, {0, x.stride(1), x.stride(0), x.stride(2)}};
+}
+
+void need_slots(const at::Tensor& slots, int64_t tokens) {
+  need(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == tokens && (slots.size(0) <= 1 || slots.stride(0) == 1),
+       "slot_map must be a contiguous int64 tensor with one entry per token");
+}
+
 // append(k, v, k_pages, v_pages, slot_map, stream): k / v [tokens, Hkv, dh]
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -164,19 +180,68 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   need(k.dim() == 3 && v.dim() == 3, "k and v must be [tokens, Hkv, dh]");
   const auto dt = k.scalar_type();
   need(v.scalar_type() == dt && kp.scalar_type() == dt && vp.scalar_type() == dt, "k, v and the pools must have one dtype");
-  need(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == k.size(0) &&
-           (slots.size(0) <= 1 || slots.stride(0) == 1),
-       "slot_map must be a contiguous int64 tensor with one entry per token");
-  bna_tensor4 rows[2];
-  const at::Tensor* src[2] = {&k, &v};
-  for (int i = 0; i < 2; ++i) {
-    const at::Tensor& x = *src[i];
-    rows[i] = bna_tensor4{x.data_ptr(), {1, x.size(1), x.size(0), x.size(2)}, {0, x.stride(1), x.stride(0), x.stride(2)}};
-  }
+  need_slots(slots, k.size(0));
+  const bna_tensor4 rows[2] = {rows4(k), rows4(v)};
   bna_tensor4 tkp = view4(kp, "k_pages"), tvp = view4(vp, "v_pages");
   return PyLong_FromLong(g_append(&rows[0], &rows[1], &tkp, &tvp, static_cast<const int64_t*>(slots.data_ptr()), dtype_code(k),
                                   address(a[5])));
   END_HANDLE_TH_ERRORS
+}
+
+// What both forms of decode check and pass on: the new rows, the requests that have them, tables, window and scale.
+struct DecodeCall {
+  bna_tensor4 q, kn, vn, out4;
+  const bna_tensor4 *k_new = nullptr, *v_new = nullptr;
+  const uint8_t* active = nullptr;
+  at::Tensor out, lse;
+  int64_t window;
+  double scale;
+  int32_t code;
+};
+void decode_call(DecodeCall& c, const at::Tensor& q, const at::Tensor& table, const at::Tensor& lens, const at::Tensor& ws, PyObject* k_new,
+                 PyObject* v_new, PyObject* active, PyObject* window, PyObject* scale, PyObject* lse) {
+  c.q = view4(q, "q");
+  const int64_t B = q.size(0), Hq = q.size(1), Tq = q.size(2), dh = q.size(3);
+  const auto dt = q.scalar_type();
+  need_ints(table, 2, "block_table");
+  need_ints(lens, 1, "lens");
+  need(table.size(0) == B && lens.size(0) == B, "block_table and lens must have one row per request");
+  need(table.size(1) <= INT32_MAX, "block_table: too many columns");
+  need(ws.scalar_type() == at::kByte && ws.is_contiguous(), "workspace must be a contiguous uint8 tensor (decode_workspace)");
+  const bool has_k = k_new != Py_None, has_v = v_new != Py_None;
+  need(has_k == has_v, "k_new and v_new go together");
+  if (has_k) {
+    const at::Tensor &kn = tensor(k_new, "k_new"), &vn = tensor(v_new, "v_new");
+    need_cuda({&q, &kn, &vn});
+    need(kn.scalar_type() == dt && vn.scalar_type() == dt, "q, k_new, v_new dtype mismatch");
+    c.kn = view4(kn, "k_new");
+    c.vn = view4(vn, "v_new");
+    c.k_new = &c.kn;
+    c.v_new = &c.vn;
+  }
+  if (active != Py_None) {
+    const at::Tensor& x = tensor(active, "active");
+    need_cuda({&q, &x});
+    need(x.scalar_type() == at::kBool && x.dim() == 1 && x.size(0) == B && x.is_contiguous(),
+         "active must be a contiguous bool tensor with one entry per request");
+    c.active = static_cast<const uint8_t*>(x.data_ptr());
+    need(has_k, "active says which requests have k_new / v_new rows");
+  }
+  c.window = integer(window);
+  need(c.window >= 0 && c.window <= INT32_MAX, "window must be in [0, 2^31) (0: every key)");
+  c.scale = PyFloat_AsDouble(scale);
+  if (c.scale == -1.0 && PyErr_Occurred()) throw python_error();
+  const int want_lse = PyObject_IsTrue(lse);
+  if (want_lse < 0) throw python_error();
+  c.code = dtype_code(q);
+  c.out = empty(q, {B, Hq, Tq, dh}, dt);
+  if (want_lse) c.lse = empty(q, {B, Hq, Tq}, at::kFloat);
+  c.out4 = view4(c.out, "out");
+}
+PyObject* decode_result(int st, const DecodeCall& c) {
+  if (st != BNA_OK) return PyLong_FromLong(st);
+  if (c.lse.defined()) return tuple_of({c.out, c.lse});
+  return THPVariable_Wrap(c.out);
 }
 
 // decode(q, k_pages, v_pages, block_table, lens, k_new, v_new, active, window, scale, want_lse, workspace, stream)
@@ -187,53 +252,81 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
                    &table = tensor(a[3], "block_table"), &lens = tensor(a[4], "lens"), &ws = tensor(a[11], "workspace");
   need_cuda({&q, &kp, &vp, &table, &lens, &ws});
   const c10::DeviceGuard guard(q.device());
-  const bna_tensor4 tq = view4(q, "q");
   bna_tensor4 tkp = view4(kp, "k_pages"), tvp = view4(vp, "v_pages");
-  const int64_t B = q.size(0), Hq = q.size(1), Tq = q.size(2), dh = q.size(3);
-  const auto dt = q.scalar_type();
-  need(kp.scalar_type() == dt && vp.scalar_type() == dt, "the pools must have q's dtype");
-  need_ints(table, 2, "block_table");
-  need_ints(lens, 1, "lens");
-  need(table.size(0) == B && lens.size(0) == B, "block_table and lens must have one row per request");
-  need(table.size(1) <= INT32_MAX, "block_table: too many columns");
-  need(ws.scalar_type() == at::kByte && ws.is_contiguous(), "workspace must be a contiguous uint8 tensor (decode_workspace)");
-  const bool has_k = a[5] != Py_None, has_v = a[6] != Py_None;
-  need(has_k == has_v, "k_new and v_new go together");
-  bna_tensor4 tkn, tvn;
-  if (has_k) {
-    const at::Tensor &kn = tensor(a[5], "k_new"), &vn = tensor(a[6], "v_new");
-    need_cuda({&q, &kn, &vn});
-    need(kn.scalar_type() == dt && vn.scalar_type() == dt, "q, k_new, v_new dtype mismatch");
-    tkn = view4(kn, "k_new");
-    tvn = view4(vn, "v_new");
-  }
-  const uint8_t* active = nullptr;
-  if (a[7] != Py_None) {
-    const at::Tensor& x = tensor(a[7], "active");
-    need_cuda({&q, &x});
-    need(x.scalar_type() == at::kBool && x.dim() == 1 && x.size(0) == B && x.is_contiguous(),
-         "active must be a contiguous bool tensor with one entry per request");
-    active = static_cast<const uint8_t*>(x.data_ptr());
-    need(has_k, "active says which requests have k_new / v_new rows");
-  }
-  const int64_t window = integer(a[8]);
-  need(window >= 0 && window <= INT32_MAX, "window must be in [0, 2^31) (0: every key)");
-  const double scale = PyFloat_AsDouble(a[9]);
-  if (scale == -1.0 && PyErr_Occurred()) throw python_error();
-  const int want_lse = PyObject_IsTrue(a[10]);
-  if (want_lse < 0) throw python_error();
-  const int32_t code = dtype_code(q);
-  at::Tensor out = empty(q, {B, Hq, Tq, dh}, dt), lse;
-  if (want_lse) lse = empty(q, {B, Hq, Tq}, at::kFloat);
-  bna_tensor4 to = view4(out, "out");
-  const int st = g_decode(&tq, &tkp, &tvp, has_k ? &tkn : nullptr, has_k ? &tvn : nullptr, active, &to,
-                          want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, Hq * Tq, Tq, code,
-                          static_cast<const int32_t*>(table.data_ptr()), table.stride(0), (int32_t)table.size(1),
-                          static_cast<const int32_t*>(lens.data_ptr()), (int32_t)window, (float)scale, ws.data_ptr(), ws.numel(),
-                          address(a[12]));
+  need(kp.scalar_type() == q.scalar_type() && vp.scalar_type() == q.scalar_type(), "the pools must have q's dtype");
+  DecodeCall c;
+  decode_call(c, q, table, lens, ws, a[5], a[6], a[7], a[8], a[9], a[10]);
+  const int64_t Hq = q.size(1), Tq = q.size(2);
+  return decode_result(g_decode(&c.q, &tkp, &tvp, c.k_new, c.v_new, c.active, &c.out4,
+                                c.lse.defined() ? static_cast<float*>(c.lse.data_ptr()) : nullptr, Hq * Tq, Tq, c.code,
+                                static_cast<const int32_t*>(table.data_ptr()), table.stride(0), (int32_t)table.size(1),
+                                static_cast<const int32_t*>(lens.data_ptr()), (int32_t)c.window, (float)c.scale, ws.data_ptr(), ws.numel(),
+                                address(a[12])),
+                       c);
+  END_HANDLE_TH_ERRORS
+}
+
+bna_tensor4 pool4(const at::Tensor& x) {
+  need(x.scalar_type() == at::kByte, "kv_pages must be a uint8 tensor");
+  return view4(x, "kv_pages");
+}
+
+// append_int4(k, v, kv_pages, slot_map, stream): k / v [tokens, Hkv, dh]
+PyObject* append_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 5);
+  const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &pool = tensor(a[2], "kv_pages"), &slots = tensor(a[3], "slot_map");
+  need_cuda({&k, &v, &pool, &slots});
+  const c10::DeviceGuard guard(k.device());
+  need(k.dim() == 3 && v.dim() == 3, "k and v must be [tokens, Hkv, dh]");
+  need(v.scalar_type() == k.scalar_type(), "k and v must have one dtype");
+  need_slots(slots, k.size(0));
+  const bna_tensor4 rows[2] = {rows4(k), rows4(v)};
+  bna_tensor4 p = pool4(pool);
+  return PyLong_FromLong(g_append_int4(&rows[0], &rows[1], &p, static_cast<const int64_t*>(slots.data_ptr()), dtype_code(k), address(a[4])));
+  END_HANDLE_TH_ERRORS
+}
+
+// read_int4(kv_pages, slot_map, f16, stream) -> k, v [tokens, Hkv, dh]
+PyObject* read_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 4);
+  const at::Tensor &pool = tensor(a[0], "kv_pages"), &slots = tensor(a[1], "slot_map");
+  need_cuda({&pool, &slots});
+  const c10::DeviceGuard guard(pool.device());
+  const bna_tensor4 p = pool4(pool);
+  need(slots.dim() == 1, "slot_map must be a contiguous int64 tensor with one entry per token");
+  const int64_t tokens = slots.size(0), heads = pool.size(1), dh = pool.size(3) / 18;
+  need(pool.size(3) % 18 == 0, "kv_pages: blocks must have 18 * head_dim bytes");
+  need_slots(slots, tokens);
+  const int f16 = PyObject_IsTrue(a[2]);
+  if (f16 < 0) throw python_error();
+  const at::Tensor k = empty(pool, {tokens, heads, dh}, f16 ? at::kHalf : at::kBFloat16), v = at::empty_like(k);
+  bna_tensor4 rows[2] = {rows4(k), rows4(v)};
+  const int st = g_read_int4(&p, static_cast<const int64_t*>(slots.data_ptr()), &rows[0], &rows[1], f16 ? BNA_F16 : BNA_BF16, address(a[3]));
   if (st != BNA_OK) return PyLong_FromLong(st);
-  if (want_lse) return tuple_of({out, lse});
-  return THPVariable_Wrap(out);
+  return tuple_of({k, v});
+  END_HANDLE_TH_ERRORS
+}
+
+// decode_int4(q, kv_pages, block_table, lens, k_new, v_new, active, window, scale, want_lse, workspace, stream)
+PyObject* decode_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 12);
+  const at::Tensor &q = tensor(a[0], "q"), &pool = tensor(a[1], "kv_pages"), &table = tensor(a[2], "block_table"),
+                   &lens = tensor(a[3], "lens"), &ws = tensor(a[10], "workspace");
+  need_cuda({&q, &pool, &table, &lens, &ws});
+  const c10::DeviceGuard guard(q.device());
+  bna_tensor4 p = pool4(pool);
+  DecodeCall c;
+  decode_call(c, q, table, lens, ws, a[4], a[5], a[6], a[7], a[8], a[9]);
+  const int64_t Hq = q.size(1), Tq = q.size(2);
+  return decode_result(g_decode_int4(&c.q, &p, c.k_new, c.v_new, c.active, &c.out4,
+                                     c.lse.defined() ? static_cast<float*>(c.lse.data_ptr()) : nullptr, Hq * Tq, Tq, c.code,
+                                     static_cast<const int32_t*>(table.data_ptr()), table.stride(0), (int32_t)table.size(1),
+                                     static_cast<const int32_t*>(lens.data_ptr()), (int32_t)c.window, (float)c.scale, ws.data_ptr(),
+                                     ws.numel(), address(a[11])),
+                       c);
   END_HANDLE_TH_ERRORS
 }
 
@@ -315,6 +408,9 @@ PyMethodDef methods[] = {{"init", fast<init>(), METH_FASTCALL, nullptr},
                          {"append", fast<append>(), METH_FASTCALL, nullptr},
                          {"decode", fast<decode>(), METH_FASTCALL, nullptr},
                          {"logprobs", fast<logprobs>(), METH_FASTCALL, nullptr},
+                         {"append_int4", fast<append_int4>(), METH_FASTCALL, nullptr},
+                         {"read_int4", fast<read_int4>(), METH_FASTCALL, nullptr},
+                         {"decode_int4", fast<decode_int4>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

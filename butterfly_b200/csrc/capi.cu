@@ -45,6 +45,10 @@ int launch_paged_decode(const bna_tensor4*, bna_tensor4*, bna_tensor4*, const bn
                         const uint8_t*, bna_tensor4*, float*, int64_t, int64_t, int, const int32_t*, int64_t, int, const int32_t*, int,
                         float, void*, cudaStream_t);
 int64_t paged_decode_workspace_bytes();
+int launch_int4_rows(bool, const bna_tensor4*, const bna_tensor4*, bna_tensor4*, const int64_t*, int, cudaStream_t);
+int launch_paged_decode_int4(const bna_tensor4*, bna_tensor4*, const bna_tensor4*, const bna_tensor4*, const uint8_t*, bna_tensor4*,
+                             float*, int64_t, int64_t, int, const int32_t*, int64_t, int, const int32_t*, int, float, void*, cudaStream_t);
+int64_t paged_decode_int4_workspace_bytes();
 int launch_token_logprobs(const void*, int64_t, int64_t, int64_t, int64_t, int, int, const void*, int, float*, float*, int64_t*, float*, int,
                           cudaStream_t);
 
@@ -520,6 +524,101 @@ int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_tensor4* v_
   return launch_paged_decode(q, k_pages, v_pages, k_new, v_new, active, out, lse, lse_stride_b, lse_stride_h, dtype, block_table,
                              table_stride, table_width, lens, window, scale, workspace, (cudaStream_t)stream);
 }
+
+// ---------------------------------------------------------------- paged cache in 4 bits
+// A pool [pages, Hkv, page_size / 16, 18 dh] of bytes (strides in bytes; no two blocks may share memory).
+static int check_int4_pool(const bna_tensor4* t, int64_t dh) {
+  if (dh != 64 && dh != 128 && dh != 256) return fail(BNA_UNSUPPORTED, "paged cache: head_dim must be 64, 128 or 256");
+  if (null4(t)) return fail(BNA_BAD_SHAPE, "kv_pages is null");
+  for (int d = 0; d < 4; ++d)
+    if (t->size[d] <= 0 || t->size[d] > INT32_MAX) return fail(BNA_BAD_SHAPE, "kv_pages is empty or too large");
+  if (t->size[3] != 18 * dh) return fail(BNA_BAD_SHAPE, "kv_pages: blocks must have 18 * head_dim bytes");
+  if (t->size[2] > INT32_MAX / 16) return fail(BNA_UNSUPPORTED, "kv_pages: pages of 2^31 tokens or more");
+  if (t->stride[3] != 1) return fail(BNA_BAD_STRIDE, "kv_pages: blocks must be contiguous");
+  for (int d = 0; d < 3; ++d)
+    if (t->size[d] > 1 && (t->stride[d] % 16 || t->stride[d] < 18 * dh))
+      return fail(BNA_BAD_STRIDE, "kv_pages: strides must be multiples of 16 bytes, of at least a block");
+  if (reinterpret_cast<uintptr_t>(t->data) & 15) return fail(BNA_BAD_STRIDE, "kv_pages: data pointer must be 16-byte aligned");
+  return BNA_OK;
+}
+
+static int int4_rows(bool append, const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* pool, const int64_t* slot_map, int32_t dtype,
+                     void* stream) {
+  const std::string name = append ? "paged_append_int4" : "paged_read_int4";
+  if (int rc = check_dtype(dtype)) return rc;
+  if (!k || !v || !pool) return fail(BNA_BAD_SHAPE, name + ": null tensor");
+  for (int d = 0; d < 4; ++d)
+    if (k->size[d] != v->size[d] || (d == 0 && k->size[d] != 1))
+      return fail(BNA_BAD_SHAPE, name + ": k and v must be [1, Hkv, tokens, dh] of one shape");
+  const int64_t dh = k->size[3];
+  if (int rc = check_int4_pool(pool, dh)) return rc;
+  if (k->size[1] != pool->size[1]) return fail(BNA_BAD_SHAPE, name + ": head counts of the rows and the pool differ");
+  if (k->size[2] == 0) return BNA_OK;
+  if (int rc = check_rows(k, "k", dh)) return rc;
+  if (int rc = check_rows(v, "v", dh)) return rc;
+  if (!slot_map) return fail(BNA_BAD_SHAPE, name + ": null slot_map");
+  if (reinterpret_cast<uintptr_t>(slot_map) & 7) return fail(BNA_BAD_STRIDE, name + ": slot_map must be 8-byte aligned");
+  return launch_int4_rows(append, k, v, pool, slot_map, dtype, (cudaStream_t)stream);
+}
+
+int bna_paged_append_int4(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* kv_pages, const int64_t* slot_map, int32_t dtype,
+                          void* stream) {
+  return int4_rows(true, k, v, kv_pages, slot_map, dtype, stream);
+}
+
+int bna_paged_read_int4(const bna_tensor4* kv_pages, const int64_t* slot_map, bna_tensor4* k, bna_tensor4* v, int32_t dtype, void* stream) {
+  if (k && v)
+    for (int d = 1; d < 3; ++d)
+      if ((k->size[d] > 1 && k->stride[d] < k->size[3]) || (v->size[d] > 1 && v->stride[d] < v->size[3]))
+        return fail(BNA_BAD_STRIDE, "paged_read_int4: rows of k and v must not overlap");
+  return int4_rows(false, k, v, const_cast<bna_tensor4*>(kv_pages), slot_map, dtype, stream);
+}
+
+int bna_paged_decode_int4(const bna_tensor4* q, bna_tensor4* kv_pages, const bna_tensor4* k_new, const bna_tensor4* v_new,
+                          const uint8_t* active, bna_tensor4* out, float* lse, int64_t lse_stride_b, int64_t lse_stride_h, int32_t dtype,
+                          const int32_t* block_table, int64_t table_stride, int32_t table_width, const int32_t* lens, int32_t window,
+                          float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (!q || !kv_pages || !out) return fail(BNA_BAD_SHAPE, "paged_decode_int4: null tensor");
+  const int64_t dh = q->size[3], B = q->size[0], Hq = q->size[1];
+  if (int rc = check_int4_pool(kv_pages, dh)) return rc;
+  const int64_t Hkv = kv_pages->size[1];
+  if (Hq <= 0 || Hq % Hkv) return fail(BNA_BAD_SHAPE, "num query heads must be a multiple of num kv heads");
+  if (Hq > 65535 || Hkv > 65535) return fail(BNA_UNSUPPORTED, "paged_decode_int4: too many heads");
+  if (q->size[2] != 1) return fail(BNA_BAD_SHAPE, "paged_decode_int4: q must be [B, Hq, 1, dh], one new token per request");
+  if (B == 0) return BNA_OK;
+  if (B < 0 || B > INT32_MAX) return fail(BNA_BAD_SHAPE, "paged_decode_int4: bad batch size");
+  if (int rc = check_rows(q, "q", dh)) return rc;
+  if (int rc = check_rows(out, "out", dh)) return rc;
+  for (int i = 0; i < 3; ++i)
+    if (out->size[i] != q->size[i]) return fail(BNA_BAD_SHAPE, "out shape mismatch");
+  if ((k_new == nullptr) != (v_new == nullptr)) return fail(BNA_BAD_SHAPE, "paged_decode_int4: k_new and v_new go together");
+  if (active && !k_new) return fail(BNA_BAD_SHAPE, "paged_decode_int4: active says which requests have a k_new / v_new row");
+  if (k_new) {
+    const char* names[2] = {"k_new", "v_new"};
+    const bna_tensor4* ts[2] = {k_new, v_new};
+    for (int i = 0; i < 2; ++i) {
+      if (int rc = check_rows(ts[i], names[i], dh)) return rc;
+      if (ts[i]->size[0] != B || ts[i]->size[1] != Hkv || ts[i]->size[2] != 1)
+        return fail(BNA_BAD_SHAPE, std::string(names[i]) + " must be [B, Hkv, 1, dh]");
+    }
+  }
+  if (!block_table || !lens) return fail(BNA_BAD_SHAPE, "paged_decode_int4: null block_table or lens");
+  if ((reinterpret_cast<uintptr_t>(block_table) & 3) || (reinterpret_cast<uintptr_t>(lens) & 3))
+    return fail(BNA_BAD_STRIDE, "paged_decode_int4: block_table and lens must be 4-byte aligned");
+  if (table_width <= 0 || (B > 1 && table_stride < 0)) return fail(BNA_BAD_SHAPE, "paged_decode_int4: bad block_table shape");
+  if ((int64_t)table_width * kv_pages->size[2] * 16 > INT32_MAX)
+    return fail(BNA_UNSUPPORTED, "paged_decode_int4: a table row covers 2^31 tokens or more");
+  if (window < 0) return fail(BNA_BAD_SHAPE, "window must be >= 0 (0: every key)");
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(BNA_BAD_SHAPE, "scale must be positive");
+  if (!workspace || workspace_bytes < paged_decode_int4_workspace_bytes())
+    return fail(BNA_CAPACITY, "paged_decode_int4: workspace smaller than bna_paged_decode_int4_workspace_bytes()");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BNA_BAD_STRIDE, "paged_decode_int4: workspace must be 16-byte aligned");
+  return launch_paged_decode_int4(q, kv_pages, k_new, v_new, active, out, lse, lse_stride_b, lse_stride_h, dtype, block_table, table_stride,
+                                  table_width, lens, window, scale, workspace, (cudaStream_t)stream);
+}
+
+int64_t bna_paged_decode_int4_workspace_bytes(void) { return paged_decode_int4_workspace_bytes(); }
 
 // ---------------------------------------------------------------- token log probabilities
 int bna_token_logprobs(const void* logits, int64_t stride, int64_t stride_outer, int64_t rows, int64_t inner, int64_t vocab, int32_t dtype,

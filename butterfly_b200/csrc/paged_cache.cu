@@ -9,6 +9,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "int4.cuh"
 
 namespace bna {
 namespace {
@@ -272,6 +273,118 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppendArgs
   }
 }
 
+// ------------------------------------------------------------------------------ 4-bit rows
+struct Int4RowsArgs {
+  const uint8_t *k, *v;        // append: rows in; read: rows out
+  int64_t k_h, k_t, v_h, v_t;  // element strides: head, token
+  uint8_t* pool;
+  int64_t p_p, p_h, p_g;  // byte strides: page, head, block
+  const int64_t* slots;
+  int64_t rows;  // tokens * heads
+  int64_t num_slots;
+  int heads, page_size, dh, vec_shift;  // 2^vec_shift vectors of 8 columns per row
+};
+
+// A token's row of one head: where the keys' half of its block lies, and the token's place in it (null: no slot).
+__device__ __forceinline__ uint8_t* int4_row(const Int4RowsArgs& a, int64_t slot, int head, int& token) {
+  if (slot < 0 || slot >= a.num_slots) return nullptr;
+  const int64_t page = a.num_slots <= UINT_MAX ? (int64_t)((unsigned)slot / (unsigned)a.page_size) : slot / a.page_size;
+  const int off = (int)(slot - page * a.page_size);
+  token = off % kInt4Tokens;
+  return a.pool + page * a.p_p + head * a.p_h + off / kInt4Tokens * a.p_g;
+}
+__device__ __forceinline__ int64_t token_of(const Int4RowsArgs& a, int64_t row) {
+  return a.rows <= UINT_MAX ? (int64_t)((unsigned)row / (unsigned)a.heads) : row / a.heads;
+}
+
+// A thread packs 8 columns of the keys and of the values of N rows that lie a block apart; 8 threads share a
+// group's extremes.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) int4_append_kernel(const Int4RowsArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int c = threadIdx.x & ((1 << a.vec_shift) - 1);
+  const int step = 256 >> a.vec_shift;
+  const int64_t row0 = (int64_t)blockIdx.x * (N * step) + (threadIdx.x >> a.vec_shift);
+  uint4 k[N], v[N];
+  int64_t slot[N];
+  int head[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t row = row0 + i * step;
+    slot[i] = -1;
+    head[i] = 0;
+    k[i] = v[i] = make_uint4(0, 0, 0, 0);
+    if (row < a.rows) {
+      const int64_t t = token_of(a, row);
+      head[i] = (int)(row - t * a.heads);
+      slot[i] = a.slots[t];
+      k[i] = ld_nc_128(a.k + 2 * (t * a.k_t + head[i] * a.k_h) + 16 * c);
+      v[i] = ld_nc_128(a.v + 2 * (t * a.v_t + head[i] * a.v_h) + 16 * c);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    uint32_t kw, kp, vw, vp;
+    int4_pack<T>(k[i], kw, kp);
+    int4_pack<T>(v[i], vw, vp);
+    int token = 0;
+    uint8_t* block = int4_row(a, slot[i], head[i], token);
+    if (!block) continue;  // (whole rows: the lanes of a group stay together)
+    const int word = int4_word_at(a.dh, token, c), pair = int4_pair_at(a.dh, token, c), half = int4_half_bytes(a.dh);
+    *reinterpret_cast<uint32_t*>(block + word) = kw;
+    *reinterpret_cast<uint32_t*>(block + half + word) = vw;
+    if ((c & 7) == 0) {
+      *reinterpret_cast<uint32_t*>(block + pair) = kp;
+      *reinterpret_cast<uint32_t*>(block + half + pair) = vp;
+    }
+  }
+}
+
+// A thread reads 8 columns of the keys and of the values of N rows; tokens without a slot get zeros.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) int4_read_kernel(const Int4RowsArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int c = threadIdx.x & ((1 << a.vec_shift) - 1);
+  const int step = 256 >> a.vec_shift;
+  const int64_t row0 = (int64_t)blockIdx.x * (N * step) + (threadIdx.x >> a.vec_shift);
+  uint32_t word[N][2], pair[N][2];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t row = row0 + i * step;
+    word[i][0] = word[i][1] = pair[i][0] = pair[i][1] = 0;
+    if (row < a.rows) {
+      const int64_t t = token_of(a, row);
+      int token = 0;
+      const uint8_t* block = int4_row(a, a.slots[t], (int)(row - t * a.heads), token);
+      if (block) {
+        const uint8_t *w = block + int4_word_at(a.dh, token, c), *p = block + int4_pair_at(a.dh, token, c);
+        const int half = int4_half_bytes(a.dh);
+        word[i][0] = *reinterpret_cast<const uint32_t*>(w);
+        pair[i][0] = *reinterpret_cast<const uint32_t*>(p);
+        word[i][1] = *reinterpret_cast<const uint32_t*>(w + half);
+        pair[i][1] = *reinterpret_cast<const uint32_t*>(p + half);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t row = row0 + i * step;
+    if (row >= a.rows) continue;
+    const int64_t t = token_of(a, row), head = row - t * a.heads;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float2 p = ElemTraits<T>::unpack2(pair[i][x]);
+      uint32_t u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = ElemTraits<T>::pack2(int4_value(word[i][x], 2 * j, p), int4_value(word[i][x], 2 * j + 1, p));
+      uint8_t* dst = const_cast<uint8_t*>(x ? a.v + 2 * (t * a.v_t + head * a.v_h) : a.k + 2 * (t * a.k_t + head * a.k_h));
+      st_128(dst + 16 * c, make_uint4(u[0], u[1], u[2], u[3]));
+    }
+  }
+}
+
 // Launch that may be set up while the stream's previous kernel runs (the kernel waits for it).
 template <typename Args>
 int launch_dependent(void (*kern)(Args), const std::remove_const_t<Args>& a, unsigned grid, unsigned block, int smem, cudaStream_t s,
@@ -334,6 +447,25 @@ int launch_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4*
   if (blocks > INT_MAX) return fail(BNA_UNSUPPORTED, "paged_append: too many elements");
   return launch_dependent(n == 4 ? paged_append_kernel<4> : paged_append_kernel<1>, a, (unsigned)blocks, 256, 0, s,
                           "paged_append launch");
+}
+
+// Rows of k / v into (append) or out of (read) 4-bit blocks.
+int launch_int4_rows(bool append, const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* pool, const int64_t* slots, int dtype, cudaStream_t s) {
+  const int heads = (int)k->size[1], dh = (int)k->size[3], page_size = (int)pool->size[2] * kInt4Tokens;
+  const int64_t rows = k->size[2] * heads;
+  const int vecs = dh / 8, vec_shift = vecs == 8 ? 3 : vecs == 16 ? 4 : 5;
+  Int4RowsArgs a{static_cast<const uint8_t*>(k->data), static_cast<const uint8_t*>(v->data), k->stride[1], k->stride[2], v->stride[1],
+                 v->stride[2], static_cast<uint8_t*>(pool->data), pool->stride[0], pool->stride[1], pool->stride[2], slots, rows,
+                 pool->size[0] * page_size, heads, page_size, dh, vec_shift};
+  const int n = rows * vecs >= (int64_t)4 * 256 * 148 * 4 ? 4 : 1;  // as in the 16-bit append
+  const int64_t per = (int64_t)n * (256 >> vec_shift), blocks = (rows + per - 1) / per;
+  if (blocks > INT_MAX) return fail(BNA_UNSUPPORTED, "paged 4-bit rows: too many elements");
+  auto pick = [&](auto t) {
+    using T = decltype(t);
+    return append ? (n == 4 ? int4_append_kernel<T, 4> : int4_append_kernel<T, 1>) : (n == 4 ? int4_read_kernel<T, 4> : int4_read_kernel<T, 1>);
+  };
+  return launch_dependent(dtype == BNA_BF16 ? pick(__nv_bfloat16()) : pick(__half()), a, (unsigned)blocks, 256, 0, s,
+                          append ? "paged_append_int4 launch" : "paged_read_int4 launch");
 }
 
 }  // namespace bna

@@ -1,0 +1,854 @@
+// paged_decode_int4.cu — attention of one new token per request over a paged cache held in 4 bits (int4.cuh).
+//   s_j = scale * q . k_j   for keys j in [max(0, len - window), len)
+//   out = sum_j softmax(s)_j v_j,   lse = log sum_j exp(s_j);  no key: out = 0, lse = -inf
+// With x = s c + m per group y of 64 columns both products are taken on the codes, which are exact in 16 bits:
+//   q . k_j = sum_y  sk_jy (q_y . ck_jy) + mk_jy sum(q_y)
+//   out     = sum_j  (p_j sv_jy) cv_jy + sum_j p_j mv_jy
+// so nothing is rounded in undoing the quantisation; the scales work on fp32 scores and probabilities.
+//
+// Tensor-core form (m16n8k16, 16 keys x up to 8 query heads): S^T = C_k Q^T and O^T = C_v^T P^T.  A code
+// c masked in place in a 16-bit half of a code word is the fp16 subnormal 2^-24 c, or 2^-20 c for the
+// odd code beside it, so a code word becomes four operand registers with five integer instructions and
+// no conversion.  q is scaled by a power of two into the fp16 range (by head; exact but for entries 2^-24 of
+// the head's largest), and 2^-4 of that meets the odd codes; p sv is held in fp16 around its largest.
+//
+// Bytes: 18 dh / 16 a token and head.  A read serves up to 8 query heads (16 at head_dim 64 and 128 with more than 8).
+//
+// Schedule: the keys of every pair (request, KV head) in granules of 16 form one line, which is cut evenly over
+// the CTAs.  A cut that falls within kSlack granules of a pair's end moves there, so that short pairs stay whole;
+// of a pair that is cut each CTA leaves a part in the workspace, and a second kernel joins the parts.  Every warp
+// copies its granules into a ring of its own by cp.async and waits for nobody until a pair ends.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <string>
+#include <type_traits>
+
+#include "common.cuh"
+#include "int4.cuh"
+#include "mma.cuh"
+#include "sm100.cuh"
+
+namespace bna {
+namespace {
+using namespace sm100;
+
+constexpr int kGran = kInt4Tokens;  // keys of a granule: a block
+constexpr int kMaxCtas = 320;       // the workspace is sized for this many
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kSlack = 40;    // granules
+constexpr int kMinShare = 32;  // granules a CTA gets at least (fewer CTAs otherwise)
+constexpr int kKeepLens = 1024;  // lengths kept in shared memory
+constexpr int kShift = 11;  // probabilities are held times 2^kShift, and so are l and o; the divisions undo it
+constexpr float kMove = 4.f;  // a reference moves when a score lies more than 2^kMove above it
+constexpr float kNone = -1e30f;  // the offset of a reference that has seen no key
+
+struct Int4Args {
+  const uint8_t* q;
+  int64_t q_b, q_h;
+  uint8_t* pool;
+  int64_t p_p, p_h, p_g;  // byte strides: page, head, block
+  const uint8_t *kn, *vn;  // the new token's rows, or null
+  int64_t kn_b, kn_h, vn_b, vn_h;
+  const uint8_t* active;  // requests that have a new row (null: all)
+  uint8_t* out;
+  int64_t o_b, o_h;
+  float* lse;
+  int64_t ls_b, ls_h;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  int B, Hkv, G, width, num_pages, page_size, window;
+  int page_grans;          // blocks of a page
+  int chunks, chunk_rows;  // the G heads in `chunks` groups of chunk_rows
+  float scale_log2;
+  uint8_t* ws;
+};
+
+// Workspace: (the first 4 KB belong to the 16-bit kernel and stay zero), a record of the cut pair that begins in each
+// CTA, (m, l) of every part, their outputs.  CTA c has the slots 2 c and 2 c + 1: the pair that ends in it, and the one that begins.
+constexpr int kPartRows = 16;
+struct CutPair {
+  int b, h, r0, rows, parts, pad[3];
+};
+constexpr int64_t kWsCut = 4096;
+constexpr int64_t kWsMl = kWsCut + kMaxCtas * (int64_t)sizeof(CutPair);
+constexpr int64_t kWsO = kWsMl + (int64_t)2 * kMaxCtas * kPartRows * 8;
+constexpr int64_t kWsBytes = kWsO + (int64_t)2 * kMaxCtas * 2048 * 4;  // (a part has 8 rows of 256 or 16 of 128 at most)
+
+__device__ __forceinline__ int first_key(const Int4Args& a, int len) { return a.window > 0 ? max(0, len - a.window) : 0; }
+__device__ __forceinline__ int clamp_len(const Int4Args& a, int len) {
+  return (int)min((int64_t)max(len, 0), (int64_t)a.width * a.page_size);
+}
+__device__ __forceinline__ int granules_of(const Int4Args& a, int len) {
+  return len == 0 ? 0 : (len + kGran - 1) / kGran - first_key(a, len) / kGran;
+}
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {  // zeros where not valid
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int N>  // N words of 32 bits
+__device__ __forceinline__ void lds(uint32_t addr, uint32_t (&r)[N]) {
+  static_assert(N == 1 || N == 2 || N % 4 == 0, "");
+  if constexpr (N == 1) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+                   : "r"(addr + 4 * i)
+                   : "memory");
+  }
+}
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// 8x8 matrix of 16-bit entries, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ float lane_max(float x) {  // over the lanes with the same lane % 4
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+}
+__device__ __forceinline__ float lane_sum(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  return x + __shfl_xor_sync(0xffffffffu, x, 16);
+}
+// (m, l) with l times 2^kShift
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? -INFINITY : (m + log2f(l) - (float)kShift) * 0.6931471805599453f;
+}
+
+// A stretch of a (request, KV head, head group) inside a CTA: granules [g0, g0 + n), keys attended to [lo, hi).
+struct Seg {
+  int b, h, r0, rows, g0, n, lo, hi, slot;  // slot of the part (-1: the whole pair)
+};
+
+template <typename T_, int DH_, bool WIDE_>
+struct Form {
+  using T = T_;
+  static constexpr int DH = DH_;
+  static constexpr bool WIDE = WIDE_;
+  static constexpr int kTiles = WIDE ? 2 : 1;  // of 8 query heads
+  static constexpr int kHeads = 8 * kTiles;
+  // two CTAs an SM where their registers fit, so that the end of one's pair overlaps the other's reads
+  static constexpr int kCtas = WIDE || DH == 256 ? 1 : 2;
+  static constexpr int GR = DH / kInt4Group;
+  static constexpr int kBlock = int4_block_bytes(DH);
+  static constexpr int kStages = DH == 256 ? 5 : WIDE ? 8 : 4;  // granules of a warp's ring
+  static constexpr int kRing = kStages * kBlock;
+  static constexpr int kPitch = DH + 4;  // floats of a row, as the warps join
+  static_assert(kHeads * kPitch * 4 <= kRing, "a warp's outputs take its ring's place");
+  static constexpr int kMl = kWarps * kRing;                   // (m, l) [warp][head]
+  static constexpr int kRuns = kMl + kWarps * kHeads * 8;      // granules up to the end of each thread's run of requests
+  static constexpr int kLens = kRuns + kThreads * 8;
+  static constexpr int kBytes = kLens + 4 * kKeepLens;
+  static_assert(kCtas * (kBytes + 1024) <= 233472, "shared memory of an SM");
+};
+
+// What a warp holds of a segment.  Scores come as S^T: lane 4 g + t has keys row(g) and row(g) + 8 and heads 2 t, 2 t + 1
+// (of every tile); matrix row g is key row(g) = g ^ (g >> 1 & 1), which spreads the rows that a read of values
+// touches over the banks.  Outputs o come as O^T: columns 64 y + 8 g .. + 7 of heads 2 t, 2 t + 1.
+template <class F>
+struct Acc {
+  using T = typename F::T;
+  static constexpr int GR = F::GR, NT = F::kTiles, DH = F::DH;
+  static constexpr bool kTwoParts = std::is_same<T, __half>::value;
+  uint32_t qb[NT][GR][2][2][2];  // Q^T fragments: tile, group, word of the lane, step, register
+  float qs[NT][GR][2];           // sum(q_y), scaled as the products with codes are
+  float f[NT][2];                // from those to scores in the exp2 domain
+  float ref[NT][2], off[NT][2];  // running reference (no score lies 2^kMove above it), and it less kShift
+  float l[NT][2], wm[NT][GR][2];  // this lane's keys: sum p, sum p mv_y
+  float o[NT][GR][4][4];          // sum p sv cv, in units of 2^-24 (odd columns 2^-20) 2^e
+  float bound, inv;               // 2^e, above every value scale so far, and 2^-e
+
+  // q: the head group's first row; rows from `rows` on count as zeros
+  __device__ __forceinline__ void begin(const uint8_t* q, int64_t q_h, int rows, float scale_log2, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      uint4 raw[GR][2];
+#pragma unroll
+      for (int y = 0; y < GR; ++y)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          raw[y][j] = g + 8 * n < rows ? ld_nc_128(q + 2 * ((g + 8 * n) * q_h + 64 * y + 16 * t + 8 * j)) : make_uint4(0, 0, 0, 0);
+      float top = 0.f;
+#pragma unroll
+      for (int y = 0; y < GR; ++y)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t u[4] = {raw[y][j].x, raw[y][j].y, raw[y][j].z, raw[y][j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 p = ElemTraits<T>::unpack2(u[i]);
+            top = fmaxf(top, fmaxf(fabsf(p.x), fabsf(p.y)));
+          }
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = min(max(140 - (int)(__float_as_uint(top) >> 23), -100), 120);  // the largest in [2^13, 2^14)
+      const float up = pow2(e);
+      float sums[GR];
+#pragma unroll
+      for (int y = 0; y < GR; ++y) {
+        sums[y] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t u[4] = {raw[y][j].x, raw[y][j].y, raw[y][j].z, raw[y][j].w};
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 p = ElemTraits<T>::unpack2(u[i]);
+            x[2 * i] = p.x * up;
+            x[2 * i + 1] = p.y * up;
+            sums[y] += x[2 * i] + x[2 * i + 1];
+          }
+          // the codes of a word meet as (0, 4), 2^4 (1, 5), (2, 6), 2^4 (3, 7)
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            qb[n][y][j][st][0] = ElemTraits<__half>::pack2(x[2 * st], x[2 * st + 4]);
+            qb[n][y][j][st][1] = ElemTraits<__half>::pack2(x[2 * st + 1] * 0.0625f, x[2 * st + 5] * 0.0625f);
+          }
+        }
+        sums[y] += __shfl_xor_sync(0xffffffffu, sums[y], 1);
+        sums[y] += __shfl_xor_sync(0xffffffffu, sums[y], 2);
+        sums[y] *= 0x1p-24f;
+      }
+      const float down = pow2(min(24 - e, 124)) * scale_log2;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int src = 4 * (2 * t + x);
+        f[n][x] = __shfl_sync(0xffffffffu, down, src);
+#pragma unroll
+        for (int y = 0; y < GR; ++y) {
+          qs[n][y][x] = __shfl_sync(0xffffffffu, sums[y], src);
+          wm[n][y][x] = 0.f;
+        }
+        ref[n][x] = -INFINITY;
+        off[n][x] = kNone;
+        l[n][x] = 0.f;
+      }
+#pragma unroll
+      for (int y = 0; y < GR; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[n][y][i][x] = 0.f;
+    }
+    bound = pow2(-100);
+    inv = pow2(100);
+  }
+
+  // A granule in shared memory, its first key at `pos`; with `edge` keys outside [lo, hi) are masked.
+  __device__ __forceinline__ void granule(uint32_t tile, int pos, bool edge, int lo, int hi, int lane) {
+    constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
+    const int g = lane >> 2, t = lane & 3;
+    const int row = g ^ ((g >> 1) & 1);
+    const uint32_t values = tile + int4_half_bytes(DH);
+    // scores
+    float u[NT][4];
+    {
+      uint32_t w[2][2 * GR], p[2][GR];
+      lds(tile + row * (DH / 2) + t * (8 * GR), w[0]);
+      lds(tile + (row + 8) * (DH / 2) + t * (8 * GR), w[1]);
+      lds(tile + 8 * DH + row * (4 * GR), p[0]);
+      lds(tile + 8 * DH + (row + 8) * (4 * GR), p[1]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) u[n][x] = 0.f;
+#pragma unroll
+      for (int y = 0; y < GR; ++y) {
+        float acc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[n][x] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t a0 = w[0][j * GR + y], a1 = w[1][j * GR + y];
+          const uint32_t even[4] = {a0 & M0, a1 & M0, a0 & M1, a1 & M1};
+          const uint32_t odd[4] = {(a0 >> 8) & M0, (a1 >> 8) & M0, (a0 >> 8) & M1, (a1 >> 8) & M1};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_16816<__half>(acc[n], even, qb[n][y][j][0][0], qb[n][y][j][0][1]);
+            mma_16816<__half>(acc[n], odd, qb[n][y][j][1][0], qb[n][y][j][1][1]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float2 sm = ElemTraits<T>::unpack2(p[r][y]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) u[n][2 * r + x] = fmaf(sm.x, acc[n][2 * r + x], fmaf(sm.y, qs[n][y][x], u[n][2 * r + x]));
+        }
+      }
+    }
+    float sv[2][GR], mv[2][GR];
+    {
+      uint32_t p[2][GR];
+      lds(values + 8 * DH + row * (4 * GR), p[0]);
+      lds(values + 8 * DH + (row + 8) * (4 * GR), p[1]);
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int y = 0; y < GR; ++y) {
+          const float2 sm = ElemTraits<T>::unpack2(p[r][y]);
+          sv[r][y] = sm.x;
+          mv[r][y] = r == 0 ? sm.y : fmaf(15.f, sm.x, sm.y);
+        }
+    }
+    if (edge) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int key = pos + row + 8 * r;
+        if (key < lo || key >= hi) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) u[n][2 * r] = u[n][2 * r + 1] = -INFINITY;
+#pragma unroll
+          for (int y = 0; y < GR; ++y) sv[r][y] = mv[r][y] = 0.f;  // what the page holds there could be NaN
+        }
+      }
+    }
+    // probabilities times 2^kShift
+    float e[NT][4], top = 0.f;
+    bool move = false;
+#pragma unroll
+    for (int y = 0; y < GR; ++y) top = fmaxf(top, fmaxf(sv[0][y], sv[1][y]));
+    move = top >= bound;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        e[n][x] = fmaf(f[n][x & 1], u[n][x], -off[n][x & 1]);
+        move |= e[n][x] > kShift + kMove;
+      }
+    if (__any_sync(0xffffffffu, move)) {
+      float scale = 1.f;
+      top = lane_max(top);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (top >= bound) {
+        const int x = min((int)(__float_as_uint(top) >> 23) - 127 + 3, 126);  // room for scales up to four times as large
+        scale = bound * pow2(-x);
+        bound = pow2(x);
+        inv = pow2(-x);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float mx = fmaxf(ref[n][x], lane_max(fmaxf(f[n][x] * u[n][x], f[n][x] * u[n][2 + x])));
+          const float to = mx == -INFINITY ? kNone : mx - (float)kShift, al = ex2_approx(off[n][x] - to);
+          ref[n][x] = mx;
+          off[n][x] = to;
+          l[n][x] *= al;
+#pragma unroll
+          for (int y = 0; y < GR; ++y) {
+            wm[n][y][x] *= al;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[n][y][i][x] *= al * scale;
+              o[n][y][i][2 + x] *= al * scale;
+            }
+          }
+          e[n][x] = fmaf(f[n][x], u[n][x], -to);
+          e[n][2 + x] = fmaf(f[n][x], u[n][2 + x], -to);
+        }
+    }
+    uint32_t pb[NT][GR][2], pl[NT][GR][2];  // P^T sv fragments: high parts, and low ones for fp16 results
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) e[n][x] = ex2_approx(e[n][x]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) l[n][x] += e[n][x] + e[n][2 + x];
+#pragma unroll
+      for (int y = 0; y < GR; ++y) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) wm[n][y][x] = fmaf(e[n][x], mv[0][y], fmaf(e[n][2 + x], mv[1][y], wm[n][y][x]));
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float s = sv[r][y] * (r == 0 ? inv : -inv), w0 = e[n][2 * r] * s, w1 = e[n][2 * r + 1] * s;
+          const uint32_t hi16 = ElemTraits<__half>::pack2(w0, w1);
+          pb[n][y][r] = transposed(hi16);
+          if (kTwoParts) {
+            const float2 h = ElemTraits<__half>::unpack2(hi16);
+            pl[n][y][r] = transposed(ElemTraits<__half>::pack2(w0 - h.x, w1 - h.y));
+          }
+        }
+      }
+    }
+    // outputs: keys 2 t, 2 t + 1 of the matrix rows, and 8 further
+    uint32_t w[4][GR];
+    const int k0 = (2 * t) ^ (t & 1), k1 = (2 * t + 1) ^ (t & 1);
+    lds(values + k0 * (DH / 2) + g * (4 * GR), w[0]);
+    lds(values + k1 * (DH / 2) + g * (4 * GR), w[1]);
+    lds(values + (k0 + 8) * (DH / 2) + g * (4 * GR), w[2]);
+    lds(values + (k1 + 8) * (DH / 2) + g * (4 * GR), w[3]);
+#pragma unroll
+    for (int y = 0; y < GR; ++y) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // columns 0-3, then 4-7 of the word, of a pair of keys each
+        uint32_t x0 = __byte_perm(w[0][y], w[1][y], half ? 0x7632 : 0x5410), x1 = __byte_perm(w[2][y], w[3][y], half ? 0x7632 : 0x5410);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t a[4] = {x0 & M0, x0 & M1, ~x1 & M0, ~x1 & M1};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_16816<__half>(o[n][y][2 * half + i], a, pb[n][y][0], pb[n][y][1]);
+            if (kTwoParts) mma_16816<__half>(o[n][y][2 * half + i], a, pl[n][y][0], pl[n][y][1]);
+          }
+          x0 >>= 8;
+          x1 >>= 8;
+        }
+      }
+    }
+  }
+
+  // Sums over the warp; o becomes the output over this warp's keys alone (0 without any).
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        l[n][x] = lane_sum(l[n][x]);
+        const float d = l[n][x] == 0.f ? 0.f : 1.f / l[n][x];
+#pragma unroll
+        for (int y = 0; y < GR; ++y) {
+          const float m = lane_sum(wm[n][y][x]) * d;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[n][y][i][x] = fmaf(o[n][y][i][x] * (d * 0x1p24f), bound, m);
+            o[n][y][i][2 + x] = fmaf(o[n][y][i][2 + x] * (d * 0x1p20f), bound, m);
+          }
+        }
+      }
+  }
+  // Columns 64 y + 8 g .. + 7 of head 8 n + 2 t + x
+  __device__ __forceinline__ void columns(int n, int y, int x, float (&c)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[2 * i] = o[n][y][i][x];
+      c[2 * i + 1] = o[n][y][i][2 + x];
+    }
+  }
+};
+
+template <class F>
+__global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const __grid_constant__ Int4Args a) {
+  using T = typename F::T;
+  constexpr int DH = F::DH, GR = F::GR;
+  extern __shared__ __align__(128) uint8_t sm[];
+  int64_t* runs = reinterpret_cast<int64_t*>(sm + F::kRuns);
+  int* lens = reinterpret_cast<int*>(sm + F::kLens);
+  __shared__ int64_t warp_sums[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- the line: granules up to the end of each thread's run of requests
+  const int per = (a.B + kThreads - 1) / kThreads, per_b = a.Hkv * a.chunks;
+  {
+    int64_t mine = 0;
+    for (int b = tid * per; b < min((tid + 1) * per, a.B); ++b) {
+      const int len = clamp_len(a, a.lens[b]);
+      if (b < kKeepLens) lens[b] = len;
+      mine += granules_of(a, len);
+    }
+    mine *= per_b;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      if (w < warp) incl += warp_sums[w];
+    runs[tid] = incl;
+    __syncthreads();
+  }
+  auto len_of = [&](int b) { return b < kKeepLens ? lens[b] : clamp_len(a, a.lens[b]); };
+  const int64_t U = runs[kThreads - 1];
+  const int C = (int)min((int64_t)gridDim.x, max((int64_t)1, (U + kMinShare - 1) / kMinShare));
+  const int64_t cq = U / C, cr = U - cq * C;
+  auto raw_cut = [&](int64_t c) { return c * cq + min(c, cr); };
+  // The pair at place x of the line: its request, where the request begins, and the granules of each of its pairs.
+  struct At {
+    int b, nt;
+    int64_t begin;
+  };
+  auto locate = [&](int64_t x) {
+    int lo = 0, hi = kThreads - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (runs[mid] > x) hi = mid;
+      else lo = mid + 1;
+    }
+    At r{lo * per, 0, lo > 0 ? runs[lo - 1] : 0};
+    for (;; ++r.b) {
+      r.nt = granules_of(a, r.b < a.B ? len_of(r.b) : 0);
+      if (r.b >= a.B - 1 || r.begin + (int64_t)r.nt * per_b > x) return r;
+      r.begin += (int64_t)r.nt * per_b;
+    }
+  };
+  // A cut moved to the nearest end of its pair where that is close.
+  auto cut = [&](int64_t c) -> int64_t {
+    const int64_t x = raw_cut(c);
+    if (x <= 0 || x >= U) return min(max(x, (int64_t)0), U);
+    const At at = locate(x);
+    const int t = (int)((x - at.begin) % at.nt);
+    return t <= kSlack && t <= at.nt - t ? x - t : at.nt - t <= kSlack ? x + at.nt - t : x;
+  };
+  int64_t cur = 0, end = 0;
+  if ((int)blockIdx.x < C) {
+    cur = cut(blockIdx.x);
+    end = cut((int64_t)blockIdx.x + 1);
+  }
+  CutPair begun{};
+  bool uncut = true;
+
+  // ---- the pairs of this CTA's stretch
+  const uint32_t ring = smem_u32(sm) + warp * F::kRing;
+  float2* ml = reinterpret_cast<float2*>(sm + F::kMl);
+  At at{0, 0, 0};
+  if (cur < end) at = locate(cur);
+  while (cur < end) {
+    while (cur >= at.begin + (int64_t)at.nt * per_b && at.b + 1 < a.B) {  // (requests without keys are passed over)
+      at.begin += (int64_t)at.nt * per_b;
+      ++at.b;
+      at.nt = granules_of(a, len_of(at.b));
+    }
+    const int64_t local = cur - at.begin;
+    if (at.nt == 0 || local >= (int64_t)at.nt * per_b) break;  // (only where lengths changed under the call)
+    const int pair = (int)(local / at.nt), t0 = (int)(local - (int64_t)pair * at.nt);
+    const int len = len_of(at.b);
+    Seg s;
+    s.b = at.b;
+    s.h = pair / a.chunks;
+    s.r0 = (pair - s.h * a.chunks) * a.chunk_rows;
+    s.rows = min(a.chunk_rows, a.G - s.r0);
+    s.lo = first_key(a, len);
+    s.hi = len;
+    s.g0 = s.lo / kGran + t0;
+    s.n = (int)min((int64_t)(at.nt - t0), end - cur);
+    s.slot = s.n == at.nt ? -1 : 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0);
+    if (s.slot >= 0 && t0 == 0) {  // a cut pair begins here: its parts are the CTAs up to the one that holds its end
+      const int64_t p1 = cur + at.nt;
+      int c = (int)blockIdx.x + 1;
+      // (cuts within the pair keep their places; those near its end have moved there)
+      const int64_t last = p1 - kSlack - 1;  // the last place that a cut inside can have
+      const int64_t wide = cr * (cq + 1);
+      // the CTA whose raw stretch holds `last`: cuts up to its start lie inside
+      c = min(max(c, (int)(last < wide ? last / (cq + 1) : cr + (last - wide) / max(cq, (int64_t)1))), C - 1);
+      begun = CutPair{s.b, s.h, s.r0, s.rows, c - (int)blockIdx.x + 1, {0, 0, 0}};
+      uncut = false;
+    }
+    cur += s.n;
+
+    // this warp's granules: warp, warp + kWarps, ...
+    const int mine = (s.n - warp + kWarps - 1) / kWarps;
+    const int32_t* table = a.table + s.b * a.table_stride;
+    // lane i: where granule i of a batch of 32 lies, or null
+    auto look_up = [&](int k0) -> const uint8_t* {
+      const int k = k0 + lane;
+      if (k >= mine) return nullptr;
+      const int gr = s.g0 + warp + k * kWarps, pi = gr / a.page_grans, page = table[pi];
+      return page >= 0 && page < a.num_pages ? a.pool + page * a.p_p + s.h * a.p_h + (gr - pi * a.page_grans) * a.p_g : nullptr;
+    };
+    const uint8_t *batch = look_up(0), *next = look_up(32);
+    auto issue = [&](int k) {
+      if (k > 0 && (k & 31) == 0) {
+        batch = next;
+        next = look_up(k + 32);
+      }
+      if (k < mine) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(batch), k & 31));
+        const uint32_t dst = ring + (k % F::kStages) * F::kBlock;
+#pragma unroll
+        for (int i = 0; i < (F::kBlock / 16 + 31) / 32; ++i)
+          if (32 * i + 32 <= F::kBlock / 16 || 32 * i + lane < F::kBlock / 16)
+            cp_async_16(dst + 512 * i + 16 * lane, src ? src + 512 * i + 16 * lane : a.pool, src != nullptr);
+      }
+      cp_async_commit();  // (a group for every granule, empty ones past the end)
+    };
+#pragma unroll 1
+    for (int k = 0; k < F::kStages - 1; ++k) issue(k);
+    Acc<F> acc;
+    acc.begin(a.q + 2 * (s.b * a.q_b + (int64_t)(s.h * a.G + s.r0) * a.q_h), a.q_h, s.rows, a.scale_log2, lane);
+    const bool fresh = a.kn && (!a.active || a.active[s.b]);
+#pragma unroll 1
+    for (int k = 0; k < mine; ++k) {
+      issue(k + F::kStages - 1);
+      cp_async_wait<F::kStages - 1>();
+      __syncwarp();
+      const int pos = (s.g0 + warp + k * kWarps) * kGran;
+      const uint32_t tile = ring + (k % F::kStages) * F::kBlock;
+      const bool edge = pos < s.lo || pos + kGran > s.hi;
+      if (fresh && pos + kGran >= s.hi) {
+        // the new token's rows, packed, into the granule and (once, where several head groups share it) its page
+        const int token = s.hi - 1 - pos, gr = (s.hi - 1) / kGran, pi = gr / a.page_grans, page = table[pi];
+        uint8_t* block = s.r0 == 0 && page >= 0 && page < a.num_pages
+                             ? a.pool + page * a.p_p + s.h * a.p_h + (gr - pi * a.page_grans) * a.p_g : nullptr;
+#pragma unroll
+        for (int i = 0; i < (2 * (DH / 8) + 31) / 32; ++i) {
+          const int x = 32 * i + lane, c = x % (DH / 8);
+          const bool isv = x >= DH / 8, any = x < 2 * (DH / 8);
+          uint4 raw = make_uint4(0, 0, 0, 0);
+          if (any)
+            raw = isv ? ld_128(a.vn + 2 * (s.b * a.vn_b + s.h * a.vn_h) + 16 * c) : ld_128(a.kn + 2 * (s.b * a.kn_b + s.h * a.kn_h) + 16 * c);
+          uint32_t word, sm_pair;
+          int4_pack<T>(raw, word, sm_pair);
+          if (any) {
+            const int at_word = (isv ? int4_half_bytes(DH) : 0) + int4_word_at(DH, token, c);
+            const int at_pair = (isv ? int4_half_bytes(DH) : 0) + int4_pair_at(DH, token, c);
+            sts32(tile + at_word, word);
+            if (block) *reinterpret_cast<uint32_t*>(block + at_word) = word;
+            if ((c & 7) == 0) {
+              sts32(tile + at_pair, sm_pair);
+              if (block) *reinterpret_cast<uint32_t*>(block + at_pair) = sm_pair;
+            }
+          }
+        }
+        __syncwarp();
+      }
+      acc.granule(tile, pos, edge, s.lo, s.hi, lane);
+      __syncwarp();  // the slot has been read
+    }
+    acc.finish();
+
+    // ---- the warps' results joined: each leaves (m, l) and its outputs in its ring's place
+    const int g = lane >> 2, t = lane & 3;
+    cp_async_wait<0>();
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < F::kTiles; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = 8 * n + 2 * t + x;
+        if (r >= s.rows) continue;
+        if (g == 0) ml[warp * F::kHeads + r] = make_float2(acc.ref[n][x], acc.l[n][x]);
+        float* dst = reinterpret_cast<float*>(sm + warp * F::kRing) + r * F::kPitch;
+#pragma unroll
+        for (int y = 0; y < GR; ++y) {
+          float c[8];
+          acc.columns(n, y, x, c);
+          *reinterpret_cast<float4*>(dst + 64 * y + 8 * g) = make_float4(c[0], c[1], c[2], c[3]);
+          *reinterpret_cast<float4*>(dst + 64 * y + 8 * g + 4) = make_float4(c[4], c[5], c[6], c[7]);
+        }
+      }
+    __syncthreads();
+    for (int it = tid; it < s.rows * (DH / 4); it += kThreads) {
+      const int r = it / (DH / 4), c = it % (DH / 4) * 4;
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w * F::kHeads + r].x);
+      const float base = M == -INFINITY ? 0.f : M;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 x = ml[w * F::kHeads + r];
+        const float4 y = *reinterpret_cast<const float4*>(sm + w * F::kRing + 4 * (r * F::kPitch + c));
+        const float p = x.y * ex2_approx(x.x - base);
+        L += p;
+        v.x = fmaf(y.x, p, v.x);
+        v.y = fmaf(y.y, p, v.y);
+        v.z = fmaf(y.z, p, v.z);
+        v.w = fmaf(y.w, p, v.w);
+      }
+      const float d = L == 0.f ? 0.f : 1.f / L;
+      v = make_float4(v.x * d, v.y * d, v.z * d, v.w * d);
+      if (s.slot < 0) {
+        const int64_t hq = s.h * a.G + s.r0 + r;
+        *reinterpret_cast<uint2*>(a.out + 2 * (s.b * a.o_b + hq * a.o_h + c)) =
+            make_uint2(ElemTraits<T>::pack2(v.x, v.y), ElemTraits<T>::pack2(v.z, v.w));
+        if (a.lse && c == 0) a.lse[s.b * a.ls_b + hq * a.ls_h] = lse_of(M, L);
+      } else {
+        *reinterpret_cast<float4*>(a.ws + kWsO + 4 * ((int64_t)s.slot * 2048 + r * DH + c)) = v;
+        if (c == 0) reinterpret_cast<float2*>(a.ws + kWsMl)[s.slot * kPartRows + r] = make_float2(M, L);
+      }
+    }
+    __syncthreads();  // the rings are free again
+  }
+  // for the join: the cut pair that begins in this CTA, if one does
+  if (tid == 0) {
+    if (uncut) begun.parts = 0;
+    reinterpret_cast<CutPair*>(a.ws + kWsCut)[blockIdx.x] = begun;
+  }
+  // requests without keys
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (len_of(b) != 0) continue;
+    const int hq = a.Hkv * a.G;
+    for (int i = tid; i < hq * (DH / 8); i += kThreads)
+      st_128(a.out + 2 * (b * a.o_b + (int64_t)(i / (DH / 8)) * a.o_h) + 16 * (i % (DH / 8)), make_uint4(0, 0, 0, 0));
+    if (a.lse)
+      for (int i = tid; i < hq; i += kThreads) a.lse[b * a.ls_b + i * a.ls_h] = -INFINITY;
+  }
+}
+
+// The cut pair that begins in CTA blockIdx.x: 32 columns of its parts' outputs, weighted and summed in the order
+// of the line.
+template <typename T, int DH>
+__global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_constant__ Int4Args a) {
+  __shared__ float weight[kPartRows][kMaxCtas];
+  __shared__ float4 sums[kThreads];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int first = blockIdx.x, c0 = 32 * blockIdx.y;
+  const CutPair p = reinterpret_cast<const CutPair*>(a.ws + kWsCut)[first];
+  if (p.parts == 0) return;
+  auto slot = [&](int i) { return 2 * (first + i) + (i == 0 ? 1 : 0); };
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + kWsMl);
+  for (int r = warp; r < p.rows; r += kWarps) {
+    float M = -INFINITY, L = 0.f;
+    for (int i = lane; i < p.parts; i += 32) M = fmaxf(M, ml[slot(i) * kPartRows + r].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float base = M == -INFINITY ? 0.f : M;
+    for (int i = lane; i < p.parts; i += 32) {
+      const float2 x = ml[slot(i) * kPartRows + r];
+      const float w = x.y * ex2_approx(x.x - base);
+      weight[r][i] = w;
+      L += w;
+    }
+    L = warp_sum(L);
+    const float d = L == 0.f ? 0.f : 1.f / L;
+    __syncwarp();
+    for (int i = lane; i < p.parts; i += 32) weight[r][i] *= d;
+    if (a.lse && c0 == 0 && lane == 0) a.lse[p.b * a.ls_b + (int64_t)(p.h * a.G + p.r0 + r) * a.ls_h] = lse_of(M, L);
+  }
+  __syncthreads();
+  const int items = p.rows * 8, groups = kThreads / items, grp = tid / items, it = tid % items;
+  const int r = it >> 3, c = c0 + 4 * (it & 7);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (grp < groups) {
+#pragma unroll 4
+    for (int i = grp; i < p.parts; i += groups) {
+      const float4 u = *reinterpret_cast<const float4*>(a.ws + kWsO + 4 * ((int64_t)slot(i) * 2048 + r * DH + c));
+      const float w = weight[r][i];
+      v.x = fmaf(u.x, w, v.x);
+      v.y = fmaf(u.y, w, v.y);
+      v.z = fmaf(u.z, w, v.z);
+      v.w = fmaf(u.w, w, v.w);
+    }
+  }
+  sums[tid] = v;
+  __syncthreads();
+  if (tid >= items) return;
+  for (int x = 1; x < groups; ++x) {
+    const float4 u = sums[x * items + tid];
+    v.x += u.x;
+    v.y += u.y;
+    v.z += u.z;
+    v.w += u.w;
+  }
+  *reinterpret_cast<uint2*>(a.out + 2 * (p.b * a.o_b + (int64_t)(p.h * a.G + p.r0 + r) * a.o_h + c)) =
+      make_uint2(ElemTraits<T>::pack2(v.x, v.y), ElemTraits<T>::pack2(v.z, v.w));
+}
+
+template <class K>
+int launch_dependent(K kern, const Int4Args& a, dim3 grid, int smem, cudaStream_t s, const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a), what);
+}
+
+template <class F>
+int launch(const Int4Args& a, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};  // devices (bits) whose kernel has its shared memory allowed
+  static std::atomic<int> sms[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int n = dev < 64 ? sms[dev].load() : 0;
+  if (n == 0 || !(ready.load() >> dev & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(int4_decode_kernel<F>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kBytes);
+    if (e != cudaSuccess) return check_cuda(e, "paged_decode_int4 attributes");
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (dev < 64) {
+      sms[dev].store(n);
+      ready.fetch_or(1ull << dev);
+    }
+  }
+  // No more CTAs than there could be shares; pairs of up to 2 kSlack granules are never cut.
+  const int64_t keys = a.window > 0 ? std::min((int64_t)a.width * a.page_size, (int64_t)a.window + 2 * kGran) : (int64_t)a.width * a.page_size;
+  const int64_t longest = (keys + kGran - 1) / kGran;
+  const double most = (double)a.B * a.Hkv * a.chunks * (double)longest / kMinShare;
+  const int grid = (int)std::max(1.0, std::min((double)std::min(n * F::kCtas, kMaxCtas), std::ceil(most)));
+  if (int rc = launch_dependent(int4_decode_kernel<F>, a, dim3(grid), F::kBytes, s, "paged_decode_int4 launch")) return rc;
+  if (grid == 1 || longest <= 2 * kSlack) return BNA_OK;
+  return launch_dependent(int4_join_kernel<typename F::T, F::DH>, a, dim3(grid, F::DH / 32), 0, s, "paged_decode_int4 join launch");
+}
+
+}  // namespace
+
+int64_t paged_decode_int4_workspace_bytes() { return kWsBytes; }
+
+int launch_paged_decode_int4(const bna_tensor4* q, bna_tensor4* pool, const bna_tensor4* kn, const bna_tensor4* vn, const uint8_t* active,
+                             bna_tensor4* out, float* lse, int64_t ls_b, int64_t ls_h, int dtype, const int32_t* table,
+                             int64_t table_stride, int width, const int32_t* lens, int window, float scale, void* ws, cudaStream_t s) {
+  Int4Args a{};
+  a.q = static_cast<const uint8_t*>(q->data);
+  a.q_b = q->stride[0], a.q_h = q->stride[1];
+  a.pool = static_cast<uint8_t*>(pool->data);
+  a.p_p = pool->stride[0], a.p_h = pool->stride[1], a.p_g = pool->stride[2];
+  if (kn) {
+    a.kn = static_cast<const uint8_t*>(kn->data), a.vn = static_cast<const uint8_t*>(vn->data);
+    a.active = active;
+    a.kn_b = kn->stride[0], a.kn_h = kn->stride[1], a.vn_b = vn->stride[0], a.vn_h = vn->stride[1];
+  }
+  a.out = static_cast<uint8_t*>(out->data);
+  a.o_b = out->stride[0], a.o_h = out->stride[1];
+  a.lse = lse, a.ls_b = ls_b, a.ls_h = ls_h;
+  a.table = table, a.table_stride = table_stride, a.lens = lens;
+  const int dh = (int)q->size[3];
+  a.B = (int)q->size[0], a.Hkv = (int)pool->size[1], a.G = (int)(q->size[1] / pool->size[1]);
+  a.width = width, a.num_pages = (int)pool->size[0], a.page_grans = (int)pool->size[2], a.page_size = a.page_grans * kGran, a.window = window;
+  const int most_rows = dh == 256 ? 8 : 16;
+  a.chunks = (a.G + most_rows - 1) / most_rows;
+  a.chunk_rows = (a.G + a.chunks - 1) / a.chunks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.ws = static_cast<uint8_t*>(ws);
+  const bool bf = dtype == BNA_BF16, wide = a.chunk_rows > 8;
+  switch (dh) {
+    case 64:
+      if (bf) return wide ? launch<Form<__nv_bfloat16, 64, true>>(a, s) : launch<Form<__nv_bfloat16, 64, false>>(a, s);
+      return wide ? launch<Form<__half, 64, true>>(a, s) : launch<Form<__half, 64, false>>(a, s);
+    case 128:
+      if (bf) return wide ? launch<Form<__nv_bfloat16, 128, true>>(a, s) : launch<Form<__nv_bfloat16, 128, false>>(a, s);
+      return wide ? launch<Form<__half, 128, true>>(a, s) : launch<Form<__half, 128, false>>(a, s);
+    case 256:
+      return bf ? launch<Form<__nv_bfloat16, 256, false>>(a, s) : launch<Form<__half, 256, false>>(a, s);
+    default: return fail(BNA_UNSUPPORTED, "paged_decode_attention_int4: head_dim must be 64, 128 or 256");
+  }
+}
+
+}  // namespace bna

@@ -167,6 +167,51 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     return r
 
 
+def int4_pool(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, device: torch.device | str = "cuda") -> torch.Tensor:
+    """An empty 4-bit pool for the functions below: bytes [pages, Hkv, page_size / 16, 18 dh]."""
+    if page_size % 16 or head_dim not in (64, 128, 256):
+        raise ValueError("a 4-bit pool needs a page_size that is a multiple of 16 and a head_dim of 64, 128 or 256")
+    return torch.empty((num_pages, num_kv_heads, page_size // 16, 18 * head_dim), dtype=torch.uint8, device=device)
+
+
+def paged_append_int4(k: torch.Tensor, v: torch.Tensor, kv_pages: torch.Tensor, slot_map: torch.Tensor) -> None:
+    """``paged_append`` into a 4-bit pool ``kv_pages`` [pages, Hkv, page_size / 16, 18 dh] of bytes (``int4_pool``).
+
+    Each group of 64 columns of a row keeps its minimum m and the scale s = (maximum - m) / 15, in the rows'
+    type, and 4-bit codes c = round((x - m) / s); x is read as s c + m, off by s / 2 or little more: 4.5
+    bits a column.  A group with a NaN or an infinity, or whose range passes the type's, reads as NaN.  The
+    slots of a call must differ (but for negative ones, which are skipped)."""
+    _lib.check((_native or _binding()).append_int4(k, v, kv_pages, slot_map, _stream(k)))
+
+
+def paged_read_int4(kv_pages: torch.Tensor, slot_map: torch.Tensor, *, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows in slots ``slot_map`` (int64 [tokens]) as k, v [tokens, Hkv, dh] of ``dtype``, the type they were
+    appended in; zeros for negative slots."""
+    r = (_native or _binding()).read_int4(kv_pages, slot_map, _lib.dtype_code(dtype) == _lib.F16, _stream(kv_pages))
+    if r.__class__ is int:
+        _lib.check(r)
+    return r
+
+
+def paged_decode_attention_int4(q: torch.Tensor, kv_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
+                                k_new: Optional[torch.Tensor] = None, v_new: Optional[torch.Tensor] = None,
+                                active: Optional[torch.Tensor] = None, window: int = 0, scale: Optional[float] = None,
+                                return_lse: bool = False, workspace: Optional[torch.Tensor] = None):
+    """``paged_decode_attention`` over a 4-bit pool whose rows were appended in q's type.
+
+    Keys and values count as s c + m without another rounding.  ``k_new`` / ``v_new`` are packed as
+    ``paged_append_int4`` would and attended to in that form.  A row that attends to a NaN is NaN.  Entries of
+    q from 2^114 on in magnitude count as infinite, values from 2^100 on may overflow."""
+    stream = _stream(q)
+    r = (_native or _binding()).decode_int4(
+        q, kv_pages, block_table, lens, k_new, v_new, active, window,
+        1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else scale, return_lse,
+        _workspace_for(q, stream) if workspace is None else workspace, stream)
+    if r.__class__ is int:
+        _lib.check(r)
+    return r
+
+
 class PagedKVCache:
     """Pools of ``num_layers`` layers under one set of block tables, lengths and free pages.
 

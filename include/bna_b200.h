@@ -408,6 +408,34 @@ BNA_API int bna_paged_decode(const bna_tensor4* q, bna_tensor4* k_pages, bna_ten
                              const int32_t* lens, int32_t window, float scale, void* workspace,
                              int64_t workspace_bytes, void* stream);
 
+/* ---- Paged key/value cache in 4 bits -----------------------------------------------------------
+ * A pool is [pages, Hkv, page_size / 16, 18 dh] bytes (strides in bytes, multiples of 16): a block of 16 tokens of a
+ * head holds key codes [16][dh / 2], key (scale, minimum) pairs [16][dh / 64][2] in the cache's 16-bit type, and
+ * the same of the values.  A row is cut into groups of 64 columns with minimum m, scale s = (maximum - m) / 15
+ * rounded to the type, and codes c = rint((x - m) / s), clipped to 0..15 (0 where s is 0): x is read as s c + m.  Code
+ * word (8 codes, the first in the lowest bits) g * (dh / 64) + y of a row holds columns 64 y + 8 g .. + 7.  A
+ * group with a NaN or an infinity, or whose range passes the type's, reads as NaN.  Tables, slots and lengths are
+ * those of the 16-bit pools (bna_paged_reserve serves both).  dtype: the type of the rows that go in and come out. */
+
+/* Rows t of k / v [1, Hkv, tokens, dh] into slot slot_map[t] of every head's pages; a slot outside the pool (-1) is
+ * skipped.  Two tokens with one slot leave a mixture of both. */
+BNA_API int bna_paged_append_int4(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* kv_pages, const int64_t* slot_map,
+                                  int32_t dtype, void* stream);
+/* The rows in slots slot_map[t] into k / v [1, Hkv, tokens, dh], rounded once; zeros for a slot outside the pool. */
+BNA_API int bna_paged_read_int4(const bna_tensor4* kv_pages, const int64_t* slot_map, bna_tensor4* k, bna_tensor4* v, int32_t dtype,
+                                void* stream);
+/* bna_paged_decode over such a pool: attention to the rows' values s c + m, unrounded.  k_new / v_new are packed as an
+ * append would, written, and attended to in that form.  Rows that attend to a NaN are NaN; entries of q from 2^114 on in
+ * magnitude count as infinite, and values from 2^100 on may overflow.  workspace: bna_paged_decode_int4_workspace_bytes() of device memory,
+ * 16-byte aligned; one of bna_paged_decode_workspace_bytes() serves both kinds of calls (its first 4096 bytes are
+ * left alone here).  Calls that may overlap on the GPU need a workspace each. */
+BNA_API int64_t bna_paged_decode_int4_workspace_bytes(void);
+BNA_API int bna_paged_decode_int4(const bna_tensor4* q, bna_tensor4* kv_pages, const bna_tensor4* k_new, const bna_tensor4* v_new,
+                                  const uint8_t* active, bna_tensor4* out, float* lse, int64_t lse_stride_b, int64_t lse_stride_h,
+                                  int32_t dtype, const int32_t* block_table, int64_t table_stride, int32_t table_width,
+                                  const int32_t* lens, int32_t window, float scale, void* workspace, int64_t workspace_bytes,
+                                  void* stream);
+
 /* ---- Token log probabilities -----------------------------------------------------------------
  * No counterpart in the reference.  Row r of the logits (bf16, fp16 or fp32, `vocab` contiguous entries) starts at element
  * (r / inner) * stride_outer + (r % inner) * stride.  Per row, in fp32 and natural logarithms, with p = softmax(row):
