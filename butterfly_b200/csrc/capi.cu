@@ -556,6 +556,9 @@ static int int4_rows(bool append, const bna_tensor4* k, const bna_tensor4* v, bn
   if (k->size[2] == 0) return BNA_OK;
   if (int rc = check_rows(k, "k", dh)) return rc;
   if (int rc = check_rows(v, "v", dh)) return rc;
+  for (const bna_tensor4* t : {k, v})
+    for (int d = 1; d < 3; ++d)
+      if (!append && t->size[d] > 1 && t->stride[d] < dh) return fail(BNA_BAD_STRIDE, name + ": rows of k and v must not overlap");
   if (!slot_map) return fail(BNA_BAD_SHAPE, name + ": null slot_map");
   if (reinterpret_cast<uintptr_t>(slot_map) & 7) return fail(BNA_BAD_STRIDE, name + ": slot_map must be 8-byte aligned");
   return launch_int4_rows(append, k, v, pool, slot_map, dtype, (cudaStream_t)stream);
@@ -567,10 +570,6 @@ int bna_paged_append_int4(const bna_tensor4* k, const bna_tensor4* v, bna_tensor
 }
 
 int bna_paged_read_int4(const bna_tensor4* kv_pages, const int64_t* slot_map, bna_tensor4* k, bna_tensor4* v, int32_t dtype, void* stream) {
-  if (k && v)
-    for (int d = 1; d < 3; ++d)
-      if ((k->size[d] > 1 && k->stride[d] < k->size[3]) || (v->size[d] > 1 && v->stride[d] < v->size[3]))
-        return fail(BNA_BAD_STRIDE, "paged_read_int4: rows of k and v must not overlap");
   return int4_rows(false, k, v, const_cast<bna_tensor4*>(kv_pages), slot_map, dtype, stream);
 }
 
