@@ -40,6 +40,8 @@ constexpr int kGran = kInt4Tokens;  // keys of a granule: a block
 constexpr int kMaxCtas = 320;       // the workspace is sized for this many
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kSlack = 40;    // granules
+constexpr int kWhole = 80;    // granules of the longest pair up to which every pair gets a CTA of its own
+static_assert(kWhole <= 2 * kSlack + 1, "pairs that are never cut");
 constexpr int kMinShare = 32;  // granules a CTA gets at least (fewer CTAs otherwise)
 constexpr int kKeepLens = 1024;  // lengths kept in shared memory
 constexpr int kShift = 11;  // probabilities are held times 2^kShift, and so are l and o; the divisions undo it
@@ -62,7 +64,8 @@ struct Int4Args {
   int64_t table_stride;
   const int32_t* lens;
   int B, Hkv, G, width, num_pages, page_size, window;
-  int page_grans;          // blocks of a page
+  int page_grans, page_shift;  // blocks of a page, and their log2 (or -1)
+  int whole;               // one pair a CTA
   int chunks, chunk_rows;  // the G heads in `chunks` groups of chunk_rows
   float scale_log2;
   uint8_t* ws;
@@ -77,7 +80,8 @@ struct CutPair {
 constexpr int64_t kWsCut = 4096;
 constexpr int64_t kWsMl = kWsCut + kMaxCtas * (int64_t)sizeof(CutPair);
 constexpr int64_t kWsO = kWsMl + (int64_t)2 * kMaxCtas * kPartRows * 8;
-constexpr int64_t kWsBytes = kWsO + (int64_t)2 * kMaxCtas * 2048 * 4;  // (a part has 8 rows of 256 or 16 of 128 at most)
+constexpr int kPartFloats = 2048;  // a part has 8 rows of 256 or 16 of 128 at most
+constexpr int64_t kWsBytes = kWsO + (int64_t)2 * kMaxCtas * kPartFloats * 4;
 
 __device__ __forceinline__ int first_key(const Int4Args& a, int len) { return a.window > 0 ? max(0, len - a.window) : 0; }
 __device__ __forceinline__ int clamp_len(const Int4Args& a, int len) {
@@ -87,8 +91,8 @@ __device__ __forceinline__ int granules_of(const Int4Args& a, int len) {
   return len == 0 ? 0 : (len + kGran - 1) / kGran - first_key(a, len) / kGran;
 }
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {  // zeros where not valid
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -111,7 +115,16 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t (&r)[N]) {
                    : "memory");
   }
 }
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// D = A B for one m16n8k16 tile of fp16 (mma_16816 without a sum to start from)
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 // 8x8 matrix of 16-bit entries, transposed
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -156,7 +169,7 @@ struct Form {
   static_assert(kHeads * kPitch * 4 <= kRing, "a warp's outputs take its ring's place");
   static constexpr int kMl = kWarps * kRing;                   // (m, l) [warp][head]
   static constexpr int kRuns = kMl + kWarps * kHeads * 8;      // granules up to the end of each thread's run of requests
-  static constexpr int kLens = kRuns + kThreads * 8;
+  static constexpr int kLens = kRuns + kThreads * 4;
   static constexpr int kBytes = kLens + 4 * kKeepLens;
   static_assert(kCtas * (kBytes + 1024) <= 233472, "shared memory of an SM");
 };
@@ -177,17 +190,25 @@ struct Acc {
   float o[NT][GR][4][4];          // sum p sv cv, in units of 2^-24 (odd columns 2^-20) 2^e
   float bound, inv;               // 2^e, above every value scale so far, and 2^-e
 
-  // q: the head group's first row; rows from `rows` on count as zeros
-  __device__ __forceinline__ void begin(const uint8_t* q, int64_t q_h, int rows, float scale_log2, int lane) {
-    const int g = lane >> 2, t = lane & 3;
+  // This lane's part of the queries.  q: the head group's first row; rows from `rows` on count as zeros
+  struct Queries {
+    uint4 raw[NT][GR][2];
+    __device__ __forceinline__ void load(const uint8_t* q, int64_t q_h, int rows, int lane) {
+      const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int y = 0; y < GR; ++y)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            raw[n][y][j] = g + 8 * n < rows ? ld_nc_128(q + 2 * ((g + 8 * n) * q_h + 64 * y + 16 * t + 8 * j)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  __device__ __forceinline__ void begin(const Queries& from, float scale_log2, int lane) {
+    const int t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      uint4 raw[GR][2];
-#pragma unroll
-      for (int y = 0; y < GR; ++y)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          raw[y][j] = g + 8 * n < rows ? ld_nc_128(q + 2 * ((g + 8 * n) * q_h + 64 * y + 16 * t + 8 * j)) : make_uint4(0, 0, 0, 0);
+      const uint4(&raw)[GR][2] = from.raw[n];
       float top = 0.f;
 #pragma unroll
       for (int y = 0; y < GR; ++y)
@@ -270,16 +291,8 @@ struct Acc {
       lds(tile + 8 * DH + row * (4 * GR), p[0]);
       lds(tile + 8 * DH + (row + 8) * (4 * GR), p[1]);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) u[n][x] = 0.f;
-#pragma unroll
       for (int y = 0; y < GR; ++y) {
         float acc[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) acc[n][x] = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t a0 = w[0][j * GR + y], a1 = w[1][j * GR + y];
@@ -287,7 +300,8 @@ struct Acc {
           const uint32_t odd[4] = {(a0 >> 8) & M0, (a1 >> 8) & M0, (a0 >> 8) & M1, (a1 >> 8) & M1};
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            mma_16816<__half>(acc[n], even, qb[n][y][j][0][0], qb[n][y][j][0][1]);
+            if (j == 0) mma_first(acc[n], even, qb[n][y][j][0][0], qb[n][y][j][0][1]);
+            else mma_16816<__half>(acc[n], even, qb[n][y][j][0][0], qb[n][y][j][0][1]);
             mma_16816<__half>(acc[n], odd, qb[n][y][j][1][0], qb[n][y][j][1][1]);
           }
         }
@@ -297,7 +311,10 @@ struct Acc {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) u[n][2 * r + x] = fmaf(sm.x, acc[n][2 * r + x], fmaf(sm.y, qs[n][y][x], u[n][2 * r + x]));
+            for (int x = 0; x < 2; ++x) {
+              const float base = y == 0 ? sm.y * qs[n][y][x] : fmaf(sm.y, qs[n][y][x], u[n][2 * r + x]);
+              u[n][2 * r + x] = fmaf(sm.x, acc[n][2 * r + x], base);
+            }
         }
       }
     }
@@ -328,19 +345,16 @@ struct Acc {
       }
     }
     // probabilities times 2^kShift
-    float e[NT][4], top = 0.f;
-    bool move = false;
+    float e[NT][4], top = fmaxf(sv[0][0], sv[1][0]), most = -INFINITY;
 #pragma unroll
-    for (int y = 0; y < GR; ++y) top = fmaxf(top, fmaxf(sv[0][y], sv[1][y]));
-    move = top >= bound;
+    for (int y = 1; y < GR; ++y) top = fmax3(top, sv[0][y], sv[1][y]);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        e[n][x] = fmaf(f[n][x & 1], u[n][x], -off[n][x & 1]);
-        move |= e[n][x] > kShift + kMove;
-      }
-    if (__any_sync(0xffffffffu, move)) {
+      for (int x = 0; x < 4; ++x) e[n][x] = fmaf(f[n][x & 1], u[n][x], -off[n][x & 1]);
+      most = fmax3(most, fmaxf(e[n][0], e[n][1]), fmaxf(e[n][2], e[n][3]));
+    }
+    if (__any_sync(0xffffffffu, top >= bound || most > kShift + kMove)) {
       float scale = 1.f;
       top = lane_max(top);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -452,97 +466,129 @@ struct Acc {
   }
 };
 
+// Granules up to the end of each thread's run of requests, cut evenly over C CTAs (the first U % C get one more).
+struct Line {
+  const int* runs;
+  const int* lens;  // the first kKeepLens lengths
+  int per, per_b, U, C, q, r;
+
+  __device__ int raw(int c) const { return c * q + min(c, r); }
+  __device__ int cta_of(int x) const {  // whose raw stretch holds x
+    const int wide = r * (q + 1);
+    return x < wide ? x / (q + 1) : r + (x - wide) / max(q, 1);
+  }
+};
+// A request's place on the line, and the granules of each of its pairs.
+struct At {
+  int b, nt, begin;
+};
+
 template <class F>
 __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const __grid_constant__ Int4Args a) {
   using T = typename F::T;
   constexpr int DH = F::DH, GR = F::GR;
   extern __shared__ __align__(128) uint8_t sm[];
-  int64_t* runs = reinterpret_cast<int64_t*>(sm + F::kRuns);
-  int* lens = reinterpret_cast<int*>(sm + F::kLens);
-  __shared__ int64_t warp_sums[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per_b = a.Hkv * a.chunks;
+  int* lens = reinterpret_cast<int*>(sm + F::kLens);
+  auto len_of = [&](int b) { return b < kKeepLens ? lens[b] : clamp_len(a, a.lens[b]); };
+  Line line{reinterpret_cast<const int*>(sm + F::kRuns), lens, (a.B + kThreads - 1) / kThreads, per_b, 0, 1, 0, 0};
+  At at{0, 0, 0};
+  int cur = 0, end = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ---- the line: granules up to the end of each thread's run of requests
-  const int per = (a.B + kThreads - 1) / kThreads, per_b = a.Hkv * a.chunks;
-  {
-    int64_t mine = 0;
-    for (int b = tid * per; b < min((tid + 1) * per, a.B); ++b) {
-      const int len = clamp_len(a, a.lens[b]);
+  if (!a.whole) {
+    // ---- the line
+    __shared__ int warp_sums[kWarps];
+    int* runs = reinterpret_cast<int*>(sm + F::kRuns);
+    int mine = 0, pairs = 0;
+    for (int b = tid * line.per; b < min((tid + 1) * line.per, a.B); ++b) {
+      const int len = clamp_len(a, a.lens[b]), nt = granules_of(a, len);
       if (b < kKeepLens) lens[b] = len;
-      mine += granules_of(a, len);
+      mine += nt;
+      pairs += nt > 0;
     }
     mine *= per_b;
-    int64_t incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += x;
     }
-    if (lane == 31) warp_sums[warp] = incl;
+    pairs = __reduce_add_sync(0xffffffffu, pairs) * per_b;
+    __shared__ int warp_pairs[kWarps];
+    if (lane == 31) {
+      warp_sums[warp] = incl;
+      warp_pairs[warp] = pairs;
+    }
     __syncthreads();
+    pairs = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w)
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) incl += warp_sums[w];
+      pairs += warp_pairs[w];
+    }
     runs[tid] = incl;
     __syncthreads();
-  }
-  auto len_of = [&](int b) { return b < kKeepLens ? lens[b] : clamp_len(a, a.lens[b]); };
-  const int64_t U = runs[kThreads - 1];
-  const int C = (int)min((int64_t)gridDim.x, max((int64_t)1, (U + kMinShare - 1) / kMinShare));
-  const int64_t cq = U / C, cr = U - cq * C;
-  auto raw_cut = [&](int64_t c) { return c * cq + min(c, cr); };
-  // The pair at place x of the line: its request, where the request begins, and the granules of each of its pairs.
-  struct At {
-    int b, nt;
-    int64_t begin;
-  };
-  auto locate = [&](int64_t x) {
-    int lo = 0, hi = kThreads - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (runs[mid] > x) hi = mid;
-      else lo = mid + 1;
+    line.U = runs[kThreads - 1];
+    // a CTA for every kMinShare granules, or for every pair, where that is more
+    line.C = min((int)gridDim.x, max(1, max(pairs, (line.U + kMinShare - 1) / kMinShare)));
+    line.q = line.U / line.C;
+    line.r = line.U - line.q * line.C;
+    auto locate = [&](int x) {
+      int lo = 0, hi = kThreads - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (line.runs[mid] > x) hi = mid;
+        else lo = mid + 1;
+      }
+      At r{lo * line.per, 0, lo > 0 ? line.runs[lo - 1] : 0};
+      for (;; ++r.b) {
+        r.nt = granules_of(a, r.b < a.B ? len_of(r.b) : 0);
+        if (r.b >= a.B - 1 || r.begin + r.nt * per_b > x) return r;
+        r.begin += r.nt * per_b;
+      }
+    };
+    if ((int)blockIdx.x < line.C) {
+      // both ends of the stretch, moved to the nearest end of their pair where that is close
+#pragma unroll 1
+      for (int i = 1; i >= 0; --i) {
+        int x = line.raw((int)blockIdx.x + i);
+        if (x < line.U) {
+          at = locate(x);
+          if (x > 0) {
+            const int t = (x - at.begin) % max(at.nt, 1), rest = at.nt - t;
+            x = t <= kSlack && t <= rest ? x - t : rest <= kSlack ? x + rest : x;
+          }
+        }
+        if (i == 1) end = x;
+        else cur = x;
+      }
     }
-    At r{lo * per, 0, lo > 0 ? runs[lo - 1] : 0};
-    for (;; ++r.b) {
-      r.nt = granules_of(a, r.b < a.B ? len_of(r.b) : 0);
-      if (r.b >= a.B - 1 || r.begin + (int64_t)r.nt * per_b > x) return r;
-      r.begin += (int64_t)r.nt * per_b;
-    }
-  };
-  // A cut moved to the nearest end of its pair where that is close.
-  auto cut = [&](int64_t c) -> int64_t {
-    const int64_t x = raw_cut(c);
-    if (x <= 0 || x >= U) return min(max(x, (int64_t)0), U);
-    const At at = locate(x);
-    const int t = (int)((x - at.begin) % at.nt);
-    return t <= kSlack && t <= at.nt - t ? x - t : at.nt - t <= kSlack ? x + at.nt - t : x;
-  };
-  int64_t cur = 0, end = 0;
-  if ((int)blockIdx.x < C) {
-    cur = cut(blockIdx.x);
-    end = cut((int64_t)blockIdx.x + 1);
+  } else {
+    // ---- one pair a CTA, none of them long enough to be cut: nothing to find out but its length
+    at.b = (int)blockIdx.x / per_b;
+    const int len = clamp_len(a, a.lens[at.b]);
+    at.nt = granules_of(a, len);
+    cur = ((int)blockIdx.x - at.b * per_b) * at.nt;
+    end = cur + at.nt;
   }
   CutPair begun{};
-  bool uncut = true;
 
   // ---- the pairs of this CTA's stretch
   const uint32_t ring = smem_u32(sm) + warp * F::kRing;
   float2* ml = reinterpret_cast<float2*>(sm + F::kMl);
-  At at{0, 0, 0};
-  if (cur < end) at = locate(cur);
   while (cur < end) {
-    while (cur >= at.begin + (int64_t)at.nt * per_b && at.b + 1 < a.B) {  // (requests without keys are passed over)
-      at.begin += (int64_t)at.nt * per_b;
+    while (cur >= at.begin + at.nt * per_b && at.b + 1 < a.B) {  // (requests without keys are passed over)
+      at.begin += at.nt * per_b;
       ++at.b;
       at.nt = granules_of(a, len_of(at.b));
     }
-    const int64_t local = cur - at.begin;
-    if (at.nt == 0 || local >= (int64_t)at.nt * per_b) break;  // (only where lengths changed under the call)
-    const int pair = (int)(local / at.nt), t0 = (int)(local - (int64_t)pair * at.nt);
-    const int len = len_of(at.b);
+    const int local = cur - at.begin;
+    if (at.nt == 0 || local >= at.nt * per_b) break;  // (only where lengths changed under the call)
+    const int pair = local / at.nt, t0 = local - pair * at.nt;
+    const int len = a.whole ? clamp_len(a, a.lens[at.b]) : len_of(at.b);
     Seg s;
     s.b = at.b;
     s.h = pair / a.chunks;
@@ -551,52 +597,80 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
     s.lo = first_key(a, len);
     s.hi = len;
     s.g0 = s.lo / kGran + t0;
-    s.n = (int)min((int64_t)(at.nt - t0), end - cur);
+    s.n = min(at.nt - t0, end - cur);
     s.slot = s.n == at.nt ? -1 : 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0);
-    if (s.slot >= 0 && t0 == 0) {  // a cut pair begins here: its parts are the CTAs up to the one that holds its end
-      const int64_t p1 = cur + at.nt;
-      int c = (int)blockIdx.x + 1;
-      // (cuts within the pair keep their places; those near its end have moved there)
-      const int64_t last = p1 - kSlack - 1;  // the last place that a cut inside can have
-      const int64_t wide = cr * (cq + 1);
-      // the CTA whose raw stretch holds `last`: cuts up to its start lie inside
-      c = min(max(c, (int)(last < wide ? last / (cq + 1) : cr + (last - wide) / max(cq, (int64_t)1))), C - 1);
-      begun = CutPair{s.b, s.h, s.r0, s.rows, c - (int)blockIdx.x + 1, {0, 0, 0}};
-      uncut = false;
+    if (s.slot >= 0 && t0 == 0) {
+      // A cut pair begins here: its parts are those of the CTAs up to the one that holds its end.  Cuts within it kept their
+      // places (those near its end have moved there): the last of them lies at or before this place.
+      const int last = min(max((int)blockIdx.x + 1, line.cta_of(cur + at.nt - kSlack - 1)), line.C - 1);
+      begun = CutPair{s.b, s.h, s.r0, s.rows, last - (int)blockIdx.x + 1, {0, 0, 0}};
     }
     cur += s.n;
 
     // this warp's granules: warp, warp + kWarps, ...
     const int mine = (s.n - warp + kWarps - 1) / kWarps;
     const int32_t* table = a.table + s.b * a.table_stride;
-    // lane i: where granule i of a batch of 32 lies, or null
-    auto look_up = [&](int k0) -> const uint8_t* {
-      const int k = k0 + lane;
-      if (k >= mine) return nullptr;
-      const int gr = s.g0 + warp + k * kWarps, pi = gr / a.page_grans, page = table[pi];
+    auto block_at = [&](int gr) -> uint8_t* {  // where the request's granule gr lies (null: its page is outside the pool)
+      const int pi = a.page_shift >= 0 ? gr >> a.page_shift : gr / a.page_grans, page = table[pi];
       return page >= 0 && page < a.num_pages ? a.pool + page * a.p_p + s.h * a.p_h + (gr - pi * a.page_grans) * a.p_g : nullptr;
     };
+    auto look_up = [&](int k0) -> const uint8_t* {  // lane i: granule i of a batch of 32
+      const int k = k0 + lane;
+      return k < mine ? block_at(s.g0 + warp + k * kWarps) : nullptr;
+    };
     const uint8_t *batch = look_up(0), *next = look_up(32);
+    typename Acc<F>::Queries queries;
+    queries.load(a.q + 2 * (s.b * a.q_b + (int64_t)(s.h * a.G + s.r0) * a.q_h), a.q_h, s.rows, lane);
+    // The new token's row, if this warp gets its granule (the request's last): packed, for the granule and, once where
+    // several head groups share it, for its page.
+    constexpr int kNew = (2 * (DH / 8) + 31) / 32;
+    uint32_t new_word[kNew], new_pair[kNew];
+    const bool owns_new = a.kn && s.g0 + s.n == (s.hi + kGran - 1) / kGran && (s.n - 1) % kWarps == warp && (!a.active || a.active[s.b]);
+    auto new_at = [&](int i, int& word, int& pair) {  // byte offsets in the block of what the lane has of it; false: none
+      const int x = 32 * i + lane, c = x % (DH / 8), half = x >= DH / 8 ? int4_half_bytes(DH) : 0, token = (s.hi - 1) % kGran;
+      word = half + int4_word_at(DH, token, c);
+      pair = (c & 7) == 0 ? half + int4_pair_at(DH, token, c) : -1;
+      return x < 2 * (DH / 8);
+    };
+    if (owns_new) {
+      uint8_t* block = s.r0 == 0 ? block_at((s.hi - 1) / kGran) : nullptr;
+#pragma unroll
+      for (int i = 0; i < kNew; ++i) {
+        const int x = 32 * i + lane, c = x % (DH / 8);
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (x < DH / 8) raw = ld_128(a.kn + 2 * (s.b * a.kn_b + s.h * a.kn_h) + 16 * c);
+        else if (x < 2 * (DH / 8)) raw = ld_128(a.vn + 2 * (s.b * a.vn_b + s.h * a.vn_h) + 16 * c);
+        int4_pack<T>(raw, new_word[i], new_pair[i]);
+        int word, pair;
+        if (new_at(i, word, pair) && block) {
+          *reinterpret_cast<uint32_t*>(block + word) = new_word[i];
+          if (pair >= 0) *reinterpret_cast<uint32_t*>(block + pair) = new_pair[i];
+        }
+      }
+    }
     auto issue = [&](int k) {
-      if (k > 0 && (k & 31) == 0) {
+      if ((k & 31) == 0 && k > 0) {
         batch = next;
         next = look_up(k + 32);
       }
       if (k < mine) {
         const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(batch), k & 31));
-        const uint32_t dst = ring + (k % F::kStages) * F::kBlock;
+        const uint32_t dst = ring + (k % F::kStages) * F::kBlock + 16 * lane;
+        if (src) {
+          src += 16 * lane;
 #pragma unroll
-        for (int i = 0; i < (F::kBlock / 16 + 31) / 32; ++i)
-          if (32 * i + 32 <= F::kBlock / 16 || 32 * i + lane < F::kBlock / 16)
-            cp_async_16(dst + 512 * i + 16 * lane, src ? src + 512 * i + 16 * lane : a.pool, src != nullptr);
+          for (int i = 0; i < F::kBlock / 512; ++i) cp_async_16(dst + 512 * i, src + 512 * i);
+          if (F::kBlock % 512 && lane < F::kBlock % 512 / 16) cp_async_16(dst + F::kBlock / 512 * 512, src + F::kBlock / 512 * 512);
+        } else {  // a page outside the pool reads as zeros
+          for (int i = lane; i < F::kBlock / 16; i += 32) sts128(dst + 16 * (i - lane), make_uint4(0, 0, 0, 0));
+        }
       }
       cp_async_commit();  // (a group for every granule, empty ones past the end)
     };
 #pragma unroll 1
     for (int k = 0; k < F::kStages - 1; ++k) issue(k);
     Acc<F> acc;
-    acc.begin(a.q + 2 * (s.b * a.q_b + (int64_t)(s.h * a.G + s.r0) * a.q_h), a.q_h, s.rows, a.scale_log2, lane);
-    const bool fresh = a.kn && (!a.active || a.active[s.b]);
+    acc.begin(queries, a.scale_log2, lane);
 #pragma unroll 1
     for (int k = 0; k < mine; ++k) {
       issue(k + F::kStages - 1);
@@ -605,29 +679,13 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
       const int pos = (s.g0 + warp + k * kWarps) * kGran;
       const uint32_t tile = ring + (k % F::kStages) * F::kBlock;
       const bool edge = pos < s.lo || pos + kGran > s.hi;
-      if (fresh && pos + kGran >= s.hi) {
-        // the new token's rows, packed, into the granule and (once, where several head groups share it) its page
-        const int token = s.hi - 1 - pos, gr = (s.hi - 1) / kGran, pi = gr / a.page_grans, page = table[pi];
-        uint8_t* block = s.r0 == 0 && page >= 0 && page < a.num_pages
-                             ? a.pool + page * a.p_p + s.h * a.p_h + (gr - pi * a.page_grans) * a.p_g : nullptr;
+      if (owns_new && k == mine - 1) {
 #pragma unroll
-        for (int i = 0; i < (2 * (DH / 8) + 31) / 32; ++i) {
-          const int x = 32 * i + lane, c = x % (DH / 8);
-          const bool isv = x >= DH / 8, any = x < 2 * (DH / 8);
-          uint4 raw = make_uint4(0, 0, 0, 0);
-          if (any)
-            raw = isv ? ld_128(a.vn + 2 * (s.b * a.vn_b + s.h * a.vn_h) + 16 * c) : ld_128(a.kn + 2 * (s.b * a.kn_b + s.h * a.kn_h) + 16 * c);
-          uint32_t word, sm_pair;
-          int4_pack<T>(raw, word, sm_pair);
-          if (any) {
-            const int at_word = (isv ? int4_half_bytes(DH) : 0) + int4_word_at(DH, token, c);
-            const int at_pair = (isv ? int4_half_bytes(DH) : 0) + int4_pair_at(DH, token, c);
-            sts32(tile + at_word, word);
-            if (block) *reinterpret_cast<uint32_t*>(block + at_word) = word;
-            if ((c & 7) == 0) {
-              sts32(tile + at_pair, sm_pair);
-              if (block) *reinterpret_cast<uint32_t*>(block + at_pair) = sm_pair;
-            }
+        for (int i = 0; i < kNew; ++i) {
+          int word, pair;
+          if (new_at(i, word, pair)) {
+            sts32(tile + word, new_word[i]);
+            if (pair >= 0) sts32(tile + pair, new_pair[i]);
           }
         }
         __syncwarp();
@@ -684,87 +742,96 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
             make_uint2(ElemTraits<T>::pack2(v.x, v.y), ElemTraits<T>::pack2(v.z, v.w));
         if (a.lse && c == 0) a.lse[s.b * a.ls_b + hq * a.ls_h] = lse_of(M, L);
       } else {
-        *reinterpret_cast<float4*>(a.ws + kWsO + 4 * ((int64_t)s.slot * 2048 + r * DH + c)) = v;
+        *reinterpret_cast<float4*>(a.ws + kWsO + 4 * ((int64_t)s.slot * kPartFloats + r * DH + c)) = v;
         if (c == 0) reinterpret_cast<float2*>(a.ws + kWsMl)[s.slot * kPartRows + r] = make_float2(M, L);
       }
     }
-    __syncthreads();  // the rings are free again
+    if (cur < end) __syncthreads();  // the rings are free again
   }
-  // for the join: the cut pair that begins in this CTA, if one does
-  if (tid == 0) {
-    if (uncut) begun.parts = 0;
-    reinterpret_cast<CutPair*>(a.ws + kWsCut)[blockIdx.x] = begun;
-  }
-  // requests without keys
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (len_of(b) != 0) continue;
+  // for the join: the cut pair that begins in this CTA, if one does (else it has no parts)
+  if (!a.whole && tid == 0) reinterpret_cast<CutPair*>(a.ws + kWsCut)[blockIdx.x] = begun;
+  auto no_keys = [&](int b) {
     const int hq = a.Hkv * a.G;
     for (int i = tid; i < hq * (DH / 8); i += kThreads)
       st_128(a.out + 2 * (b * a.o_b + (int64_t)(i / (DH / 8)) * a.o_h) + 16 * (i % (DH / 8)), make_uint4(0, 0, 0, 0));
     if (a.lse)
       for (int i = tid; i < hq; i += kThreads) a.lse[b * a.ls_b + i * a.ls_h] = -INFINITY;
+  };
+  if (a.whole) {
+    if (at.nt == 0 && (int)blockIdx.x == at.b * per_b) no_keys(at.b);
+  } else {
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      if (len_of(b) == 0) no_keys(b);
   }
 }
 
-// The cut pair that begins in CTA blockIdx.x: 32 columns of its parts' outputs, weighted and summed in the order
-// of the line.
+// A head of the cut pair that begins in CTA blockIdx.x of the decode: its parts' outputs, weighted and summed in the
+// order of the line.  A warp takes every kWarps-th part; the weights of part i are in lane i % 32.
 template <typename T, int DH>
 __global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_constant__ Int4Args a) {
-  __shared__ float weight[kPartRows][kMaxCtas];
-  __shared__ float4 sums[kThreads];
+  constexpr int kPer = (kMaxCtas + 31) / 32;  // parts a lane has the weights of
+  constexpr int V = DH / 32;                  // columns of a lane
+  __shared__ float sums[kWarps][DH];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int first = blockIdx.x, c0 = 32 * blockIdx.y;
+  const int first = blockIdx.x, r = blockIdx.y;
   const CutPair p = reinterpret_cast<const CutPair*>(a.ws + kWsCut)[first];
-  if (p.parts == 0) return;
+  if (r >= p.rows || p.parts == 0) return;
   auto slot = [&](int i) { return 2 * (first + i) + (i == 0 ? 1 : 0); };
   const float2* ml = reinterpret_cast<const float2*>(a.ws + kWsMl);
-  for (int r = warp; r < p.rows; r += kWarps) {
-    float M = -INFINITY, L = 0.f;
-    for (int i = lane; i < p.parts; i += 32) M = fmaxf(M, ml[slot(i) * kPartRows + r].x);
+  float2 x[kPer];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float base = M == -INFINITY ? 0.f : M;
-    for (int i = lane; i < p.parts; i += 32) {
-      const float2 x = ml[slot(i) * kPartRows + r];
-      const float w = x.y * ex2_approx(x.x - base);
-      weight[r][i] = w;
-      L += w;
+  for (int k = 0; k < kPer; ++k) x[k] = 32 * k + lane < p.parts ? ml[slot(32 * k + lane) * kPartRows + r] : make_float2(-INFINITY, 0.f);
+  const float* o = reinterpret_cast<const float*>(a.ws + kWsO) + r * DH + V * lane;
+  float M = -INFINITY, L = 0.f, v[V];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) M = fmaxf(M, x[k].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    x[k].x = x[k].y * ex2_approx(x[k].x - base);
+    L += x[k].x;
+  }
+  L = warp_sum(L);
+#pragma unroll
+  for (int c = 0; c < V; ++c) v[c] = 0.f;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    if (32 * k >= p.parts) break;
+#pragma unroll
+    for (int j = 0; j < 32 / kWarps; ++j) {
+      const int i = 32 * k + j * kWarps + warp;
+      const float w = __shfl_sync(0xffffffffu, x[k].x, j * kWarps + warp);
+      if (i < p.parts) {
+        float u[V];
+        if constexpr (V == 2) *reinterpret_cast<float2*>(u) = *reinterpret_cast<const float2*>(o + (int64_t)slot(i) * kPartFloats);
+        else
+#pragma unroll
+          for (int c = 0; c < V; c += 4)
+            *reinterpret_cast<float4*>(u + c) = *reinterpret_cast<const float4*>(o + (int64_t)slot(i) * kPartFloats + c);
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[c] = fmaf(u[c], w, v[c]);
+      }
     }
-    L = warp_sum(L);
-    const float d = L == 0.f ? 0.f : 1.f / L;
-    __syncwarp();
-    for (int i = lane; i < p.parts; i += 32) weight[r][i] *= d;
-    if (a.lse && c0 == 0 && lane == 0) a.lse[p.b * a.ls_b + (int64_t)(p.h * a.G + p.r0 + r) * a.ls_h] = lse_of(M, L);
   }
+#pragma unroll
+  for (int c = 0; c < V; ++c) sums[warp][V * lane + c] = v[c];
   __syncthreads();
-  const int items = p.rows * 8, groups = kThreads / items, grp = tid / items, it = tid % items;
-  const int r = it >> 3, c = c0 + 4 * (it & 7);
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (grp < groups) {
-#pragma unroll 4
-    for (int i = grp; i < p.parts; i += groups) {
-      const float4 u = *reinterpret_cast<const float4*>(a.ws + kWsO + 4 * ((int64_t)slot(i) * 2048 + r * DH + c));
-      const float w = weight[r][i];
-      v.x = fmaf(u.x, w, v.x);
-      v.y = fmaf(u.y, w, v.y);
-      v.z = fmaf(u.z, w, v.z);
-      v.w = fmaf(u.w, w, v.w);
+  const float d = L == 0.f ? 0.f : 1.f / L;
+  const int64_t hq = p.h * a.G + p.r0 + r;
+  if (tid < DH / 2) {
+    float y[2] = {0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      y[0] += sums[w][2 * tid];
+      y[1] += sums[w][2 * tid + 1];
     }
+    *reinterpret_cast<uint32_t*>(a.out + 2 * (p.b * a.o_b + hq * a.o_h + 2 * tid)) = ElemTraits<T>::pack2(y[0] * d, y[1] * d);
   }
-  sums[tid] = v;
-  __syncthreads();
-  if (tid >= items) return;
-  for (int x = 1; x < groups; ++x) {
-    const float4 u = sums[x * items + tid];
-    v.x += u.x;
-    v.y += u.y;
-    v.z += u.z;
-    v.w += u.w;
-  }
-  *reinterpret_cast<uint2*>(a.out + 2 * (p.b * a.o_b + (int64_t)(p.h * a.G + p.r0 + r) * a.o_h + c)) =
-      make_uint2(ElemTraits<T>::pack2(v.x, v.y), ElemTraits<T>::pack2(v.z, v.w));
+  if (a.lse && tid == 0) a.lse[p.b * a.ls_b + hq * a.ls_h] = lse_of(M, L);
 }
 
 template <class K>
@@ -798,14 +865,17 @@ int launch(const Int4Args& a, cudaStream_t s) {
       ready.fetch_or(1ull << dev);
     }
   }
-  // No more CTAs than there could be shares; pairs of up to 2 kSlack granules are never cut.
   const int64_t keys = a.window > 0 ? std::min((int64_t)a.width * a.page_size, (int64_t)a.window + 2 * kGran) : (int64_t)a.width * a.page_size;
-  const int64_t longest = (keys + kGran - 1) / kGran;
-  const double most = (double)a.B * a.Hkv * a.chunks * (double)longest / kMinShare;
-  const int grid = (int)std::max(1.0, std::min((double)std::min(n * F::kCtas, kMaxCtas), std::ceil(most)));
-  if (int rc = launch_dependent(int4_decode_kernel<F>, a, dim3(grid), F::kBytes, s, "paged_decode_int4 launch")) return rc;
-  if (grid == 1 || longest <= 2 * kSlack) return BNA_OK;
-  return launch_dependent(int4_join_kernel<typename F::T, F::DH>, a, dim3(grid, F::DH / 32), 0, s, "paged_decode_int4 join launch");
+  const int64_t longest = (keys + kGran - 1) / kGran, pairs = (int64_t)a.B * a.Hkv * a.chunks;
+  if (pairs > INT_MAX / longest) return fail(BNA_UNSUPPORTED, "paged_decode_int4: requests x heads x tokens of a table row beyond 2^35");
+  Int4Args b = a;
+  b.whole = longest <= kWhole;
+  // No more CTAs than there could be pairs or shares.
+  const int64_t most = std::max(pairs, (pairs * longest + kMinShare - 1) / kMinShare);
+  const int grid = (int)(b.whole ? pairs : std::min<int64_t>(std::min(n * F::kCtas, kMaxCtas), most));
+  if (int rc = launch_dependent(int4_decode_kernel<F>, b, dim3(grid), F::kBytes, s, "paged_decode_int4 launch")) return rc;
+  if (b.whole || grid == 1) return BNA_OK;
+  return launch_dependent(int4_join_kernel<typename F::T, F::DH>, b, dim3(grid, a.chunk_rows), 0, s, "paged_decode_int4 join launch");
 }
 
 }  // namespace
@@ -833,6 +903,7 @@ int launch_paged_decode_int4(const bna_tensor4* q, bna_tensor4* pool, const bna_
   a.B = (int)q->size[0], a.Hkv = (int)pool->size[1], a.G = (int)(q->size[1] / pool->size[1]);
   a.width = width, a.num_pages = (int)pool->size[0], a.page_grans = (int)pool->size[2], a.page_size = a.page_grans * kGran, a.window = window;
   const int most_rows = dh == 256 ? 8 : 16;
+  a.page_shift = (a.page_grans & (a.page_grans - 1)) == 0 ? __builtin_ctz((unsigned)a.page_grans) : -1;
   a.chunks = (a.G + most_rows - 1) / most_rows;
   a.chunk_rows = (a.G + a.chunks - 1) / a.chunks;
   a.scale_log2 = scale * 1.4426950408889634f;
