@@ -137,6 +137,12 @@ __device__ __forceinline__ void st_128(void* p, uint4 v) {
   asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
 }
+// 256-bit global load (sm_100) of 32-byte aligned data that no one writes meanwhile.
+__device__ __forceinline__ void ld_nc_256(const void* p, uint32_t (&v)[8]) {
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p));
+}
 // 256-bit global store (sm_100): one 32-byte chunk per lane halves the cache-line
 // requests of row-per-lane stores compared with 16-byte stores.
 __device__ __forceinline__ void st_256(void* p, const uint32_t* v) {

@@ -22,42 +22,110 @@ __host__ __device__ constexpr int int4_block_bytes(int dh) { return 18 * dh; }
 __device__ __forceinline__ int int4_word_at(int dh, int token, int c) { return token * (dh / 2) + 4 * ((c & 7) * (dh / 64) + (c >> 3)); }
 __device__ __forceinline__ int int4_pair_at(int dh, int token, int c) { return 8 * dh + 4 * (token * (dh / 64) + (c >> 3)); }
 
-// The code word and the group's (s, m) of 8 columns in each lane; lanes 8 i .. 8 i + 7 hold a group, and all 32
-// lanes of the warp take part.  A group with a NaN or an infinity gets s = m = NaN, one whose range passes the
-// type's gets s = inf: both read as NaN.
+// Two columns in a register: the smaller and the larger of each half (NaN if either is), one half alone, and both negated.
+template <typename T> struct Pair16;
+template <> struct Pair16<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+  static constexpr float kTiny = 0x1p-100f;  // scales below this are divided by
+};
+template <> struct Pair16<__half> {
+  using V = __half2;
+  static constexpr float kTiny = 0x1p-14f;  // (subnormal: rounding one may leave codes above 15)
+};
 template <typename T>
-__device__ __forceinline__ void int4_pack(const uint4& raw, uint32_t& word, uint32_t& pair) {
-  const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  using V = typename Pair16<T>::V;
+  const V r = __hmin2_nan(*reinterpret_cast<V*>(&a), *reinterpret_cast<V*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  using V = typename Pair16<T>::V;
+  const V r = __hmax2_nan(*reinterpret_cast<V*>(&a), *reinterpret_cast<V*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// (a, b) of lower halves as the two halves
+__device__ __forceinline__ uint32_t lower2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The smallest column and minus the largest, as the two halves, of N registers of columns in each of L lanes side by
+// side (L a power of two; the lanes of the mask take part).  NaN where a column is.
+template <typename T, int N, int L>
+__device__ __forceinline__ uint32_t int4_extremes(const uint32_t (&u)[N]) {
+  uint32_t lo = u[0], hi = u[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    lo = min2<T>(lo, u[i]);
+    hi = max2<T>(hi, u[i]);
+  }
+  // (lower halves, upper halves) of both, the largest negated
+  uint32_t e = min2<T>(lower2(lo, hi ^ 0x80008000u), __byte_perm(lo, hi ^ 0x80008000u, 0x7632));
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) e = min2<T>(e, __shfl_xor_sync(0xffffffffu, e, o));
+  return e;
+}
+
+// A group's (s, m) from its extremes.  With a NaN or an infinity s = m = NaN; where the range passes the type's s = inf.
+template <typename T>
+__device__ __forceinline__ uint32_t int4_pair(uint32_t extremes) {
+  const float2 e = ElemTraits<T>::unpack2(extremes);
+  const bool good = e.x > -INFINITY && e.y > -INFINITY;  // (neither NaN nor infinite: e.x <= -e.y)
+  const float m = good ? e.x : __int_as_float(0x7fc00000);
+  return ElemTraits<T>::pack2(good ? __fdiv_rn(-e.y - m, 15.f) : m, m);
+}
+
+// The code word of 8 columns (4 registers): rint(d / s) of each difference d = x - m, ties to even, 15 at most; 0 for
+// all where s is not a positive number.
+// c = rint(d (1 / s)) can only be wrong beside a tie, and the residual e = d - c s shows it: it is exact (both
+// terms are multiples of the smaller one's last place, and no more than 24 bits of it apart), so |e| > s / 2 means
+// the next code, and |e| = s / 2 the even one.
+template <typename T>
+__device__ __forceinline__ uint32_t int4_codes(const uint32_t* u, float2 sm) {
+  const float s = sm.x, m = sm.y;
+  if (!(s > 0.f && s < INFINITY)) return 0;
+  float x[8], c[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 p = ElemTraits<T>::unpack2(u[i]);
-    x[2 * i] = p.x;
-    x[2 * i + 1] = p.y;
+    x[2 * i] = p.x - m;
+    x[2 * i + 1] = p.y - m;
   }
-  float lo = x[0], hi = x[0];
-  bool finite = true;
+  if (s < Pair16<T>::kTiny) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    finite &= fabsf(x[i]) < INFINITY;
-  }
+    for (int i = 0; i < 8; ++i) c[i] = fminf(rintf(__fdiv_rn(x[i], s)), 15.f);
+  } else {  // (the scale is off by 2^-9 of itself at most: no code passes 15)
+    const float r = rcp_approx(s), h = 0.5f * s;
+    float e[8], worst = 0.f;
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  const int lane = threadIdx.x & 31;
-  const bool good = ((__ballot_sync(0xffffffffu, finite) >> (lane & 24)) & 255u) == 255u;
-  const float m = good ? lo : __int_as_float(0x7fc00000);
-  pair = ElemTraits<T>::pack2(good ? __fdiv_rn(hi - lo, 15.f) : m, m);
-  const float s = ElemTraits<T>::unpack2(pair).x;
-  word = 0;
-  if (s > 0.f && s < INFINITY) {
+    for (int i = 0; i < 8; ++i) {
+      c[i] = fmaf(x[i], r, 0x1.8p23f) - 0x1.8p23f;  // rint
+      e[i] = fmaf(-c[i], s, x[i]);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) word |= (uint32_t)fminf(rintf(__fdiv_rn(x[i] - m, s)), 15.f) << (4 * i);
+    for (int i = 0; i < 8; i += 2) worst = fmax3(worst, fabsf(e[i]), fabsf(e[i + 1]));
+    if (worst >= h) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(e[i]) > h || (fabsf(e[i]) == h && ((int)c[i] & 1))) c[i] += copysignf(1.f, e[i]);
+    }
   }
+  const float lo = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 0x1p23f;  // the sum's last 16 bits
+  const float hi = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 0x1p23f;
+  return lower2(__float_as_uint(lo), __float_as_uint(hi));
+}
+
+// The code word and the group's (s, m) of 8 columns in each lane; lanes 8 i .. 8 i + 7 hold a group, and all 32
+// lanes of the warp take part.
+template <typename T>
+__device__ __forceinline__ void int4_pack(const uint4& raw, uint32_t& word, uint32_t& pair) {
+  const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+  pair = int4_pair<T>(int4_extremes<T, 4, 8>(u));
+  word = int4_codes<T>(u, ElemTraits<T>::unpack2(pair));
 }
 
 // Column i (0..7) of a code word, read with its group's (s, m).

@@ -275,122 +275,123 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppendArgs
 
 // ------------------------------------------------------------------------------ 4-bit rows
 struct Int4RowsArgs {
-  const uint8_t *k, *v;        // append: rows in; read: rows out
-  int64_t k_h, k_t, v_h, v_t;  // element strides: head, token
+  uint8_t* rows[2];      // keys, values: in (append) or out (read)
+  int64_t h[2], t[2];    // their element strides: head, token
   uint8_t* pool;
   int64_t p_p, p_h, p_g;  // byte strides: page, head, block
   const int64_t* slots;
-  int64_t rows;  // tokens * heads
+  int64_t count;  // tokens * heads
   int64_t num_slots;
-  int heads, page_size, dh, vec_shift;  // 2^vec_shift vectors of 8 columns per row
+  int heads, page_size;
+  int wide;  // every 16 columns of the rows are 32-byte aligned
 };
 
-// A token's row of one head: where the keys' half of its block lies, and the token's place in it (null: no slot).
-__device__ __forceinline__ uint8_t* int4_row(const Int4RowsArgs& a, int64_t slot, int head, int& token) {
-  if (slot < 0 || slot >= a.num_slots) return nullptr;
-  const int64_t page = a.num_slots <= UINT_MAX ? (int64_t)((unsigned)slot / (unsigned)a.page_size) : slot / a.page_size;
-  const int off = (int)(slot - page * a.page_size);
-  token = off % kInt4Tokens;
-  return a.pool + page * a.p_p + head * a.p_h + off / kInt4Tokens * a.p_g;
-}
-__device__ __forceinline__ int64_t token_of(const Int4RowsArgs& a, int64_t row) {
-  return a.rows <= UINT_MAX ? (int64_t)((unsigned)row / (unsigned)a.heads) : row / a.heads;
-}
-
-// A thread packs 8 columns of the keys and of the values of N rows that lie a block apart; 8 threads share a
-// group's extremes.
-template <typename T, int N>
-__global__ void __launch_bounds__(256) int4_append_kernel(const Int4RowsArgs a) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int c = threadIdx.x & ((1 << a.vec_shift) - 1);
-  const int step = 256 >> a.vec_shift;
-  const int64_t row0 = (int64_t)blockIdx.x * (N * step) + (threadIdx.x >> a.vec_shift);
-  uint4 k[N], v[N];
-  int64_t slot[N];
-  int head[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t row = row0 + i * step;
-    slot[i] = -1;
-    head[i] = 0;
-    k[i] = v[i] = make_uint4(0, 0, 0, 0);
-    if (row < a.rows) {
-      const int64_t t = token_of(a, row);
-      head[i] = (int)(row - t * a.heads);
-      slot[i] = a.slots[t];
-      k[i] = ld_nc_128(a.k + 2 * (t * a.k_t + head[i] * a.k_h) + 16 * c);
-      v[i] = ld_nc_128(a.v + 2 * (t * a.v_t + head[i] * a.v_h) + 16 * c);
-    }
+// A row is a token's of one head, and four lanes share it: lane t has columns 64 y + 16 t .. + 15 of every group y, whose code
+// words lie side by side.  blockIdx.y: keys, values.
+struct Int4Row {
+  uint8_t *row, *half;  // the 16-bit row, its half of the block (null: no slot)
+  int token;            // in the block
+};
+__device__ __forceinline__ bool int4_row(const Int4RowsArgs& a, int dh, Int4Row& r) {
+  const int64_t i = (int64_t)blockIdx.x * (blockDim.x / 4) + threadIdx.x / 4;
+  if (i >= a.count) return false;
+  const bool x = blockIdx.y;
+  const int64_t t = a.count <= UINT_MAX ? (int64_t)((unsigned)i / (unsigned)a.heads) : i / a.heads;
+  const int head = (int)(i - t * a.heads);
+  const int64_t slot = a.slots[t];
+  r.row = x ? a.rows[1] + 2 * (t * a.t[1] + head * a.h[1]) : a.rows[0] + 2 * (t * a.t[0] + head * a.h[0]);
+  if (slot >= 0 && slot < a.num_slots) {
+    const int64_t page = a.num_slots <= UINT_MAX ? (int64_t)((unsigned)slot / (unsigned)a.page_size) : slot / a.page_size;
+    const int off = (int)(slot - page * a.page_size);
+    r.token = off % kInt4Tokens;
+    r.half = a.pool + page * a.p_p + head * a.p_h + off / kInt4Tokens * a.p_g + x * int4_half_bytes(dh);
   }
+  return true;
+}
+template <int N>  // N words, 4 N bytes aligned (16 at most)
+__device__ __forceinline__ void move_words(uint32_t* dst, const uint32_t* src) {
+  if constexpr (N == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+  else
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    uint32_t kw, kp, vw, vp;
-    int4_pack<T>(k[i], kw, kp);
-    int4_pack<T>(v[i], vw, vp);
-    int token = 0;
-    uint8_t* block = int4_row(a, slot[i], head[i], token);
-    if (!block) continue;  // (whole rows: the lanes of a group stay together)
-    const int word = int4_word_at(a.dh, token, c), pair = int4_pair_at(a.dh, token, c), half = int4_half_bytes(a.dh);
-    *reinterpret_cast<uint32_t*>(block + word) = kw;
-    *reinterpret_cast<uint32_t*>(block + half + word) = vw;
-    if ((c & 7) == 0) {
-      *reinterpret_cast<uint32_t*>(block + pair) = kp;
-      *reinterpret_cast<uint32_t*>(block + half + pair) = vp;
-    }
-  }
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
 }
 
-// A thread reads 8 columns of the keys and of the values of N rows; tokens without a slot get zeros.
-template <typename T, int N>
-__global__ void __launch_bounds__(256) int4_read_kernel(const Int4RowsArgs a) {
+// GR groups of 64 columns a row
+template <typename T, int GR>
+__global__ void __launch_bounds__(256) int4_append_kernel(const __grid_constant__ Int4RowsArgs a) {
+  constexpr int DH = kInt4Group * GR;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int c = threadIdx.x & ((1 << a.vec_shift) - 1);
-  const int step = 256 >> a.vec_shift;
-  const int64_t row0 = (int64_t)blockIdx.x * (N * step) + (threadIdx.x >> a.vec_shift);
-  uint32_t word[N][2], pair[N][2];
+  const int t = threadIdx.x & 3;
+  Int4Row r{};
+  const bool any = int4_row(a, DH, r);
+  uint32_t u[GR][8];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t row = row0 + i * step;
-    word[i][0] = word[i][1] = pair[i][0] = pair[i][1] = 0;
-    if (row < a.rows) {
-      const int64_t t = token_of(a, row);
-      int token = 0;
-      const uint8_t* block = int4_row(a, a.slots[t], (int)(row - t * a.heads), token);
-      if (block) {
-        const uint8_t *w = block + int4_word_at(a.dh, token, c), *p = block + int4_pair_at(a.dh, token, c);
-        const int half = int4_half_bytes(a.dh);
-        word[i][0] = *reinterpret_cast<const uint32_t*>(w);
-        pair[i][0] = *reinterpret_cast<const uint32_t*>(p);
-        word[i][1] = *reinterpret_cast<const uint32_t*>(w + half);
-        pair[i][1] = *reinterpret_cast<const uint32_t*>(p + half);
-      }
+  for (int y = 0; y < GR; ++y) {
+    const uint8_t* src = r.row + 128 * y + 32 * t;
+    if (any && a.wide) {
+      ld_nc_256(src, u[y]);
+    } else {
+      const uint4 lo = any ? ld_nc_128(src) : make_uint4(0, 0, 0, 0), hi = any ? ld_nc_128(src + 16) : make_uint4(0, 0, 0, 0);
+      u[y][0] = lo.x, u[y][1] = lo.y, u[y][2] = lo.z, u[y][3] = lo.w;
+      u[y][4] = hi.x, u[y][5] = hi.y, u[y][6] = hi.z, u[y][7] = hi.w;
     }
   }
+  uint32_t word[2 * GR], mine = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t row = row0 + i * step;
-    if (row >= a.rows) continue;
-    const int64_t t = token_of(a, row), head = row - t * a.heads;
+  for (int y = 0; y < GR; ++y) {
+    const uint32_t pair = int4_pair<T>(int4_extremes<T, 8, 4>(u[y]));
+    const float2 sm = ElemTraits<T>::unpack2(pair);
+    word[y] = int4_codes<T>(u[y], sm);
+    word[GR + y] = int4_codes<T>(u[y] + 4, sm);
+    if (y == t) mine = pair;
+  }
+  if (!any || !r.half) return;
+  move_words<2 * GR>(reinterpret_cast<uint32_t*>(r.half + r.token * (DH / 2) + t * (8 * GR)), word);
+  if (t < GR) *reinterpret_cast<uint32_t*>(r.half + 8 * DH + 4 * (r.token * GR + t)) = mine;
+}
+
+// Rows without a slot get zeros.
+template <typename T, int GR>
+__global__ void __launch_bounds__(256) int4_read_kernel(const __grid_constant__ Int4RowsArgs a) {
+  constexpr int DH = kInt4Group * GR;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int t = threadIdx.x & 3;
+  Int4Row r{};
+  if (!int4_row(a, DH, r)) return;
+  uint32_t word[2 * GR] = {}, pair[GR] = {};
+  if (r.half) {
+    move_words<2 * GR>(word, reinterpret_cast<const uint32_t*>(r.half + r.token * (DH / 2) + t * (8 * GR)));
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(r.half + 8 * DH + 4 * r.token * GR);
+    if constexpr (GR == 1) pair[0] = *p;
+    else move_words<GR>(pair, p);
+  }
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float2 p = ElemTraits<T>::unpack2(pair[i][x]);
-      uint32_t u[4];
+  for (int y = 0; y < GR; ++y) {
+    const float2 sm = ElemTraits<T>::unpack2(pair[y]);
+    uint32_t u[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = ElemTraits<T>::pack2(int4_value(word[i][x], 2 * j, p), int4_value(word[i][x], 2 * j + 1, p));
-      uint8_t* dst = const_cast<uint8_t*>(x ? a.v + 2 * (t * a.v_t + head * a.v_h) : a.k + 2 * (t * a.k_t + head * a.k_h));
-      st_128(dst + 16 * c, make_uint4(u[0], u[1], u[2], u[3]));
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w = word[(j >> 2) * GR + y];
+      u[j] = ElemTraits<T>::pack2(int4_value(w, 2 * (j & 3), sm), int4_value(w, 2 * (j & 3) + 1, sm));
+    }
+    uint8_t* dst = r.row + 128 * y + 32 * t;
+    if (a.wide) {
+      st_256(dst, u);
+    } else {
+      st_128(dst, make_uint4(u[0], u[1], u[2], u[3]));
+      st_128(dst + 16, make_uint4(u[4], u[5], u[6], u[7]));
     }
   }
 }
 
 // Launch that may be set up while the stream's previous kernel runs (the kernel waits for it).
 template <typename Args>
-int launch_dependent(void (*kern)(Args), const std::remove_const_t<Args>& a, unsigned grid, unsigned block, int smem, cudaStream_t s,
+int launch_dependent(void (*kern)(Args), const std::remove_const_t<Args>& a, dim3 grid, unsigned block, int smem, cudaStream_t s,
                      const char* what) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -429,7 +430,7 @@ int launch_reserve(const int32_t* lens, const int32_t* add, int B, int32_t* tabl
   const int64_t given = std::min((int64_t)num_pages, (int64_t)B * width) / 2;
   const int64_t items = std::max((num_tokens + k - 1) / k, std::max(given, (int64_t)B));
   const unsigned grid = (unsigned)std::min<int64_t>(kReserveCtas, (items + threads - 1) / threads);
-  return launch_dependent(kern, a, grid, threads, smem, s, "paged_reserve launch");
+  return launch_dependent(kern, a, dim3(grid), threads, smem, s, "paged_reserve launch");
 }
 
 int launch_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* kp, bna_tensor4* vp,
@@ -445,26 +446,38 @@ int launch_paged_append(const bna_tensor4* k, const bna_tensor4* v, bna_tensor4*
   const int n = rows * vecs >= (int64_t)4 * 256 * 148 * 4 ? 4 : 1;
   const int64_t per = (int64_t)n * (256 >> vec_shift), blocks = (rows + per - 1) / per;
   if (blocks > INT_MAX) return fail(BNA_UNSUPPORTED, "paged_append: too many elements");
-  return launch_dependent(n == 4 ? paged_append_kernel<4> : paged_append_kernel<1>, a, (unsigned)blocks, 256, 0, s,
+  return launch_dependent(n == 4 ? paged_append_kernel<4> : paged_append_kernel<1>, a, dim3((unsigned)blocks), 256, 0, s,
                           "paged_append launch");
 }
 
 // Rows of k / v into (append) or out of (read) 4-bit blocks.
 int launch_int4_rows(bool append, const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* pool, const int64_t* slots, int dtype, cudaStream_t s) {
-  const int heads = (int)k->size[1], dh = (int)k->size[3], page_size = (int)pool->size[2] * kInt4Tokens;
-  const int64_t rows = k->size[2] * heads;
-  const int vecs = dh / 8, vec_shift = vecs == 8 ? 3 : vecs == 16 ? 4 : 5;
-  Int4RowsArgs a{static_cast<const uint8_t*>(k->data), static_cast<const uint8_t*>(v->data), k->stride[1], k->stride[2], v->stride[1],
-                 v->stride[2], static_cast<uint8_t*>(pool->data), pool->stride[0], pool->stride[1], pool->stride[2], slots, rows,
-                 pool->size[0] * page_size, heads, page_size, dh, vec_shift};
-  const int n = rows * vecs >= (int64_t)4 * 256 * 148 * 4 ? 4 : 1;  // as in the 16-bit append
-  const int64_t per = (int64_t)n * (256 >> vec_shift), blocks = (rows + per - 1) / per;
+  const bna_tensor4* x[2] = {k, v};
+  Int4RowsArgs a{};
+  a.pool = static_cast<uint8_t*>(pool->data);
+  a.p_p = pool->stride[0], a.p_h = pool->stride[1], a.p_g = pool->stride[2];
+  a.slots = slots;
+  a.heads = (int)k->size[1], a.page_size = (int)pool->size[2] * kInt4Tokens;
+  a.count = k->size[2] * a.heads, a.num_slots = pool->size[0] * a.page_size;
+  a.wide = 1;
+  for (int i = 0; i < 2; ++i) {
+    a.rows[i] = static_cast<uint8_t*>(x[i]->data);
+    a.h[i] = x[i]->stride[1], a.t[i] = x[i]->stride[2];
+    if (reinterpret_cast<uintptr_t>(x[i]->data) % 32 || (x[i]->size[1] > 1 && a.h[i] % 16) || (x[i]->size[2] > 1 && a.t[i] % 16)) a.wide = 0;
+  }
+  // Short calls in small CTAs on many SMs: 64 tokens of 2 heads are 512 lanes a tensor.
+  const int block = a.count <= 64 * 148 ? 64 : 256;
+  const int64_t blocks = (a.count + block / 4 - 1) / (block / 4);
   if (blocks > INT_MAX) return fail(BNA_UNSUPPORTED, "paged 4-bit rows: too many elements");
-  auto pick = [&](auto t) {
+  auto pick = [&](auto t) -> void (*)(const Int4RowsArgs) {
     using T = decltype(t);
-    return append ? (n == 4 ? int4_append_kernel<T, 4> : int4_append_kernel<T, 1>) : (n == 4 ? int4_read_kernel<T, 4> : int4_read_kernel<T, 1>);
+    switch (k->size[3]) {
+      case 64: return append ? int4_append_kernel<T, 1> : int4_read_kernel<T, 1>;
+      case 128: return append ? int4_append_kernel<T, 2> : int4_read_kernel<T, 2>;
+      default: return append ? int4_append_kernel<T, 4> : int4_read_kernel<T, 4>;
+    }
   };
-  return launch_dependent(dtype == BNA_BF16 ? pick(__nv_bfloat16()) : pick(__half()), a, (unsigned)blocks, 256, 0, s,
+  return launch_dependent(dtype == BNA_BF16 ? pick(__nv_bfloat16()) : pick(__half()), a, dim3((unsigned)blocks, 2), block, 0, s,
                           append ? "paged_append_int4 launch" : "paged_read_int4 launch");
 }
 

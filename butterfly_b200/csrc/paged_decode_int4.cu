@@ -99,19 +99,22 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-template <int N>  // N words of 32 bits
+template <int AT, int N>  // N words of 32 bits at `AT` bytes past addr
 __device__ __forceinline__ void lds(uint32_t addr, uint32_t (&r)[N]) {
-  static_assert(N == 1 || N == 2 || N % 4 == 0, "");
+  static_assert(N == 1 || N == 2 || N == 4 || N == 8, "");
   if constexpr (N == 1) {
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
+    asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(r[0]) : "r"(addr), "n"(AT) : "memory");
   } else if constexpr (N == 2) {
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr), "n"(AT) : "memory");
   } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
-                   : "r"(addr + 4 * i)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr), "n"(AT)
+                 : "memory");
+    if constexpr (N == 8)
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+                   : "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                   : "r"(addr), "n"(AT + 16)
                    : "memory");
   }
 }
@@ -174,9 +177,10 @@ struct Form {
   static_assert(kCtas * (kBytes + 1024) <= 233472, "shared memory of an SM");
 };
 
-// What a warp holds of a segment.  Scores come as S^T: lane 4 g + t has keys row(g) and row(g) + 8 and heads 2 t, 2 t + 1
-// (of every tile); matrix row g is key row(g) = g ^ (g >> 1 & 1), which spreads the rows that a read of values
-// touches over the banks.  Outputs o come as O^T: columns 64 y + 8 g .. + 7 of heads 2 t, 2 t + 1.
+// What a warp holds of a segment.  Scores come as S^T: lane 4 g + t has two keys, row(g) and row(g) + 4, and heads 2 t,
+// 2 t + 1 (of every tile).  Matrix row g is key row(g) = g / 2 + 8 (g % 2), so that lane t's keys in P V are t, t + 8 and t + 4,
+// t + 12: one address and fixed offsets, two lanes to a bank.  Outputs o come as O^T: columns 64 y + 8 g .. + 7 of
+// heads 2 t, 2 t + 1.
 template <class F>
 struct Acc {
   using T = typename F::T;
@@ -280,16 +284,15 @@ struct Acc {
   __device__ __forceinline__ void granule(uint32_t tile, int pos, bool edge, int lo, int hi, int lane) {
     constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
     const int g = lane >> 2, t = lane & 3;
-    const int row = g ^ ((g >> 1) & 1);
-    const uint32_t values = tile + int4_half_bytes(DH);
+    const int row = (g >> 1) + 8 * (g & 1);
     // scores
     float u[NT][4];
     {
       uint32_t w[2][2 * GR], p[2][GR];
-      lds(tile + row * (DH / 2) + t * (8 * GR), w[0]);
-      lds(tile + (row + 8) * (DH / 2) + t * (8 * GR), w[1]);
-      lds(tile + 8 * DH + row * (4 * GR), p[0]);
-      lds(tile + 8 * DH + (row + 8) * (4 * GR), p[1]);
+      lds<0>(tile + row * (DH / 2) + t * (8 * GR), w[0]);
+      lds<4 * (DH / 2)>(tile + row * (DH / 2) + t * (8 * GR), w[1]);
+      lds<8 * DH>(tile + row * (4 * GR), p[0]);
+      lds<8 * DH + 16 * GR>(tile + row * (4 * GR), p[1]);
 #pragma unroll
       for (int y = 0; y < GR; ++y) {
         float acc[NT][4];
@@ -321,8 +324,8 @@ struct Acc {
     float sv[2][GR], mv[2][GR];
     {
       uint32_t p[2][GR];
-      lds(values + 8 * DH + row * (4 * GR), p[0]);
-      lds(values + 8 * DH + (row + 8) * (4 * GR), p[1]);
+      lds<17 * DH>(tile + row * (4 * GR), p[0]);
+      lds<17 * DH + 16 * GR>(tile + row * (4 * GR), p[1]);
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -335,7 +338,7 @@ struct Acc {
     if (edge) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int key = pos + row + 8 * r;
+        const int key = pos + row + 4 * r;
         if (key < lo || key >= hi) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) u[n][2 * r] = u[n][2 * r + 1] = -INFINITY;
@@ -410,13 +413,13 @@ struct Acc {
         }
       }
     }
-    // outputs: keys 2 t, 2 t + 1 of the matrix rows, and 8 further
+    // outputs
     uint32_t w[4][GR];
-    const int k0 = (2 * t) ^ (t & 1), k1 = (2 * t + 1) ^ (t & 1);
-    lds(values + k0 * (DH / 2) + g * (4 * GR), w[0]);
-    lds(values + k1 * (DH / 2) + g * (4 * GR), w[1]);
-    lds(values + (k0 + 8) * (DH / 2) + g * (4 * GR), w[2]);
-    lds(values + (k1 + 8) * (DH / 2) + g * (4 * GR), w[3]);
+    const uint32_t at = tile + t * (DH / 2) + g * (4 * GR);
+    lds<9 * DH>(at, w[0]);
+    lds<9 * DH + 8 * (DH / 2)>(at, w[1]);
+    lds<9 * DH + 4 * (DH / 2)>(at, w[2]);
+    lds<9 * DH + 12 * (DH / 2)>(at, w[3]);
 #pragma unroll
     for (int y = 0; y < GR; ++y) {
 #pragma unroll
