@@ -7,7 +7,7 @@
 // reference that moves only when an entry lies more than kSlack above it, and where its largest
 // entry lies.  The k largest need no second pass over the row: of 64 groups of threads the k-th
 // largest of their largest entries is a bound that at least k entries reach, and only the few threads
-// whose own largest reaches it look at their entries again (from L2, a warp for each of them).
+// whose own largest reaches it have their entries looked at again (from L2, by all lanes of their warp).
 // A row is shared by a cluster of CTAs where there are few rows; the CTAs' sums and lists are joined
 // through distributed shared memory by the cluster's first one.
 #include <cuda_runtime.h>
@@ -30,7 +30,8 @@ constexpr int kList = 4096;   // entries that reach the bound, as long as they f
 constexpr int kMaxCluster = 8;
 constexpr float kSlack = 8.f;  // e^kSlack times the row's length stays far below the fp32 range
 constexpr float kLog2e = 1.4426950408889634f;
-// e^kFloor is 0 in fp32; differences are cut there, so that a masked entry adds 0 to W and not 0 * inf
+// Entries are cut at the type's lowest value as they are summed, so that a masked one adds 0 to W and not 0 * inf; where
+// the reference itself is about as low, differences are cut instead: e^kFloor is 0 in fp32.
 constexpr float kFloor = -120.f;
 static_assert(kMaxCluster * kTop <= kList && kThreads % kTop == 0, "");
 
@@ -62,6 +63,65 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// Two floats in a register pair, and operations on both.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 apart(Two x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// What a type's lowest value is, below which reference the differences are cut, and (16 bits) maxima of two entries in a register.
+template <typename T> struct Low;
+template <> struct Low<float> {
+  static constexpr float kLowest = -3.4028234663852886e38f, kNear = -1e38f;
+};
+template <> struct Low<__nv_bfloat16> {
+  static constexpr uint32_t kLowest = 0xff7fff7fu;
+  static constexpr float kNear = -1e38f;
+  __device__ static uint32_t top(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ static uint32_t cut(uint32_t a) {
+    uint32_t b = kLowest;
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+template <> struct Low<__half> {
+  static constexpr uint32_t kLowest = 0xfbfffbffu;
+  static constexpr float kNear = -6e4f;
+  __device__ static uint32_t top(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ static uint32_t cut(uint32_t a) {
+    uint32_t b = kLowest;
+    const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
 
 // Z and W around a reference.  ref = -inf: no entry but masked ones (Z = W = 0).
 struct Sums {
@@ -133,6 +193,7 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
   __shared__ uint64_t group[kTop], top[kTop];
   __shared__ Sums warp_sums[kWarps], cta_sums;
   __shared__ uint64_t bound;
+  __shared__ uint8_t owners[kWarps][32];
   __shared__ int count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = cluster > 1 ? (int)cluster_ctarank() : 0;
@@ -152,41 +213,79 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
     if (token >= 0 && token < a.V) picked = row.at(token);
   }
 
-  Sums s{-INFINITY, 0.f, 0.f};
+  float ref = -INFINITY;
+  Two z2 = two(0.f, 0.f), w2 = two(0.f, 0.f);  // Z and W of the entries at even and at odd places
   float best = -INFINITY;
   int best_v = first;
   auto take = [&](const uint4& raw, int v) {
-    float f[E];
-    Row<T>::unpack(raw, f);
-    float mx = f[0];
-#pragma unroll
-    for (int j = 1; j < E; ++j) mx = fmaxf(mx, f[j]);
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+    float mx;
+    if constexpr (sizeof(T) == 4) {
+      mx = fmaxf(fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1])), fmaxf(__uint_as_float(u[2]), __uint_as_float(u[3])));
+    } else {
+      const float2 m = ElemTraits<T>::unpack2(Low<T>::top(Low<T>::top(u[0], u[1]), Low<T>::top(u[2], u[3])));
+      mx = fmaxf(m.x, m.y);
+    }
     if (mx > best) {
       best = mx;
       best_v = v;
     }
-    if (mx > s.ref + kSlack) s = moved(s, mx);
-    const float base = s.ref == -INFINITY ? 0.f : s.ref;
+    if (mx > ref + kSlack) {
+      const float2 z = apart(z2), w = apart(w2);
+      const Sums x = moved({ref, z.x, w.x}, mx), y = moved({ref, z.y, w.y}, mx);
+      z2 = two(x.z, y.z);
+      w2 = two(x.w, y.w);
+      ref = mx;
+    }
+    if (ref < Low<T>::kNear) {  // (nothing but masked entries so far, by either kind of mask)
+      float f[E];
+      Row<T>::unpack(raw, f);
+      const float base = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const float d = max_nan(f[j] - base, kFloor), e = ex2_approx(d * kLog2e);
-      s.z += e;
-      s.w = fmaf(d, e, s.w);
+      for (int j = 0; j < E; j += 2) {
+        const float d0 = max_nan(f[j] - base, kFloor), d1 = max_nan(f[j + 1] - base, kFloor);
+        const Two e = two(ex2_approx(d0 * kLog2e), ex2_approx(d1 * kLog2e));
+        z2 = add2(z2, e);
+        w2 = fma2(two(d0, d1), e, w2);
+      }
+      return;
+    }
+    const Two base = two(-ref, -ref), log2e = two(kLog2e, kLog2e);
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) {
+      Two x;
+      if constexpr (sizeof(T) == 4) {
+        x = two(max_nan(__uint_as_float(u[2 * j]), Low<T>::kLowest), max_nan(__uint_as_float(u[2 * j + 1]), Low<T>::kLowest));
+      } else {
+        const float2 f = ElemTraits<T>::unpack2(Low<T>::cut(u[j]));
+        x = two(f.x, f.y);
+      }
+      const Two d = add2(x, base);
+      const float2 t = apart(mul2(d, log2e));
+      const Two e = two(ex2_approx(t.x), ex2_approx(t.y));
+      z2 = add2(z2, e);
+      w2 = fma2(d, e, w2);
     }
   };
   constexpr int U = 4;  // vectors in flight
-  for (int v = first; v < v1; v += U * kThreads) {
+  const int inside = min(v1, row.whole1);
+  int v = first;
+  if (v < row.whole0 && v < v1) {
+    take(row.load(v), v);
+    v += kThreads;
+  }
+  for (; v + (U - 1) * kThreads < inside; v += U * kThreads) {
     uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * kThreads < v1) raw[u] = row.load(v + u * kThreads);
+    for (int u = 0; u < U; ++u) raw[u] = ld_128(row.base + 16 * (int64_t)(v + u * kThreads));
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * kThreads < v1) take(raw[u], v + u * kThreads);
+    for (int u = 0; u < U; ++u) take(raw[u], v + u * kThreads);
   }
+  for (; v < v1; v += kThreads) take(row.load(v), v);
+  const float2 z = apart(z2), w = apart(w2);
 
   // sums of the CTA
-  Sums t = s;
+  Sums t{ref, z.x + z.y, w.x + w.y};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const Sums other{__shfl_xor_sync(0xffffffffu, t.ref, o), __shfl_xor_sync(0xffffffffu, t.z, o), __shfl_xor_sync(0xffffffffu, t.w, o)};
@@ -222,21 +321,24 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
     int n;
     for (;;) {
       const uint64_t b = bound;
-      unsigned todo = __ballot_sync(0xffffffffu, any && most >= b);
-      while (todo) {
-        const int owner = __ffs(todo) - 1;
-        todo &= todo - 1;
-        for (int v = v0 + warp * 32 + owner + lane * kThreads; v < v1; v += 32 * kThreads) {
-          float f[E];
-          Row<T>::unpack(row.load(v), f);
+      // the threads whose largest entry may reach it, then all their vectors, shared out over the warp's lanes
+      const bool reaches = any && most >= b;
+      const unsigned todo = __ballot_sync(0xffffffffu, reaches);
+      if (reaches) owners[warp][__popc(todo & ((1u << lane) - 1))] = (uint8_t)lane;
+      __syncwarp();
+      const int span = (v1 - v0 + kThreads - 1) / kThreads, items = __popc(todo) * span;
+      for (int it = lane; it < items; it += 32) {
+        const int who = it / span, v = v0 + warp * 32 + owners[warp][who] + (it - who * span) * kThreads;
+        if (v >= v1) continue;
+        float f[E];
+        Row<T>::unpack(row.load(v), f);
 #pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const int64_t i = v * (int64_t)E + j - row.shift;
-            const uint64_t key = key_of(f[j], (uint32_t)i);
-            if (i >= 0 && i < row.V && key >= b) {
-              const int at = atomicAdd(&count, 1);
-              if (at < kList) list[at] = key;
-            }
+        for (int j = 0; j < E; ++j) {
+          const int64_t i = v * (int64_t)E + j - row.shift;
+          const uint64_t key = key_of(f[j], (uint32_t)i);
+          if (i >= 0 && i < row.V && key >= b) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kList) list[at] = key;
           }
         }
       }
