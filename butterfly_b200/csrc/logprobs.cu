@@ -33,7 +33,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Entries are cut at the type's lowest value as they are summed, so that a masked one adds 0 to W and not 0 * inf; where
 // the reference itself is about as low, differences are cut instead: e^kFloor is 0 in fp32.
 constexpr float kFloor = -120.f;
-static_assert(kMaxCluster * kTop <= kList && kThreads % kTop == 0, "");
 
 struct LogprobArgs {
   const uint8_t* x;
@@ -133,10 +132,23 @@ __device__ __forceinline__ Sums moved(const Sums& s, float M) {
   const float d = s.ref - M, f = ex2_approx(d * kLog2e);
   return {M, s.z * f, f == 0.f ? s.w * f : (s.w + d * s.z) * f};
 }
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-  const float M = fmaxf(a.ref, b.ref);
-  const Sums x = moved(a, M), y = moved(b, M);
-  return {M, x.z + y.z, x.w + y.w};
+// All lanes' sums as one (in every lane).
+__device__ __forceinline__ Sums warp_join(const Sums& s) {
+  float M = s.ref;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const Sums x = moved(s, M);
+  return {M, warp_sum(x.z), warp_sum(x.w)};
+}
+static_assert(kMaxCluster * kTop <= kList && kThreads % kTop == 0, "");
+// The warp's keys' ranks: of the keys list[0 .. n) the number above `key`, counted by the eight lanes 8 i .. 8 i + 7 that hold
+// the same key.
+__device__ __forceinline__ int rank_in(const uint64_t* list, int n, uint64_t key, int lane) {
+  int above = 0;
+  for (int i = lane & 7; i < n; i += 8) above += list[i] > key;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+  return above;
 }
 
 template <typename T>
@@ -170,16 +182,16 @@ struct Row {
   // A vector; entries before and after the row are -inf, and are not read.
   __device__ __forceinline__ uint4 load(int v) const {
     if (v >= whole0 && v < whole1) return ld_128(base + 16 * (int64_t)v);
-    const T* row = reinterpret_cast<const T*>(base) + shift;
     uint32_t u[4];
-    T* e = reinterpret_cast<T*>(u);
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int64_t i = v * (int64_t)E + j - shift;
-      e[j] = i >= 0 && i < V ? row[i] : static_cast<T>(-INFINITY);
+    for (int j = 0; j < 4; ++j) {
+      const int64_t i = (int64_t)v * E + j * (E / 4) - shift;
+      if constexpr (sizeof(T) == 4) u[j] = __float_as_uint(entry(i));
+      else u[j] = ElemTraits<T>::pack2(entry(i), entry(i + 1));
     }
     return make_uint4(u[0], u[1], u[2], u[3]);
   }
+  __device__ __forceinline__ float entry(int64_t i) const { return i >= 0 && i < V ? at(i) : -INFINITY; }
   __device__ __forceinline__ float at(int64_t i) const {
     if constexpr (sizeof(T) == 4) return reinterpret_cast<const float*>(base)[shift + i];
     else return static_cast<float>(reinterpret_cast<const T*>(base)[shift + i]);
@@ -187,13 +199,13 @@ struct Row {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, int cluster) {
+__global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs a, int cluster) {
   constexpr int E = Row<T>::E;
   __shared__ uint64_t list[kList];
   __shared__ uint64_t group[kTop], top[kTop];
-  __shared__ Sums warp_sums[kWarps], cta_sums;
+  __shared__ float sums[3][kWarps];  // ref, Z, W of the warps, then of the CTA in column 0
   __shared__ uint64_t bound;
-  __shared__ uint8_t owners[kWarps][32];
+  __shared__ int owners[kThreads];
   __shared__ int count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = cluster > 1 ? (int)cluster_ctarank() : 0;
@@ -285,13 +297,20 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
   const float2 z = apart(z2), w = apart(w2);
 
   // sums of the CTA
-  Sums t{ref, z.x + z.y, w.x + w.y};
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums other{__shfl_xor_sync(0xffffffffu, t.ref, o), __shfl_xor_sync(0xffffffffu, t.z, o), __shfl_xor_sync(0xffffffffu, t.w, o)};
-    t = joined(t, other);
-  }
-  if (lane == 0) warp_sums[warp] = t;
+  Sums t = warp_join({ref, z.x + z.y, w.x + w.y});
+  auto keep = [&](int column) {
+    sums[0][column] = t.ref;
+    sums[1][column] = t.z;
+    sums[2][column] = t.w;
+  };
+  if (lane == 0) keep(warp);
+  auto join_warps = [&]() {  // by one warp, after a barrier
+    t = {-INFINITY, 0.f, 0.f};
+    if (lane < kWarps) t = {sums[0][lane], sums[1][lane], sums[2][lane]};
+    t = warp_join(t);
+    __syncwarp();
+    if (lane == 0) keep(0);
+  };
 
   if (a.k > 0) {
     // Keys of what a thread could hold at best (the first entry of its best vector), and of what its
@@ -309,12 +328,17 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
     }
     if (tid < kTop) top[tid] = 0;
     __syncthreads();
-    if (tid < kTop && group[tid] != 0) {
+    constexpr int kShare = kThreads / kTop;  // threads that count the groups above one
+    {
+      const uint64_t mine = group[tid / kShare];
       int above = 0;
-#pragma unroll 8
-      for (int i = 0; i < kTop; ++i) above += group[i] > group[tid];
-      if (above == a.k - 1) bound = group[tid];
+#pragma unroll
+      for (int i = 0; i < kTop / kShare; ++i) above += group[i * kShare + tid % kShare] > mine;
+#pragma unroll
+      for (int o = 1; o < kShare; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+      if (tid % kShare == 0 && mine != 0 && above == a.k - 1) bound = mine;
     }
+    if (warp == kWarps - 1) join_warps();
     __syncthreads();
     // Entries that reach the bound.  If they do not fit, the k-th largest of those that did is a higher
     // bound; each round leaves at least kList - k of them out, so the rounds end.
@@ -324,11 +348,11 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
       // the threads whose largest entry may reach it, then all their vectors, shared out over the warp's lanes
       const bool reaches = any && most >= b;
       const unsigned todo = __ballot_sync(0xffffffffu, reaches);
-      if (reaches) owners[warp][__popc(todo & ((1u << lane) - 1))] = (uint8_t)lane;
+      if (reaches) owners[32 * warp + __popc(todo & ((1u << lane) - 1))] = tid;
       __syncwarp();
       const int span = (v1 - v0 + kThreads - 1) / kThreads, items = __popc(todo) * span;
       for (int it = lane; it < items; it += 32) {
-        const int who = it / span, v = v0 + warp * 32 + owners[warp][who] + (it - who * span) * kThreads;
+        const int who = it / span, v = v0 + owners[32 * warp + who] + (it - who * span) * kThreads;
         if (v >= v1) continue;
         float f[E];
         Row<T>::unpack(row.load(v), f);
@@ -345,10 +369,11 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
       __syncthreads();
       n = min(count, kList);
       const bool fits = count <= kList;
-      for (int c = tid; c < n; c += kThreads) {
-        int above = 0;
-        for (int i = 0; i < n; ++i) above += list[i] > list[c];
-        if (above < a.k) top[above] = list[c];
+      for (int c0 = 0; c0 < n; c0 += kThreads / 8) {
+        const int c = c0 + tid / 8;
+        const uint64_t key = c < n ? list[c] : 0;
+        const int above = rank_in(list, n, key, lane);
+        if (c < n && (lane & 7) == 0 && above < a.k) top[above] = key;
       }
       __syncthreads();
       if (fits) break;
@@ -360,24 +385,16 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
     }
   } else {
     __syncthreads();
-  }
-  if (warp == 0) {
-    t = lane < kWarps ? warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Sums other{__shfl_xor_sync(0xffffffffu, t.ref, o), __shfl_xor_sync(0xffffffffu, t.z, o), __shfl_xor_sync(0xffffffffu, t.w, o)};
-      t = joined(t, other);
-    }
-    if (lane == 0) cta_sums = t;
+    if (warp == kWarps - 1) join_warps();
   }
   if (cluster == 1) {
     __syncthreads();
   } else {
     cluster_sync_all();  // (every thread of every CTA comes here)
     if (part == 0) {
-      auto remote32 = [](const void* p, int rank) {
-        uint32_t v;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+      auto remote32 = [](const float* p, int rank) {
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
         return v;
       };
       for (int i = tid; i < cluster * a.k; i += kThreads) {
@@ -386,31 +403,24 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
         asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(src), i / a.k)) : "memory");
         list[i] = v;
       }
-      Sums all = cta_sums;
-      if (warp == 0) {
-        const Sums mine = lane < cluster ? Sums{__uint_as_float(remote32(&cta_sums.ref, lane)), __uint_as_float(remote32(&cta_sums.z, lane)),
-                                                __uint_as_float(remote32(&cta_sums.w, lane))}
-                                         : Sums{-INFINITY, 0.f, 0.f};
-        all = mine;
-#pragma unroll
-        for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
-          const Sums other{__shfl_xor_sync(0xffffffffu, all.ref, o), __shfl_xor_sync(0xffffffffu, all.z, o),
-                           __shfl_xor_sync(0xffffffffu, all.w, o)};
-          all = joined(all, other);
-        }
+      if (warp == kWarps - 1) {
+        t = {-INFINITY, 0.f, 0.f};
+        if (lane < cluster) t = {remote32(&sums[0][0], lane), remote32(&sums[1][0], lane), remote32(&sums[2][0], lane)};
+        t = warp_join(t);
       }
       __syncthreads();  // (the lists have been read before `top` is written again)
-      if (tid == 0) cta_sums = all;
-      for (int c = tid; c < cluster * a.k; c += kThreads) {
-        int above = 0;
-        for (int i = 0; i < cluster * a.k; ++i) above += list[i] > list[c];
-        if (above < a.k && list[c] != 0) top[above] = list[c];
+      if (tid == kThreads - 1) keep(0);
+      for (int c0 = 0; c0 < cluster * a.k; c0 += kThreads / 8) {
+        const int c = c0 + tid / 8;
+        const uint64_t key = c < cluster * a.k ? list[c] : 0;
+        const int above = rank_in(list, cluster * a.k, key, lane);
+        if (key != 0 && (lane & 7) == 0 && above < a.k) top[above] = key;
       }
       __syncthreads();
     }
   }
   if (part == 0) {
-    const Sums all = cta_sums;
+    const Sums all{sums[0][0], sums[1][0], sums[2][0]};
     // a row of masked entries only: no distribution; log probabilities -inf, entropy 0
     const bool none = all.z == 0.f;
     const float base = none ? 0.f : all.ref, log_z = none ? 0.f : logf(all.z);
@@ -431,6 +441,7 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a, 
 template <typename T>
 int launch(const LogprobArgs& a, int64_t rows, cudaStream_t s) {
   const int64_t vectors = ((int64_t)a.V + Row<T>::E - 1) / Row<T>::E;
+  // A row to several CTAs as long as these do not outnumber two on every SM, and have two vectors a thread.
   int cluster = 1;
   while (cluster < kMaxCluster && rows * cluster * 2 <= 2 * 148 && vectors >= (int64_t)2 * cluster * kThreads) cluster *= 2;
   if (rows * cluster > INT_MAX) return fail(BNA_UNSUPPORTED, "token_logprobs: too many rows");

@@ -77,6 +77,13 @@ def test_sizes(V, dtype):
         check(x, _tokens(x), min(V, 20))
 
 
+@pytest.mark.parametrize("rows,V", [(149, 5000), (900, 1000), (3000, 77), (1200, 20011)])
+def test_many_rows(rows, V):
+    for dtype in TYPES:
+        x = _rand(rows, V, dtype=dtype, seed=rows)
+        check(x, _tokens(x), 20)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_row_starts_and_strides(dtype):
     for pad in range(9):
