@@ -6,8 +6,9 @@
 // Each logit is read once from HBM and the rest is held in registers: a thread keeps (ref, Z, W) with a
 // reference that moves only when an entry lies more than kSlack above it, and where its largest
 // entry lies.  The k largest need no second pass over the row: of 64 groups of threads the k-th
-// largest of their largest entries is a bound that at least k entries reach, and only the few threads
-// whose own largest reaches it have their entries looked at again (from L2, by all lanes of their warp).
+// largest of their largest entries is a bound that at least k entries reach.  A thread keeps in mind which vector
+// holds its largest entry and reads that one again (from L2), and the few threads whose second-best vector reaches
+// the bound too have all their entries looked at, by all lanes of their warp.
 // A row is shared by a cluster of CTAs where there are few rows; the CTAs' sums and lists are joined
 // through distributed shared memory by the cluster's first one.
 #include <cuda_runtime.h>
@@ -37,8 +38,7 @@ constexpr float kFloor = -120.f;
 struct LogprobArgs {
   const uint8_t* x;
   int64_t ld, ld_outer;  // elements between rows, and between runs of `inner` rows
-  int64_t inner;
-  int V;
+  int inner, V;
   const void* tokens;  // or null
   int tokens64;
   float *logprob, *entropy;
@@ -209,25 +209,23 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
   __shared__ int count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = cluster > 1 ? (int)cluster_ctarank() : 0;
-  const int64_t r = blockIdx.x / cluster;
+  const int r = (int)blockIdx.x / cluster;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t outer = r / a.inner;
+  const int outer = r / a.inner;
   const Row<T> row(a.x + (outer * a.ld_outer + (r - outer * a.inner) * a.ld) * (int64_t)sizeof(T), a.V);
   const int nv = row.vectors(), per = (nv + cluster - 1) / cluster;
   const int v0 = part * per, v1 = min(v0 + per, nv), first = v0 + tid;
 
-  // the given token's logit, asked for first
+  // the given token, asked for before the row's entries, and its logit after them
   int64_t token = -1;
-  float picked = -INFINITY;
-  if (part == 0 && tid == 0 && a.tokens) {
+  if (part == 0 && tid == 0 && a.tokens)
     token = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[r] : static_cast<const int32_t*>(a.tokens)[r];
-    if (token >= 0 && token < a.V) picked = row.at(token);
-  }
 
   float ref = -INFINITY;
   Two z2 = two(0.f, 0.f), w2 = two(0.f, 0.f);  // Z and W of the entries at even and at odd places
-  float best = -INFINITY;
+  // the largest entry, its vector, and the largest of the other vectors
+  float best = -INFINITY, second = -INFINITY;
   int best_v = first;
   auto take = [&](const uint4& raw, int v) {
     const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -238,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
       const float2 m = ElemTraits<T>::unpack2(Low<T>::top(Low<T>::top(u[0], u[1]), Low<T>::top(u[2], u[3])));
       mx = fmaxf(m.x, m.y);
     }
+    second = fmaxf(second, fminf(mx, best));
     if (mx > best) {
       best = mx;
       best_v = v;
@@ -295,6 +294,8 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
   }
   for (; v < v1; v += kThreads) take(row.load(v), v);
   const float2 z = apart(z2), w = apart(w2);
+  float picked = -INFINITY;
+  if (token >= 0 && token < a.V) picked = row.at(token);
 
   // sums of the CTA
   Sums t = warp_join({ref, z.x + z.y, w.x + w.y});
@@ -345,17 +346,9 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
     int n;
     for (;;) {
       const uint64_t b = bound;
-      // the threads whose largest entry may reach it, then all their vectors, shared out over the warp's lanes
-      const bool reaches = any && most >= b;
-      const unsigned todo = __ballot_sync(0xffffffffu, reaches);
-      if (reaches) owners[32 * warp + __popc(todo & ((1u << lane) - 1))] = tid;
-      __syncwarp();
-      const int span = (v1 - v0 + kThreads - 1) / kThreads, items = __popc(todo) * span;
-      for (int it = lane; it < items; it += 32) {
-        const int who = it / span, v = v0 + owners[32 * warp + who] + (it - who * span) * kThreads;
-        if (v >= v1) continue;
+      auto look = [&](const uint4& raw, int v) {
         float f[E];
-        Row<T>::unpack(row.load(v), f);
+        Row<T>::unpack(raw, f);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           const int64_t i = v * (int64_t)E + j - row.shift;
@@ -365,6 +358,25 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
             if (at < kList) list[at] = key;
           }
         }
+      };
+      // the vectors with the threads' largest entries (but where there was no entry above -inf) ...
+      const bool kept = best > -INFINITY;
+      if (any && kept && most >= b) look(row.load(best_v), best_v);
+      // ... and of threads that hold more, all vectors are read again, shared out over the warp's lanes
+      const bool more = any && key_of(kept ? second : best, 0) >= b;
+      const unsigned todo = __ballot_sync(0xffffffffu, more);
+      if (more) owners[32 * warp + __popc(todo & ((1u << lane) - 1))] = tid;
+      if (todo) {
+        const int skip = kept ? best_v : -1;
+        __syncwarp();
+        const int span = (v1 - v0 + kThreads - 1) / kThreads, items = __popc(todo) * span;
+        for (int it0 = 0; it0 < items; it0 += 32) {
+          const int it = it0 + lane, who = min(it, items - 1) / span, owner = owners[32 * warp + who];
+          const int v = v0 + owner + (it - who * span) * kThreads;
+          const int done = __shfl_sync(0xffffffffu, skip, owner & 31);  // the vector looked at already
+          if (it < items && v < v1 && v != done) look(row.load(v), v);
+        }
+        __syncwarp();
       }
       __syncthreads();
       n = min(count, kList);
@@ -464,7 +476,7 @@ int launch(const LogprobArgs& a, int64_t rows, cudaStream_t s) {
 
 int launch_token_logprobs(const void* x, int64_t ld, int64_t ld_outer, int64_t rows, int64_t inner, int V, int dtype, const void* tokens,
                           int tokens64, float* logprob, float* entropy, int64_t* top_ids, float* top_lp, int k, cudaStream_t s) {
-  const LogprobArgs a{static_cast<const uint8_t*>(x), ld, ld_outer, inner, V, tokens, tokens64, logprob, entropy, top_ids, top_lp, k};
+  const LogprobArgs a{static_cast<const uint8_t*>(x), ld, ld_outer, (int)std::min(inner, std::min(rows, (int64_t)INT_MAX)), V, tokens, tokens64, logprob, entropy, top_ids, top_lp, k};
   if (dtype == BNA_F32) return launch<float>(a, rows, s);
   return dtype == BNA_BF16 ? launch<__nv_bfloat16>(a, rows, s) : launch<__half>(a, rows, s);
 }
