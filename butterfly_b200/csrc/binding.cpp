@@ -79,12 +79,12 @@ at::Tensor empty(const at::Tensor& like, at::IntArrayRef size, at::ScalarType ty
   return at::empty(size, like.options().dtype(type));
 }
 
-// n elements of `type` at byte `offset` of a byte buffer, sharing its storage (a fraction of the
+// A contiguous tensor of `type` at byte `offset` of a byte buffer, sharing its storage (a fraction of the
 // time of an allocation).
-at::Tensor part(const at::Tensor& bytes, int64_t offset, int64_t n, at::ScalarType type) {
+at::Tensor part(const at::Tensor& bytes, int64_t offset, at::IntArrayRef size, at::ScalarType type) {
   auto impl = c10::make_intrusive<at::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(),
                                                   caffe2::TypeMeta::fromScalarType(type));
-  impl->set_sizes_contiguous({n});
+  impl->set_sizes_contiguous(size);
   impl->set_storage_offset(bytes.storage_offset() + offset / (int64_t)c10::elementSize(type));
   return at::Tensor(std::move(impl));
 }
@@ -143,8 +143,8 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // one allocation for what lives on as the cache's state, one for the step's tokens
   const int64_t round = (tokens + 1) / 2 * 16;  // slots, to a multiple of 16 bytes
   const at::Tensor state = empty(lens, {4 * B + 4 + B}, at::kByte), step = empty(lens, {round + 4 * tokens}, at::kByte);
-  at::Tensor out = part(state, 0, B, at::kInt), left = part(state, 4 * B, 1, at::kInt), granted = part(state, 4 * B + 4, B, at::kBool),
-             slots = part(step, 0, tokens, at::kLong), positions = part(step, round, tokens, at::kInt);
+  at::Tensor out = part(state, 0, {B}, at::kInt), left = part(state, 4 * B, {1}, at::kInt), granted = part(state, 4 * B + 4, {B}, at::kBool),
+             slots = part(step, 0, {tokens}, at::kLong), positions = part(step, round, {tokens}, at::kInt);
   if (B == 0) left.copy_(num_free);  // (no request: the call writes nothing)
   const int st = g_reserve(static_cast<const int32_t*>(lens.data_ptr()), static_cast<const int32_t*>(add.data_ptr()), (int32_t)B,
                            static_cast<int32_t*>(table.data_ptr()), B > 1 ? table.stride(0) : width, (int32_t)width,
@@ -154,7 +154,7 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
                            static_cast<uint8_t*>(granted.data_ptr()), static_cast<int64_t*>(slots.data_ptr()),
                            static_cast<int32_t*>(positions.data_ptr()), tokens, address(a[7]));
   if (st != BNA_OK) return PyLong_FromLong(st);
-  if (keep) keep->copy_(part(state, 0, B + 1, at::kInt));
+  if (keep) keep->copy_(part(state, 0, {B + 1}, at::kInt));
   return tuple_of({out, left, slots, positions, granted});
   END_HANDLE_TH_ERRORS
 }
@@ -234,8 +234,14 @@ void decode_call(DecodeCall& c, const at::Tensor& q, const at::Tensor& table, co
   const int want_lse = PyObject_IsTrue(lse);
   if (want_lse < 0) throw python_error();
   c.code = dtype_code(q);
-  c.out = empty(q, {B, Hq, Tq, dh}, dt);
-  if (want_lse) c.lse = empty(q, {B, Hq, Tq}, at::kFloat);
+  if (want_lse) {  // one allocation: outputs (16-bit rows of dh, a multiple of 64), then sums
+    const int64_t rows = B * Hq * Tq;
+    const at::Tensor both = empty(q, {rows * (2 * dh + 4)}, at::kByte);
+    c.out = part(both, 0, {B, Hq, Tq, dh}, dt);
+    c.lse = part(both, 2 * rows * dh, {B, Hq, Tq}, at::kFloat);
+  } else {
+    c.out = empty(q, {B, Hq, Tq, dh}, dt);
+  }
   c.out4 = view4(c.out, "out");
 }
 PyObject* decode_result(int st, const DecodeCall& c) {
@@ -301,7 +307,9 @@ PyObject* read_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   need_slots(slots, tokens);
   const int f16 = PyObject_IsTrue(a[2]);
   if (f16 < 0) throw python_error();
-  const at::Tensor k = empty(pool, {tokens, heads, dh}, f16 ? at::kHalf : at::kBFloat16), v = at::empty_like(k);
+  const auto type = f16 ? at::kHalf : at::kBFloat16;
+  const at::Tensor both = empty(pool, {4 * tokens * heads * dh}, at::kByte);
+  const at::Tensor k = part(both, 0, {tokens, heads, dh}, type), v = part(both, 2 * tokens * heads * dh, {tokens, heads, dh}, type);
   bna_tensor4 rows[2] = {rows4(k), rows4(v)};
   const int st = g_read_int4(&p, static_cast<const int64_t*>(slots.data_ptr()), &rows[0], &rows[1], f16 ? BNA_F16 : BNA_BF16, address(a[3]));
   if (st != BNA_OK) return PyLong_FromLong(st);
@@ -376,9 +384,11 @@ PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // one allocation: ids, then log probabilities of the top, entropies, log probabilities of the tokens
   const int64_t top = rows * k;
   const at::Tensor all = empty(x, {12 * top + 8 * rows}, at::kByte);
-  at::Tensor ids = part(all, 0, top, at::kLong), top_lp = part(all, 8 * top, top, at::kFloat),
-             entropy = part(all, 12 * top, rows, at::kFloat), lp;
-  if (tokens.defined()) lp = part(all, 12 * top + 4 * rows, rows, at::kFloat);
+  c10::SmallVector<int64_t, 6> topped(lead.begin(), lead.end());
+  topped.push_back(k);
+  at::Tensor ids = part(all, 0, topped, at::kLong), top_lp = part(all, 8 * top, topped, at::kFloat),
+             entropy = part(all, 12 * top, lead, at::kFloat), lp;
+  if (tokens.defined()) lp = part(all, 12 * top + 4 * rows, lead, at::kFloat);
   const int st = g_logprobs(x.data_ptr(), stride, outer_stride, rows, inner, V,
                             type == at::kFloat ? BNA_F32 : type == at::kHalf ? BNA_F16 : BNA_BF16,
                             tokens.defined() && rows ? tokens.data_ptr() : nullptr, tokens.defined() && tokens.scalar_type() == at::kLong,
@@ -386,14 +396,6 @@ PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
                             static_cast<float*>(entropy.data_ptr()), static_cast<int64_t*>(ids.data_ptr()),
                             static_cast<float*>(top_lp.data_ptr()), (int32_t)k, address(a[3]));
   if (st != BNA_OK) return PyLong_FromLong(st);
-  c10::SmallVector<int64_t, 6> shape(lead.begin(), lead.end());
-  if (dims != 2) {
-    entropy.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
-    if (lp.defined()) lp.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
-  }
-  shape.push_back(k);
-  ids.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
-  top_lp.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
   return tuple_of({lp, entropy, ids, top_lp});
   END_HANDLE_TH_ERRORS
 }

@@ -544,23 +544,23 @@ static int check_int4_pool(const bna_tensor4* t, int64_t dh) {
 
 static int int4_rows(bool append, const bna_tensor4* k, const bna_tensor4* v, bna_tensor4* pool, const int64_t* slot_map, int32_t dtype,
                      void* stream) {
-  const std::string name = append ? "paged_append_int4" : "paged_read_int4";
+  auto refuse = [&](int status, const char* why) { return fail(status, std::string(append ? "paged_append_int4: " : "paged_read_int4: ") + why); };
   if (int rc = check_dtype(dtype)) return rc;
-  if (!k || !v || !pool) return fail(BNA_BAD_SHAPE, name + ": null tensor");
+  if (!k || !v || !pool) return refuse(BNA_BAD_SHAPE, "null tensor");
   for (int d = 0; d < 4; ++d)
     if (k->size[d] != v->size[d] || (d == 0 && k->size[d] != 1))
-      return fail(BNA_BAD_SHAPE, name + ": k and v must be [1, Hkv, tokens, dh] of one shape");
+      return refuse(BNA_BAD_SHAPE, "k and v must be [1, Hkv, tokens, dh] of one shape");
   const int64_t dh = k->size[3];
   if (int rc = check_int4_pool(pool, dh)) return rc;
-  if (k->size[1] != pool->size[1]) return fail(BNA_BAD_SHAPE, name + ": head counts of the rows and the pool differ");
+  if (k->size[1] != pool->size[1]) return refuse(BNA_BAD_SHAPE, "head counts of the rows and the pool differ");
   if (k->size[2] == 0) return BNA_OK;
   if (int rc = check_rows(k, "k", dh)) return rc;
   if (int rc = check_rows(v, "v", dh)) return rc;
   for (const bna_tensor4* t : {k, v})
     for (int d = 1; d < 3; ++d)
-      if (!append && t->size[d] > 1 && t->stride[d] < dh) return fail(BNA_BAD_STRIDE, name + ": rows of k and v must not overlap");
-  if (!slot_map) return fail(BNA_BAD_SHAPE, name + ": null slot_map");
-  if (reinterpret_cast<uintptr_t>(slot_map) & 7) return fail(BNA_BAD_STRIDE, name + ": slot_map must be 8-byte aligned");
+      if (!append && t->size[d] > 1 && t->stride[d] < dh) return refuse(BNA_BAD_STRIDE, "rows of k and v must not overlap");
+  if (!slot_map) return refuse(BNA_BAD_SHAPE, "null slot_map");
+  if (reinterpret_cast<uintptr_t>(slot_map) & 7) return refuse(BNA_BAD_STRIDE, "slot_map must be 8-byte aligned");
   return launch_int4_rows(append, k, v, pool, slot_map, dtype, (cudaStream_t)stream);
 }
 

@@ -155,18 +155,22 @@ struct Seg {
   int b, h, r0, rows, g0, n, lo, hi, slot;  // slot of the part (-1: the whole pair)
 };
 
-template <typename T_, int DH_, bool WIDE_>
+// ROWS: query heads served together at most: 4 (fp16 alone), 8 or 16
+template <typename T_, int DH_, int ROWS>
 struct Form {
   using T = T_;
   static constexpr int DH = DH_;
-  static constexpr bool WIDE = WIDE_;
-  static constexpr int kTiles = WIDE ? 2 : 1;  // of 8 query heads
+  static constexpr int kTiles = ROWS > 8 ? 2 : 1;  // of 8 columns
   static constexpr int kHeads = 8 * kTiles;
+  // For fp16 results a probability times the scale is held as two fp16 parts: one would add as much error to the output
+  // as its final rounding does (for bf16 ones an eighth of it).  With up to 4 heads the low parts ride in
+  // columns 4-7, with more they take products of their own.
+  static constexpr bool kTwoParts = std::is_same<T, __half>::value && ROWS > 4, kLowColumns = std::is_same<T, __half>::value && ROWS <= 4;
   // two CTAs an SM where their registers fit, so that the end of one's pair overlaps the other's reads
-  static constexpr int kCtas = WIDE || DH == 256 ? 1 : 2;
+  static constexpr int kCtas = ROWS > 8 || DH == 256 ? 1 : 2;
   static constexpr int GR = DH / kInt4Group;
   static constexpr int kBlock = int4_block_bytes(DH);
-  static constexpr int kStages = DH == 256 ? 5 : WIDE ? 8 : 4;  // granules of a warp's ring
+  static constexpr int kStages = DH == 256 ? 5 : ROWS > 8 ? 8 : 4;  // granules of a warp's ring
   static constexpr int kRing = kStages * kBlock;
   static constexpr int kPitch = DH + 4;  // floats of a row, as the warps join
   static_assert(kHeads * kPitch * 4 <= kRing, "a warp's outputs take its ring's place");
@@ -185,7 +189,6 @@ template <class F>
 struct Acc {
   using T = typename F::T;
   static constexpr int GR = F::GR, NT = F::kTiles, DH = F::DH;
-  static constexpr bool kTwoParts = std::is_same<T, __half>::value;
   uint32_t qb[NT][GR][2][2][2];  // Q^T fragments: tile, group, word of the lane, step, register
   float qs[NT][GR][2];           // sum(q_y), scaled as the products with codes are
   float f[NT][2];                // from those to scores in the exp2 domain
@@ -198,7 +201,7 @@ struct Acc {
   struct Queries {
     uint4 raw[NT][GR][2];
     __device__ __forceinline__ void load(const uint8_t* q, int64_t q_h, int rows, int lane) {
-      const int g = lane >> 2, t = lane & 3;
+      const int g = F::kLowColumns ? (lane >> 2) & 3 : lane >> 2, t = lane & 3;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -404,12 +407,14 @@ struct Acc {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float s = sv[r][y] * (r == 0 ? inv : -inv), w0 = e[n][2 * r] * s, w1 = e[n][2 * r + 1] * s;
-          const uint32_t hi16 = ElemTraits<__half>::pack2(w0, w1);
-          pb[n][y][r] = transposed(hi16);
-          if (kTwoParts) {
-            const float2 h = ElemTraits<__half>::unpack2(hi16);
-            pl[n][y][r] = transposed(ElemTraits<__half>::pack2(w0 - h.x, w1 - h.y));
+          uint32_t part = ElemTraits<__half>::pack2(w0, w1), low = 0;
+          if (F::kTwoParts || F::kLowColumns) {
+            const float2 h = ElemTraits<__half>::unpack2(part);
+            low = ElemTraits<__half>::pack2(w0 - h.x, w1 - h.y);
           }
+          if (F::kLowColumns && t >= 2) part = low;
+          pb[n][y][r] = transposed(part);
+          if (F::kTwoParts) pl[n][y][r] = transposed(low);
         }
       }
     }
@@ -431,7 +436,7 @@ struct Acc {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma_16816<__half>(o[n][y][2 * half + i], a, pb[n][y][0], pb[n][y][1]);
-            if (kTwoParts) mma_16816<__half>(o[n][y][2 * half + i], a, pl[n][y][0], pl[n][y][1]);
+            if (F::kTwoParts) mma_16816<__half>(o[n][y][2 * half + i], a, pl[n][y][0], pl[n][y][1]);
           }
           x0 >>= 8;
           x1 >>= 8;
@@ -453,6 +458,10 @@ struct Acc {
           const float m = lane_sum(wm[n][y][x]) * d;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
+            if (F::kLowColumns) {
+              o[n][y][i][x] += __shfl_xor_sync(0xffffffffu, o[n][y][i][x], 2);
+              o[n][y][i][2 + x] += __shfl_xor_sync(0xffffffffu, o[n][y][i][2 + x], 2);
+            }
             o[n][y][i][x] = fmaf(o[n][y][i][x] * (d * 0x1p24f), bound, m);
             o[n][y][i][2 + x] = fmaf(o[n][y][i][2 + x] * (d * 0x1p20f), bound, m);
           }
@@ -539,14 +548,10 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
     line.C = min((int)gridDim.x, max(1, max(pairs, (line.U + kMinShare - 1) / kMinShare)));
     line.q = line.U / line.C;
     line.r = line.U - line.q * line.C;
-    auto locate = [&](int x) {
-      int lo = 0, hi = kThreads - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (line.runs[mid] > x) hi = mid;
-        else lo = mid + 1;
-      }
-      At r{lo * line.per, 0, lo > 0 ? line.runs[lo - 1] : 0};
+    auto locate = [&](int x) {  // of a place before U: the warp whose runs reach past it, the run, the request
+      const int w = __popc(__ballot_sync(0xffffffffu, lane < kWarps && line.runs[32 * (lane & (kWarps - 1)) + 31] <= x));
+      const int i = 32 * w + __popc(__ballot_sync(0xffffffffu, line.runs[32 * w + lane] <= x));
+      At r{i * line.per, 0, i > 0 ? line.runs[i - 1] : 0};
       for (;; ++r.b) {
         r.nt = granules_of(a, r.b < a.B ? len_of(r.b) : 0);
         if (r.b >= a.B - 1 || r.begin + r.nt * per_b > x) return r;
@@ -911,16 +916,22 @@ int launch_paged_decode_int4(const bna_tensor4* q, bna_tensor4* pool, const bna_
   a.chunk_rows = (a.G + a.chunks - 1) / a.chunks;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.ws = static_cast<uint8_t*>(ws);
-  const bool bf = dtype == BNA_BF16, wide = a.chunk_rows > 8;
+  const int rows = a.chunk_rows;
+  auto pick = [&](auto form) {
+    constexpr int DH = decltype(form)::DH;
+    if (dtype == BNA_BF16) {
+      if constexpr (DH < 256)
+        if (rows > 8) return launch<Form<__nv_bfloat16, DH, 16>>(a, s);
+      return launch<Form<__nv_bfloat16, DH, 8>>(a, s);
+    }
+    if constexpr (DH < 256)
+      if (rows > 8) return launch<Form<__half, DH, 16>>(a, s);
+    return rows > 4 ? launch<Form<__half, DH, 8>>(a, s) : launch<Form<__half, DH, 4>>(a, s);
+  };
   switch (dh) {
-    case 64:
-      if (bf) return wide ? launch<Form<__nv_bfloat16, 64, true>>(a, s) : launch<Form<__nv_bfloat16, 64, false>>(a, s);
-      return wide ? launch<Form<__half, 64, true>>(a, s) : launch<Form<__half, 64, false>>(a, s);
-    case 128:
-      if (bf) return wide ? launch<Form<__nv_bfloat16, 128, true>>(a, s) : launch<Form<__nv_bfloat16, 128, false>>(a, s);
-      return wide ? launch<Form<__half, 128, true>>(a, s) : launch<Form<__half, 128, false>>(a, s);
-    case 256:
-      return bf ? launch<Form<__nv_bfloat16, 256, false>>(a, s) : launch<Form<__half, 256, false>>(a, s);
+    case 64: return pick(Form<__half, 64, 8>());
+    case 128: return pick(Form<__half, 128, 8>());
+    case 256: return pick(Form<__half, 256, 8>());
     default: return fail(BNA_UNSUPPORTED, "paged_decode_attention_int4: head_dim must be 64, 128 or 256");
   }
 }
