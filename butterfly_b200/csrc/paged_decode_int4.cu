@@ -75,7 +75,7 @@ struct Int4Args {
 // CTA, (m, l) of every part, their outputs.  CTA c has the slots 2 c and 2 c + 1: the pair that ends in it, and the one that begins.
 constexpr int kPartRows = 16;
 struct CutPair {
-  int b, h, r0, rows, parts, pad[3];
+  int b, h, r0, rows_parts;  // rows and, from bit 8 on, parts (0: no cut pair begins in the CTA)
 };
 constexpr int64_t kWsCut = 4096;
 constexpr int64_t kWsMl = kWsCut + kMaxCtas * (int64_t)sizeof(CutPair);
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
       // A cut pair begins here: its parts are those of the CTAs up to the one that holds its end.  Cuts within it kept their
       // places (those near its end have moved there): the last of them lies at or before this place.
       const int last = min(max((int)blockIdx.x + 1, line.cta_of(cur + at.nt - kSlack - 1)), line.C - 1);
-      begun = CutPair{s.b, s.h, s.r0, s.rows, last - (int)blockIdx.x + 1, {0, 0, 0}};
+      begun = CutPair{s.b, s.h, s.r0, s.rows | (last - (int)blockIdx.x + 1) << 8};
     }
     cur += s.n;
 
@@ -773,26 +773,72 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
   }
 }
 
-// A head of the cut pair that begins in CTA blockIdx.x of the decode: its parts' outputs, weighted and summed in the
-// order of the line.  A warp takes every kWarps-th part; the weights of part i are in lane i % 32.
+// Head blockIdx.y of the blockIdx.x-th cut pair: its parts' outputs, weighted and summed in the order of the line.  A
+// warp takes every kWarps-th part, eight at a time, and asks for the first eight before it knows their weights;
+// the weights of part i are in lane i % 32 of every warp.
 template <typename T, int DH>
-__global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_constant__ Int4Args a) {
-  constexpr int kPer = (kMaxCtas + 31) / 32;  // parts a lane has the weights of
-  constexpr int V = DH / 32;                  // columns of a lane
+__global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_constant__ Int4Args a, int ctas) {
+  constexpr int kPer = kMaxCtas / 32;      // parts a lane has the weights of
+  constexpr int kMine = kMaxCtas / kWarps;  // parts of a warp
+  constexpr int kBatch = 8;
+  constexpr int V = DH / 32;  // columns of a lane
   __shared__ float sums[kWarps][DH];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ CutPair found;
+  __shared__ int found_cta, before[2 * kWarps];
+  static_assert(kMaxCtas <= 2 * kThreads && kMine % kBatch == 0, "");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = blockIdx.y;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int first = blockIdx.x, r = blockIdx.y;
-  const CutPair p = reinterpret_cast<const CutPair*>(a.ws + kWsCut)[first];
-  if (r >= p.rows || p.parts == 0) return;
+  // the pair's record among those of all CTAs
+  CutPair mine[2];
+  unsigned some[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c = k * kThreads + tid;
+    mine[k] = c < ctas ? reinterpret_cast<const CutPair*>(a.ws + kWsCut)[c] : CutPair{};
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    some[k] = __ballot_sync(0xffffffffu, mine[k].rows_parts != 0);
+    if (lane == 0) before[k * kWarps + warp] = __popc(some[k]);
+  }
+  if (tid == 0) found_cta = -1;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    int at = __popc(some[k] & ((1u << lane) - 1));
+    for (int w = 0; w < k * kWarps + warp; ++w) at += before[w];
+    if (mine[k].rows_parts != 0 && at == (int)blockIdx.x) {
+      found = mine[k];
+      found_cta = k * kThreads + tid;
+    }
+  }
+  __syncthreads();
+  const int first = found_cta;
+  const CutPair p = found;
+  const int rows = p.rows_parts & 255, parts = p.rows_parts >> 8;
+  if (first < 0 || r >= rows) return;
   auto slot = [&](int i) { return 2 * (first + i) + (i == 0 ? 1 : 0); };
-  const float2* ml = reinterpret_cast<const float2*>(a.ws + kWsMl);
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + kWsMl) + r;
+  const float* o = reinterpret_cast<const float*>(a.ws + kWsO) + r * DH + V * lane;
   float2 x[kPer];
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) x[k] = 32 * k + lane < p.parts ? ml[slot(32 * k + lane) * kPartRows + r] : make_float2(-INFINITY, 0.f);
-  const float* o = reinterpret_cast<const float*>(a.ws + kWsO) + r * DH + V * lane;
-  float M = -INFINITY, L = 0.f, v[V];
+  for (int k = 0; k < kPer; ++k) x[k] = 32 * k + lane < parts ? ml[slot(32 * k + lane) * kPartRows] : make_float2(-INFINITY, 0.f);
+  float u[kBatch][V], v[V];
+  auto fetch = [&](int j0) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = (j0 + j) * kWarps + warp;
+      if (i >= parts) break;
+      const float* src = o + (int64_t)slot(i) * kPartFloats;
+      if constexpr (V == 2) *reinterpret_cast<float2*>(u[j]) = *reinterpret_cast<const float2*>(src);
+      else
+#pragma unroll
+        for (int c = 0; c < V; c += 4) *reinterpret_cast<float4*>(u[j] + c) = *reinterpret_cast<const float4*>(src + c);
+    }
+  };
+  fetch(0);
+  float M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) M = fmaxf(M, x[k].x);
 #pragma unroll
@@ -807,22 +853,16 @@ __global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_consta
 #pragma unroll
   for (int c = 0; c < V; ++c) v[c] = 0.f;
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    if (32 * k >= p.parts) break;
+  for (int j0 = 0; j0 < kMine; j0 += kBatch) {
+    if (j0 * kWarps >= parts) break;
+    if (j0 > 0) fetch(j0);
 #pragma unroll
-    for (int j = 0; j < 32 / kWarps; ++j) {
-      const int i = 32 * k + j * kWarps + warp;
-      const float w = __shfl_sync(0xffffffffu, x[k].x, j * kWarps + warp);
-      if (i < p.parts) {
-        float u[V];
-        if constexpr (V == 2) *reinterpret_cast<float2*>(u) = *reinterpret_cast<const float2*>(o + (int64_t)slot(i) * kPartFloats);
-        else
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = (j0 + j) * kWarps + warp;  // part i: lane i % 32, its weight i / 32
+      const float w = __shfl_sync(0xffffffffu, x[(j0 + j) * kWarps / 32].x, (j0 + j) * kWarps % 32 + warp);
+      if (i < parts)
 #pragma unroll
-          for (int c = 0; c < V; c += 4)
-            *reinterpret_cast<float4*>(u + c) = *reinterpret_cast<const float4*>(o + (int64_t)slot(i) * kPartFloats + c);
-#pragma unroll
-        for (int c = 0; c < V; ++c) v[c] = fmaf(u[c], w, v[c]);
-      }
+        for (int c = 0; c < V; ++c) v[c] = fmaf(u[j][c], w, v[c]);
     }
   }
 #pragma unroll
@@ -842,8 +882,8 @@ __global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_consta
   if (a.lse && tid == 0) a.lse[p.b * a.ls_b + hq * a.ls_h] = lse_of(M, L);
 }
 
-template <class K>
-int launch_dependent(K kern, const Int4Args& a, dim3 grid, int smem, cudaStream_t s, const char* what) {
+template <class K, class... Args>
+int launch_dependent(K kern, dim3 grid, int smem, cudaStream_t s, const char* what, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads);
@@ -854,7 +894,7 @@ int launch_dependent(K kern, const Int4Args& a, dim3 grid, int smem, cudaStream_
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a), what);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), what);
 }
 
 template <class F>
@@ -881,9 +921,11 @@ int launch(const Int4Args& a, cudaStream_t s) {
   // No more CTAs than there could be pairs or shares.
   const int64_t most = std::max(pairs, (pairs * longest + kMinShare - 1) / kMinShare);
   const int grid = (int)(b.whole ? pairs : std::min<int64_t>(std::min(n * F::kCtas, kMaxCtas), most));
-  if (int rc = launch_dependent(int4_decode_kernel<F>, b, dim3(grid), F::kBytes, s, "paged_decode_int4 launch")) return rc;
+  if (int rc = launch_dependent(int4_decode_kernel<F>, dim3(grid), F::kBytes, s, "paged_decode_int4 launch", b)) return rc;
   if (b.whole || grid == 1) return BNA_OK;
-  return launch_dependent(int4_join_kernel<typename F::T, F::DH>, b, dim3(grid, a.chunk_rows), 0, s, "paged_decode_int4 join launch");
+  // A cut pair begins in each CTA at most, and there are no more of them than pairs.
+  const dim3 joins((unsigned)std::min<int64_t>(grid, pairs), (unsigned)a.chunk_rows);
+  return launch_dependent(int4_join_kernel<typename F::T, F::DH>, joins, 0, s, "paged_decode_int4 join launch", b, grid);
 }
 
 }  // namespace
