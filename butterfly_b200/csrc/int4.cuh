@@ -10,6 +10,8 @@
 // Code word (8 codes, the first in the lowest bits) g * groups + y of a row holds columns
 // 64 y + 8 g .. + 7: the lanes g of a matrix fragment then find the same part of every group side by side.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace bna {
@@ -79,44 +81,75 @@ __device__ __forceinline__ uint32_t int4_pair(uint32_t extremes) {
   return ElemTraits<T>::pack2(good ? __fdiv_rn(-e.y - m, 15.f) : m, m);
 }
 
+// Both halves of a register plus a float, each rounded once (the adder takes 16-bit terms as they are).
+template <typename T>
+__device__ __forceinline__ float2 halves_plus(uint32_t u, float c) {
+  float2 r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "add.f32.f16 %0, l, %3;\n\t"
+        "add.f32.f16 %1, h, %3;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(u), "f"(c));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "add.f32.bf16 %0, l, %3;\n\t"
+        "add.f32.bf16 %1, h, %3;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(u), "f"(c));
+  return r;
+}
+
 // The code word of 8 columns (4 registers): rint(d / s) of each difference d = x - m, ties to even, 15 at most; 0 for
 // all where s is not a positive number.
-// c = rint(d (1 / s)) can only be wrong beside a tie, and the residual e = d - c s shows it: it is exact (both
-// terms are multiples of the smaller one's last place, and no more than 24 bits of it apart), so |e| > s / 2 means
-// the next code, and |e| = s / 2 the even one.
+// c = rint(d r) with r a little below 1 / s (by more than its own error) is the code, or the one below it where d / s lies
+// at a tie or 15 2^-21 above one.  The residual e = d - c s tells: it is exact (both terms are multiples of the
+// smaller one's last place, and no more than 24 bits of it apart), so e = s / 2 means a tie, and rint(c + 1 / 2) is
+// its even code; e > s / 2, the next code, needs a difference that was rounded.  Ties are common in 16-bit
+// data (one value in 200 of a normal sample), so they take no branch.  Columns i and i + 4 go as a pair.
 template <typename T>
 __device__ __forceinline__ uint32_t int4_codes(const uint32_t* u, float2 sm) {
   const float s = sm.x, m = sm.y;
   if (!(s > 0.f && s < INFINITY)) return 0;
-  float x[8], c[8];
+  Two d[4], c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = ElemTraits<T>::unpack2(u[i]);
-    x[2 * i] = p.x - m;
-    x[2 * i + 1] = p.y - m;
+  for (int j = 0; j < 2; ++j) {
+    const float2 a = halves_plus<T>(u[j], -m), b = halves_plus<T>(u[2 + j], -m);
+    d[2 * j] = two(a.x, b.x);
+    d[2 * j + 1] = two(a.y, b.y);
   }
   if (s < Pair16<T>::kTiny) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = fminf(rintf(__fdiv_rn(x[i], s)), 15.f);
-  } else {  // (the scale is off by 2^-9 of itself at most: no code passes 15)
-    const float r = rcp_approx(s), h = 0.5f * s;
-    float e[8], worst = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = fmaf(x[i], r, 0x1.8p23f) - 0x1.8p23f;  // rint
-      e[i] = fmaf(-c[i], s, x[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = apart(d[i]);
+      c[i] = two(fminf(rintf(__fdiv_rn(x.x, s)), 15.f), fminf(rintf(__fdiv_rn(x.y, s)), 15.f));
     }
+  } else {  // (the scale is off by 2^-9 of itself at most: no code passes 15)
+    constexpr float kRint = 0x1.8p23f;  // adding it rounds to an integer
+    const float r = rcp_approx(s) * (1.f - 0x1p-21f), h = 0.5f * s;
+    const Two r2 = two(r, r), s2 = two(-s, -s), up = two(kRint, kRint), down = two(-kRint, -kRint), half = two(0.5f, 0.5f);
+    float worst = -1.f;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) worst = fmax3(worst, fabsf(e[i]), fabsf(e[i + 1]));
-    if (worst >= h) {
+    for (int i = 0; i < 4; ++i) {
+      const Two t = fma2(d[i], r2, up);
+      const float2 e = apart(fma2(add2(t, down), s2, d[i]));
+      worst = fmax3(worst, e.x, e.y);
+      c[i] = add2(fma2(two(e.x >= h ? 1.f : 0.f, e.y >= h ? 1.f : 0.f), half, t), down);
+    }
+    if (worst > h) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (fabsf(e[i]) > h || (fabsf(e[i]) == h && ((int)c[i] & 1))) c[i] += copysignf(1.f, e[i]);
+      for (int i = 0; i < 4; ++i) {
+        const Two t = add2(fma2(d[i], r2, up), down);
+        const float2 k = apart(t), e = apart(fma2(t, s2, d[i])), even = apart(c[i]);
+        c[i] = two(e.x > h ? k.x + 1.f : even.x, e.y > h ? k.y + 1.f : even.y);
+      }
     }
   }
-  const float lo = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 0x1p23f;  // the sum's last 16 bits
-  const float hi = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 0x1p23f;
-  return lower2(__float_as_uint(lo), __float_as_uint(hi));
+  const Two by = two(16.f, 16.f);  // the sums' last 16 bits are the codes
+  const float2 w = apart(add2(fma2(fma2(fma2(c[3], by, c[2]), by, c[1]), by, c[0]), two(0x1p23f, 0x1p23f)));
+  return lower2(__float_as_uint(w.x), __float_as_uint(w.y));
 }
 
 // The code word and the group's (s, m) of 8 columns in each lane; lanes 8 i .. 8 i + 7 hold a group, and all 32

@@ -145,19 +145,11 @@ __device__ __forceinline__ float lane_sum(float x) {
   x += __shfl_xor_sync(0xffffffffu, x, 8);
   return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
-// Both halves of a register as floats.  bf16: by the adder that takes 16-bit terms (exact), as the integer pipe, which
+// Both halves of a register as floats.  bf16: by the adder that takes 16-bit terms, as the integer pipe, which
 // would shift and mask, is the busiest one here (64 x 65,536 tokens: 241 -> 233 us).
 template <typename T>
 __device__ __forceinline__ float2 halves(uint32_t w) {
-  if constexpr (std::is_same<T, __half>::value) return ElemTraits<T>::unpack2(w);
-  float2 r;
-  asm("{\n\t.reg .b16 l, h;\n\t"
-      "mov.b32 {l, h}, %2;\n\t"
-      "add.f32.bf16 %0, l, %3;\n\t"
-      "add.f32.bf16 %1, h, %3;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "r"(w), "f"(0.f));
-  return r;
+  return std::is_same<T, __half>::value ? ElemTraits<T>::unpack2(w) : halves_plus<T>(w, 0.f);
 }
 // (m, l) with l times 2^kShift
 __device__ __forceinline__ float lse_of(float m, float l) {
