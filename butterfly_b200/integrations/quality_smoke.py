@@ -7,7 +7,8 @@ with stock (dense) attention and once swapped onto the B200 compressed kernels, 
 * KL of the next-token distributions at the end of prefill, both directions, over the
   stock top-k tokens that also appear in the compressed top-k (reference ``_kl``, :228-238)
 * top-k overlap and top-1 agreement of those distributions (:241-262)
-* exact match and token-by-token agreement of the greedy suffix.
+* exact match and token-by-token agreement of the greedy suffix
+* the prompt's own tokens: mean negative log likelihood and mean entropy under each (``prompt_scores``).
 
 The smoke is descriptive, as the reference's: it reports, it does not assert.
 
@@ -22,6 +23,22 @@ import math
 from typing import Any, Dict, List
 
 import torch
+
+from ..logits import token_logprobs
+
+
+def prompt_scores(model, input_ids: torch.Tensor, chunk: int = 1024) -> Dict[str, float]:
+    """Mean negative log likelihood (nats) of each token of ``input_ids`` [1, T] after those before it, and mean
+    entropy of the distributions it is drawn from.  The logits exist ``chunk`` rows at a time."""
+    with torch.no_grad():
+        hidden = model.model(input_ids=input_ids, use_cache=False).last_hidden_state[0, :-1]
+        targets = input_ids[0, 1:]
+        sums = torch.zeros(2, dtype=torch.float64, device=hidden.device)
+        for i in range(0, hidden.shape[0], chunk):
+            r = token_logprobs(model.lm_head(hidden[i:i + chunk]), targets[i:i + chunk])
+            sums += torch.stack([-r.logprobs.double().sum(), r.entropy.double().sum()])
+    nll, entropy = (sums / max(1, hidden.shape[0])).tolist()
+    return {"nll": nll, "entropy": entropy}
 
 
 def run_mode(model, input_ids: torch.Tensor, decode_len: int, top_k: int = 50, cache=None) -> Dict[str, Any]:
@@ -90,6 +107,7 @@ def quality_smoke(model, input_ids: torch.Tensor, decode_len: int = 32, top_k: i
     from .qwen_fused import fuse_qwen_decoder_layers, unfuse_qwen_decoder_layers
     qt.patch_qwen35_full_attention_decode()
     stock = run_mode(model, input_ids, decode_len, top_k, DynamicCache(config=model.config))
+    scores = {"stock": prompt_scores(model, input_ids)}
     qt.swap_qwen_attention_with_butterfly_cuda(model, qt.compressed_config())
     if fused:
         fuse_qwen_decoder_layers(model)
@@ -98,10 +116,12 @@ def quality_smoke(model, input_ids: torch.Tensor, decode_len: int = 32, top_k: i
                                          max_kv_size=int(input_ids.shape[1]) + decode_len + 64,
                                          max_chunk_size=4096)
         comp = run_mode(model, input_ids, decode_len, top_k, cache)
+        scores["compressed"] = prompt_scores(model, input_ids)
     finally:
         unfuse_qwen_decoder_layers(model)
         qt.restore_qwen_dense_attention(model)
-    return {"metrics": compare(stock, comp), "stock": stock, "compressed": comp,
+    metrics = {**compare(stock, comp), **{f"prompt_{k}_{mode}": v for mode, x in scores.items() for k, v in x.items()}}
+    return {"metrics": metrics, "stock": stock, "compressed": comp,
             "seq_len": int(input_ids.shape[1]), "decode_len": decode_len}
 
 

@@ -19,6 +19,9 @@ sizes that are multiples of 256 up to 8,192).
     logits, granted = dec.step(tokens)                  # tokens [max_requests], rows not live ignored
     dec.finish([3])
 
+``cache_bits=4`` keeps the keys and values in 4 bits; ``butterfly_b200.logits.token_logprobs`` gives the log
+probabilities of the tokens that are sampled from the logits, and their alternatives.
+
 ``python -m butterfly_b200.integrations.qwen_paged`` runs a random-init model this way.
 """
 from __future__ import annotations
@@ -30,6 +33,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import glue
+from ..logits import token_logprobs
 from ..paged import PagedKVCache, PagedReservation
 from .qwen_fused import _is_qwen35_norm, _merge_weights
 from .qwen_torch import _get_decoder_with_layers, _has_required_qwen_attention_attrs, patch_qwen35_full_attention_decode
@@ -62,7 +66,7 @@ class _Layer:
 class PagedQwenDecoder:
     @torch.no_grad()
     def __init__(self, model: nn.Module, *, num_pages: int, max_tokens_per_request: int, max_requests: int = 8,
-                 page_size: int = 64):
+                 page_size: int = 64, cache_bits: int = 16):
         patch_qwen35_full_attention_decode()
         self.model, self.decoder = model, _get_decoder_with_layers(model)
         head = getattr(model, "lm_head", None)
@@ -72,7 +76,8 @@ class PagedQwenDecoder:
         w = self.layers[0].w_qkv
         self.cache = PagedKVCache(num_layers=len(self.layers), num_pages=num_pages, page_size=page_size,
                                   num_kv_heads=self.layers[0].hkv, head_dim=128, max_requests=max_requests,
-                                  max_tokens_per_request=max_tokens_per_request, dtype=w.dtype, device=w.device)
+                                  max_tokens_per_request=max_tokens_per_request, dtype=w.dtype, device=w.device,
+                                  cache_bits=cache_bits)
         # the weight-streaming GEMVs take up to 8 rows, and inputs of these sizes; else library products
         sizes = [n for st in self.layers for n in (st.w_qkv.shape[1], 128 * st.hq, st.inter)]
         self._few = max_requests <= 8 and all(n % 256 == 0 and n <= 8192 for n in sizes)
@@ -190,6 +195,7 @@ def main() -> None:
     ap.add_argument("--requests", type=int, default=8)
     ap.add_argument("--prompt", type=int, default=4096, help="longest prompt; request i has a 1 / (i + 1) of it")
     ap.add_argument("--steps", type=int, default=64)
+    ap.add_argument("--cache-bits", type=int, default=16, choices=(16, 4))
     args = ap.parse_args()
     if args.steps < 1:
         ap.error("--steps must be at least 1")
@@ -202,20 +208,23 @@ def main() -> None:
     page = 64
     width = args.prompt + args.steps + page
     dec = PagedQwenDecoder(model, max_requests=args.requests, page_size=page, max_tokens_per_request=width,
-                           num_pages=args.requests * -(-width // page))
+                           num_pages=args.requests * -(-width // page), cache_bits=args.cache_bits)
     lens = [max(1, args.prompt // (i + 1)) for i in range(args.requests)]
     logits = dec.add({i: torch.randint(0, 32000, (n,), device="cuda") for i, n in enumerate(lens)})
     tokens = torch.stack([logits[i].argmax() for i in range(args.requests)])
+    total = torch.zeros((), device="cuda")
     for s in range(args.steps):
         if s == untimed:
             torch.cuda.synchronize()
             t0 = time.perf_counter()
         logits, _ = dec.step(tokens)
-        tokens = logits.argmax(-1)
+        best = token_logprobs(logits, top_k=1)
+        tokens = best.top_ids[:, 0]
+        total += best.top_logprobs.sum()
     torch.cuda.synchronize()
     ms = (time.perf_counter() - t0) / (args.steps - untimed) * 1e3
-    print(f"{args.requests} requests of {min(lens)} to {max(lens)} prompt tokens: {ms:.3f} ms a step, "
-          f"{args.requests / ms * 1e3:.0f} tokens/s; lengths now {dec.cache.lens.tolist()}, "
+    print(f"{args.requests} requests of {min(lens)} to {max(lens)} prompt tokens, {args.cache_bits}-bit cache of {dec.cache.nbytes / 1e6:.1f} MB: "
+          f"{ms:.3f} ms a step, {args.requests / ms * 1e3:.0f} tokens/s, mean log probability {float(total) / (args.requests * args.steps):.3f}; lengths now {dec.cache.lens.tolist()}, "
           f"{int(dec.cache.num_free)} of {int(dec.cache.free_pages.numel())} pages free")
 
 

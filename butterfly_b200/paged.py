@@ -10,10 +10,14 @@ request, and attention that reads through the table.
   paged_append             the tokens' key / value rows into their slots
   paged_decode_attention   one new token per request over its pages, optionally writing that
                            token's rows in the same launch
-  PagedKVCache             the three of them over per-layer pools
+  paged_append_int4, paged_read_int4, paged_decode_attention_int4
+                           the same over pools that hold keys and values in 4 bits (4.5 with their
+                           scales), and the rows read back
+  PagedKVCache             all of them over per-layer pools, in 16 or 4 bits
 
-Pools are ``[pages, Hkv, page_size, dh]`` views (``page_size`` a multiple of 16, ``dh`` 64, 128
-or 256; rows of ``dh`` contiguous), so token-major pages are a transposed view.  Everything is
+16-bit pools are ``[pages, Hkv, page_size, dh]`` views (``page_size`` a multiple of 16, ``dh`` 64, 128
+or 256; rows of ``dh`` contiguous), so token-major pages are a transposed view; 4-bit pools are bytes
+(``int4_pool``).  Everything is
 enqueued on the current stream and nothing waits for the host.
 """
 from __future__ import annotations
@@ -215,6 +219,9 @@ def paged_decode_attention_int4(q: torch.Tensor, kv_pages: torch.Tensor, block_t
 class PagedKVCache:
     """Pools of ``num_layers`` layers under one set of block tables, lengths and free pages.
 
+    ``cache_bits=4`` holds the rows (of type ``dtype``) in 4 bits (``paged_append_int4``): ``kv_pages`` in place of
+    ``k_pages`` and ``v_pages``, 3.56 times the tokens in the same memory.
+
     The requests are the ``max_requests`` rows of the tables; a row of length 0 is vacant.  The
     cache's state (lengths, stack height, tables, the attention's workspace) stays at one address
     and moves on in stream order, so calls may be captured: a replayed ``reserve`` (with a device
@@ -223,14 +230,22 @@ class PagedKVCache:
 
     def __init__(self, *, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  max_requests: int, max_tokens_per_request: int, dtype: torch.dtype = torch.bfloat16,
-                 device: torch.device | str = "cuda") -> None:
+                 device: torch.device | str = "cuda", cache_bits: int = 16) -> None:
+        if cache_bits not in (4, 16):
+            raise ValueError(f"cache_bits must be 16 or 4, got {cache_bits}")
         if not 0 < int(max_requests) <= MAX_REQUESTS:
             raise ValueError(f"max_requests must be in [1, {MAX_REQUESTS}], what one reservation serves")
-        self.page_size = int(page_size)
+        self.page_size, self.cache_bits, self.dtype = int(page_size), int(cache_bits), dtype
         shape = (int(num_pages), int(num_kv_heads), self.page_size, int(head_dim))
         # every read goes through a row written before, so the pools need no clearing
-        self.k_pages = [torch.empty(shape, dtype=dtype, device=device) for _ in range(int(num_layers))]
-        self.v_pages = [torch.empty(shape, dtype=dtype, device=device) for _ in range(int(num_layers))]
+        self.k_pages, self.v_pages, self.kv_pages = [], [], []
+        for _ in range(int(num_layers)):
+            if self.cache_bits == 4:
+                _lib.dtype_code(dtype)
+                self.kv_pages.append(int4_pool(*shape, device=device))
+            else:
+                self.k_pages.append(torch.empty(shape, dtype=dtype, device=device))
+                self.v_pages.append(torch.empty(shape, dtype=dtype, device=device))
         width = -(-int(max_tokens_per_request) // self.page_size)
         self.block_table = torch.full((int(max_requests), width), -1, dtype=torch.int32, device=device)
         with torch.inference_mode(False):  # (updated in place, in whichever mode the caller is then)
@@ -265,7 +280,7 @@ class PagedKVCache:
     @property
     def nbytes(self) -> int:
         """Bytes of all pools (what the cache holds on the device, used or not)."""
-        return sum(x.numel() * x.element_size() for x in self.k_pages + self.v_pages)
+        return sum(x.numel() * x.element_size() for x in self.k_pages + self.v_pages + self.kv_pages)
 
     def reserve(self, add: torch.Tensor | Sequence[int], num_tokens: Optional[int] = None) -> PagedReservation:
         """Advance every request by ``add`` tokens (see ``paged_reserve``); done once per step, for
@@ -299,17 +314,38 @@ class PagedKVCache:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
         """The reserved tokens' rows [tokens, Hkv, dh] of one layer into their slots."""
-        paged_append(k, v, self.k_pages[layer], self.v_pages[layer], slot_map)
+        if self.cache_bits == 4:
+            self._check_type("k", k)
+            paged_append_int4(k, v, self.kv_pages[layer], slot_map)
+        else:
+            paged_append(k, v, self.k_pages[layer], self.v_pages[layer], slot_map)
+
+    def _check_type(self, name: str, x: torch.Tensor) -> None:
+        # 4-bit pools are bytes, whose scales are of the type that the rows came in
+        if x.dtype != self.dtype:
+            raise ValueError(f"{name} must have the cache's dtype {self.dtype}, got {x.dtype}")
+
+    def read(self, layer: int, slot_map: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """The rows in slots ``slot_map`` of one layer of a 4-bit cache (see ``paged_read_int4``)."""
+        if self.cache_bits != 4:
+            raise ValueError("read is for a cache of 4 bits: 16-bit pools hold the rows as they are")
+        return paged_read_int4(self.kv_pages[layer], slot_map, dtype=self.dtype)
 
     def attend(self, layer: int, q: torch.Tensor, *, k_new: Optional[torch.Tensor] = None,
                v_new: Optional[torch.Tensor] = None, active: Optional[torch.Tensor] = None, window: int = 0,
                scale: Optional[float] = None, return_lse: bool = False):
         """One new token per request, q [max_requests,Hq,1,dh], over its cached context (see
         ``paged_decode_attention``)."""
+        if self.cache_bits == 4:
+            self._check_type("q", q)
+            return paged_decode_attention_int4(q, self.kv_pages[layer], self.block_table, self._lens, k_new=k_new, v_new=v_new,
+                                               active=active, window=window, scale=scale, return_lse=return_lse,
+                                               workspace=self.workspace)
         return paged_decode_attention(q, self.k_pages[layer], self.v_pages[layer], self.block_table, self._lens,
                                       k_new=k_new, v_new=v_new, active=active, window=window, scale=scale,
                                       return_lse=return_lse, workspace=self.workspace)
 
 
-__all__ = ["PagedKVCache", "PagedReservation", "RELEASE", "decode_workspace", "paged_append", "paged_decode_attention", "paged_reserve",
-           "reset_workspaces", "take_device_error"]
+__all__ = ["PagedKVCache", "PagedReservation", "RELEASE", "decode_workspace", "int4_pool", "paged_append", "paged_append_int4",
+           "paged_decode_attention", "paged_decode_attention_int4", "paged_read_int4", "paged_reserve", "reset_workspaces",
+           "take_device_error"]

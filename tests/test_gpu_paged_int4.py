@@ -435,7 +435,7 @@ def test_queries_far_apart_in_one_head():
 
 def test_nan_stays_in_its_head_and_request():
     c = Case([50, 60, 70], 4, 2, seed=5)
-    rows = [b for b in range(3)]
+    rows = list(range(3))
     c.pool[int(c.table[1, 0]), 1, 0, 8 * 128:8 * 128 + 2] = 255  # a key scale of request 1, head 1
     out, lse = c.run()
     assert torch.isnan(out[1, 2:]).all() and torch.isnan(lse[1, 2:]).all()

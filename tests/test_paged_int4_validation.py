@@ -105,3 +105,32 @@ def test_wrappers_refuse_cpu_tensors():
         with pytest.raises(ValueError):
             bb.paged.int4_pool(*bad, device="cpu")
     assert bb.paged.int4_pool(3, 2, 48, 64, device="cpu").shape == (3, 2, 3, 18 * 64)
+
+
+def _cache(**kw):
+    a = dict(num_layers=2, num_pages=4, page_size=32, num_kv_heads=2, head_dim=64, max_requests=3, max_tokens_per_request=64, device="cpu")
+    return bb.PagedKVCache(**{**a, **kw})
+
+
+def test_cache_bits():
+    c = _cache(cache_bits=4)
+    assert [x.shape for x in c.kv_pages] == [(4, 2, 2, 18 * 64)] * 2 and not c.k_pages and not c.v_pages
+    assert c.nbytes * 32 == _cache().nbytes * 9  # 4.5 bits a column for 16
+    for bits in (8, 0, 32):
+        with pytest.raises(ValueError, match="cache_bits"):
+            _cache(cache_bits=bits)
+    with pytest.raises(ValueError):
+        _cache(cache_bits=4, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        _cache(cache_bits=4, page_size=24)
+    with pytest.raises(ValueError, match="4 bits"):
+        _cache().read(0, torch.zeros(1, dtype=torch.int64))
+
+
+def test_a_cache_takes_rows_of_its_own_type():
+    c = _cache(cache_bits=4)
+    rows = torch.zeros(4, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="dtype"):
+        c.append(0, rows, rows, torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="dtype"):
+        c.attend(0, rows[:3, :, None])
