@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 #include <string>
+#include <type_traits>
 
 #include "../../include/bna_b200.h"
 
@@ -137,6 +138,27 @@ __device__ __forceinline__ void st_128(void* p, uint4 v) {
   asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
 }
+// Both halves of a register plus a float, each rounded once (the adder takes 16-bit terms as they are).
+template <typename T>
+__device__ __forceinline__ float2 halves_plus(uint32_t u, float c) {
+  float2 r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "add.f32.f16 %0, l, %3;\n\t"
+        "add.f32.f16 %1, h, %3;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(u), "f"(c));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "add.f32.bf16 %0, l, %3;\n\t"
+        "add.f32.bf16 %1, h, %3;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(u), "f"(c));
+  return r;
+}
+
 // Two floats in a register pair, and operations on both.
 using Two = unsigned long long;
 __device__ __forceinline__ Two two(float a, float b) {

@@ -10,8 +10,6 @@
 // Code word (8 codes, the first in the lowest bits) g * groups + y of a row holds columns
 // 64 y + 8 g .. + 7: the lanes g of a matrix fragment then find the same part of every group side by side.
 #pragma once
-#include <type_traits>
-
 #include "common.cuh"
 
 namespace bna {
@@ -79,27 +77,6 @@ __device__ __forceinline__ uint32_t int4_pair(uint32_t extremes) {
   const bool good = e.x > -INFINITY && e.y > -INFINITY;  // (neither NaN nor infinite: e.x <= -e.y)
   const float m = good ? e.x : __int_as_float(0x7fc00000);
   return ElemTraits<T>::pack2(good ? __fdiv_rn(-e.y - m, 15.f) : m, m);
-}
-
-// Both halves of a register plus a float, each rounded once (the adder takes 16-bit terms as they are).
-template <typename T>
-__device__ __forceinline__ float2 halves_plus(uint32_t u, float c) {
-  float2 r;
-  if constexpr (std::is_same<T, __half>::value)
-    asm("{\n\t.reg .b16 l, h;\n\t"
-        "mov.b32 {l, h}, %2;\n\t"
-        "add.f32.f16 %0, l, %3;\n\t"
-        "add.f32.f16 %1, h, %3;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "r"(u), "f"(c));
-  else
-    asm("{\n\t.reg .b16 l, h;\n\t"
-        "mov.b32 {l, h}, %2;\n\t"
-        "add.f32.bf16 %0, l, %3;\n\t"
-        "add.f32.bf16 %1, h, %3;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "r"(u), "f"(c));
-  return r;
 }
 
 // The code word of 8 columns (4 registers): rint(d / s) of each difference d = x - m, ties to even, 15 at most; 0 for

@@ -112,7 +112,7 @@ __device__ __forceinline__ Sums warp_join(const Sums& s) {
   const Sums x = moved(s, M);
   return {M, warp_sum(x.z), warp_sum(x.w)};
 }
-static_assert(kMaxCluster * kTop <= kList && kThreads % kTop == 0, "");
+static_assert(kThreads % kTop == 0, "");
 // The warp's keys' ranks: of the keys list[0 .. n) the number above `key`, counted by the eight lanes 8 i .. 8 i + 7 that hold
 // the same key.
 __device__ __forceinline__ int rank_in(const uint64_t* list, int n, uint64_t key, int lane) {
@@ -178,10 +178,13 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
   __shared__ float sums[3][kWarps];  // ref, Z, W of the warps, then of the CTA in column 0
   __shared__ uint64_t bound;
   __shared__ int owners[kThreads];
+  __shared__ uint64_t all_top[kMaxCluster * kTop];  // of the cluster's CTAs, in the first one
+  __shared__ float all_sums[3][kMaxCluster];
   __shared__ int count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = cluster > 1 ? (int)cluster_ctarank() : 0;
   const int r = (int)blockIdx.x / cluster;
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int outer = r / a.inner;
@@ -233,17 +236,17 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
       }
       return;
     }
-    const Two base = two(-ref, -ref), log2e = two(kLog2e, kLog2e);
+    const Two log2e = two(kLog2e, kLog2e);
 #pragma unroll
     for (int j = 0; j < E / 2; ++j) {
-      Two x;
+      Two d;
       if constexpr (sizeof(T) == 4) {
-        x = two(max_nan(__uint_as_float(u[2 * j]), Low<T>::kLowest), max_nan(__uint_as_float(u[2 * j + 1]), Low<T>::kLowest));
+        d = add2(two(max_nan(__uint_as_float(u[2 * j]), Low<T>::kLowest), max_nan(__uint_as_float(u[2 * j + 1]), Low<T>::kLowest)),
+                 two(-ref, -ref));
       } else {
-        const float2 f = ElemTraits<T>::unpack2(Low<T>::cut(u[j]));
-        x = two(f.x, f.y);
+        const float2 f = halves_plus<T>(Low<T>::cut(u[j]), -ref);
+        d = two(f.x, f.y);
       }
-      const Two d = add2(x, base);
       const float2 t = apart(mul2(d, log2e));
       const Two e = two(ex2_approx(t.x), ex2_approx(t.y));
       z2 = add2(z2, e);
@@ -374,30 +377,28 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
   if (cluster == 1) {
     __syncthreads();
   } else {
+    // each CTA leaves its sums and its list in the first one's shared memory
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // (all of them run by now)
+    if (tid < a.k)
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&all_top[part * a.k + tid]), 0)), "l"(top[tid]) : "memory");
+    if (tid == kThreads - 32) {  // (whose warp joined the sums)
+      const float x[3] = {t.ref, t.z, t.w};
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&all_sums[i][part]), 0)), "f"(x[i]) : "memory");
+    }
     cluster_sync_all();  // (every thread of every CTA comes here)
     if (part == 0) {
-      auto remote32 = [](const float* p, int rank) {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
-        return v;
-      };
-      for (int i = tid; i < cluster * a.k; i += kThreads) {
-        const uint64_t* src = &top[i % a.k];
-        uint64_t v;
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(src), i / a.k)) : "memory");
-        list[i] = v;
-      }
       if (warp == kWarps - 1) {
         t = {-INFINITY, 0.f, 0.f};
-        if (lane < cluster) t = {remote32(&sums[0][0], lane), remote32(&sums[1][0], lane), remote32(&sums[2][0], lane)};
+        if (lane < cluster) t = {all_sums[0][lane], all_sums[1][lane], all_sums[2][lane]};
         t = warp_join(t);
+        if (lane == 0) keep(0);
       }
-      __syncthreads();  // (the lists have been read before `top` is written again)
-      if (tid == kThreads - 1) keep(0);
       for (int c0 = 0; c0 < cluster * a.k; c0 += kThreads / 8) {
         const int c = c0 + tid / 8;
-        const uint64_t key = c < cluster * a.k ? list[c] : 0;
-        const int above = rank_in(list, cluster * a.k, key, lane);
+        const uint64_t key = c < cluster * a.k ? all_top[c] : 0;
+        const int above = rank_in(all_top, cluster * a.k, key, lane);
         if (key != 0 && (lane & 7) == 0 && above < a.k) top[above] = key;
       }
       __syncthreads();
@@ -415,11 +416,10 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
     }
     if (tid < a.k) {
       const uint64_t key = top[tid];
-      a.top_ids[r * a.k + tid] = (int64_t)(uint32_t)~(uint32_t)key;
-      a.top_lp[r * a.k + tid] = (value_of((uint32_t)(key >> 32)) - base) - log_z;
+      a.top_ids[(int64_t)r * a.k + tid] = (int64_t)(uint32_t)~(uint32_t)key;
+      a.top_lp[(int64_t)r * a.k + tid] = (value_of((uint32_t)(key >> 32)) - base) - log_z;
     }
   }
-  if (cluster > 1) cluster_sync_all();  // no CTA ends while its shared memory may be read
 }
 
 template <typename T>
