@@ -31,8 +31,9 @@ constexpr int kList = 4096;   // entries that reach the bound, as long as they f
 constexpr int kMaxCluster = 8;
 constexpr float kSlack = 8.f;  // e^kSlack times the row's length stays far below the fp32 range
 constexpr float kLog2e = 1.4426950408889634f;
-// Entries are cut at the type's lowest value as they are summed, so that a masked one adds 0 to W and not 0 * inf; where
-// the reference itself is about as low, differences are cut instead: e^kFloor is 0 in fp32.
+// Entries are cut from below (Low) as they are summed, so that a masked one adds 0 to W and not 0 * inf: what lies so far
+// below the reference adds nothing else.  Where the reference itself is about as low, differences are cut
+// instead: e^kFloor is 0 in fp32.
 constexpr float kFloor = -120.f;
 
 struct LogprobArgs {
@@ -62,14 +63,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// What a type's lowest value is, below which reference the differences are cut, and (16 bits) maxima of two entries in a register.
+// Where entries are cut, below which reference the differences are cut instead, and (16 bits) maxima of two entries in a
+// register.  A cut entry less the largest finite one is still finite.
 template <typename T> struct Low;
 template <> struct Low<float> {
-  static constexpr float kLowest = -3.4028234663852886e38f, kNear = -1e38f;
+  static constexpr float kLowest = -0x1p100f, kNear = -0x1p99f;
 };
 template <> struct Low<__nv_bfloat16> {
-  static constexpr uint32_t kLowest = 0xff7fff7fu;
-  static constexpr float kNear = -1e38f;
+  static constexpr uint32_t kLowest = 0xfb00fb00u;  // -2^119
+  static constexpr float kNear = -0x1p118f;
   __device__ static uint32_t top(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -81,7 +83,7 @@ template <> struct Low<__nv_bfloat16> {
   }
 };
 template <> struct Low<__half> {
-  static constexpr uint32_t kLowest = 0xfbfffbffu;
+  static constexpr uint32_t kLowest = 0xfbfffbffu;  // -65504
   static constexpr float kNear = -6e4f;
   __device__ static uint32_t top(uint32_t a, uint32_t b) {
     const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));

@@ -34,6 +34,7 @@ def check(x, tokens=None, k=0, got=None):
     assert r.entropy.shape == x.shape[:-1] and r.top_ids.shape == (*x.shape[:-1], k) == r.top_logprobs.shape
     d = x.double().reshape(-1, V)
     logp = torch.log_softmax(d, -1)
+    logp = torch.where(logp < -torch.finfo(torch.float32).max, -math.inf, logp)  # (what fp32 results can hold)
     p = logp.exp()
     M = d.max(-1, keepdim=True).values
     A = torch.where(p > 0, p * (d - M).abs(), 0).sum(-1)
@@ -168,6 +169,25 @@ def test_large_and_small_logits():
     for scale, shift in ((300.0, 0.0), (1e-3, 0.0), (5.0, 2000.0), (5.0, -2000.0)):
         x = _rand(7, 12345, dtype="f32", scale=scale) + shift
         check(x, _tokens(x), 20)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_entries_at_the_ends_of_the_range(dtype):
+    fi = torch.finfo(TYPES[dtype])
+    for rows in (1, 200):
+        x = _rand(rows, 9001, dtype=dtype).clone()
+        x[:, ::7] = -math.inf
+        x[:, 1::7] = fi.min
+        x[:, 2::7] = fi.min / 2
+        check(x, _tokens(x), 20)
+        x[:, 40] = fi.max  # beside masked entries and the lowest ones
+        x[:, 51] = fi.max
+        check(x, _tokens(x), 20)
+        low = torch.full_like(x, fi.min)
+        low[:, 5::9] = -math.inf
+        low[:, 17] = fi.min * (1 - 2 * fi.eps)
+        check(low, _tokens(low), 20)
+        check((low.double() / 2).to(x.dtype), _tokens(low), 20)
 
 
 def test_tokens():
