@@ -465,7 +465,8 @@ int launch_int4_rows(bool append, const bna_tensor4* k, const bna_tensor4* v, bn
     a.h[i] = x[i]->stride[1], a.t[i] = x[i]->stride[2];
     if (reinterpret_cast<uintptr_t>(x[i]->data) % 32 || (x[i]->size[1] > 1 && a.h[i] % 16) || (x[i]->size[2] > 1 && a.t[i] % 16)) a.wide = 0;
   }
-  // Short calls in small CTAs on many SMs: 64 tokens of 2 heads are 512 lanes a tensor.
+  // Short calls in small CTAs on many SMs (64 tokens x 2 heads: append 2.1, read 1.6 us with 64 threads, 2.3 and 1.8 with
+  // 256; 8,000 tokens 4.2 and 3.6 with 64, 4.0 and 3.2 with 256).
   const int block = a.count <= 64 * 148 ? 64 : 256;
   const int64_t blocks = (a.count + block / 4 - 1) / (block / 4);
   if (blocks > INT_MAX) return fail(BNA_UNSUPPORTED, "paged 4-bit rows: too many elements");

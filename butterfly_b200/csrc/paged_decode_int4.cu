@@ -39,10 +39,15 @@ using namespace sm100;
 constexpr int kGran = kInt4Tokens;  // keys of a granule: a block
 constexpr int kMaxCtas = 320;       // the workspace is sized for this many
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kSlack = 40;    // granules
-constexpr int kWhole = 80;    // granules of the longest pair up to which every pair gets a CTA of its own
-static_assert(kWhole <= 2 * kSlack + 1, "pairs that are never cut");
-constexpr int kMinShare = 32;  // granules a CTA gets at least (fewer CTAs otherwise)
+// Granules within which a cut moves to the end of its pair, and of the longest pair up to which none is cut where there
+// are pairs enough or the table has room for no longer one.  A cut costs its parts' way through memory and the
+// join, some 4 us.  2 heads of 128, slack 10 / 20 / 40: one request of 2,500 tokens 10.1 / 10.0 / 12.2 us, 8 of
+// 4,000 13.2 / 12.6 / 16.0.  Whole / cut: 64 requests of 1,200 tokens with a table for no more 10.5 / 15.8 us
+// (with one for 4,000 17.7 / 15.9), 128 of 1,250 and 4 heads 33.0 / 36.0, one of 1,000 (table 2,000) 11.0 / 9.4.
+constexpr int kSlack = 20, kWhole = 80;
+// Granules a CTA gets at least of a cut line (fewer CTAs otherwise); 16 / 32: one request of 20,000 tokens 12.1 / 10.5 us,
+// of 6,000 10.0 / 10.1.
+constexpr int kMinShare = 32;
 constexpr int kKeepLens = 1024;  // lengths kept in shared memory
 constexpr int kShift = 11;  // probabilities are held times 2^kShift, and so are l and o; the divisions undo it
 constexpr float kMove = 4.f;  // a reference moves when a score lies more than 2^kMove above it
@@ -487,8 +492,7 @@ struct Acc {
 // Granules up to the end of each thread's run of requests, cut evenly over C CTAs (the first U % C get one more).
 struct Line {
   const int* runs;
-  const int* lens;  // the first kKeepLens lengths
-  int per, per_b, U, C, q, r;
+  int per, per_b, U, C, q, r, slack;
 
   __device__ int raw(int c) const { return c * q + min(c, r); }
   __device__ int cta_of(int x) const {  // whose raw stretch holds x
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
   const int per_b = a.Hkv * a.chunks;
   int* lens = reinterpret_cast<int*>(sm + F::kLens);
   auto len_of = [&](int b) { return b < kKeepLens ? lens[b] : clamp_len(a, a.lens[b]); };
-  Line line{reinterpret_cast<const int*>(sm + F::kRuns), lens, (a.B + kThreads - 1) / kThreads, per_b, 0, 1, 0, 0};
+  Line line{reinterpret_cast<const int*>(sm + F::kRuns), (a.B + kThreads - 1) / kThreads, per_b, 0, 1, 0, 0, kSlack};
   At at{0, 0, 0};
   int cur = 0, end = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -520,12 +524,13 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
     // ---- the line
     __shared__ int warp_sums[kWarps];
     int* runs = reinterpret_cast<int*>(sm + F::kRuns);
-    int mine = 0, pairs = 0;
+    int mine = 0, pairs = 0, longest = 0;
     for (int b = tid * line.per; b < min((tid + 1) * line.per, a.B); ++b) {
       const int len = clamp_len(a, a.lens[b]), nt = granules_of(a, len);
       if (b < kKeepLens) lens[b] = len;
       mine += nt;
       pairs += nt > 0;
+      longest = max(longest, nt);
     }
     mine *= per_b;
     int incl = mine;
@@ -535,10 +540,12 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
       if (lane >= o) incl += x;
     }
     pairs = __reduce_add_sync(0xffffffffu, pairs) * per_b;
-    __shared__ int warp_pairs[kWarps];
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    __shared__ int warp_pairs[kWarps], warp_longest[kWarps];
     if (lane == 31) {
       warp_sums[warp] = incl;
       warp_pairs[warp] = pairs;
+      warp_longest[warp] = longest;
     }
     __syncthreads();
     pairs = 0;
@@ -546,12 +553,16 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) incl += warp_sums[w];
       pairs += warp_pairs[w];
+      longest = max(longest, warp_longest[w]);
     }
     runs[tid] = incl;
     __syncthreads();
     line.U = runs[kThreads - 1];
-    // a CTA for every kMinShare granules, or for every pair, where that is more
+    // A CTA for every kMinShare granules, or for every pair, where that is more.  Where all pairs are short, and enough
+    // for every CTA, cuts move to the nearest end however far it is.
+    const bool whole = longest <= kWhole && pairs >= (int)gridDim.x;
     line.C = min((int)gridDim.x, max(1, max(pairs, (line.U + kMinShare - 1) / kMinShare)));
+    line.slack = whole ? kWhole : kSlack;
     line.q = line.U / line.C;
     line.r = line.U - line.q * line.C;
     auto locate = [&](int x) {  // of a place before U: the warp whose runs reach past it, the run, the request
@@ -573,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
           at = locate(x);
           if (x > 0) {
             const int t = (x - at.begin) % max(at.nt, 1), rest = at.nt - t;
-            x = t <= kSlack && t <= rest ? x - t : rest <= kSlack ? x + rest : x;
+            x = t <= line.slack && t <= rest ? x - t : rest <= line.slack ? x + rest : x;
           }
         }
         if (i == 1) end = x;
@@ -616,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
     if (s.slot >= 0 && t0 == 0) {
       // A cut pair begins here: its parts are those of the CTAs up to the one that holds its end.  Cuts within it kept their
       // places (those near its end have moved there): the last of them lies at or before this place.
-      const int last = min(max((int)blockIdx.x + 1, line.cta_of(cur + at.nt - kSlack - 1)), line.C - 1);
+      const int last = min(max((int)blockIdx.x + 1, line.cta_of(cur + at.nt - line.slack - 1)), line.C - 1);
       begun = CutPair{s.b, s.h, s.r0, s.rows | (last - (int)blockIdx.x + 1) << 8};
     }
     cur += s.n;

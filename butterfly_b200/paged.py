@@ -239,9 +239,10 @@ class PagedKVCache:
         shape = (int(num_pages), int(num_kv_heads), self.page_size, int(head_dim))
         # every read goes through a row written before, so the pools need no clearing
         self.k_pages, self.v_pages, self.kv_pages = [], [], []
+        if self.cache_bits == 4:
+            _lib.dtype_code(dtype)  # (bytes in any other type would not be refused by the calls)
         for _ in range(int(num_layers)):
             if self.cache_bits == 4:
-                _lib.dtype_code(dtype)
                 self.kv_pages.append(int4_pool(*shape, device=device))
             else:
                 self.k_pages.append(torch.empty(shape, dtype=dtype, device=device))
