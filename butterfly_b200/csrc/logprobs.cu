@@ -11,6 +11,10 @@
 // the bound too have all their entries looked at, by all lanes of their warp.
 // A row is shared by a cluster of CTAs where there are few rows; the CTAs' sums and lists are joined
 // through distributed shared memory by the cluster's first one.
+//
+// Measured, with the likeliest entry: 4,096 rows of 151,936 in bf16 212 us for 1.24 GB, 5.9 TB/s (0.90 of a copy; the issue slots are 67% and
+// the exponential's pipe 56% busy).  512 threads and three CTAs an SM, so that the end of one row (bound,
+// candidates, ranks) lies beside the reads of two others.  One row with 20 alternatives 7.8 us: latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -316,9 +316,12 @@ __device__ __forceinline__ void move_words(uint32_t* dst, const uint32_t* src) {
     for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
 }
 
-// GR groups of 64 columns a row
+// GR groups of 64 columns a row.  131,072 tokens x 2 heads of 128 in bf16: 42 us for 172 MB, 4.1 TB/s (0.63 of a copy), bound by
+// instructions and their latency.  Ten CTAs of 128 threads an SM hold it to 48 registers; with 54 and four of 256 it takes 47 us, with twelve
+// and 40 registers 41, but 8,000 tokens 5.4 us instead of 4.4.  The first form, with eight lanes to a group and a division for each
+// code, took 182 us.
 template <typename T, int GR>
-__global__ void __launch_bounds__(256) int4_append_kernel(const __grid_constant__ Int4RowsArgs a) {
+__global__ void __launch_bounds__(128, GR == 4 ? 6 : 10) int4_append_kernel(const __grid_constant__ Int4RowsArgs a) {
   constexpr int DH = kInt4Group * GR;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -351,9 +354,9 @@ __global__ void __launch_bounds__(256) int4_append_kernel(const __grid_constant_
   if (t < GR) *reinterpret_cast<uint32_t*>(r.half + 8 * DH + 4 * (r.token * GR + t)) = mine;
 }
 
-// Rows without a slot get zeros.
+// Rows without a slot get zeros.  131,072 tokens x 2 heads of 128: 30 us for 172 MB, 5.8 TB/s (0.88 of a copy): HBM.
 template <typename T, int GR>
-__global__ void __launch_bounds__(256) int4_read_kernel(const __grid_constant__ Int4RowsArgs a) {
+__global__ void __launch_bounds__(128) int4_read_kernel(const __grid_constant__ Int4RowsArgs a) {
   constexpr int DH = kInt4Group * GR;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -466,8 +469,8 @@ int launch_int4_rows(bool append, const bna_tensor4* k, const bna_tensor4* v, bn
     if (reinterpret_cast<uintptr_t>(x[i]->data) % 32 || (x[i]->size[1] > 1 && a.h[i] % 16) || (x[i]->size[2] > 1 && a.t[i] % 16)) a.wide = 0;
   }
   // Short calls in small CTAs on many SMs (64 tokens x 2 heads: append 2.1, read 1.6 us with 64 threads, 2.3 and 1.8 with
-  // 256; 8,000 tokens 4.2 and 3.6 with 64, 4.0 and 3.2 with 256).
-  const int block = a.count <= 64 * 148 ? 64 : 256;
+  // 256); read of 131,072 tokens: 30 us with 128 threads, 36 with 64.
+  const int block = a.count <= 64 * 148 ? 64 : 128;
   const int64_t blocks = (a.count + block / 4 - 1) / (block / 4);
   if (blocks > INT_MAX) return fail(BNA_UNSUPPORTED, "paged 4-bit rows: too many elements");
   auto pick = [&](auto t) -> void (*)(const Int4RowsArgs) {
