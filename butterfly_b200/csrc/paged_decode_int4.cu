@@ -26,8 +26,8 @@
 //
 // Measured: 64 requests of 65,536 tokens, 8 / 2 heads of 128, bf16: 241 us for 1.21 GB, 5.0 TB/s (0.77 of a copy; the 16-bit
 // kernel takes 610 us for its 4.3 GB).  Bound by the instructions of a granule, some 300: 0.61 issued a cycle and
-// scheduler, the integer pipe 48% busy, the tensor pipe 22%.  One request of 131,072 tokens: 20 us, some 4 of
-// them before the first keys and 5 in the join.  4 requests of 37 to 513 tokens: 10 us, latency.
+// scheduler, the integer pipe 48% busy, the tensor pipe 22%.  One request of 131,072 tokens: 19 us, some 4 of
+// them before the first keys and 4 in the join.  4 requests of 37 to 513 tokens: 10 us, latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -801,20 +801,19 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
 }
 
 // Head blockIdx.y of the blockIdx.x-th cut pair: its parts' outputs, weighted and summed in the order of the line.  A
-// warp takes every kWarps-th part, eight at a time, and asks for the first eight before it knows their weights;
+// warp takes every kWarps-th part, BATCH at a time, and asks for the first ones before it knows their weights;
 // the weights of part i are in lane i % 32 of every warp.
 // A launch of its own, as a CTA that waited for the others' parts would hold its SM meanwhile.  Bound by latency: the launch and two
 // reads that depend on one another (the records, then weights and outputs).
-template <typename T, int DH>
+template <typename T, int DH, int BATCH>
 __global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_constant__ Int4Args a, int ctas) {
   constexpr int kPer = kMaxCtas / 32;      // parts a lane has the weights of
   constexpr int kMine = kMaxCtas / kWarps;  // parts of a warp
-  constexpr int kBatch = 8;
   constexpr int V = DH / 32;  // columns of a lane
   __shared__ float sums[kWarps][DH];
   __shared__ CutPair found;
   __shared__ int found_cta, before[2 * kWarps];
-  static_assert(kMaxCtas <= 2 * kThreads && kMine % kBatch == 0, "");
+  static_assert(kMaxCtas <= 2 * kThreads && kMine % BATCH == 0, "");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = blockIdx.y;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -853,10 +852,10 @@ __global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_consta
   float2 x[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) x[k] = 32 * k + lane < parts ? ml[slot(32 * k + lane) * kPartRows] : make_float2(-INFINITY, 0.f);
-  float u[kBatch][V], v[V];
+  float u[BATCH][V], v[V];
   auto fetch = [&](int j0) {
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
+    for (int j = 0; j < BATCH; ++j) {
       const int i = (j0 + j) * kWarps + warp;
       if (i >= parts) break;
       const float* src = o + (int64_t)slot(i) * kPartFloats;
@@ -882,11 +881,11 @@ __global__ void __launch_bounds__(kThreads) int4_join_kernel(const __grid_consta
 #pragma unroll
   for (int c = 0; c < V; ++c) v[c] = 0.f;
 #pragma unroll
-  for (int j0 = 0; j0 < kMine; j0 += kBatch) {
+  for (int j0 = 0; j0 < kMine; j0 += BATCH) {
     if (j0 * kWarps >= parts) break;
     if (j0 > 0) fetch(j0);
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
+    for (int j = 0; j < BATCH; ++j) {
       const int i = (j0 + j) * kWarps + warp;  // part i: lane i % 32, its weight i / 32
       const float w = __shfl_sync(0xffffffffu, x[(j0 + j) * kWarps / 32].x, (j0 + j) * kWarps % 32 + warp);
       if (i < parts)
@@ -954,7 +953,11 @@ int launch(const Int4Args& a, cudaStream_t s) {
   if (b.whole || grid == 1) return BNA_OK;
   // A cut pair begins in each CTA at most, and there are no more of them than pairs.
   const dim3 joins((unsigned)std::min<int64_t>(grid, pairs), (unsigned)a.chunk_rows);
-  return launch_dependent(int4_join_kernel<typename F::T, F::DH>, joins, 0, s, "paged_decode_int4 join launch", b, grid);
+  // Few pairs have many parts each, and then fewer rounds are faster (one request of 131,072 tokens, 2 heads of 128: 18.8 us against
+  // 20.3); else the longer code and its registers cost more than they give (64 of 1,200: 17.3 against 16.1).
+  constexpr int kMany = F::DH == 256 ? 10 : 20;
+  const auto join = grid >= 64 * pairs ? int4_join_kernel<typename F::T, F::DH, kMany> : int4_join_kernel<typename F::T, F::DH, 8>;
+  return launch_dependent(join, joins, 0, s, "paged_decode_int4 join launch", b, grid);
 }
 
 }  // namespace
