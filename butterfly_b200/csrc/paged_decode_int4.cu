@@ -24,10 +24,9 @@
 // Half of the keys enter P V as 15 - c with scale -s and minimum m + 15 s, so that what the tensor core cuts off its
 // sums cancels.
 //
-// Measured: 64 requests of 65,536 tokens, 8 / 2 heads of 128, bf16: 241 us for 1.21 GB, 5.0 TB/s (0.77 of a copy; the 16-bit
-// kernel takes 610 us for its 4.3 GB).  Bound by the instructions of a granule, some 300: 0.61 issued a cycle and
-// scheduler, the integer pipe 48% busy, the tensor pipe 22%.  One request of 131,072 tokens: 19 us, some 4 of
-// them before the first keys and 4 in the join.  4 requests of 37 to 513 tokens: 10 us, latency.
+// Measured: 64 requests of 65,536 tokens, 8 / 2 heads of 128, bf16: 209 us for 1.21 GB, 5.8 TB/s (0.88 of a copy; the 16-bit
+// kernel takes 610 us for its 4.3 GB).  Bound by the instructions of a granule as much as by HBM.  One request of
+// 131,072 tokens: 19 us, some 4 of them before the first keys and 4 in the join.  4 requests of 37 to 513 tokens: 10 us, latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -176,7 +175,7 @@ struct Seg {
   int b, h, r0, rows, g0, n, lo, hi, slot;  // slot of the part (-1: the whole pair)
 };
 
-// ROWS: query heads served together at most: 4 (fp16 alone), 8 or 16
+// ROWS: query heads served together at most: 4, 8 or 16
 template <typename T_, int DH_, int ROWS>
 struct Form {
   using T = T_;
@@ -187,19 +186,28 @@ struct Form {
   // as its final rounding does (for bf16 ones an eighth of it).  With up to 4 heads the low parts ride in
   // columns 4-7, with more they take products of their own.
   static constexpr bool kTwoParts = std::is_same<T, __half>::value && ROWS > 4, kLowColumns = std::is_same<T, __half>::value && ROWS <= 4;
+  // For bf16 results with up to 4 heads two granules share the columns: all 8 get the same queries, and of the scores
+  // lanes t < 2 keep the first granule's, the others the second one's.  What follows on scores and probabilities is then done once
+  // for both, and the two halves' sums meet as the warps join: 64 x 65,536 tokens 240 -> 209 us, 64 of 1,200 10.5 -> 9.5, one of
+  // 131,072 18.8 -> 19.2.  (fp16, whose columns hold low parts, gains nothing by products for those instead: 84 us on 13
+  // requests to 262,144 either way.)
+  static constexpr bool kPaired = std::is_same<T, __nv_bfloat16>::value && ROWS <= 4;
+  static constexpr int kStep = kPaired ? 2 : 1;  // granules at a time
   // two CTAs an SM where their registers fit, so that the end of one's pair overlaps the other's reads
   static constexpr int kCtas = ROWS > 8 || DH == 256 ? 1 : 2;
   static constexpr int GR = DH / kInt4Group;
   static constexpr int kBlock = int4_block_bytes(DH);
-  static constexpr int kStages = DH == 256 ? 5 : ROWS > 8 ? 8 : 4;  // granules of a warp's ring
+  // (paired with 4 / 5 / 6 slots: 64 x 65,536 tokens 211 / 216 / 217 us)
+  static constexpr int kStages = kPaired ? 4 : DH == 256 ? 5 : ROWS > 8 ? 8 : 4;  // granules of a warp's ring
   static constexpr int kRing = kStages * kBlock;
+  static_assert(kStages % kStep == 0, "a pair of granules lies side by side");
   static constexpr int kPitch = DH + 4;  // floats of a row, as the warps join
   static_assert(kHeads * kPitch * 4 <= kRing, "a warp's outputs take its ring's place");
   static constexpr int kMl = kWarps * kRing;                   // (m, l) [warp][head]
   static constexpr int kRuns = kMl + kWarps * kHeads * 8;      // granules up to the end of each thread's run of requests
   static constexpr int kLens = kRuns + kThreads * 4;
   static constexpr int kBytes = kLens + 4 * kKeepLens;
-  static_assert(kCtas * (kBytes + 1024) <= 233472, "shared memory of an SM");
+  static_assert(kCtas * (kBytes + 1024 + 256) <= 233472, "shared memory of an SM (1 KB a CTA is the system's, and some static)");
 };
 
 // What a warp holds of a segment.  Scores come as S^T: lane 4 g + t has two keys, row(g) and row(g) + 4, and heads 2 t,
@@ -222,7 +230,7 @@ struct Acc {
   struct Queries {
     uint4 raw[NT][GR][2];
     __device__ __forceinline__ void load(const uint8_t* q, int64_t q_h, int rows, int lane) {
-      const int g = F::kLowColumns ? (lane >> 2) & 3 : lane >> 2, t = lane & 3;
+      const int g = F::kLowColumns || F::kPaired ? (lane >> 2) & 3 : lane >> 2, t = lane & 3;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -304,34 +312,51 @@ struct Acc {
     inv = pow2(100);
   }
 
-  // A granule in shared memory, its first key at `pos`; with `edge` keys outside [lo, hi) are masked.
-  __device__ __forceinline__ void granule(uint32_t tile, int pos, bool edge, int lo, int hi, int lane) {
+  // A granule in shared memory, its first key at `pos`; with `edge` keys outside [lo, hi) are masked.  Paired: also the
+  // one at `second`; `pos` is that of the lane's granule.
+  __device__ __forceinline__ void granule(uint32_t tile, uint32_t second, int pos, bool edge, int lo, int hi, int lane) {
     constexpr uint32_t M0 = 0x000f000fu, M1 = 0x00f000f0u;
     const int g = lane >> 2, t = lane & 3;
     const int row = (g >> 1) + 8 * (g & 1);
+    const uint32_t own = F::kPaired && t >= 2 ? second : tile;  // the granule of the lane's scores
     // scores
     float u[NT][4];
     {
-      uint32_t w[2][2 * GR], p[2][GR];
-      lds<0>(tile + row * (DH / 2) + t * (8 * GR), w[0]);
-      lds<4 * (DH / 2)>(tile + row * (DH / 2) + t * (8 * GR), w[1]);
-      lds<8 * DH>(tile + row * (4 * GR), p[0]);
-      lds<8 * DH + 16 * GR>(tile + row * (4 * GR), p[1]);
+      float acc[GR][NT][4];
+      uint32_t p[2][GR];
 #pragma unroll
-      for (int y = 0; y < GR; ++y) {
-        float acc[NT][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t a0 = w[0][j * GR + y], a1 = w[1][j * GR + y];
-          const uint32_t even[4] = {a0 & M0, a1 & M0, a0 & M1, a1 & M1};
-          const uint32_t odd[4] = {(a0 >> 8) & M0, (a1 >> 8) & M0, (a0 >> 8) & M1, (a1 >> 8) & M1};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (j == 0) mma_first(acc[n], even, qb[n][y][j][0][0], qb[n][y][j][0][1]);
-            else mma_16816<__half>(acc[n], even, qb[n][y][j][0][0], qb[n][y][j][0][1]);
-            mma_16816<__half>(acc[n], odd, qb[n][y][j][1][0], qb[n][y][j][1][1]);
-          }
+      for (int x = 0; x < F::kStep; ++x) {
+        const uint32_t from = x == 0 ? tile : second;
+        uint32_t w[2][2 * GR];
+        lds<0>(from + row * (DH / 2) + t * (8 * GR), w[0]);
+        lds<4 * (DH / 2)>(from + row * (DH / 2) + t * (8 * GR), w[1]);
+        if (x == 0) {
+          lds<8 * DH>(own + row * (4 * GR), p[0]);
+          lds<8 * DH + 16 * GR>(own + row * (4 * GR), p[1]);
         }
+#pragma unroll
+        for (int y = 0; y < GR; ++y) {
+          float c[NT][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t a0 = w[0][j * GR + y], a1 = w[1][j * GR + y];
+            const uint32_t even[4] = {a0 & M0, a1 & M0, a0 & M1, a1 & M1};
+            const uint32_t odd[4] = {(a0 >> 8) & M0, (a1 >> 8) & M0, (a0 >> 8) & M1, (a1 >> 8) & M1};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              if (j == 0) mma_first(c[n], even, qb[n][y][j][0][0], qb[n][y][j][0][1]);
+              else mma_16816<__half>(c[n], even, qb[n][y][j][0][0], qb[n][y][j][0][1]);
+              mma_16816<__half>(c[n], odd, qb[n][y][j][1][0], qb[n][y][j][1][1]);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[y][n][i] = x == 0 || t >= 2 ? c[n][i] : acc[y][n][i];
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < GR; ++y)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float2 sm = halves<T>(p[r][y]);
@@ -340,16 +365,15 @@ struct Acc {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const float base = y == 0 ? sm.y * qs[n][y][x] : fmaf(sm.y, qs[n][y][x], u[n][2 * r + x]);
-              u[n][2 * r + x] = fmaf(sm.x, acc[n][2 * r + x], base);
+              u[n][2 * r + x] = fmaf(sm.x, acc[y][n][2 * r + x], base);
             }
         }
-      }
     }
     float sv[2][GR], mv[2][GR];
     {
       uint32_t p[2][GR];
-      lds<17 * DH>(tile + row * (4 * GR), p[0]);
-      lds<17 * DH + 16 * GR>(tile + row * (4 * GR), p[1]);
+      lds<17 * DH>(own + row * (4 * GR), p[0]);
+      lds<17 * DH + 16 * GR>(own + row * (4 * GR), p[1]);
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -440,27 +464,36 @@ struct Acc {
       }
     }
     // outputs
-    uint32_t w[4][GR];
-    const uint32_t at = tile + t * (DH / 2) + g * (4 * GR);
-    lds<9 * DH>(at, w[0]);
-    lds<9 * DH + 8 * (DH / 2)>(at, w[1]);
-    lds<9 * DH + 4 * (DH / 2)>(at, w[2]);
-    lds<9 * DH + 12 * (DH / 2)>(at, w[3]);
 #pragma unroll
-    for (int y = 0; y < GR; ++y) {
+    for (int z = 0; z < F::kStep; ++z) {
+      uint32_t w[4][GR];
+      const uint32_t at = (z == 0 ? tile : second) + t * (DH / 2) + g * (4 * GR);
+      lds<9 * DH>(at, w[0]);
+      lds<9 * DH + 8 * (DH / 2)>(at, w[1]);
+      lds<9 * DH + 4 * (DH / 2)>(at, w[2]);
+      lds<9 * DH + 12 * (DH / 2)>(at, w[3]);
+      const bool here = !F::kPaired || (lane >= 16) == (z == 1);  // the granule's columns
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {  // columns 0-3, then 4-7 of the word, of a pair of keys each
-        uint32_t x0 = __byte_perm(w[0][y], w[1][y], half ? 0x7632 : 0x5410), x1 = __byte_perm(w[2][y], w[3][y], half ? 0x7632 : 0x5410);
+      for (int y = 0; y < GR; ++y) {
+        uint32_t b[NT][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t a[4] = {x0 & M0, x0 & M1, ~x1 & M0, ~x1 & M1};
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_16816<__half>(o[n][y][2 * half + i], a, pb[n][y][0], pb[n][y][1]);
-            if (F::kTwoParts) mma_16816<__half>(o[n][y][2 * half + i], a, pl[n][y][0], pl[n][y][1]);
+          for (int r = 0; r < 2; ++r) b[n][r] = here ? pb[n][y][r] : 0u;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // columns 0-3, then 4-7 of the word, of a pair of keys each
+          uint32_t x0 = __byte_perm(w[0][y], w[1][y], half ? 0x7632 : 0x5410), x1 = __byte_perm(w[2][y], w[3][y], half ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t a[4] = {x0 & M0, x0 & M1, ~x1 & M0, ~x1 & M1};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_16816<__half>(o[n][y][2 * half + i], a, b[n][0], b[n][1]);
+              if (F::kTwoParts) mma_16816<__half>(o[n][y][2 * half + i], a, pl[n][y][0], pl[n][y][1]);
+            }
+            x0 >>= 8;
+            x1 >>= 8;
           }
-          x0 >>= 8;
-          x1 >>= 8;
         }
       }
     }
@@ -702,31 +735,41 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
       }
       cp_async_commit();  // (a group for every granule, empty ones past the end)
     };
+    constexpr int kAhead = F::kStages - F::kStep;  // granules in flight beside those at hand
 #pragma unroll 1
-    for (int k = 0; k < F::kStages - 1; ++k) issue(k);
+    for (int k = 0; k < kAhead; ++k) issue(k);
     Acc<F> acc;
     acc.begin(queries, a.scale_log2, lane);
 #pragma unroll 1
-    for (int k = 0; k < mine; ++k) {
-      issue(k + F::kStages - 1);
-      cp_async_wait<F::kStages - 1>();
+    for (int k = 0; k < mine; k += F::kStep) {
+#pragma unroll
+      for (int i = 0; i < F::kStep; ++i) issue(k + kAhead + i);
+      cp_async_wait<kAhead>();
       __syncwarp();
-      const int pos = (s.g0 + warp + k * kWarps) * kGran;
-      const uint32_t tile = ring + (k % F::kStages) * F::kBlock;
-      const bool edge = pos < s.lo || pos + kGran > s.hi;
-      if (owns_new && k == mine - 1) {
+      int pos = (s.g0 + warp + k * kWarps) * kGran;
+      bool edge = pos < s.lo || pos + kGran > s.hi;
+      const uint32_t tile = ring + (k % F::kStages) * F::kBlock, second = tile + F::kBlock;
+      if (F::kPaired) {
+        // without a second granule the slot's scores are those of keys behind all others
+        const bool two = k + 1 < mine;
+        const int other = two ? pos + kWarps * kGran : INT_MAX - 2 * kGran;
+        edge = edge || !two || other + kGran > s.hi;
+        pos = lane & 2 ? other : pos;
+      }
+      if (owns_new && k + F::kStep >= mine) {
+        const uint32_t slot = F::kPaired && k + 1 < mine ? second : tile;
 #pragma unroll
         for (int i = 0; i < kNew; ++i) {
           int word, pair;
           if (new_at(i, word, pair)) {
-            sts32(tile + word, new_word[i]);
-            if (pair >= 0) sts32(tile + pair, new_pair[i]);
+            sts32(slot + word, new_word[i]);
+            if (pair >= 0) sts32(slot + pair, new_pair[i]);
           }
         }
         __syncwarp();
       }
-      acc.granule(tile, pos, edge, s.lo, s.hi, lane);
-      __syncwarp();  // the slot has been read
+      acc.granule(tile, second, pos, edge, s.lo, s.hi, lane);
+      __syncwarp();  // the slots have been read
     }
     acc.finish();
 
@@ -739,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r = 8 * n + 2 * t + x;
-        if (r >= s.rows) continue;
+        if ((F::kPaired ? r & 3 : r) >= s.rows) continue;
         if (g == 0) ml[warp * F::kHeads + r] = make_float2(acc.ref[n][x], acc.l[n][x]);
         float* dst = reinterpret_cast<float*>(sm + warp * F::kRing) + r * F::kPitch;
 #pragma unroll
@@ -755,13 +798,14 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
       const int r = it / (DH / 4), c = it % (DH / 4) * 4;
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w * F::kHeads + r].x);
+      for (int w = 0; w < F::kStep * kWarps; ++w) M = fmaxf(M, ml[w / F::kStep * F::kHeads + r + w % F::kStep * 4].x);
       const float base = M == -INFINITY ? 0.f : M;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float2 x = ml[w * F::kHeads + r];
-        const float4 y = *reinterpret_cast<const float4*>(sm + w * F::kRing + 4 * (r * F::kPitch + c));
+      for (int w = 0; w < F::kStep * kWarps; ++w) {  // (paired: rows r and r + 4 of each warp)
+        const int at = w / F::kStep, row = r + w % F::kStep * 4;
+        const float2 x = ml[at * F::kHeads + row];
+        const float4 y = *reinterpret_cast<const float4*>(sm + at * F::kRing + 4 * (row * F::kPitch + c));
         const float p = x.y * ex2_approx(x.x - base);
         L += p;
         v.x = fmaf(y.x, p, v.x);
@@ -996,7 +1040,7 @@ int launch_paged_decode_int4(const bna_tensor4* q, bna_tensor4* pool, const bna_
     if (dtype == BNA_BF16) {
       if constexpr (DH < 256)
         if (rows > 8) return launch<Form<__nv_bfloat16, DH, 16>>(a, s);
-      return launch<Form<__nv_bfloat16, DH, 8>>(a, s);
+      return rows > 4 ? launch<Form<__nv_bfloat16, DH, 8>>(a, s) : launch<Form<__nv_bfloat16, DH, 4>>(a, s);
     }
     if constexpr (DH < 256)
       if (rows > 8) return launch<Form<__half, DH, 16>>(a, s);
