@@ -308,6 +308,18 @@ def test_pairs_cut_between_ctas(lens, Hq, Hkv, dh):
     assert all(torch.equal(a, b) for a, b in zip(first, c.run()))  # equal calls, equal bits
 
 
+@pytest.mark.parametrize("G", [1, 3, 4])
+@pytest.mark.parametrize("dh", [64, 128, 256])
+def test_granules_without_a_second_one(G, dh):
+    """Up to 4 heads take a warp's granules two at a time: odd and even numbers of them, in whole and cut pairs, of
+    windows that begin in either one, with the new row in either one."""
+    lens = [128 * i + d for i in (0, 1, 2, 3, 7) for d in (1, 16, 17, 33, 127, 128)]
+    for case, window in ((lens, 0), (lens, 150), ([20011, 9001, 4999], 0), ([33333], 0), ([33333], 7001)):
+        for step in (False, True):
+            c = Case(case, 2 * G, 2, dh=dh, step=step, seed=G + dh)
+            c.check(c.run(window=window), window=window)
+
+
 def test_lengths_around_a_cut():
     """One pair just below and above the lengths at which it is cut, and where cuts move to its ends."""
     for ln in list(range(16 * 79, 16 * 84, 16)) + [16 * 127 + 1, 16 * 128, 16 * 161, 16 * 200]:
