@@ -9,6 +9,7 @@
 // largest of their largest entries is a bound that at least k entries reach.  A thread keeps in mind which vector
 // holds its largest entry and reads that one again (from L2), and the few threads whose second-best vector reaches
 // the bound too have all their entries looked at, by all lanes of their warp.
+// Many short rows take a warp each (logprob_short_kernel).
 // A row is shared by a cluster of CTAs where there are few rows; the CTAs' sums and lists are joined
 // through distributed shared memory by the cluster's first one.
 //
@@ -301,6 +302,13 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
     auto key_at = [&](int v, int j) { return key_of(best, (uint32_t)max((int64_t)0, v * (int64_t)E + j - row.shift)); };
     const uint64_t most = any ? key_at(best_v, 0) : 0, least = any ? key_at(best_v, E - 1) : 0;
     uint64_t g = least;
+    if (v1 - v0 < kThreads) {
+      // Of threads side by side whole groups would have no vector, and with fewer groups than k all entries would
+      // count: threads 64 apart instead (1,000 entries, 20 alternatives: 40 -> 4.6 us).
+      list[tid] = least;
+      __syncthreads();
+      g = list[tid / (kThreads / kTop) + kTop * (tid % (kThreads / kTop))];
+    }
 #pragma unroll
     for (int o = kThreads / kTop / 2; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
     if (lane % (kThreads / kTop) == 0) group[tid / (kThreads / kTop)] = g;
@@ -428,9 +436,177 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
   }
 }
 
+// Rows of up to kShort entries, a warp to each, held in registers: the sums around the row's maximum, then the rank of the k-th
+// largest entry by bisection (a count over the warp each), the entries above it and the first of those that equal it.  65,536 rows of 1,000 in
+// bf16: 82 us without alternatives, 245 with 5, 348 with 64 (131 MB: 20 us of a copy), bound by instructions.
+constexpr int kShort = 1024, kShortWarps = 4;
+template <typename T>
+__global__ void __launch_bounds__(32 * kShortWarps) logprob_short_kernel(const LogprobArgs a, int rows) {
+  constexpr int E = Row<T>::E, N = kShort / 32 / E;
+  // ranks without the bits that no entry of the type sets
+  constexpr int kDrop = std::is_same<T, __nv_bfloat16>::value ? 16 : std::is_same<T, __half>::value ? 13 : 0;
+  __shared__ uint64_t picks[kShortWarps][kTop];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t r64 = (int64_t)blockIdx.x * kShortWarps + warp;
+  if (r64 >= rows) return;
+  const int r = (int)r64, outer = r / a.inner;
+  const Row<T> row(a.x + (outer * a.ld_outer + (r - outer * a.inner) * a.ld) * (int64_t)sizeof(T), a.V);
+  const int nv = row.vectors();  // (32 N at most)
+  int64_t token = -1;
+  if (a.tokens) token = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[r] : static_cast<const int32_t*>(a.tokens)[r];
+  float f[N][E];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int v = lane + 32 * i;
+    if (v < nv) {
+      Row<T>::unpack(row.load(v), f[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) f[i][j] = -INFINITY;
+    }
+  }
+  const float picked = token >= 0 && token < a.V ? row.at(token) : -INFINITY;
+  float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < E; ++j) M = fmaxf(M, f[i][j]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float base = M == -INFINITY ? 0.f : M;
+  Two z2 = two(0.f, 0.f), w2 = two(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (32 * i >= nv) break;
+#pragma unroll
+    for (int j = 0; j < E; j += 2) {
+      const float d0 = max_nan(f[i][j] - base, kFloor), d1 = max_nan(f[i][j + 1] - base, kFloor);
+      const Two e = two(ex2_approx(d0 * kLog2e), ex2_approx(d1 * kLog2e));
+      z2 = add2(z2, e);
+      w2 = fma2(two(d0, d1), e, w2);
+    }
+  }
+  const float2 za = apart(z2), wa = apart(w2);
+  const float z = warp_sum(za.x + za.y), w = warp_sum(wa.x + wa.y);
+  const bool none = z == 0.f;  // (a row of masked entries only)
+  const float log_z = none ? 0.f : logf(z);
+  if (none) base = 0.f;
+  if (lane == 0) {
+    if (a.logprob) a.logprob[r] = token < 0 ? 0.f : (picked - base) - log_z;
+    const float h = none ? 0.f : log_z - w / z;
+    a.entropy[r] = h < 0.f ? 0.f : h;  // (a rounding below 0)
+  }
+  if (a.k == 0) return;
+
+  // ranks, 0 beside the row (any entry's is above that); the smallest of the largest of 32 or 64 groups is reached
+  // by k entries
+  uint32_t u[N][E], lo = 0, hi = 0, least = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = (lane + 32 * i) * E - row.shift;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      u[i][j] = at + j >= 0 && at + j < a.V ? rank_of(f[i][j]) >> kDrop : 0u;
+      lo = max(lo, u[i][j]);
+    }
+    if (i % (N / 2) == N / 2 - 1) {
+      least = a.k > 32 ? min(least, lo) : max(hi, lo);
+      hi = max(hi, lo);
+      lo = 0;
+    }
+  }
+  lo = __reduce_min_sync(0xffffffffu, least);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  auto reach = [&](uint32_t x) {  // entries that reach x
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (32 * i < nv) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) n += u[i][j] >= x;
+      }
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  int n = -1;  // of those that reach lo, where it has been counted
+  while (lo < hi && n != a.k) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    const int c = reach(mid);
+    if (c >= a.k) {
+      lo = mid;
+      n = c;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  if (n < 0) n = reach(lo);
+  // the k entries into the list: with ties too many first those above, then the ties in the order of their indices
+  int count = 0;
+  auto append = [&](bool ties, bool above) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (32 * i >= nv) break;
+      int mine = 0;
+#pragma unroll
+      for (int j = 0; j < E; ++j) mine += (above && u[i][j] > lo) || (ties && u[i][j] == lo);
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+      }
+      int to = count + incl - mine;
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if ((above && u[i][j] > lo) || (ties && u[i][j] == lo)) {
+          if (to < a.k) picks[warp][to] = key_of(f[i][j], (uint32_t)((lane + 32 * i) * E + j - row.shift));
+          ++to;
+        }
+      count += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  };
+  if (n == a.k) {
+    append(true, true);
+  } else {
+    append(false, true);
+    append(true, false);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int x = 0; x < kTop; x += 32) {
+    if (x >= a.k) break;
+    const uint64_t key = x + lane < a.k ? picks[warp][x + lane] : 0;
+    int above = 0;
+    for (int i = 0; i < a.k; ++i) above += picks[warp][i] > key;
+    if (x + lane < a.k) {
+      a.top_ids[(int64_t)r * a.k + above] = (int64_t)(uint32_t)~(uint32_t)key;
+      a.top_lp[(int64_t)r * a.k + above] = (value_of((uint32_t)(key >> 32)) - base) - log_z;
+    }
+  }
+}
+
 template <typename T>
 int launch(const LogprobArgs& a, int64_t rows, cudaStream_t s) {
+  if (rows > INT_MAX) return fail(BNA_UNSUPPORTED, "token_logprobs: too many rows");
   const int64_t vectors = ((int64_t)a.V + Row<T>::E - 1) / Row<T>::E;
+  constexpr int kWave = 3 * 148;  // rows that the CTAs of the other form hold at once
+  // Short rows (one that begins inside a vector has E - 1 places before it at most) to a warp each where there are more of them than
+  // CTAs at once, or alternatives for most of the groups, or groups without a vector; else the CTAs' latency is the shorter one.  A warp /
+  // a CTA each, rows of 1,000: 65,536 with 64 alternatives 348 us / 15 ms, 444 with 64 12 / 28 us, 444 with 5 8.6 / 6.8, one in fp32
+  // with 20 6.6 / 4.2.
+  if (a.V <= kShort - (Row<T>::E - 1) && (rows > kWave || vectors < kTop || a.k > kTop / 2)) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((rows + kShortWarps - 1) / kShortWarps));
+    cfg.blockDim = dim3(32 * kShortWarps);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, logprob_short_kernel<T>, a, (int)rows), "token_logprobs launch");
+  }
   // A row to several CTAs as long as there is an SM for each and eight vectors a thread to share: 20 alternatives of one row of
   // 151,936 take 7.8 us with eight CTAs and 12.6 with one, of 40 rows 10.4 with two each and 13.3; 64 rows of 32,000 take
   // 6.5 us with one CTA each and 7.5 with two.

@@ -286,3 +286,50 @@ def test_under_grad_and_inference_mode():
     with torch.inference_mode():
         i = bb.token_logprobs(x.detach(), _tokens(x), top_k=3)
     assert torch.equal(r.logprobs, i.logprobs) and torch.equal(r.top_ids, i.top_ids)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,k", [(1, 1), (2, 2), (31, 31), (32, 32), (33, 33), (64, 64), (65, 64), (257, 50), (513, 33), (1016, 20), (1017, 64), (1018, 64),
+                                 (1021, 1), (1022, 5), (1024, 64), (1030, 64)])
+def test_short_rows(V, k, dtype):
+    """Rows that a warp holds, up to where they end being short, that begin at every place of a 16-byte vector."""
+    for offset in range(0, 8, 3 if V > 100 else 1):
+        x = _rand(37, V, dtype=dtype, seed=V + offset, pad=5, offset=offset)
+        check(x, _tokens(x), k=k)
+    x = _rand(4099, V, dtype=dtype, seed=V)
+    check(x, _tokens(x, dtype=torch.int32), k=min(k, 7))
+    check(x[:, :], None, k=0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_short_rows_with_ties_and_masks(dtype):
+    t = TYPES[dtype]
+    for V in (40, 64, 200, 1000):
+        k = min(V, 64)
+        x = _rand(24, V, dtype=dtype, seed=V)
+        x[0] = 1.5                                            # all equal
+        x[1] = torch.arange(V, device=DEV).to(t)              # ascending
+        x[2] = -torch.arange(V, device=DEV).to(t)             # descending
+        x[3] = (torch.arange(V, device=DEV) % 3).to(t)        # three values
+        x[4, 1::2] = -math.inf                                # masks by either kind of lowest value
+        x[5, 3:] = -math.inf
+        x[6, ::2] = torch.finfo(t).min
+        x[7, :-1] = torch.finfo(t).min
+        x[8] = 0.0
+        x[8, ::2] = -0.0                                      # zeros of both signs are equal
+        x[9, V // 2] = torch.finfo(t).max / 4
+        x[10] = torch.finfo(t).tiny * (torch.arange(V, device=DEV) % 5).to(t)
+        check(x, _tokens(x), k=k)
+    y = _rand(6, 100, dtype=dtype, seed=5)
+    y[0] = -math.inf
+    y[1, 7] = math.nan
+    y[2, 9] = math.inf
+    y[3] = math.nan
+    r = bb.token_logprobs(y, _tokens(y), top_k=30)
+    assert r.logprobs[0] == -math.inf and r.entropy[0] == 0 and (r.top_logprobs[0] == -math.inf).all()
+    assert torch.equal(r.top_ids[0], torch.arange(30, device=DEV)) and torch.equal(r.top_ids[3], r.top_ids[0])
+    assert r.logprobs[1:4].isnan().all() and r.entropy[1:4].isnan().all() and r.top_logprobs[1:4].isnan().all()
+    assert r.top_ids[2, 0] == 9 and not (r.top_ids[1] == 7).any()
+    check(y[4:], _tokens(y[4:]), k=30)
+    assert all(torch.equal(a, b) for a, b in zip((z[4:] for z in bb.token_logprobs(y, _tokens(y), top_k=30)[1:]),
+                                                 (z[4:] for z in r[1:])))
