@@ -33,6 +33,7 @@ using namespace sm100;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kTop = 64;      // alternatives at most, and groups of threads
 constexpr int kList = 4096;   // entries that reach the bound, as long as they fit
+constexpr int kFew = 512;     // of more candidates than this, those that a second bound leaves are ranked
 constexpr int kMaxCluster = 8;
 constexpr float kSlack = 8.f;  // e^kSlack times the row's length stays far below the fp32 range
 constexpr float kLog2e = 1.4426950408889634f;
@@ -183,7 +184,9 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
   __shared__ uint64_t list[kList];
   __shared__ uint64_t group[kTop], top[kTop];
   __shared__ float sums[3][kWarps];  // ref, Z, W of the warps, then of the CTA in column 0
-  __shared__ uint64_t bound;
+  __shared__ uint64_t few[kFew];
+  __shared__ uint64_t bound, few_bound;
+  __shared__ int few_count;
   __shared__ int owners[kThreads];
   __shared__ uint64_t all_top[kMaxCluster * kTop];  // of the cluster's CTAs, in the first one
   __shared__ float all_sums[3][kMaxCluster];
@@ -302,32 +305,37 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
     auto key_at = [&](int v, int j) { return key_of(best, (uint32_t)max((int64_t)0, v * (int64_t)E + j - row.shift)); };
     const uint64_t most = any ? key_at(best_v, 0) : 0, least = any ? key_at(best_v, E - 1) : 0;
     uint64_t g = least;
-    if (v1 - v0 < kThreads) {
+    if (v1 - v0 < kThreads || a.k > 16) {
       // Of threads side by side whole groups would have no vector, and with fewer groups than k all entries would
-      // count: threads 64 apart instead (1,000 entries, 20 alternatives: 40 -> 4.6 us).
+      // count; and in a masked end the k-th group's bound would be 64 k entries into it.  Threads 64 apart instead, for one more
+      // barrier (1,000 entries, 20 alternatives: 40 -> 4.6 us; five rows of 151,936, a seventh masked, 64 alternatives 558 -> 30).
       list[tid] = least;
       __syncthreads();
       g = list[tid / (kThreads / kTop) + kTop * (tid % (kThreads / kTop))];
     }
+    constexpr int kShare = kThreads / kTop;  // threads of a group, and threads that count the groups above one
+    auto leave = [&](uint64_t x) {  // the group's largest
 #pragma unroll
-    for (int o = kThreads / kTop / 2; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if (lane % (kThreads / kTop) == 0) group[tid / (kThreads / kTop)] = g;
-    if (tid == 0) {
-      bound = 0;  // fewer than k threads have entries: all entries count
-      count = 0;
-    }
-    if (tid < kTop) top[tid] = 0;
-    __syncthreads();
-    constexpr int kShare = kThreads / kTop;  // threads that count the groups above one
-    {
+      for (int o = kShare / 2; o > 0; o >>= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+      if (lane % kShare == 0) group[tid / kShare] = x;
+    };
+    auto kth = [&](uint64_t& to) {  // the k-th largest of the groups', if so many have one
       const uint64_t mine = group[tid / kShare];
       int above = 0;
 #pragma unroll
       for (int i = 0; i < kTop / kShare; ++i) above += group[i * kShare + tid % kShare] > mine;
 #pragma unroll
       for (int o = 1; o < kShare; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-      if (tid % kShare == 0 && mine != 0 && above == a.k - 1) bound = mine;
+      if (tid % kShare == 0 && mine != 0 && above == a.k - 1) to = mine;
+    };
+    leave(g);
+    if (tid == 0) {
+      bound = 0;  // fewer than k threads have entries: all entries count
+      count = 0;
     }
+    if (tid < kTop) top[tid] = 0;
+    __syncthreads();
+    kth(bound);
     if (warp == kWarps - 1) join_warps();
     __syncthreads();
     // Entries that reach the bound.  If they do not fit, the k-th largest of those that did is a higher
@@ -370,10 +378,33 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
       __syncthreads();
       n = min(count, kList);
       const bool fits = count <= kList;
+      // Ranking takes n^2 steps; where masks left many groups without another entry n is large, and the k-th largest of 64
+      // groups of candidates is a higher bound (2,939 rows of 4,233, 604 of them masked, 64 alternatives: 10.7 -> 0.12 ms).
+      const uint64_t* from = list;
+      if (n > kFew) {
+        uint64_t x = 0;
+        // (places 64 apart: the list is partly in order, and then the first k places are those of k groups)
+        for (int c = tid / kShare + kTop * (tid % kShare); c < n; c += kThreads) x = max(x, list[c]);
+        leave(x);
+        if (tid == 0) few_count = 0;
+        __syncthreads();
+        kth(few_bound);
+        __syncthreads();
+        for (int c = tid; c < n; c += kThreads)
+          if (list[c] >= few_bound) {
+            const int at = atomicAdd(&few_count, 1);
+            if (at < kFew) few[at] = list[c];
+          }
+        __syncthreads();
+        if (few_count <= kFew) {
+          from = few;
+          n = few_count;
+        }
+      }
       for (int c0 = 0; c0 < n; c0 += kThreads / 8) {
         const int c = c0 + tid / 8;
-        const uint64_t key = c < n ? list[c] : 0;
-        const int above = rank_in(list, n, key, lane);
+        const uint64_t key = c < n ? from[c] : 0;
+        const int above = rank_in(from, n, key, lane);
         if (c < n && (lane & 7) == 0 && above < a.k) top[above] = key;
       }
       __syncthreads();

@@ -333,3 +333,28 @@ def test_short_rows_with_ties_and_masks(dtype):
     check(y[4:], _tokens(y[4:]), k=30)
     assert all(torch.equal(a, b) for a, b in zip((z[4:] for z in bb.token_logprobs(y, _tokens(y), top_k=30)[1:]),
                                                  (z[4:] for z in r[1:])))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,R", [(1100, 500), (4233, 37), (5000, 3), (30011, 2), (151936, 3), (151936, 200)])
+def test_many_entries_that_reach_the_bound(V, R, dtype):
+    """Long masked ends, rows in order and rows of few values: whole groups of threads with nothing large, so that far
+    more entries than are asked for reach the first bound."""
+    t = TYPES[dtype]
+    x = _rand(R, V, dtype=dtype, seed=V)
+    x[:, V - V // 7:] = -math.inf
+    x[0, : V // 3] = torch.finfo(t).min
+    x[1] = torch.linspace(-50, 50, V, device=DEV).to(t)
+    x[-1] = torch.linspace(9, -9, V, device=DEV).to(t)
+    if R > 3:
+        x[2, 20:] = -math.inf
+        x[3] = 0.25
+        x[4] = (torch.arange(V, device=DEV) % 7).to(t)
+        x[5, : V - 70] = -math.inf
+    for k in (64, 33, 5):
+        tokens = _tokens(x)
+        r = bb.token_logprobs(x, tokens, top_k=k)
+        some = (x > -math.inf).any(-1)  # (a plain log softmax has no value for a row of masks alone)
+        check(x[some], tokens[some], k=k, got=type(r)(*(y[some] for y in r)))
+        assert (r.logprobs[~some] == -math.inf).all() and (r.entropy[~some] == 0).all() and (r.top_logprobs[~some] == -math.inf).all()
+        assert (r.top_ids[~some] == torch.arange(k, device=DEV)).all()
