@@ -10,7 +10,7 @@
 // c masked in place in a 16-bit half of a code word is the fp16 subnormal 2^-24 c, or 2^-20 c for the
 // odd code beside it, so a code word becomes four operand registers with five integer instructions and
 // no conversion.  q is scaled by a power of two into the fp16 range (by head; exact but for entries 2^-24 of
-// the head's largest), and 2^-4 of that meets the odd codes; p sv is held in fp16 around its largest.
+// the head's largest), and 2^-4 of that meets the odd codes.
 //
 // Bytes: 18 dh / 16 a token and head.  A read serves up to 8 query heads (16 at head_dim 64 and 128 with more than 8).
 //
@@ -21,12 +21,14 @@
 //
 // Warp-level matrix instructions, as their operand is made in registers: the fifth-generation ones read it from shared
 // or tensor memory, where the unpacked codes would be four times the bytes that came, written and read once more.
+// p sv is held in fp16 in a unit of its head and column group, in which the largest product so far is 2^(kLeast - 1) or more: what
+// falls below fp16's 2^-24 is lost against the group's own sum.
 // Half of the keys enter P V as 15 - c with scale -s and minimum m + 15 s, so that what the tensor core cuts off its
 // sums cancels.
 //
-// Measured: 64 requests of 65,536 tokens, 8 / 2 heads of 128, bf16: 209 us for 1.21 GB, 5.8 TB/s (0.88 of a copy; the 16-bit
-// kernel takes 610 us for its 4.3 GB).  Bound by the instructions of a granule as much as by HBM.  One request of
-// 131,072 tokens: 19 us, some 4 of them before the first keys and 4 in the join.  4 requests of 37 to 513 tokens: 10 us, latency.
+// Measured (in a CUDA graph): 64 requests of 65,536 tokens, 8 / 2 heads of 128, bf16: 215 us for 1.21 GB, 5.6 TB/s (0.86 of a copy; the
+// 16-bit kernel takes 610 us for its 4.3 GB; one unit for all groups and heads, which lost small ones, 211 us).  Bound by the instructions of a
+// granule as much as by HBM.  One request of 131,072 tokens: 18.3 us, some 4 of them before the first keys and 4 in the join.  4 requests of 37 to 513 tokens: 10 us, latency.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -60,6 +62,9 @@ constexpr int kMinShare = 32;
 constexpr int kKeepLens = 1024;  // lengths kept in shared memory
 constexpr int kShift = 11;  // probabilities are held times 2^kShift, and so are l and o; the divisions undo it
 constexpr float kMove = 4.f;  // a reference moves when a score lies more than 2^kMove above it
+// A new unit of products is 2^kRoom times the largest scale or more, so that ones up to 2^(kRoom - 1) times as large need no other,
+// but leaves the largest product at 2^kLeast or more, however large the scales of keys without weight are.
+constexpr int kRoom = 3, kLeast = 3;
 constexpr float kNone = -1e30f;  // the offset of a reference that has seen no key
 
 struct Int4Args {
@@ -148,7 +153,9 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+constexpr int kMaxExp = 126;
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }  // of x >= 0 (0: -127)
 __device__ __forceinline__ float lane_max(float x) {  // over the lanes with the same lane % 4
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
@@ -223,8 +230,11 @@ struct Acc {
   float f[NT][2];                // from those to scores in the exp2 domain
   float ref[NT][2], off[NT][2];  // running reference (no score lies 2^kMove above it), and it less kShift
   float l[NT][2], wm[NT][GR][2];  // this lane's keys: sum p, sum p mv_y
-  float o[NT][GR][4][4];          // sum p sv cv, in units of 2^-24 (odd columns 2^-20) 2^e
-  float bound, inv;               // 2^e, above every value scale so far, and 2^-e
+  float o[NT][GR][4][4];          // sum p sv cv, in units of 2^-24 (odd columns 2^-20) 2^k
+  // 2^-k of each head and group.  The unit follows the group's largest product p sv, also down as the reference moves, so that what is
+  // lost below fp16's range is lost against the column's own sum, whatever scales other groups, keys without
+  // weight or other heads have.
+  float inv[NT][GR][2];
 
   // This lane's part of the queries.  q: the head group's first row; rows from `rows` on count as zeros
   struct Queries {
@@ -296,6 +306,7 @@ struct Acc {
         for (int y = 0; y < GR; ++y) {
           qs[n][y][x] = __shfl_sync(0xffffffffu, sums[y], src);
           wm[n][y][x] = 0.f;
+          inv[n][y][x] = pow2(kMaxExp);
         }
         ref[n][x] = -INFINITY;
         off[n][x] = kNone;
@@ -308,8 +319,6 @@ struct Acc {
 #pragma unroll
           for (int x = 0; x < 4; ++x) o[n][y][i][x] = 0.f;
     }
-    bound = pow2(-100);
-    inv = pow2(100);
   }
 
   // A granule in shared memory, its first key at `pos`; with `edge` keys outside [lo, hi) are masked.  Paired: also the
@@ -395,54 +404,81 @@ struct Acc {
         }
       }
     }
-    // probabilities times 2^kShift
-    float e[NT][4], top = fmaxf(sv[0][0], sv[1][0]), most = -INFINITY;
-#pragma unroll
-    for (int y = 1; y < GR; ++y) top = fmax3(top, sv[0][y], sv[1][y]);
+    // probabilities times 2^kShift, and their products with the scales, in the units held
+    float e[NT][4], w[NT][GR][4], most = -INFINITY, top = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int y = 0; y < GR; ++y) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float2 v = apart(mul2(two(sv[r][y], sv[r][y]), two(inv[n][y][0], inv[n][y][1])));
+          w[n][y][2 * r] = v.x;
+          w[n][y][2 * r + 1] = v.y;
+        }
+        top = fmax3(fmax3(top, w[n][y][0], w[n][y][1]), w[n][y][2], w[n][y][3]);
+      }
 #pragma unroll
       for (int x = 0; x < 4; ++x) e[n][x] = fmaf(f[n][x & 1], u[n][x], -off[n][x & 1]);
       most = fmax3(most, fmaxf(e[n][0], e[n][1]), fmaxf(e[n][2], e[n][3]));
     }
-    if (__any_sync(0xffffffffu, top >= bound || most > kShift + kMove)) {
-      float scale = 1.f;
-      top = lane_max(top);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (top >= bound) {
-        const int x = min((int)(__float_as_uint(top) >> 23) - 127 + 3, 126);  // room for scales up to four times as large
-        scale = bound * pow2(-x);
-        bound = pow2(x);
-        inv = pow2(-x);
-      }
+    // without a move no product is above 2^(kShift + kMove) = 2^15
+    const bool move = __any_sync(0xffffffffu, top > 1.f || most > kShift + kMove);
+    if (move) {
+      int high[GR];  // of the largest scale
+#pragma unroll
+      for (int y = 0; y < GR; ++y) high[y] = exponent(lane_max(fmaxf(sv[0][y], sv[1][y])));
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float mx = fmaxf(ref[n][x], lane_max(fmaxf(f[n][x] * u[n][x], f[n][x] * u[n][2 + x])));
-          const float to = mx == -INFINITY ? kNone : mx - (float)kShift, al = ex2_approx(off[n][x] - to);
+          const float s0 = f[n][x] * u[n][x], s1 = f[n][x] * u[n][2 + x], mx = fmaxf(ref[n][x], lane_max(fmaxf(s0, s1)));
+          const float to = mx == -INFINITY ? kNone : mx - (float)kShift, by = off[n][x] - to, al = ex2_approx(by);
+          // (differences of whole parts: many small moves take the unit as far as one large one)
+          const int less = (int)fmaxf(floorf(off[n][x]) - floorf(to), -4.f * kMaxExp);
           ref[n][x] = mx;
           off[n][x] = to;
           l[n][x] *= al;
+          e[n][x] = ex2_approx(fmaf(f[n][x], u[n][x], -to));
+          e[n][2 + x] = ex2_approx(fmaf(f[n][x], u[n][2 + x], -to));
 #pragma unroll
           for (int y = 0; y < GR; ++y) {
             wm[n][y][x] *= al;
+            // the largest product's exponent, or one less
+            const float largest = lane_max(fmaxf(s0 + (float)exponent(sv[0][y]), s1 + (float)exponent(sv[1][y]))) - to;
+            const int old = -exponent(inv[n][y][x]);
+            const int k = min(max(max(old + less, min(high[y] + kRoom, (int)floorf(fmaxf(largest, -4.f * kMaxExp)) - kLeast)), -kMaxExp), kMaxExp);
+            const float scale = ex2_approx(by + (float)(old - k));
+            inv[n][y][x] = pow2(-k);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              o[n][y][i][x] *= al * scale;
-              o[n][y][i][2 + x] *= al * scale;
+              o[n][y][i][x] *= scale;
+              o[n][y][i][2 + x] *= scale;
             }
+            // (in this order: a scale by 2^-k might overflow under a probability of 0)
+            w[n][y][x] = e[n][x] * sv[0][y] * inv[n][y][x];
+            w[n][y][2 + x] = e[n][2 + x] * sv[1][y] * inv[n][y][x];
           }
-          e[n][x] = fmaf(f[n][x], u[n][x], -to);
-          e[n][2 + x] = fmaf(f[n][x], u[n][2 + x], -to);
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float(&p)[4] = e[n];
+          p[2 * r] = ex2_approx(p[2 * r]);
+          p[2 * r + 1] = ex2_approx(p[2 * r + 1]);
+#pragma unroll
+          for (int y = 0; y < GR; ++y) {
+            const float2 v = apart(mul2(two(w[n][y][2 * r], w[n][y][2 * r + 1]), two(p[2 * r], p[2 * r + 1])));
+            w[n][y][2 * r] = v.x;
+            w[n][y][2 * r + 1] = v.y;
+          }
         }
     }
     uint32_t pb[NT][GR][2], pl[NT][GR][2];  // P^T sv fragments: high parts, and low ones for fp16 results
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x) e[n][x] = ex2_approx(e[n][x]);
 #pragma unroll
       for (int x = 0; x < 2; ++x) l[n][x] += e[n][x] + e[n][2 + x];
 #pragma unroll
@@ -451,7 +487,7 @@ struct Acc {
         for (int x = 0; x < 2; ++x) wm[n][y][x] = fmaf(e[n][x], mv[0][y], fmaf(e[n][2 + x], mv[1][y], wm[n][y][x]));
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float s = sv[r][y] * (r == 0 ? inv : -inv), w0 = e[n][2 * r] * s, w1 = e[n][2 * r + 1] * s;
+          const float w0 = r == 0 ? w[n][y][0] : -w[n][y][2], w1 = r == 0 ? w[n][y][1] : -w[n][y][3];
           uint32_t part = ElemTraits<__half>::pack2(w0, w1), low = 0;
           if (F::kTwoParts || F::kLowColumns) {
             const float2 h = ElemTraits<__half>::unpack2(part);
@@ -466,12 +502,12 @@ struct Acc {
     // outputs
 #pragma unroll
     for (int z = 0; z < F::kStep; ++z) {
-      uint32_t w[4][GR];
+      uint32_t c[4][GR];
       const uint32_t at = (z == 0 ? tile : second) + t * (DH / 2) + g * (4 * GR);
-      lds<9 * DH>(at, w[0]);
-      lds<9 * DH + 8 * (DH / 2)>(at, w[1]);
-      lds<9 * DH + 4 * (DH / 2)>(at, w[2]);
-      lds<9 * DH + 12 * (DH / 2)>(at, w[3]);
+      lds<9 * DH>(at, c[0]);
+      lds<9 * DH + 8 * (DH / 2)>(at, c[1]);
+      lds<9 * DH + 4 * (DH / 2)>(at, c[2]);
+      lds<9 * DH + 12 * (DH / 2)>(at, c[3]);
       const bool here = !F::kPaired || (lane >= 16) == (z == 1);  // the granule's columns
 #pragma unroll
       for (int y = 0; y < GR; ++y) {
@@ -482,7 +518,7 @@ struct Acc {
           for (int r = 0; r < 2; ++r) b[n][r] = here ? pb[n][y][r] : 0u;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {  // columns 0-3, then 4-7 of the word, of a pair of keys each
-          uint32_t x0 = __byte_perm(w[0][y], w[1][y], half ? 0x7632 : 0x5410), x1 = __byte_perm(w[2][y], w[3][y], half ? 0x7632 : 0x5410);
+          uint32_t x0 = __byte_perm(c[0][y], c[1][y], half ? 0x7632 : 0x5410), x1 = __byte_perm(c[2][y], c[3][y], half ? 0x7632 : 0x5410);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t a[4] = {x0 & M0, x0 & M1, ~x1 & M0, ~x1 & M1};
@@ -510,14 +546,15 @@ struct Acc {
 #pragma unroll
         for (int y = 0; y < GR; ++y) {
           const float m = lane_sum(wm[n][y][x]) * d;
+          const float unit = __uint_as_float((254u << 23) - __float_as_uint(inv[n][y][x]));  // 2^k
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (F::kLowColumns) {
               o[n][y][i][x] += __shfl_xor_sync(0xffffffffu, o[n][y][i][x], 2);
               o[n][y][i][2 + x] += __shfl_xor_sync(0xffffffffu, o[n][y][i][2 + x], 2);
             }
-            o[n][y][i][x] = fmaf(o[n][y][i][x] * (d * 0x1p24f), bound, m);
-            o[n][y][i][2 + x] = fmaf(o[n][y][i][2 + x] * (d * 0x1p20f), bound, m);
+            o[n][y][i][x] = fmaf(o[n][y][i][x] * (d * 0x1p24f), unit, m);
+            o[n][y][i][2 + x] = fmaf(o[n][y][i][2 + x] * (d * 0x1p20f), unit, m);
           }
         }
       }

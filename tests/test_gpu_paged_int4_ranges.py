@@ -1,0 +1,112 @@
+"""Attention over the 4-bit cache where scales, scores and lengths lie far apart.
+
+Compared with float64 arithmetic on the values s c + m, as in test_gpu_paged_int4.py, with the bar of each column taken from its
+own group y of 64 columns and its own head: with G_y = sum_j p_j (15 s_jy + |m_jy|), n keys, u the type's unit roundoff (2^-8 bf16,
+2^-11 fp16) and ds the score's error (there),
+  * sums of p (c s + m), or of p ((15 - c) (-s) + m + 15 s), have terms of 2 G_y at most, p off by a factor of 1 +- (2 ds + 2^-20)
+    and fp32 sums by n 2^-23: 2 G_y (2 ds + 2^-20 + n 2^-23);
+  * a product p s is rounded to fp16, 2^-11 of itself for bf16 results and (two parts) 2^-22 for fp16 ones, and 2^-25 at least in a unit
+    where the group's largest one is 2^2 or more: G_y (w + n 2^-27), w = 2^-11 or 2^-22;
+  * the result is rounded once: u |ref|.
+"""
+import math
+
+import pytest
+import torch
+
+from .test_gpu_paged_int4 import DEV, DTYPES, U, Case, pack, value
+
+pytestmark = pytest.mark.gpu
+W = {torch.bfloat16: 2.0 ** -11, torch.float16: 2.0 ** -22}
+
+
+def _check(c, got, window=0, scale=None):
+    out, lse = got
+    G, dh = c.Hq // c.Hkv, c.dh
+    scale = 1 / math.sqrt(dh) if scale is None else scale
+    for b, ln in enumerate(c.host):
+        first = max(0, ln - window) if window else 0
+        k, v = c.k[b][:, first:], c.v[b][:, first:]
+        n = k.shape[1]
+        q = c.q[b, :, 0].double().view(c.Hkv, G, dh)
+        z = scale * q @ value(k).transpose(1, 2)
+        p = torch.softmax(z, -1)
+        ref = p @ value(v)
+        _, s, m = pack(k)
+        S = scale * (q.abs() @ (15 * s.double() + m.double().abs()).repeat_interleave(64, -1).transpose(1, 2)).amax(-1, keepdim=True)
+        ds = (dh + 10) * 2 ** -23 * S
+        _, s, m = pack(v)
+        own = (p @ (15 * s.double() + m.double().abs())).repeat_interleave(64, -1)
+        bar = U[c.dtype] * ref.abs() + own * (4 * ds + 2 ** -19 + n * 2 ** -22 + W[c.dtype] + n * 2 ** -27)
+        o, ls = out[b, :, 0].double().view(c.Hkv, G, dh), lse[b, :, 0].double().view(c.Hkv, G)
+        assert ((o - ref).abs() <= bar).all(), (b, ln, float(((o - ref).abs() / bar).max()))
+        rl = torch.logsumexp(z, -1)
+        assert ((ls - rl).abs() <= ds[..., 0] + 2 ** -20 + n * 2 ** -23 + 2 ** -21 * rl.abs()).all(), (b, ln)
+
+
+def _normal(seed, dtype, dh, exponents):
+    """Normal rows, much alike (so that what keys lose does not cancel), times 2^exponents(key numbers [n, 1], column groups [1, groups])."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+
+    def rows(b, n):
+        x = torch.randn(2, 1, dh, generator=g, device=DEV) + 0.25 * torch.randn(2, n, dh, generator=g, device=DEV)
+        e = torch.as_tensor(exponents(torch.arange(n, device=DEV)[:, None], torch.arange(dh // 64, device=DEV)[None]), device=DEV)
+        return (x * torch.exp2(e.expand(n, dh // 64).double()).repeat_interleave(64, -1).float()).to(dtype)
+
+    return rows
+
+
+def _levels(dtype, dh, level):
+    """Keys of equal columns level(key numbers): a query of equal entries c scores c sqrt(dh) level."""
+    return lambda b, n: level(torch.arange(n, device=DEV).double())[None, :, None].expand(2, n, dh).to(dtype).contiguous()
+
+
+def _equal_queries(c, nats):
+    """Entries of each head h such that a key of level 1 scores nats[h % len]."""
+    x = torch.tensor([nats[h % len(nats)] / math.sqrt(c.dh) for h in range(c.Hq)], device=DEV)
+    c.q = x[None, :, None, None].expand_as(c.q).to(c.dtype).contiguous()
+
+
+@pytest.mark.parametrize("dtype,low,high", [(torch.bfloat16, 0, 20), (torch.bfloat16, 0, 24), (torch.bfloat16, -30, 0), (torch.bfloat16, 0, 90),
+                                            (torch.float16, -10, 12)])
+@pytest.mark.parametrize("dh,G", [(128, 2), (128, 8), (128, 16), (256, 4), (256, 7)])
+def test_one_group_far_above_another(dtype, low, high, dh, G):
+    for at in (0, 1):  # the group with large values
+        v = _normal(high, dtype, dh, lambda j, y: torch.where(y == at, high, low))
+        c = Case([40, 700, 5000], 2 * G, 2, dh=dh, dtype=dtype, v=v, seed=G)
+        _check(c, c.run())
+
+
+@pytest.mark.parametrize("dtype,low,high", [(torch.bfloat16, 0, 24), (torch.bfloat16, 0, 40), (torch.float16, -10, 12)])
+@pytest.mark.parametrize("dh,G", [(64, 3), (128, 4), (128, 5), (256, 2)])
+def test_large_values_without_weight(dtype, low, high, dh, G):
+    """One key 40 nats below the others, with values far above theirs: first, in the middle, last."""
+    for at in (0, 333, 1999):
+        v = _normal(at, dtype, dh, lambda j, y: torch.where(j == at, high, low))
+        k = _levels(dtype, dh, lambda j: -(j == at).double())
+        c = Case([2000], 2 * G, 2, dh=dh, dtype=dtype, k=k, v=v)
+        _equal_queries(c, [40.0])
+        _check(c, c.run())
+
+
+@pytest.mark.parametrize("dtype,low,high", [(torch.bfloat16, 0, 30), (torch.float16, -10, 12)])
+@pytest.mark.parametrize("dh,G", [(64, 4), (128, 2), (128, 6), (256, 8)])
+def test_heads_that_attend_to_different_keys(dtype, low, high, dh, G):
+    """Even heads see the keys with large values, odd ones those between them, 80 nats apart."""
+    v = _normal(1, dtype, dh, lambda j, y: torch.where(j % 2 == 0, high, low))
+    k = _levels(dtype, dh, lambda j: torch.where(j % 2 == 0, 1.0, -1.0))
+    c = Case([33, 3000], 2 * G, 2, dh=dh, dtype=dtype, k=k, v=v)
+    _equal_queries(c, [40.0, -40.0])
+    _check(c, c.run())
+
+
+@pytest.mark.parametrize("dtype,fall", [(torch.bfloat16, 30), (torch.bfloat16, 60), (torch.float16, 20)])
+@pytest.mark.parametrize("dh,G", [(64, 4), (128, 4), (128, 9), (256, 4)])
+def test_scores_that_rise_as_values_fall(dtype, fall, dh, G):
+    """References move often and by little, in some heads further than in others, while values lose `fall` bits."""
+    n = 4000
+    v = _normal(2, dtype, dh, lambda j, y: 10 - fall * j / n)
+    k = _levels(dtype, dh, lambda j: j / n)
+    c = Case([n], 2 * G, 2, dh=dh, dtype=dtype, k=k, v=v)
+    _equal_queries(c, [100.0, 20.0, 5.0, 50.0])
+    _check(c, c.run())
