@@ -787,9 +787,9 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) int4_decode_kernel(const _
       bool edge = pos < s.lo || pos + kGran > s.hi;
       const uint32_t tile = ring + (k % F::kStages) * F::kBlock, second = tile + F::kBlock;
       if (F::kPaired) {
-        // without a second granule the slot's scores are those of keys behind all others
+        // without a second granule the slot's scores are those of keys behind the last one
         const bool two = k + 1 < mine;
-        const int other = two ? pos + kWarps * kGran : INT_MAX - 2 * kGran;
+        const int other = two ? pos + kWarps * kGran : s.hi;
         edge = edge || !two || other + kGran > s.hi;
         pos = lane & 2 ? other : pos;
       }

@@ -110,3 +110,19 @@ def test_scores_that_rise_as_values_fall(dtype, fall, dh, G):
     c = Case([n], 2 * G, 2, dh=dh, dtype=dtype, k=k, v=v)
     _equal_queries(c, [100.0, 20.0, 5.0, 50.0])
     _check(c, c.run())
+
+
+@pytest.mark.parametrize("dh,Hq", [(64, 4), (128, 4), (128, 8)])
+def test_the_longest_table_rows(dh, Hq):
+    """Windows at the end of rows of 2^31 - 16 tokens, whose columns all name one page."""
+    page = 16 * 511  # 262,657 of them are 2^31 - 16
+    c = Case([page], Hq, 1, dh=dh, page=page, spare=0, seed=dh)
+    c.table = c.table[:, :1].expand(1, 262657).contiguous()
+    assert c.table.shape[1] * page == 2 ** 31 - 16
+    for ln in (2 ** 31 - 16, 2 ** 31 - 17, 2 ** 31 - 31, 2 ** 31 - 32, 2 ** 31 - 40):
+        for window in (1, 20, 130):
+            at = (torch.arange(ln - window, ln, device=DEV) % page)
+            d = Case([window], Hq, 1, dh=dh, page=16, k=lambda b, n: c.k[0][:, at], v=lambda b, n: c.v[0][:, at])
+            d.q, d.table, d.pool = c.q, c.table, c.pool
+            d.lens = torch.tensor([ln], dtype=torch.int32, device=DEV)
+            _check(d, d.run(window=window))
