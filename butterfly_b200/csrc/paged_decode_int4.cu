@@ -297,7 +297,8 @@ struct Acc {
         sums[y] += __shfl_xor_sync(0xffffffffu, sums[y], 2);
         sums[y] *= 0x1p-24f;
       }
-      const float down = pow2(min(24 - e, 124)) * scale_log2;
+      // (never 0, which would make a masked score of -inf a NaN: small queries, or none, under a small scale)
+      const float down = fmaxf(pow2(min(24 - e, 124)) * scale_log2, 0x1p-126f);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int src = 4 * (2 * t + x);

@@ -207,7 +207,7 @@ def paged_decode_attention_int4(q: torch.Tensor, kv_pages: torch.Tensor, block_t
     to 2^-34 of it; a probability times a value scale is rounded to 2^-11 (bf16) or 2^-22 (fp16) of itself and to 2^-27 of the largest such
     product of its head and group of columns.  ``k_new`` / ``v_new`` are packed as
     ``paged_append_int4`` would and attended to in that form.  A row that attends to a NaN is NaN.  Entries of
-    q from 2^114 on in magnitude count as infinite, values from 2^100 on may overflow."""
+    q from 2^114 (or 2^114 / scale) on in magnitude count as infinite, values from 2^100 on may overflow."""
     stream = _stream(q)
     r = (_native or _binding()).decode_int4(
         q, kv_pages, block_table, lens, k_new, v_new, active, window,

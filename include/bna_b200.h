@@ -428,7 +428,7 @@ BNA_API int bna_paged_read_int4(const bna_tensor4* kv_pages, const int64_t* slot
  * entries below 2^-24 of its head's largest, which are off by 2^-34 of that one at most; a product of a probability and a value scale
  * is rounded to 2^-11 (bf16) or 2^-22 (fp16 rows) of itself and to 2^-27 of the largest one of its head and column group.  k_new / v_new are packed as an
  * append would, written, and attended to in that form.  Rows that attend to a NaN are NaN; entries of q from 2^114 on in
- * magnitude count as infinite, and values from 2^100 on may overflow.  workspace: bna_paged_decode_int4_workspace_bytes() of device memory,
+ * magnitude, or from 2^114 / scale on, count as infinite, and values from 2^100 on may overflow.  workspace: bna_paged_decode_int4_workspace_bytes() of device memory,
  * 16-byte aligned; one of bna_paged_decode_workspace_bytes() serves both kinds of calls (its first 4096 bytes are
  * left alone here).  Calls that may overlap on the GPU need a workspace each. */
 BNA_API int64_t bna_paged_decode_int4_workspace_bytes(void);

@@ -126,3 +126,14 @@ def test_the_longest_table_rows(dh, Hq):
             d.q, d.table, d.pool = c.q, c.table, c.pool
             d.lens = torch.tensor([ln], dtype=torch.int32, device=DEV)
             _check(d, d.run(window=window))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G", [2, 8])
+def test_scores_of_next_to_nothing(dtype, G):
+    """Scales far below 1, and queries of zeros or of the type's smallest entries: the mean of the values."""
+    for scale in (1e-12, 1e-20, 1e-30, 1e-44):
+        c = Case([5, 130, 3000], 2 * G, 2, dtype=dtype, seed=G)
+        c.q[:, 0] = 0
+        c.q[:, 1] = torch.finfo(dtype).tiny
+        _check(c, c.run(scale=scale), scale=scale)
