@@ -234,14 +234,8 @@ void decode_call(DecodeCall& c, const at::Tensor& q, const at::Tensor& table, co
   const int want_lse = PyObject_IsTrue(lse);
   if (want_lse < 0) throw python_error();
   c.code = dtype_code(q);
-  if (want_lse) {  // one allocation: outputs (16-bit rows of dh, a multiple of 64), then sums
-    const int64_t rows = B * Hq * Tq;
-    const at::Tensor both = empty(q, {rows * (2 * dh + 4)}, at::kByte);
-    c.out = part(both, 0, {B, Hq, Tq, dh}, dt);
-    c.lse = part(both, 2 * rows * dh, {B, Hq, Tq}, at::kFloat);
-  } else {
-    c.out = empty(q, {B, Hq, Tq, dh}, dt);
-  }
+  c.out = empty(q, {B, Hq, Tq, dh}, dt);
+  if (want_lse) c.lse = empty(q, {B, Hq, Tq}, at::kFloat);  // (of its own: a caller that keeps it alone does not keep the outputs)
   c.out4 = view4(c.out, "out");
 }
 PyObject* decode_result(int st, const DecodeCall& c) {

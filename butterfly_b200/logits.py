@@ -31,7 +31,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     A negative token is padding: its log probability is 0, so that it drops out of sums.  One that is not below V has -inf.
     Entries of -inf are masked; a row of nothing else has log probabilities -inf and entropy 0.  A row
     with a NaN or +inf gives NaN for both (its ids are in range, NaN ordered as -inf).  fp32 sums; the
-    results carry no gradient."""
+    results carry no gradient, and share one allocation, which each keeps alive (``clone`` one that is to outlive the others)."""
     global _native
     if _native is None:
         _native = _lib.native()

@@ -190,7 +190,7 @@ def paged_append_int4(k: torch.Tensor, v: torch.Tensor, kv_pages: torch.Tensor, 
 
 def paged_read_int4(kv_pages: torch.Tensor, slot_map: torch.Tensor, *, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
     """The rows in slots ``slot_map`` (int64 [tokens]) as k, v [tokens, Hkv, dh] of ``dtype``, the type they were
-    appended in; zeros for negative slots."""
+    appended in; zeros for negative slots.  k and v share one allocation, which either keeps alive."""
     r = (_native or _binding()).read_int4(kv_pages, slot_map, _lib.dtype_code(dtype) == _lib.F16, _stream(kv_pages))
     if r.__class__ is int:
         _lib.check(r)
