@@ -8,7 +8,8 @@ with stock (dense) attention and once swapped onto the B200 compressed kernels, 
   stock top-k tokens that also appear in the compressed top-k (reference ``_kl``, :228-238)
 * top-k overlap and top-1 agreement of those distributions (:241-262)
 * exact match and token-by-token agreement of the greedy suffix
-* the prompt's own tokens: mean negative log likelihood and mean entropy under each (``prompt_scores``).
+* with ``score_prompt`` the prompt's own tokens: mean negative log likelihood and mean entropy under each (``prompt_scores``,
+  one more forward of the prompt each).
 
 The smoke is descriptive, as the reference's: it reports, it does not assert.
 
@@ -29,15 +30,20 @@ from ..logits import token_logprobs
 
 def prompt_scores(model, input_ids: torch.Tensor, chunk: int = 1024) -> Dict[str, float]:
     """Mean negative log likelihood (nats) of each token of ``input_ids`` [1, T] after those before it, and mean
-    entropy of the distributions it is drawn from.  The logits exist ``chunk`` rows at a time."""
+    entropy of the distributions it is drawn from.  The logits exist ``chunk`` rows at a time where the model has a backbone
+    ``model`` and an ``lm_head``; all at once, from its own call, where it has not."""
     with torch.no_grad():
-        hidden = model.model(input_ids=input_ids, use_cache=False).last_hidden_state[0, :-1]
+        backbone, head = getattr(model, "model", None), getattr(model, "lm_head", None)
+        if backbone is not None and head is not None:
+            rows = backbone(input_ids=input_ids, use_cache=False).last_hidden_state[0, :-1]
+        else:
+            rows, head = model(input_ids=input_ids, use_cache=False).logits[0, :-1], lambda x: x
         targets = input_ids[0, 1:]
-        sums = torch.zeros(2, dtype=torch.float64, device=hidden.device)
-        for i in range(0, hidden.shape[0], chunk):
-            r = token_logprobs(model.lm_head(hidden[i:i + chunk]), targets[i:i + chunk])
+        sums = torch.zeros(2, dtype=torch.float64, device=rows.device)
+        for i in range(0, rows.shape[0], chunk):
+            r = token_logprobs(head(rows[i:i + chunk]), targets[i:i + chunk])
             sums += torch.stack([-r.logprobs.double().sum(), r.entropy.double().sum()])
-    nll, entropy = (sums / max(1, hidden.shape[0])).tolist()
+    nll, entropy = (sums / max(1, rows.shape[0])).tolist()
     return {"nll": nll, "entropy": entropy}
 
 
@@ -98,16 +104,17 @@ def prompt_ids(vocab: int, seq_len: int, seed: int = 42) -> torch.Tensor:
 
 
 def quality_smoke(model, input_ids: torch.Tensor, decode_len: int = 32, top_k: int = 50,
-                  fused: bool = True) -> Dict[str, Any]:
+                  fused: bool = True, score_prompt: bool = False) -> Dict[str, Any]:
     """Run ``model`` (stock Qwen3.5 attention) both ways and compare; the model is left
-    with its stock attention restored."""
+    with its stock attention restored.  ``score_prompt`` adds ``prompt_scores`` of both to the metrics
+    (``prompt_nll_stock`` and so on)."""
     from transformers import DynamicCache
 
     from . import qwen_torch as qt
     from .qwen_fused import fuse_qwen_decoder_layers, unfuse_qwen_decoder_layers
     qt.patch_qwen35_full_attention_decode()
     stock = run_mode(model, input_ids, decode_len, top_k, DynamicCache(config=model.config))
-    scores = {"stock": prompt_scores(model, input_ids)}
+    scores = {"stock": prompt_scores(model, input_ids)} if score_prompt else {}
     qt.swap_qwen_attention_with_butterfly_cuda(model, qt.compressed_config())
     if fused:
         fuse_qwen_decoder_layers(model)
@@ -116,7 +123,8 @@ def quality_smoke(model, input_ids: torch.Tensor, decode_len: int = 32, top_k: i
                                          max_kv_size=int(input_ids.shape[1]) + decode_len + 64,
                                          max_chunk_size=4096)
         comp = run_mode(model, input_ids, decode_len, top_k, cache)
-        scores["compressed"] = prompt_scores(model, input_ids)
+        if score_prompt:
+            scores["compressed"] = prompt_scores(model, input_ids)
     finally:
         unfuse_qwen_decoder_layers(model)
         qt.restore_qwen_dense_attention(model)
@@ -131,6 +139,7 @@ def main() -> None:
     ap.add_argument("--seq-len", type=int, default=8192)
     ap.add_argument("--decode-len", type=int, default=32)
     ap.add_argument("--top-k", type=int, default=50)
+    ap.add_argument("--score-prompt", action="store_true", help="also score the prompt's own tokens under both")
     ap.add_argument("--seed", type=int, default=1)
     ap.add_argument("--out-path", default=None)
     args = ap.parse_args()
@@ -149,7 +158,7 @@ def main() -> None:
             model = Qwen3_5ForCausalLM(cfg)
         model = model.to(torch.bfloat16).eval()
     ids = prompt_ids(model.config.vocab_size, args.seq_len).to(dev)
-    res = quality_smoke(model, ids, args.decode_len, args.top_k)
+    res = quality_smoke(model, ids, args.decode_len, args.top_k, score_prompt=args.score_prompt)
     text = json.dumps(res, indent=1)
     if args.out_path:
         with open(args.out_path, "w") as f:
