@@ -181,16 +181,15 @@ struct Row {
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs a, int cluster) {
   constexpr int E = Row<T>::E;
-  __shared__ uint64_t list[kList];
-  __shared__ uint64_t group[kTop], top[kTop];
-  __shared__ float sums[3][kWarps];  // ref, Z, W of the warps, then of the CTA in column 0
-  __shared__ uint64_t few[kFew];
-  __shared__ uint64_t bound, few_bound;
-  __shared__ int few_count;
-  __shared__ int owners[kThreads];
-  __shared__ uint64_t all_top[kMaxCluster * kTop];  // of the cluster's CTAs, in the first one
-  __shared__ float all_sums[3][kMaxCluster];
-  __shared__ int count;
+  // Shared memory is read and written an element at a time, each of its array's type and by an index into that array, here
+  // and (all_top, all_sums) from the cluster's other CTAs, whose arrays lie at the same offsets.  Global memory: the row by 16 bytes at
+  // multiples of 16 (base) or by its elements, tokens and results by theirs; the C call checks their pointers.
+  alignas(8) __shared__ uint64_t list[kList], group[kTop], top[kTop], few[kFew], bound, few_bound;
+  alignas(8) __shared__ uint64_t all_top[kMaxCluster * kTop];  // of the cluster's CTAs, in the first one
+  alignas(4) __shared__ float sums[3][kWarps];  // ref, Z, W of the warps, then of the CTA in column 0
+  alignas(4) __shared__ float all_sums[3][kMaxCluster];
+  alignas(4) __shared__ int few_count, count, owners[kThreads];
+  static_assert(alignof(uint64_t) == 8 && alignof(float) == 4 && 16 % sizeof(T) == 0 && E * sizeof(T) == 16, "");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = cluster > 1 ? (int)cluster_ctarank() : 0;
   const int r = (int)blockIdx.x / cluster;
@@ -476,7 +475,7 @@ __global__ void __launch_bounds__(32 * kShortWarps) logprob_short_kernel(const L
   constexpr int E = Row<T>::E, N = kShort / 32 / E;
   // ranks without the bits that no entry of the type sets
   constexpr int kDrop = std::is_same<T, __nv_bfloat16>::value ? 16 : std::is_same<T, __half>::value ? 13 : 0;
-  __shared__ uint64_t picks[kShortWarps][kTop];
+  alignas(8) __shared__ uint64_t picks[kShortWarps][kTop];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
