@@ -13,8 +13,8 @@
 // A row is shared by a cluster of CTAs where there are few rows; the CTAs' sums and lists are joined
 // through distributed shared memory by the cluster's first one.
 //
-// Measured, with the likeliest entry: 4,096 rows of 151,936 in bf16 212 us for 1.24 GB, 5.9 TB/s (0.90 of a copy; the issue slots are 67% and
-// the exponential's pipe 56% busy).  512 threads and three CTAs an SM, so that the end of one row (bound,
+// Measured, with the likeliest entry: 4,096 rows of 151,936 in bf16 212 us at 1,965 MHz for 1.24 GB, 5.9 TB/s (0.90 of a copy; the issue
+// slots are 67% and the exponential's pipe 56% busy); call after call, under the power cap at 1,700 MHz, 232 to 250 us.  512 threads and three CTAs an SM, so that the end of one row (bound,
 // candidates, ranks) lies beside the reads of two others.  One row with 20 alternatives 7.8 us: latency.
 #include <cuda_runtime.h>
 
@@ -468,7 +468,8 @@ __global__ void __launch_bounds__(kThreads, 3) logprob_kernel(const LogprobArgs 
 
 // Rows of up to kShort entries, a warp to each, held in registers: the sums around the row's maximum, then the rank of the k-th
 // largest entry by bisection (a count over the warp each), the entries above it and the first of those that equal it.  65,536 rows of 1,000 in
-// bf16: 82 us without alternatives, 245 with 5, 348 with 64 (131 MB: 20 us of a copy), bound by instructions.
+// bf16: 82 us without alternatives, 242 with 5, 348 with 64 (131 MB: 20 us of a copy).  Without alternatives bound by loads that nothing
+// covers (17 warps an SM, issue slots 38% busy), with them by four times the instructions and their fetch (50%).
 constexpr int kShort = 1024, kShortWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(32 * kShortWarps) logprob_short_kernel(const LogprobArgs a, int rows) {

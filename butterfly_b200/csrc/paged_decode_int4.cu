@@ -9,7 +9,7 @@
 // Tensor-core form (m16n8k16, 16 keys x up to 8 query heads): S^T = C_k Q^T and O^T = C_v^T P^T.  A code
 // c masked in place in a 16-bit half of a code word is the fp16 subnormal 2^-24 c, or 2^-20 c for the
 // odd code beside it, so a code word becomes four operand registers with five integer instructions and
-// no conversion.  q is scaled by a power of two into the fp16 range (by head; exact but for entries 2^-24 of
+// no conversion.  q is scaled by a power of two into the fp16 range (by head; exact but for entries 2^-23 of
 // the head's largest), and 2^-4 of that meets the odd codes.
 //
 // Bytes: 18 dh / 16 a token and head.  A read serves up to 8 query heads (16 at head_dim 64 and 128 with more than 8).
@@ -26,8 +26,9 @@
 // Half of the keys enter P V as 15 - c with scale -s and minimum m + 15 s, so that what the tensor core cuts off its
 // sums cancels.
 //
-// Measured (in a CUDA graph): 64 requests of 65,536 tokens, 8 / 2 heads of 128, bf16: 215 us for 1.21 GB, 5.6 TB/s (0.86 of a copy; the
-// 16-bit kernel takes 610 us for its 4.3 GB; one unit for all groups and heads, which lost small ones, 211 us).  Bound by the instructions of a
+// Measured at 1,965 MHz: 64 requests of 65,536 tokens, 8 / 2 heads of 128, bf16: 215 us for 1.21 GB, 5.6 TB/s (0.86 of a copy; the
+// 16-bit kernel takes 610 us for its 4.3 GB; one unit for all groups and heads, which lost small ones, 211 us); call after call, under the
+// power cap at 1,700 MHz, 236 to 252 us.  Bound by the instructions of a
 // granule as much as by HBM.  One request of 131,072 tokens: 18.3 us, some 4 of them before the first keys and 4 in the join.  4 requests of 37 to 513 tokens: 10 us, latency.
 #include <cuda_runtime.h>
 

@@ -224,7 +224,7 @@ def main() -> None:
     torch.cuda.synchronize()
     ms = (time.perf_counter() - t0) / (args.steps - untimed) * 1e3
     print(f"{args.requests} requests of {min(lens)} to {max(lens)} prompt tokens, {args.cache_bits}-bit cache of {dec.cache.nbytes / 1e6:.1f} MB: "
-          f"{ms:.3f} ms a step, {args.requests / ms * 1e3:.0f} tokens/s, mean log probability {float(total) / (args.requests * args.steps):.3f}; lengths now {dec.cache.lens.tolist()}, "
+          f"{ms:.3f} ms a step, {args.requests / ms * 1e3:.0f} tokens/s, mean log probability of the tokens chosen {float(total) / (args.requests * args.steps):.3f}; lengths now {dec.cache.lens.tolist()}, "
           f"{int(dec.cache.num_free)} of {int(dec.cache.free_pages.numel())} pages free")
 
 

@@ -1,7 +1,7 @@
 """Log probabilities of given tokens, entropies and likeliest alternatives, from logits.
 
-What a server returns beside its tokens, and what a compressed cache or attention is judged by
-(``integrations.quality_smoke``): one pass over the logits, which are read once and never copied to fp32.
+What a server returns beside its tokens, and what ``integrations.quality_smoke`` can score a prompt with under stock and compressed
+attention: one pass over the logits, which are read once and never copied to fp32.
 """
 from __future__ import annotations
 

@@ -203,7 +203,7 @@ def paged_decode_attention_int4(q: torch.Tensor, kv_pages: torch.Tensor, block_t
                                 return_lse: bool = False, workspace: Optional[torch.Tensor] = None):
     """``paged_decode_attention`` over a 4-bit pool whose rows were appended in q's type.
 
-    Keys and values count as s c + m without another rounding.  Entries of q below 2^-24 of their head's largest are off by up
+    Keys and values count as s c + m without another rounding.  Entries of q below 2^-23 of their head's largest are off by up
     to 2^-34 of it; a probability times a value scale is rounded to 2^-11 (bf16) or 2^-22 (fp16) of itself and to 2^-27 of the largest such
     product of its head and group of columns.  ``k_new`` / ``v_new`` are packed as
     ``paged_append_int4`` would and attended to in that form.  A row that attends to a NaN is NaN.  Entries of

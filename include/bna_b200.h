@@ -425,7 +425,7 @@ BNA_API int bna_paged_append_int4(const bna_tensor4* k, const bna_tensor4* v, bn
 BNA_API int bna_paged_read_int4(const bna_tensor4* kv_pages, const int64_t* slot_map, bna_tensor4* k, bna_tensor4* v, int32_t dtype,
                                 void* stream);
 /* bna_paged_decode over such a pool: attention to the rows' values s c + m, which are not rounded themselves.  q is exact but for
- * entries below 2^-24 of its head's largest, which are off by 2^-34 of that one at most; a product of a probability and a value scale
+ * entries below 2^-23 of its head's largest, which are off by 2^-34 of that one at most; a product of a probability and a value scale
  * is rounded to 2^-11 (bf16) or 2^-22 (fp16 rows) of itself and to 2^-27 of the largest one of its head and column group.  k_new / v_new are packed as an
  * append would, written, and attended to in that form.  Rows that attend to a NaN are NaN; entries of q from 2^114 on in
  * magnitude, or from 2^114 / scale on, count as infinite, and values from 2^100 on may overflow.  workspace: bna_paged_decode_int4_workspace_bytes() of device memory,
