@@ -62,11 +62,11 @@ constexpr int kSlack = 20, kWhole = 80;
 constexpr int kMinShare = 32;
 constexpr int kKeepLens = 1024;  // lengths kept in shared memory
 constexpr int kShift = 11;  // probabilities are held times 2^kShift, and so are l and o; the divisions undo it
-constexpr float kMove = 4.f;  // a reference moves when a score lies more than 2^kMove above it
+constexpr float kMove = 4.f;  // a reference moves when a score lies more than that above it
 // A new unit of products is 2^kRoom times the largest scale or more, so that ones up to 2^(kRoom - 1) times as large need no other,
 // but leaves the largest product at 2^kLeast or more, however large the scales of keys without weight are.
 constexpr int kRoom = 3, kLeast = 3;
-constexpr float kNone = -1e30f;  // the offset of a reference that has seen no key
+constexpr float kNone = 1e30f;  // `add` of a reference that has seen no key
 
 struct Int4Args {
   const uint8_t* q;
@@ -229,7 +229,7 @@ struct Acc {
   uint32_t qb[NT][GR][2][2][2];  // Q^T fragments: tile, group, word of the lane, step, register
   float qs[NT][GR][2];           // sum(q_y), scaled as the products with codes are
   float f[NT][2];                // from those to scores in the exp2 domain
-  float ref[NT][2], off[NT][2];  // running reference (no score lies 2^kMove above it), and it less kShift
+  float ref[NT][2], add[NT][2];  // running reference (no score lies kMove above it), and kShift less it
   float l[NT][2], wm[NT][GR][2];  // this lane's keys: sum p, sum p mv_y
   float o[NT][GR][4][4];          // sum p sv cv, in units of 2^-24 (odd columns 2^-20) 2^k
   // 2^-k of each head and group.  The unit follows the group's largest product p sv, also down as the reference moves, so that what is
@@ -311,7 +311,7 @@ struct Acc {
           inv[n][y][x] = pow2(kMaxExp);
         }
         ref[n][x] = -INFINITY;
-        off[n][x] = kNone;
+        add[n][x] = kNone;
         l[n][x] = 0.f;
       }
 #pragma unroll
@@ -420,8 +420,10 @@ struct Acc {
         }
         top = fmax3(fmax3(top, w[n][y][0], w[n][y][1]), w[n][y][2], w[n][y][3]);
       }
+      // The scores are rounded before the reference is taken off, here and in a move: from 2^27 on their roundings are above 2^kMove, and
+      // equal ones must stay equal.  (A packed product and sum would be made one operation.)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) e[n][x] = fmaf(f[n][x & 1], u[n][x], -off[n][x & 1]);
+      for (int x = 0; x < 4; ++x) e[n][x] = __fadd_rn(__fmul_rn(f[n][x & 1], u[n][x]), add[n][x & 1]);
       most = fmax3(most, fmaxf(e[n][0], e[n][1]), fmaxf(e[n][2], e[n][3]));
     }
     // without a move no product is above 2^(kShift + kMove) = 2^15
@@ -434,20 +436,21 @@ struct Acc {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float s0 = f[n][x] * u[n][x], s1 = f[n][x] * u[n][2 + x], mx = fmaxf(ref[n][x], lane_max(fmaxf(s0, s1)));
-          const float to = mx == -INFINITY ? kNone : mx - (float)kShift, by = off[n][x] - to, al = ex2_approx(by);
+          const float s0 = __fmul_rn(f[n][x], u[n][x]), s1 = __fmul_rn(f[n][x], u[n][2 + x]), mx = fmaxf(ref[n][x], lane_max(fmaxf(s0, s1)));
+          const float to = mx == -INFINITY ? kNone : (float)kShift - mx, by = to - add[n][x], al = ex2_approx(by);
           // (differences of whole parts: many small moves take the unit as far as one large one)
-          const int less = (int)fmaxf(floorf(off[n][x]) - floorf(to), -4.f * kMaxExp);
+          const int less = (int)fmaxf(ceilf(to) - ceilf(add[n][x]), -4.f * kMaxExp);
           ref[n][x] = mx;
-          off[n][x] = to;
+          add[n][x] = to;
           l[n][x] *= al;
-          e[n][x] = ex2_approx(fmaf(f[n][x], u[n][x], -to));
-          e[n][2 + x] = ex2_approx(fmaf(f[n][x], u[n][2 + x], -to));
+          const float e0 = s0 + to, e1 = s1 + to;
+          e[n][x] = ex2_approx(e0);
+          e[n][2 + x] = ex2_approx(e1);
 #pragma unroll
           for (int y = 0; y < GR; ++y) {
             wm[n][y][x] *= al;
             // the largest product's exponent, or one less
-            const float largest = lane_max(fmaxf(s0 + (float)exponent(sv[0][y]), s1 + (float)exponent(sv[1][y]))) - to;
+            const float largest = lane_max(fmaxf(e0 + (float)exponent(sv[0][y]), e1 + (float)exponent(sv[1][y])));
             const int old = -exponent(inv[n][y][x]);
             const int k = min(max(max(old + less, min(high[y] + kRoom, (int)floorf(fmaxf(largest, -4.f * kMaxExp)) - kLeast)), -kMaxExp), kMaxExp);
             const float scale = ex2_approx(by + (float)(old - k));

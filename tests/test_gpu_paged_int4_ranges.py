@@ -137,3 +137,30 @@ def test_scores_of_next_to_nothing(dtype, G):
         c.q[:, 0] = 0
         c.q[:, 1] = torch.finfo(dtype).tiny
         _check(c, c.run(scale=scale), scale=scale)
+
+
+def _check_equal(c, got, top):
+    """All weight in equal parts on the keys `top` of a request alone, whose scores are equal sums and far above the others."""
+    out, lse = got
+    dh, G = c.dh, c.Hq // c.Hkv
+    ref = value(c.v[0])[:, top].mean(1).repeat_interleave(G, 0)
+    _, s, m = pack(c.v[0])
+    own = (15 * s.double() + m.double().abs()).repeat_interleave(64, -1)[:, top].mean(1).repeat_interleave(G, 0)
+    assert ((out[0, :, 0].double() - ref).abs() <= U[c.dtype] * ref.abs() + own * (2 ** -18 + 2 * W[c.dtype])).all()
+    z = (c.q[0, :, 0].double() * value(c.k[0])[:, top[0]].repeat_interleave(G, 0)).sum(-1) / math.sqrt(dh) + math.log(len(top))
+    assert ((lse[0, :, 0].double() - z).abs() <= (dh + 10) * 2 ** -22 * z.abs()).all()
+
+
+@pytest.mark.parametrize("dtype,sizes", [(torch.bfloat16, (2.0 ** 26, 2.0 ** 32, 2.0 ** 50, 2.0 ** 90)), (torch.float16, (2.0 ** 22, 2.0 ** 29))])
+@pytest.mark.parametrize("dh,G", [(64, 3), (128, 4), (128, 8), (256, 2)])
+def test_scores_far_above_zero(dtype, sizes, dh, G):
+    """Scores up to `sizes`, the largest far from the others, over groups of small and of large values."""
+    high = 20 if dtype == torch.bfloat16 else 10
+    for size in sizes:
+        q = min(2.0 ** 14, size ** 0.5)
+        k = _levels(dtype, dh, lambda j: torch.where(j % 39 == 7, 1.25, 0.25 + 0.5 * (j % 2)) * (size / q / math.sqrt(dh)))
+        for sign in (1, -1):  # the group with large values
+            v = _normal(3, dtype, dh, lambda j, y: sign * high * (1 - 2 * (y % 2)))
+            c = Case([500], 2 * G, 2, dh=dh, dtype=dtype, k=k, v=v)
+            _equal_queries(c, [q * math.sqrt(dh)])
+            _check_equal(c, c.run(), list(range(7, 500, 39)))
