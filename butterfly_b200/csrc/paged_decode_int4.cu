@@ -66,7 +66,7 @@ constexpr float kMove = 4.f;  // a reference moves when a score lies more than t
 // A new unit of products is 2^kRoom times the largest scale or more, so that ones up to 2^(kRoom - 1) times as large need no other,
 // but leaves the largest product at 2^kLeast or more, however large the scales of keys without weight are.
 constexpr int kRoom = 3, kLeast = 3;
-constexpr float kNone = 1e30f;  // `add` of a reference that has seen no key
+constexpr float kNone = 0x1.fffffep127f;  // `add` of a reference that has seen no key: any score moves it, however low
 
 struct Int4Args {
   const uint8_t* q;

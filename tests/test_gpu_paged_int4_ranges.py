@@ -164,3 +164,14 @@ def test_scores_far_above_zero(dtype, sizes, dh, G):
             c = Case([500], 2 * G, 2, dh=dh, dtype=dtype, k=k, v=v)
             _equal_queries(c, [q * math.sqrt(dh)])
             _check_equal(c, c.run(), list(range(7, 500, 39)))
+
+
+@pytest.mark.parametrize("dh,G", [(64, 3), (128, 4), (128, 8), (256, 2)])
+def test_scores_far_below_zero(dh, G):
+    """Nothing but scores down to -2^106: the least low ones have all weight."""
+    for size in (2.0 ** 30, 2.0 ** 98, 2.0 ** 106):
+        q = min(2.0 ** 50, size ** 0.5)
+        k = _levels(torch.bfloat16, dh, lambda j: -torch.where(j % 39 == 7, 0.25, 0.5 + 0.5 * (j % 2)) * (size / q / math.sqrt(dh)))
+        c = Case([500], 2 * G, 2, dh=dh, k=k, v=_normal(4, torch.bfloat16, dh, lambda j, y: 0 * y))
+        _equal_queries(c, [q * math.sqrt(dh)])
+        _check_equal(c, c.run(), list(range(7, 500, 39)))
