@@ -609,7 +609,7 @@ int bna_paged_decode_int4(const bna_tensor4* q, bna_tensor4* kv_pages, const bna
   if ((int64_t)table_width * kv_pages->size[2] * 16 > INT32_MAX)
     return fail(BNA_UNSUPPORTED, "paged_decode_int4: a table row covers 2^31 tokens or more");
   if (window < 0) return fail(BNA_BAD_SHAPE, "window must be >= 0 (0: every key)");
-  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(BNA_BAD_SHAPE, "scale must be positive");
+  if (!(scale > 0.f) || !std::isfinite(scale * 1.4426950408889634f)) return fail(BNA_BAD_SHAPE, "scale must be positive, and finite in powers of two");
   if (!workspace || workspace_bytes < paged_decode_int4_workspace_bytes())
     return fail(BNA_CAPACITY, "paged_decode_int4: workspace smaller than bna_paged_decode_int4_workspace_bytes()");
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BNA_BAD_STRIDE, "paged_decode_int4: workspace must be 16-byte aligned");
